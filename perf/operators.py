@@ -422,5 +422,21 @@ def _exact_attention(case, s):
 
 
 def _exact_evict(case, s):
-    # Every output is a copy of an input or a whole number.
-    return {"kept": None, "lens": None, "weights": None, "k": None, "v": None}
+    lens, _ = _lens(case)
+    page, budget = case["page"], case["budget"]
+    k, v, weights = s["k"].double(), s["v"].double(), s["weights_out"].double()
+    given = s["weights"].cpu().numpy()
+    for i, end in enumerate(lens):
+        source_page, source_row = _slots_of(case, s, i, end)
+        for h in range(case["kv_heads"]):
+            middle = [] if end <= budget else range(case["sinks"], end - case["recent"])
+            leaving = sorted(middle, key=lambda j: (-float(given[i, h, j]), j))[budget - case["sinks"] - case["recent"]:]
+            stays = torch.ones(end, dtype=torch.bool)
+            stays[leaving] = False
+            kept = stays.nonzero()[:, 0].cuda()
+            to = torch.arange(kept.shape[0], device="cuda")
+            where = s["table_out"][i].long()[to // page], h, to % page
+            k[where], v[where] = k[source_page[kept], h, source_row[kept]], v[source_page[kept], h, source_row[kept]]
+            weights[i, h, to] = s["weights"][i, h, kept].double()
+    # (The places and lengths that are kept are whole numbers.)
+    return {"kept": None, "lens": None, "weights": weights, "k": k, "v": v}
