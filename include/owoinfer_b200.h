@@ -656,6 +656,96 @@ const b2_time_embedding* b2_dit_file_time_embedding(const b2_dit_file* file);
 const b2_time_mlp_bf16* b2_dit_file_time_mlp_bf16(const b2_dit_file* file);
 void b2_dit_file_close(b2_dit_file* file);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * A language model's layer on a paged key-value cache: what the text side of the image model runs to write or rewrite a
+ * prompt and to make its text rows. No counterpart in the reference's DiT path.
+ *
+ * Element types: bf16 or fp16, every 16-bit tensor of a call alike; sums, norms and softmax statistics in fp32, each output
+ * rounded once. head_dim 64 or 128; q_heads a multiple of kv_heads (query head h reads key head h / (q_heads / kv_heads)).
+ * The calls follow the conventions above: they allocate nothing, do not synchronise and can be captured. Device data that
+ * the host cannot check (lengths, block tables, cu_seqlens, positions) is checked by the kernels: what would lead out of
+ * bounds is neither read nor written (a page outside the pool reads as zeros, a length is cut to what is allowed) and raises a
+ * bit of b2_paged_cache_status.
+ * ------------------------------------------------------------------------------------------------------------- */
+
+#define B2_DTYPE_BF16 0
+#define B2_DTYPE_F16 1
+
+/* A pool of pages for keys and one for values (of the same strides, in elements: row r of page p of head h starts at
+ * p * page_stride + h * head_stride + r * row_stride), and for each sequence its pages in order and the number of slots
+ * that are filled. Slot j of sequence b is row j % page_size of page block_table[b * table_ld + j / page_size]; entries
+ * behind a sequence's last page are not read. Pools 16-byte aligned, strides multiples of 8 elements; page_size a power of
+ * two from 16 to 1024; table_width * page_size < 2^31. What lies in slots behind seq_lens does not reach any output, NaN
+ * and infinities included. */
+typedef struct b2_paged_cache {
+  size_t struct_size;
+  void* k;
+  void* v;
+  int64_t page_stride, head_stride, row_stride;
+  int64_t num_pages;
+  int dtype;                   /* B2_DTYPE_* */
+  int kv_heads, page_size, head_dim;
+  const int32_t* block_table;  /* device int32 [batch, table_width], rows table_ld apart */
+  int64_t table_ld;
+  int table_width;
+  const int32_t* seq_lens;     /* device int32 [batch]: slots filled, the tokens of the call included */
+  int batch;
+} b2_paged_cache;
+
+/* Queries and keys of a fused projection normalised per head, rotated by their positions, keys and values put into the
+ * cache, in one pass. qkv [tokens, (q_heads + 2 kv_heads) * head_dim] (rows ld apart): query heads, key heads, value heads.
+ * Sequence b has the tokens [cu_seqlens[b], cu_seqlens[b + 1]) (device int32 [batch + 1]); they fill its last slots.
+ *   y = x * rsqrt(mean(x^2) + eps) * w        (w = q_norm or k_norm [head_dim]; both NULL: y = x)
+ *   (a, b) -> (a cos - b sin, b cos + a sin)  over the pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) with interleaved != 0
+ * rope: device fp32 [rope_rows, rot_dim], each row sin | cos of the position's rot_dim / 2 angles, contiguous, 16-byte aligned;
+ * rot_dim a multiple of 16 up to head_dim (0: no rotation, rope not read). positions: device int32 [tokens] or NULL (a token's
+ * position is its slot; after an eviction the two differ). A position outside the table raises a status bit and is clamped.
+ * q_out: [tokens, q_heads, head_dim] (row and head strides), may be the query part of qkv itself. */
+int b2_qk_norm_rope_append(const b2_paged_cache* cache, const void* qkv, int64_t ld, int64_t tokens, int q_heads,
+                           const int32_t* cu_seqlens, const int32_t* positions, const void* q_norm, const void* k_norm, float eps,
+                           const float* rope, int64_t rope_rows, int rot_dim, int interleaved, void* q_out, int64_t q_row_stride,
+                           int64_t q_head_stride, void* stream);
+
+/* Attention of a prompt's tokens over the cache that holds their keys and values already. Token i of the n a sequence has
+ * in the call sits at slot p = seq_len - n + i and sees the slots j <= p with j < sinks or p - j < window (window 0: every
+ * j <= p). out = softmax(scale * q k^T) v; lse (fp32 [tokens, q_heads], or NULL) = log sum exp(scale * q k^T). A token that
+ * sees nothing (a cache shorter than the call's tokens) gets zeros and -infinity. q, out: views of one dtype [tokens,
+ * q_heads, head_dim]; max_q: no sequence has more tokens in the call. Keys and values of slots that a token does not see do
+ * not reach its output, NaN and infinities included. */
+int b2_attention_paged(const b2_paged_cache* cache, const b2_view3* q, const b2_view3* out, float* lse, const int32_t* cu_seqlens,
+                       int max_q, float scale, int window, int sinks, void* stream);
+
+/* The same for one token per sequence (token b of q and out is sequence b's newest, at slot seq_len - 1), the cache's length
+ * split over the GPU and joined. With weights_out != NULL the attention each slot got is added up besides:
+ *   weights_out[b, h, j] = (j < seq_len - 1 ? weights[b, h, j] : 0) + sum of the softmax weight of slot j over h's query heads
+ * for every slot j < seq_len; the others are left alone. weights, weights_out: device fp32, [batch, kv_heads, slots] with
+ * rows weights_ld apart (at least max_len, or the table's slots), the same buffer or two that do not overlap.
+ * max_len: no sequence is longer (0: as long as the block table allows); the split goes by it.
+ * workspace: b2_attention_paged_decode_workspace_bytes() of the same arguments (with_weights: whether weights_out is given), 256-byte aligned;
+ * nothing in it needs clearing and nothing is kept in it. */
+size_t b2_attention_paged_decode_workspace_bytes(const b2_paged_cache* cache, int q_heads, int max_len, int window, int sinks,
+                                                 int with_weights);
+int b2_attention_paged_decode(const b2_paged_cache* cache, const b2_view3* q, const b2_view3* out, float* lse, int max_len,
+                              float scale, int window, int sinks, const float* weights, float* weights_out, int64_t weights_ld,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* Eviction by accumulated attention weight, for each sequence and key head by itself. A sequence of more than `budget` slots
+ * keeps its first `sinks` slots, its last `recent` ones and, of those between, the ones of largest weight up to `budget` in all
+ * (equal weights: the lower slot stays; NaN ranks below everything); a shorter one keeps all. What is kept moves, in
+ * order, to the pages table_out[b, :] of the same pools (device int32, rows table_out_ld apart, table_out_width * page_size >=
+ * budget): pages that none of the cache's sequences holds.
+ *   kept [batch, kv_heads, budget] int32: the slots that stayed, ascending, then -1;  lens_out [batch] int32: min(seq_len, budget);
+ *   weights_out (or NULL) [batch, kv_heads, slots] fp32, rows weights_out_ld apart: the weights of the slots that stayed.
+ * weights: fp32, rows weights_ld apart (at least table_width * page_size). weights_out must not overlap weights. */
+int b2_kv_evict(const b2_paged_cache* cache, const float* weights, int64_t weights_ld, int sinks, int recent, int budget,
+                const int32_t* table_out, int64_t table_out_ld, int table_out_width, int32_t* kept, int32_t* lens_out,
+                float* weights_out, int64_t weights_out_ld, void* stream);
+
+/* Bits that the kernels on paged caches have raised on the current device since the last clear: 1 a page outside the pool,
+ * 2 a length outside the block table, 4 cu_seqlens out of order or a token without a slot, 8 a position outside the rotation
+ * table, 16 a bounded wait that expired. Synchronises the device: for tests and post-mortems. */
+int b2_paged_cache_status(unsigned* host_value, int clear);
+
 /* Every mbarrier wait inside the tensor-core kernels is bounded (200 ms); a CTA whose wait expired raises a device word,
  * drains and returns instead of hanging. This reads the two words (GEMM, attention): 0 = no wait ever expired on this device.
  * Synchronises the device; for tests and post-mortems, not for the hot path. No counterpart in the reference (its

@@ -24,6 +24,8 @@ EXPORTS = [
     "b2_dit_file_open_expanded", "b2_silu_bf16", "b2_time_modulation_bf16_workspace_bytes", "b2_time_modulation_bf16",
     "b2_dit_graphs_create", "b2_dit_graphs_clear", "b2_dit_graphs_destroy", "b2_dit_graphs_stats", "b2_dit_forward_graphed",
     "b2_dit_file_open", "b2_dit_file_get_info", "b2_dit_file_model", "b2_dit_file_time_embedding", "b2_dit_file_time_mlp_bf16", "b2_dit_file_close",
+    "b2_qk_norm_rope_append", "b2_attention_paged", "b2_attention_paged_decode_workspace_bytes", "b2_attention_paged_decode",
+    "b2_kv_evict", "b2_paged_cache_status",
 ]
 
 
@@ -54,6 +56,13 @@ class AttentionLayout(C.Structure):
     _fields_ = [(n, C.c_size_t) for n in ("q_i8", "k_i8", "v8", "q_scale", "k_scale", "k_mean", "v_scale", "v_recp",
                                           "part_sum", "part_amax", "total")] + \
                [("padded_k", C.c_int64), ("q_blocks", C.c_int), ("k_blocks", C.c_int), ("chunks", C.c_int)]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [("struct_size", C.c_size_t), ("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("row_stride", C.c_int64), ("num_pages", C.c_int64), ("dtype", C.c_int), ("kv_heads", C.c_int), ("page_size", C.c_int),
+                ("head_dim", C.c_int), ("block_table", C.c_void_p), ("table_ld", C.c_int64), ("table_width", C.c_int),
+                ("seq_lens", C.c_void_p), ("batch", C.c_int)]
 
 
 class Linear(C.Structure):
@@ -175,6 +184,14 @@ def lib() -> C.CDLL:
         l.b2_dit_forward_workspace_bytes.argtypes = [C.POINTER(DitModel), C.POINTER(Forward)]
         l.b2_block_quant_sp_workspace_bytes.restype = C.c_size_t
         l.b2_block_quant_sp_workspace_bytes.argtypes = [C.POINTER(SpRun), C.c_int]
+        cache, view, p, i, n = C.POINTER(PagedCache), C.POINTER(View3), C.c_void_p, C.c_int, C.c_int64
+        l.b2_qk_norm_rope_append.argtypes = [cache, p, n, n, i, p, p, p, p, C.c_float, p, n, i, i, p, n, n, p]
+        l.b2_attention_paged.argtypes = [cache, view, view, p, p, i, C.c_float, i, i, p]
+        l.b2_attention_paged_decode_workspace_bytes.restype = C.c_size_t
+        l.b2_attention_paged_decode_workspace_bytes.argtypes = [cache, i, i, i, i, i]
+        l.b2_attention_paged_decode.argtypes = [cache, view, view, p, i, C.c_float, i, i, p, p, n, p, C.c_size_t, p]
+        l.b2_kv_evict.argtypes = [cache, p, n, i, i, i, p, n, i, p, p, p, n, p]
+        l.b2_paged_cache_status.argtypes = [C.POINTER(C.c_uint), i]
         _lib = l
     return _lib
 

@@ -11,7 +11,9 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "csrc", "build")
 LIB = os.path.join(HERE, "libowoinfer_b200.so")
-SOURCES = ["api.cu", "rotate_quantize.cu", "int8_gemm.cu", "attention.cu", "block.cu", "sp_block.cu", "sampler_step.cu", "dit_shell.cu", "dit_loader.cu"]
+SOURCES = ["api.cu", "rotate_quantize.cu", "int8_gemm.cu", "attention.cu", "block.cu", "sp_block.cu", "sampler_step.cu", "dit_shell.cu", "dit_loader.cu",
+           "paged_cache.cu", "paged_decode.cu", "paged_attention.cu"]
+HEADERS = ["common.cuh", "attention.cuh", "paged.cuh"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
          "-I", os.path.join(ROOT, "include"), "-I", CSRC]
@@ -26,7 +28,7 @@ def _stale(target: str, deps: list[str]) -> bool:
 
 def _compile(src: str, verbose: bool) -> str:
     obj = os.path.join(OBJ, src.replace(".cu", ".o"))
-    deps = [os.path.join(CSRC, src), os.path.join(CSRC, "common.cuh"), os.path.join(ROOT, "include", "owoinfer_b200.h")]
+    deps = [os.path.join(CSRC, src), *(os.path.join(CSRC, h) for h in HEADERS), os.path.join(ROOT, "include", "owoinfer_b200.h")]
     if _stale(obj, deps):
         cmd = [NVCC, *FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-c", os.path.join(CSRC, src), "-o", obj]
         r = subprocess.run(cmd, capture_output=True, text=True)

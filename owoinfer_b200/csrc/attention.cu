@@ -25,7 +25,7 @@
 #include <limits>
 #include <string>
 
-#include "common.cuh"
+#include "attention.cuh"
 
 namespace b2 {
 namespace {
@@ -41,48 +41,6 @@ __device__ long long g_attn_trace[8192];
 #else
 #define TRACE(slot) do { } while (0)
 #endif
-
-__device__ __forceinline__ std::uint64_t global_ns() {
-  std::uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-__device__ __forceinline__ bool wait_bar(std::uint32_t bar, std::uint32_t parity, volatile int* abort_word) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const std::uint64_t t0 = global_ns();
-  for (;;) {
-    // A tight inner loop (test, branch); the abort word and the clock are looked at once per 256 tests.
-#pragma unroll 1
-    for (int i = 0; i < 256; ++i) {
-      if (mbar_try_wait_hint(bar, parity)) return true;
-    }
-    if (*abort_word != 0) return false;
-    if (global_ns() - t0 > 200000000ull) {
-      *abort_word = 1;
-      return false;
-    }
-  }
-}
-
-// The same for a role with slack (the TMA and MMA warps share their scheduler with softmax warps): sleeps between tests so
-// that waiting costs next to no issue slots.
-template <int kSleepNs>
-__device__ __forceinline__ bool wait_bar_relaxed(std::uint32_t bar, std::uint32_t parity, volatile int* abort_word) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const std::uint64_t t0 = global_ns();
-  for (;;) {
-#pragma unroll 1
-    for (int i = 0; i < 64; ++i) {
-      __nanosleep(kSleepNs);
-      if (mbar_try_wait(bar, parity)) return true;
-    }
-    if (*abort_word != 0) return false;
-    if (global_ns() - t0 > 200000000ull) {
-      *abort_word = 1;
-      return false;
-    }
-  }
-}
 
 __device__ __forceinline__ void load8(const __nv_bfloat16* p, float* x) {
   const uint4 raw = *reinterpret_cast<const uint4*>(p);
@@ -122,46 +80,12 @@ __device__ __forceinline__ std::uint32_t e4m3x4(float a, float b, float c, float
       : "f"(a), "f"(b), "f"(c), "f"(d));
   return w;
 }
-// Packed fp32 pairs (one instruction for two lanes of work): d = a * b + c and d = a + b on (x, y) pairs.
-__device__ __forceinline__ std::uint64_t pack2(float x, float y) {
-  std::uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void unpack2(std::uint64_t v, float& x, float& y) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
-}
-__device__ __forceinline__ std::uint64_t fma2(std::uint64_t a, std::uint64_t b, std::uint64_t c) {
-  std::uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ std::uint64_t add2(std::uint64_t a, std::uint64_t b) {
-  std::uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 #ifndef B2_TRACE_WARP
 #define B2_TRACE_WARP 2
 #endif
 #ifndef B2_MMA_SLEEP_NS
 #define B2_MMA_SLEEP_NS 100
 #endif
-__device__ __forceinline__ float rcp_approx(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // ---------------------------------------------------------------------------------------------------------------
 // QK-norm + RoPE (standalone) and the RoPE table.
@@ -983,15 +907,6 @@ __device__ __forceinline__ std::uint64_t umma_desc_sw32(std::uint32_t smem_addr)
   d |= static_cast<std::uint64_t>(6) << 61;
   return d;
 }
-__device__ __forceinline__ void umma_bf16(std::uint32_t d_tmem, std::uint64_t a_desc, std::uint64_t b_desc,
-                                          std::uint32_t idesc, std::uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
 
 // Which (query tile, head, sequence) a CTA works on, and where the sequence's queries and keys lie. kByLength: a flat grid
 // of as many ids as there can be tiles instead of (tiles, heads, sequences), for 2 to 32 sequences (a lane each): longest
@@ -1142,7 +1057,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     // S(u % 2) = [12582912.0f +] Q · K(u)^T, by the elected lane. The constant operand serves as A (128 rows) and as B (its
     // first 64 rows): every row holds the same 16 values.
     const auto issue_scores = [&](std::uint32_t d_s, std::uint64_t dk) {
-      if (B2_ATTN_CONST_BIAS) umma_bf16(d_s, dconst, dconst, idesc_bias, 0u);
+      if (B2_ATTN_CONST_BIAS) umma_f16(d_s, dconst, dconst, idesc_bias, 0u);
 #pragma unroll
       for (int k4 = 0; k4 < 4; ++k4) umma_i8(d_s, dq + 2u * k4, dk + 2u * k4, idesc_qk, (B2_ATTN_CONST_BIAS || k4 != 0) ? 1u : 0u);
     };

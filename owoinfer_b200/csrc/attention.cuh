@@ -1,0 +1,106 @@
+// Device helpers of the attention kernels: bounded waits, packed fp32 arithmetic, the hardware's exponential, 16-bit MMAs.
+#pragma once
+
+#include "common.cuh"
+
+namespace b2 {
+
+__device__ __forceinline__ std::uint64_t global_ns() {
+  std::uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ bool wait_bar(std::uint32_t bar, std::uint32_t parity, volatile int* abort_word) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const std::uint64_t t0 = global_ns();
+  for (;;) {
+    // A tight inner loop (test, branch); the abort word and the clock are looked at once per 256 tests.
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i) {
+      if (mbar_try_wait_hint(bar, parity)) return true;
+    }
+    if (*abort_word != 0) return false;
+    if (global_ns() - t0 > 200000000ull) {
+      *abort_word = 1;
+      return false;
+    }
+  }
+}
+
+// The same for a role with slack (the TMA and MMA warps share their scheduler with softmax warps): sleeps between tests so
+// that waiting costs next to no issue slots.
+template <int kSleepNs>
+__device__ __forceinline__ bool wait_bar_relaxed(std::uint32_t bar, std::uint32_t parity, volatile int* abort_word) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const std::uint64_t t0 = global_ns();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i) {
+      __nanosleep(kSleepNs);
+      if (mbar_try_wait(bar, parity)) return true;
+    }
+    if (*abort_word != 0) return false;
+    if (global_ns() - t0 > 200000000ull) {
+      *abort_word = 1;
+      return false;
+    }
+  }
+}
+
+// Packed fp32 pairs (one instruction for two lanes of work): d = a * b + c and d = a + b on (x, y) pairs.
+__device__ __forceinline__ std::uint64_t pack2(float x, float y) {
+  std::uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(std::uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ std::uint64_t fma2(std::uint64_t a, std::uint64_t b, std::uint64_t c) {
+  std::uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ std::uint64_t add2(std::uint64_t a, std::uint64_t b) {
+  std::uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// D[tmem] (+)= A[smem] * B[smem] for bf16 or fp16 operands, one thread issues.
+__device__ __forceinline__ void umma_f16(std::uint32_t d_tmem, std::uint64_t a_desc, std::uint64_t b_desc,
+                                          std::uint32_t idesc, std::uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The same with A in tensor memory: row r of A is lane r, two values to a 32-bit column in K order (K = 16 is eight columns).
+__device__ __forceinline__ void umma_f16_ts(std::uint32_t d_tmem, std::uint32_t a_tmem, std::uint64_t b_desc,
+                                            std::uint32_t idesc, std::uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+}  // namespace b2

@@ -1,0 +1,112 @@
+// A key-value cache in pages, as the kernels on it see it: argument checks, slot arithmetic with bounds, the status word, and
+// what the 16-bit types need. No counterpart in the reference.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace b2 {
+
+// Why b2_paged_cache_status is not 0.
+enum PagedFault : unsigned {
+  kPagedBadPage = 1,      // a page of the block table outside the pool
+  kPagedBadLength = 2,    // seq_lens below 0 or past the block table or max_len
+  kPagedBadTokens = 4,    // cu_seqlens that do not rise from 0 to the call's tokens, or tokens without a slot
+  kPagedBadPosition = 8,  // a position outside the rotation table
+  kPagedWait = 16,        // a bounded wait expired
+};
+
+struct PagedArgs {
+  void* k;
+  void* v;
+  std::int64_t page_stride, head_stride, row_stride, num_pages;  // elements
+  const std::int32_t* table;
+  std::int64_t table_ld;
+  const std::int32_t* lens;
+  unsigned* status;
+  int most, page_shift, batch, kv_heads;  // most: slots a sequence can have
+};
+
+// Checks the cache of a call and fills `a` but for its status word (head_dim 64 or 128, a page size that is a power of two from 16 to
+// 1024). Makes no CUDA call.
+int check_paged_cache(const char* op, const b2_paged_cache* c, PagedArgs* a);
+// The current device's status word into `a`.
+int paged_status_word(const char* op, PagedArgs* a);
+// Where a call may write or read rows of `row` elements: 16-byte aligned, strides in multiples of 8 elements.
+inline bool rows_ok(const void* p, std::int64_t row, std::int64_t head) { return p != nullptr && aligned_to(p, 16) && row % 8 == 0 && head % 8 == 0; }
+// cuTensorMapEncodeTiled for a pool of pages of 16-bit elements, [pages, heads, rows, head_dim]: boxes of box_rows rows of 64
+// elements, 128-byte swizzle. Returns false (and sets the last error) on failure.
+bool make_tensor_map_pages(CUtensorMap* map, const void* base, int head_dim, int page_size, int heads, std::int64_t pages,
+                           std::int64_t row_stride, std::int64_t head_stride, std::int64_t page_stride, int box_rows, const char* op);
+
+// A window that reaches every slot is none; sinks past the last slot are all slots.
+int check_window(const char* op, const PagedArgs& c, int* window, int* sinks);
+
+#ifdef __CUDACC__
+// Slots of sequence b, at least 0 and at most what its row of the block table (or the call) allows.
+__device__ __forceinline__ int paged_len(const PagedArgs& a, int b) {
+  const int len = a.lens[b];
+  if (len >= 0 && len <= a.most) return len;
+  atomicOr(a.status, kPagedBadLength);
+  return len < 0 ? 0 : a.most;
+}
+// The page with slot `slot` (which lies in the block table) of sequence b, or -1.
+__device__ __forceinline__ int paged_page(const PagedArgs& a, int b, int slot) {
+  const int page = a.table[b * a.table_ld + (slot >> a.page_shift)];
+  if (page >= 0 && page < a.num_pages) return page;
+  atomicOr(a.status, kPagedBadPage);
+  return -1;
+}
+// Offset in elements of a slot's row of one head.
+__device__ __forceinline__ std::int64_t paged_row(const PagedArgs& a, int page, int head, int slot) {
+  return page * a.page_stride + head * a.head_stride + (slot & ((1 << a.page_shift) - 1)) * a.row_stride;
+}
+// The call's tokens of sequence b: [first, first + n) of `tokens`.
+__device__ __forceinline__ void paged_tokens(const PagedArgs& a, const std::int32_t* cu, int b, std::int64_t tokens, int& first, int& n) {
+  const int from = cu[b], to = cu[b + 1];
+  first = from, n = to - from;
+  if (from >= 0 && to >= from && to <= tokens) return;
+  atomicOr(a.status, kPagedBadTokens);
+  first = 0, n = 0;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v) { return static_cast<float>(v); }
+template <typename T>
+__device__ __forceinline__ std::uint32_t pack16(float lo, float hi);
+template <>
+__device__ __forceinline__ std::uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const std::uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ std::uint32_t pack16<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const std::uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ void unpack16(std::uint32_t w, float& lo, float& hi);
+template <>
+__device__ __forceinline__ void unpack16<__nv_bfloat16>(std::uint32_t w, float& lo, float& hi) {
+  lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xFFFF0000u);
+}
+template <>
+__device__ __forceinline__ void unpack16<__half>(std::uint32_t w, float& lo, float& hi) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  lo = f.x, hi = f.y;
+}
+template <typename T>
+__device__ __forceinline__ void load8(const uint4& raw, float (&x)[8]) {
+  unpack16<T>(raw.x, x[0], x[1]);
+  unpack16<T>(raw.y, x[2], x[3]);
+  unpack16<T>(raw.z, x[4], x[5]);
+  unpack16<T>(raw.w, x[6], x[7]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 store8(const float (&x)[8]) {
+  return make_uint4(pack16<T>(x[0], x[1]), pack16<T>(x[2], x[3]), pack16<T>(x[4], x[5]), pack16<T>(x[6], x[7]));
+}
+#endif
+
+}  // namespace b2

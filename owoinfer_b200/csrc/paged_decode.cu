@@ -1,0 +1,481 @@
+// Attention of one new token per sequence over a paged key-value cache, split over the cache's length and joined, with the
+// attention that each cached slot got added up.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <type_traits>
+
+#include "attention.cuh"
+#include "paged.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kKeys = 16;       // slots of a step of a warp: a page holds a multiple of it
+constexpr int kStages = 3;      // steps a warp has in flight
+constexpr int kRows = 16;       // query heads of a CTA: the rows of an MMA
+constexpr int kJoinThreads = 256;
+constexpr int kMostGroup = 4096;  // (a float each in shared memory)
+
+struct DecodeArgs {
+  PagedArgs c;
+  const void* q;
+  std::int64_t q_row, q_head;
+  void* out;
+  std::int64_t o_row, o_head;
+  float* lse;
+  int q_heads, group;           // query heads; query heads to a key head
+  float scale_log2;             // scale * log2(e)
+  int window, sinks;            // window 0: none
+  int chunk, splits;            // steps of a CTA; CTAs to a (sequence, key head) at most
+  float2* part_ml;              // [batch, q_heads, splits] maximum and sum of a part
+  float* part_o;                // [batch, q_heads, splits, D]
+  float* scores;                // [batch, q_heads, scores_ld] scaled scores in binades, or NULL
+  std::int64_t scores_ld;
+  const float* weights;
+  float* weights_out;
+  std::int64_t weights_ld;
+};
+
+// The steps of kKeys slots that the newest of `len` tokens sees some slot of: first the sinks', then from `from` on.
+struct Steps {
+  int sinks, from, count;
+  __device__ __forceinline__ Steps(const DecodeArgs& a, int len) {
+    const int all = (len + kKeys - 1) / kKeys;
+    from = a.window > 0 && len > a.window ? (len - a.window) / kKeys : 0;
+    sinks = min((min(a.sinks, len) + kKeys - 1) / kKeys, from);
+    count = sinks + all - from;
+  }
+  __device__ __forceinline__ int slot(int i) const { return (i < sinks ? i : i - sinks + from) * kKeys; }
+};
+__device__ __forceinline__ bool sees(const DecodeArgs& a, int len, int slot) {
+  return slot < len && (a.window == 0 || slot < a.sinks || slot >= len - a.window);
+}
+
+__device__ __forceinline__ void copy16(std::uint32_t dst, const void* src, bool there) {  // zeros where it is not
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ldsm4(std::uint32_t addr, std::uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(std::uint32_t addr, std::uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], const std::uint32_t (&a)[4], std::uint32_t b0, std::uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16<__nv_bfloat16>(float (&d)[4], const std::uint32_t (&a)[4], std::uint32_t b0, std::uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16<__half>(float (&d)[4], const std::uint32_t (&a)[4], std::uint32_t b0, std::uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The reference of a row's exponentials is its first step's maximum, raised once a score is this many binades above it: P
+// keeps its relative precision however large it is (fp16: up to 2^8 of 2^16).
+constexpr float kRaise = 8.0f;
+
+// A CTA per (part of the cache, key head and block of 16 query heads, sequence). Its warps work apart: each copies its own steps
+// of 16 slots (K and V, 16 bytes a lane, kStages ahead) and keeps its own maxima, sums and output rows in registers; they meet at the
+// end. Q·K^T and P·V are 16-row MMAs with the group's query heads as rows: the cache is read once for all of them, and at one
+// byte to every 2 group multiply-adds the memory is what bounds it.
+template <typename T, int D, bool kScores>
+__global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeArgs a) {
+  dependents_may_start();
+  extern __shared__ __align__(128) std::uint8_t smem[];
+  constexpr int kRowBytes = D * 2, kChunks = D / 8, kStageBytes = 2 * kKeys * kRowBytes;
+  constexpr bool kTwoParts = std::is_same<T, __nv_bfloat16>::value;
+  const int warp = static_cast<int>(threadIdx.x) / 32, lane = static_cast<int>(threadIdx.x) % 32;
+  const int blocks = (a.group + kRows - 1) / kRows;
+  const int split = blockIdx.x, h = blockIdx.y / blocks, g0 = (blockIdx.y % blocks) * kRows, b = blockIdx.z;
+  const int rows = min(kRows, a.group - g0), q_head0 = h * a.group + g0;
+  const int len = paged_len(a.c, b);
+  const Steps steps(a, len);
+  const int begin = split * a.chunk, end = min(steps.count, begin + a.chunk);
+  // (Part 0 of an empty sequence goes on: it writes the zeros, or the empty part that the join finds.)
+  if (begin >= end && split > 0) return;
+  const int mine = begin + warp < end ? (end - begin - warp + kWarps - 1) / kWarps : 0;  // this warp's steps
+
+  const std::uint32_t ring = smem_u32(smem) + static_cast<std::uint32_t>(warp) * (kStages * kStageBytes);
+  // Pages of 32 steps at a time, a lane each, the next 32 fetched ahead.
+  const auto fetch_pages = [&](int n) {
+    const int i = n + lane;
+    return i < mine ? paged_page(a.c, b, steps.slot(begin + warp + i * kWarps)) : -1;
+  };
+  int pages = fetch_pages(0), pages_next = fetch_pages(32);
+  const auto issue = [&](int n) {  // step n of this warp into its stage
+    if (n < mine) {
+      if (n > 0 && n % 32 == 0) {
+        pages = pages_next;
+        pages_next = fetch_pages(n + 32);
+      }
+      const int page = __shfl_sync(0xffffffffu, pages, n % 32), slot0 = steps.slot(begin + warp + n * kWarps);
+      const std::uint32_t stage = ring + static_cast<std::uint32_t>(n % kStages) * kStageBytes;
+      const int c = lane % kChunks;
+      const std::int64_t from = paged_row(a.c, max(page, 0), h, slot0) + c * 8;
+#pragma unroll
+      for (int i = 0; i < kKeys * kChunks / 32; ++i) {
+        const int r = i * (32 / kChunks) + lane / kChunks;
+        const bool there = page >= 0 && sees(a, len, slot0 + r);
+        const std::int64_t at = from + r * a.c.row_stride;
+        const std::uint32_t to = stage + r * kRowBytes + ((c ^ (r & 7)) << 4);
+        copy16(to, there ? static_cast<const T*>(a.c.k) + at : a.q, there);
+        copy16(to + kKeys * kRowBytes, there ? static_cast<const T*>(a.c.v) + at : a.q, there);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int n = 0; n < kStages - 1; ++n) issue(n);
+
+  // Q as the A operand: rows lane / 4 and + 8 (zeros past the group), two neighbouring channels to a register.
+  std::uint32_t qf[D / 16][4];
+  {
+    const T* q = static_cast<const T*>(a.q) + b * a.q_row + (lane % 4) * 2;
+    const int r0 = lane / 4, r1 = r0 + 8;
+    const auto at = [&](int r, int d) { return r < rows ? *reinterpret_cast<const std::uint32_t*>(q + (q_head0 + r) * a.q_head + d) : 0u; };
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      qf[d][0] = at(r0, d * 16), qf[d][1] = at(r1, d * 16);
+      qf[d][2] = at(r0, d * 16 + 8), qf[d][3] = at(r1, d * 16 + 8);
+    }
+  }
+  float o[D / 8][4] = {};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+  for (int n = 0; n < mine; ++n) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    __syncwarp();  // this step's rows are there for every lane, and the step before it is read
+    issue(n + kStages - 1);
+    const std::uint32_t k_rows = ring + static_cast<std::uint32_t>(n % kStages) * kStageBytes, v_rows = k_rows + kKeys * kRowBytes;
+    const int slot0 = steps.slot(begin + warp + n * kWarps);
+
+    float s[2][4] = {};  // slots 0..7 and 8..15 of the step
+    {
+      const int r = (lane >> 4) * 8 + lane % 8, half = lane >> 3 & 1;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        std::uint32_t kf[4];
+        ldsm4(k_rows + r * kRowBytes + (((2 * d + half) ^ (r & 7)) << 4), kf);
+        mma16<T>(s[0], qf[d], kf[0], kf[1]);
+        mma16<T>(s[1], qf[d], kf[2], kf[3]);
+      }
+    }
+    // In binades; what is not seen is minus infinity.
+    const int key = slot0 + (lane % 4) * 2;
+    const bool all = sees(a, len, slot0) && sees(a, len, slot0 + kKeys - 1) && (a.window == 0 || slot0 + kKeys <= a.sinks || slot0 >= len - a.window);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[t][i] *= a.scale_log2;
+        if (!all && !sees(a, len, key + t * 8 + (i & 1))) s[t][i] = -INFINITY;
+      }
+    }
+    if constexpr (kScores) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = lane / 4 + 8 * i;
+        if (r < rows) {
+          float* row = a.scores + (static_cast<std::int64_t>(b) * a.q_heads + q_head0 + r) * a.scores_ld + key;
+          *reinterpret_cast<float2*>(row) = make_float2(s[0][2 * i], s[0][2 * i + 1]);
+          *reinterpret_cast<float2*>(row + 8) = make_float2(s[1][2 * i], s[1][2 * i + 1]);
+        }
+      }
+    }
+    float top[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+    }
+    const auto above = [&](int i) { return m[i] == -INFINITY ? top[i] > -INFINITY : top[i] > m[i] + kRaise; };
+    if (__any_sync(0xffffffffu, above(0) || above(1))) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (!above(i)) continue;
+        const float grow = ex2(m[i] - top[i]);  // 0 the first time
+        m[i] = top[i], l[i] *= grow;
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d) o[d][2 * i] *= grow, o[d][2 * i + 1] *= grow;
+      }
+    }
+    float p[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float ref = m[i >> 1];
+        p[t][i] = ref == -INFINITY && s[t][i] == -INFINITY ? 0.f : ex2(s[t][i] - ref);
+        l[i >> 1] += p[t][i];
+      }
+    }
+    // P for the tensor core. bf16 keeps 8 bits of it, so the 8 bits that this leaves go in as a second operand: P·V is then as exact as
+    // the values are, for 16 more MMAs in a kernel that waits for memory. fp16's 11 bits stand alone.
+    std::uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float x = p[t][2 * i], y = p[t][2 * i + 1];
+        hi[2 * t + i] = pack16<T>(x, y);
+        if constexpr (kTwoParts) {
+          float xh, yh;
+          unpack16<T>(hi[2 * t + i], xh, yh);
+          lo[2 * t + i] = pack16<T>(x - xh, y - yh);
+        }
+      }
+    }
+    const int r = (lane >> 3 & 1) * 8 + lane % 8, half = lane >> 4;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      std::uint32_t vf[4];
+      ldsm4_trans(v_rows + r * kRowBytes + (((2 * d + half) ^ (r & 7)) << 4), vf);
+      mma16<T>(o[2 * d], hi, vf[0], vf[1]);
+      mma16<T>(o[2 * d + 1], hi, vf[2], vf[3]);
+      if constexpr (kTwoParts) {
+        mma16<T>(o[2 * d], lo, vf[0], vf[1]);
+        mma16<T>(o[2 * d + 1], lo, vf[2], vf[3]);
+      }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+  }
+
+  // The warps' parts meet in the rings' place.
+  __syncthreads();
+  float* s_o = reinterpret_cast<float*>(smem);           // [kWarps][kRows][D + 4]
+  constexpr int kLd = D + 4;
+  float* s_ml = s_o + kWarps * kRows * kLd;              // [kWarps][kRows][2]
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = warp * kRows + lane / 4 + 8 * i;
+    if (lane % 4 == 0) s_ml[2 * row] = m[i], s_ml[2 * row + 1] = l[i];
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(s_o + row * kLd + d * 8 + (lane % 4) * 2) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+  }
+  __syncthreads();
+  constexpr int kQuads = D / 4;
+  for (int at = threadIdx.x; at < rows * kQuads; at += kThreads) {
+    const int row = at / kQuads, d = (at % kQuads) * 4;
+    float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_ml[2 * (w * kRows + row)]);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float lw = s_ml[2 * (w * kRows + row) + 1];
+      const float f = lw == 0.f ? 0.f : ex2(s_ml[2 * (w * kRows + row)] - mm);  // (a warp that saw nothing has nothing to add)
+      const float4 x = *reinterpret_cast<const float4*>(s_o + (w * kRows + row) * kLd + d);
+      ll = fmaf(f, lw, ll);
+      sum.x = fmaf(f, x.x, sum.x), sum.y = fmaf(f, x.y, sum.y), sum.z = fmaf(f, x.z, sum.z), sum.w = fmaf(f, x.w, sum.w);
+    }
+    const std::int64_t head = static_cast<std::int64_t>(b) * a.q_heads + q_head0 + row;
+    if (a.part_o == nullptr) {
+      const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+      T* out = static_cast<T*>(a.out) + b * a.o_row + (q_head0 + row) * a.o_head + d;
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(sum.x * inv, sum.y * inv), pack16<T>(sum.z * inv, sum.w * inv));
+      if (d == 0 && a.lse != nullptr) a.lse[head] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+    } else {
+      *reinterpret_cast<float4*>(a.part_o + (head * a.splits + split) * D + d) = sum;
+      if (d == 0) a.part_ml[head * a.splits + split] = make_float2(mm, ll);
+    }
+  }
+}
+
+// The parts of a (sequence, key head) joined: the outputs of query heads x, x + gridDim.x, ... of its group, and what the slots of the
+// x-th range got. Every CTA works out the group's maxima and sums from the parts' for itself.
+template <typename T, int D, bool kScores>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a) {
+  extern __shared__ __align__(16) float s_lse[];  // [group] log2 of the sum of all weights, or infinity where nothing is seen
+  __shared__ __align__(16) float s_sum[kJoinThreads * 4];
+  const int h = blockIdx.y, b = blockIdx.z, warp = static_cast<int>(threadIdx.x) / 32, lane = static_cast<int>(threadIdx.x) % 32;
+  wait_for_predecessors();
+  const int len = paged_len(a.c, b);
+  const Steps steps(a, len);
+  const int parts = max(1, (steps.count + a.chunk - 1) / a.chunk);
+  const std::int64_t head0 = static_cast<std::int64_t>(b) * a.q_heads + h * a.group;
+  for (int g = warp; g < a.group; g += kJoinThreads / 32) {
+    const float2* ml = a.part_ml + (head0 + g) * a.splits;
+    float mm = -INFINITY;
+    for (int i = lane; i < parts; i += 32) mm = fmaxf(mm, ml[i].x);
+#pragma unroll
+    for (int w = 16; w > 0; w /= 2) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, w));
+    float ll = 0.f;
+    for (int i = lane; i < parts; i += 32) ll += ml[i].y == 0.f ? 0.f : ml[i].y * ex2(ml[i].x - mm);
+#pragma unroll
+    for (int w = 16; w > 0; w /= 2) ll += __shfl_xor_sync(0xffffffffu, ll, w);
+    if (lane == 0) s_lse[g] = ll == 0.f ? INFINITY : mm + log2f(ll);
+  }
+  __syncthreads();
+
+  constexpr int kQuads = D / 4, kSlices = kJoinThreads / kQuads;  // threads to a row, rows of the parts at a time
+  const int quad = static_cast<int>(threadIdx.x) % kQuads, slice = static_cast<int>(threadIdx.x) / kQuads;
+  for (int g = blockIdx.x; g < a.group; g += gridDim.x) {
+    const float lse2 = s_lse[g];
+    const float2* ml = a.part_ml + (head0 + g) * a.splits;
+    const float* part = a.part_o + (head0 + g) * a.splits * D + quad * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = slice; i < parts; i += kSlices) {
+      const float2 of = ml[i];
+      const float f = of.y == 0.f ? 0.f : ex2(of.x - lse2);
+      const float4 x = *reinterpret_cast<const float4*>(part + static_cast<std::int64_t>(i) * D);
+      sum.x = fmaf(f, x.x, sum.x), sum.y = fmaf(f, x.y, sum.y), sum.z = fmaf(f, x.z, sum.z), sum.w = fmaf(f, x.w, sum.w);
+    }
+    __syncthreads();  // (the sums of the head before are read)
+    *reinterpret_cast<float4*>(s_sum + 4 * threadIdx.x) = sum;
+    __syncthreads();
+    if (slice == 0) {
+      for (int i = 1; i < kSlices; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(s_sum + 4 * (i * kQuads + quad));
+        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+      }
+      T* out = static_cast<T*>(a.out) + b * a.o_row + (h * a.group + g) * a.o_head + quad * 4;
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(sum.x, sum.y), pack16<T>(sum.z, sum.w));
+      if (quad == 0 && a.lse != nullptr) a.lse[head0 + g] = lse2 == INFINITY ? -INFINITY : lse2 * 0.6931471805599453f;
+    }
+  }
+
+  if constexpr (kScores) {
+    const std::int64_t row = (static_cast<std::int64_t>(b) * a.c.kv_heads + h) * a.weights_ld;
+    for (int j = static_cast<int>(blockIdx.x) * kJoinThreads + static_cast<int>(threadIdx.x); j < len; j += gridDim.x * kJoinThreads) {
+      float sum = j < len - 1 ? a.weights[row + j] : 0.f;
+      if (sees(a, len, j)) {
+        const float* s = a.scores + head0 * a.scores_ld + j;
+        float got = 0.f;
+        for (int g = 0; g < a.group; ++g) got += ex2(s[g * a.scores_ld] - s_lse[g]);
+        sum += got;
+      }
+      a.weights_out[row + j] = sum;
+    }
+  }
+}
+
+constexpr int kTargetCtas = 4;  // CTAs per SM that a call is cut into, where it is long enough
+
+struct Plan {
+  int chunk, splits;
+  std::int64_t scores_ld;
+  std::size_t ml, o, scores, total;
+  bool parts;
+};
+Plan plan(const PagedArgs& c, int q_heads, int head_dim, int window, int sinks, bool weights) {
+  Plan p{};
+  p.scores_ld = (static_cast<std::int64_t>(c.most) + kKeys - 1) / kKeys * kKeys;
+  const std::int64_t group = q_heads / c.kv_heads, units = std::max<std::int64_t>(1, c.batch * c.kv_heads * ((group + kRows - 1) / kRows));
+  std::int64_t steps = p.scores_ld / kKeys;
+  if (window > 0) steps = std::min<std::int64_t>(steps, (static_cast<std::int64_t>(window) + kKeys - 1) / kKeys + 1 + (static_cast<std::int64_t>(sinks) + kKeys - 1) / kKeys);
+  const std::int64_t target = static_cast<std::int64_t>(sm_count()) * kTargetCtas;
+  std::int64_t chunk = (steps * units + target - 1) / target;
+  chunk = std::max<std::int64_t>((chunk + kWarps - 1) / kWarps * kWarps, 2 * kWarps);
+  p.chunk = static_cast<int>(std::min<std::int64_t>(chunk, INT_MAX / 2));
+  p.splits = static_cast<int>(std::max<std::int64_t>(1, (steps + p.chunk - 1) / p.chunk));
+  p.parts = p.splits > 1 || weights;
+  const auto align = [](std::size_t n) { return (n + 255) / 256 * 256; };
+  const std::size_t heads = static_cast<std::size_t>(c.batch) * q_heads;
+  if (p.parts) {
+    p.ml = 0;
+    p.o = align(heads * p.splits * sizeof(float2));
+    p.scores = p.o + align(heads * p.splits * head_dim * 4);
+    p.total = p.scores + (weights ? align(heads * p.scores_ld * 4) : 0);
+  }
+  return p;
+}
+
+int check(const char* op, const b2_paged_cache* cache, PagedArgs* c, int q_heads, int max_len, int* window, int* sinks) {
+  if (const int rc = check_paged_cache(op, cache, c)) return rc;
+  if (q_heads <= 0 || q_heads > 65535 || q_heads % cache->kv_heads != 0) return fail_invalid(op, "q_heads must be a multiple of kv_heads, at most 65535");
+  if (max_len < 0 || max_len > c->most) return fail_invalid(op, "max_len must lie within the block table");
+  if (max_len > 0) c->most = max_len;
+  if (const int rc = check_window(op, *c, window, sinks)) return rc;
+  if (q_heads / cache->kv_heads > kMostGroup) return fail_invalid(op, "at most 4096 query heads to a key head");
+  return B2_OK;
+}
+
+template <typename T, int D, bool kScores>
+int launch(const char* op, const DecodeArgs& a, const Plan& p, cudaStream_t st) {
+  constexpr int ring = kWarps * kStages * 2 * kKeys * D * 2, meet = kWarps * kRows * (D + 4 + 2) * 4;
+  constexpr int smem = ring > meet ? ring : meet;
+  const auto kernel = decode_kernel<T, D, kScores>;
+  if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) {
+    cudaGetLastError();
+    return fail_cuda(op, e);
+  }
+  const LaunchChain chain(st);
+  const unsigned blocks = static_cast<unsigned>((a.group + kRows - 1) / kRows), batch = static_cast<unsigned>(a.c.batch);
+  const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.c.kv_heads) * blocks, batch);
+  if (const int rc = enqueue(op, kernel, grid, kThreads, smem, st, 1, a)) return rc;
+  if (!p.parts) return B2_OK;
+  const int slices = std::max(std::min(a.group, 64), kScores ? std::min((a.c.most + 1023) / 1024, 1 << 20) : 1);
+  return enqueue(op, join_kernel<T, D, kScores>, dim3(static_cast<unsigned>(slices), static_cast<unsigned>(a.c.kv_heads), batch), kJoinThreads,
+                 static_cast<std::size_t>(a.group) * 4, st, 1, a);
+}
+
+}  // namespace
+}  // namespace b2
+
+using namespace b2;
+
+extern "C" {
+
+size_t b2_attention_paged_decode_workspace_bytes(const b2_paged_cache* cache, int q_heads, int max_len, int window, int sinks, int with_weights) {
+  PagedArgs c{};
+  if (check("attention_paged_decode", cache, &c, q_heads, max_len, &window, &sinks) != B2_OK) return 0;
+  return std::max<std::size_t>(plan(c, q_heads, cache->head_dim, window, sinks, with_weights != 0).total, 256);
+}
+
+int b2_attention_paged_decode(const b2_paged_cache* cache, const b2_view3* q, const b2_view3* out, float* lse, int max_len,
+                              float scale, int window, int sinks, const float* weights, float* weights_out, int64_t weights_ld,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  constexpr const char* op = "attention_paged_decode";
+  DecodeArgs a{};
+  if (q == nullptr || out == nullptr) return fail_invalid(op, "null q or out");
+  if (q->heads <= 0 || q->heads > 65535) return fail_invalid(op, "q must have from 1 to 65535 heads");
+  if (const int rc = check(op, cache, &a.c, static_cast<int>(q->heads), max_len, &window, &sinks)) return rc;
+  if (q->tokens != cache->batch || out->tokens != q->tokens || out->heads != q->heads) return fail_invalid(op, "q and out must have one token per sequence and the same heads");
+  if (!std::isfinite(scale) || !(scale > 0.0f)) return fail_invalid(op, "scale must be finite and positive");
+  if ((weights == nullptr) != (weights_out == nullptr)) return fail_invalid(op, "weights and weights_out: both or neither");
+  if (weights != nullptr && weights_ld < a.c.most) return fail_invalid(op, "weights need a place for every slot");
+  if (cache->batch == 0) return B2_OK;
+  if (!rows_ok(q->data, q->row_stride, q->head_stride) || !rows_ok(out->data, out->row_stride, out->head_stride)) {
+    return fail_invalid(op, "q and out need a 16-byte aligned base and strides that are multiples of 8");
+  }
+  a.q = q->data, a.q_row = q->row_stride, a.q_head = q->head_stride, a.out = out->data, a.o_row = out->row_stride, a.o_head = out->head_stride;
+  a.lse = lse, a.q_heads = static_cast<int>(q->heads), a.group = a.q_heads / cache->kv_heads;
+  if (static_cast<std::int64_t>(cache->kv_heads) * ((a.group + kRows - 1) / kRows) > 65535) return fail_invalid(op, "too many heads");
+  const bool scores = weights != nullptr;
+  const Plan p = plan(a.c, a.q_heads, cache->head_dim, window, sinks, scores);
+  if (p.parts && (workspace == nullptr || !aligned_to(workspace, 256) || workspace_bytes < p.total)) {
+    return fail_invalid(op, "workspace is too small or not 256-byte aligned (b2_attention_paged_decode_workspace_bytes)");
+  }
+  a.scores_ld = p.scores_ld;
+  a.scale_log2 = scale * 1.4426950408889634f, a.window = window, a.sinks = sinks, a.chunk = p.chunk, a.splits = p.splits;
+  if (p.parts) {
+    std::uint8_t* ws = static_cast<std::uint8_t*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(ws + p.ml), a.part_o = reinterpret_cast<float*>(ws + p.o);
+    if (scores) a.scores = reinterpret_cast<float*>(ws + p.scores);
+  }
+  a.weights = weights, a.weights_out = weights_out, a.weights_ld = weights_ld;
+  const cudaStream_t st = as_stream(stream);
+  if (const int rc = paged_status_word(op, &a.c)) return rc;
+  const bool wide = cache->head_dim == 128;
+  if (cache->dtype == B2_DTYPE_BF16) {
+    using T = __nv_bfloat16;
+    if (scores) return wide ? launch<T, 128, true>(op, a, p, st) : launch<T, 64, true>(op, a, p, st);
+    return wide ? launch<T, 128, false>(op, a, p, st) : launch<T, 64, false>(op, a, p, st);
+  }
+  using T = __half;
+  if (scores) return wide ? launch<T, 128, true>(op, a, p, st) : launch<T, 64, true>(op, a, p, st);
+  return wide ? launch<T, 128, false>(op, a, p, st) : launch<T, 64, false>(op, a, p, st);
+}
+
+}  // extern "C"

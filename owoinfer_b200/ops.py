@@ -666,6 +666,160 @@ def dit_prefill_references(model, latents, time_vector, tier=TIER_INT8):
     return kv
 
 
+# ------------------------------------------------------------------------------------------------ paged key-value cache
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def _raw_stream() -> int:
+    return _stream().value or 0
+
+
+def _at(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _need(t, name, dtype, dim):
+    if t.dtype != dtype or t.dim() != dim or (dim and t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name} must be a {dtype} tensor of {dim} dimensions, the last one contiguous")
+
+
+class PagedCache:
+    """b2_paged_cache: pools k and v [pages, kv_heads, page_size, head_dim] (bf16 or fp16 views of the same strides, head_dim
+    contiguous), block_table int32 [batch, width] and seq_lens int32 [batch] on the device. The struct holds addresses, so the
+    contents may change between calls (lengths that grow, pages that are added) without a new handle."""
+
+    def __init__(self, k, v, block_table, seq_lens):
+        if k.dtype not in _DTYPES or k.dtype != v.dtype or k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.stride(3) != 1:
+            raise ValueError("k and v must be bf16 or fp16 pools [pages, kv_heads, page_size, head_dim] of the same strides, head_dim contiguous")
+        _need(block_table, "block_table", torch.int32, 2)
+        _need(seq_lens, "seq_lens", torch.int32, 1)
+        if block_table.shape[0] != seq_lens.shape[0]:
+            raise ValueError("block_table and seq_lens must have a row for every sequence")
+        self.k, self.v, self.block_table, self.seq_lens, self.dtype = k, v, block_table, seq_lens, k.dtype
+        pages, heads, page, dim = k.shape
+        page_stride, head_stride, row_stride, _ = k.stride()
+        batch, width = block_table.shape
+        self.batch, self.kv_heads, self.page_size, self.head_dim, self.slots = batch, heads, page, dim, width * page
+        self.struct = _lib.PagedCache(C.sizeof(_lib.PagedCache), k.data_ptr(), v.data_ptr(), page_stride, head_stride, row_stride, pages,
+                                      _DTYPES[k.dtype], heads, page, dim, block_table.data_ptr(), max(block_table.stride(0), width), width,
+                                      seq_lens.data_ptr(), batch)
+
+
+def _heads_view(t, cache, name):
+    if t.dim() != 3 or t.dtype != cache.dtype or t.shape[2] != cache.head_dim or t.stride(2) != 1:
+        raise ValueError(f"{name} must be a [tokens, heads, head_dim] view of the cache's dtype and head_dim, head_dim contiguous")
+    return _view3(t)
+
+
+def qk_norm_rope_append(qkv, cache, cu_seqlens, q_norm, k_norm, rope, positions=None, eps=1e-6, interleaved=False, out=None):
+    """qkv [tokens, (q_heads + 2 kv_heads) * head_dim]: per-head RMS norm of queries and keys (None: none), rotation by the fp32 table
+    rope [positions, rot_dim] (sin | cos; None: none), keys and values into the cache's last slots. Returns the queries
+    [tokens, q_heads, head_dim] (into `out` when given; qkv's own query part will do)."""
+    _need(qkv, "qkv", cache.dtype, 2)
+    _need(cu_seqlens, "cu_seqlens", torch.int32, 1)
+    tokens, width = qkv.shape
+    heads, rest = divmod(width, cache.head_dim)
+    q_heads = heads - 2 * cache.kv_heads
+    if rest or q_heads <= 0 or cu_seqlens.shape[0] != cache.batch + 1:
+        raise ValueError("qkv must have q_heads + 2 kv_heads heads, cu_seqlens batch + 1 entries")
+    for norm in (q_norm, k_norm):
+        if norm is not None and (norm.dtype != cache.dtype or norm.shape != (cache.head_dim,) or not norm.is_contiguous()):
+            raise ValueError("q_norm and k_norm must be contiguous [head_dim] tensors of the cache's dtype")
+    if rope is not None and (rope.dtype != torch.float32 or rope.dim() != 2 or not rope.is_contiguous()):
+        raise ValueError("rope must be a contiguous fp32 table [positions, rot_dim]")
+    if positions is not None and (positions.dtype != torch.int32 or positions.shape != (tokens,) or not positions.is_contiguous()):
+        raise ValueError("positions must be a contiguous int32 tensor with one entry per token")
+    out = torch.empty((tokens, q_heads, cache.head_dim), dtype=cache.dtype, device=qkv.device) if out is None else out
+    if out.dtype != cache.dtype or out.shape != (tokens, q_heads, cache.head_dim) or out.stride(2) != 1:
+        raise ValueError("out must be a [tokens, q_heads, head_dim] view of the cache's dtype, head_dim contiguous")
+    rows, rot = (0, 0) if rope is None else rope.shape
+    check(_lib.lib().b2_qk_norm_rope_append(cache.struct, qkv.data_ptr(), _ld(qkv), tokens, q_heads, cu_seqlens.data_ptr(), _at(positions), _at(q_norm),
+                                            _at(k_norm), eps, _at(rope), rows, rot, int(interleaved), out.data_ptr(), out.stride(0), out.stride(1),
+                                            _raw_stream()))
+    return out
+
+
+def _lse_of(q, lse):
+    if lse is None:
+        return torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous():
+        raise ValueError("lse must be a contiguous fp32 [tokens, q_heads] tensor")
+    return lse
+
+
+def attention_paged(q, cache, cu_seqlens, max_q, scale, window=0, sinks=0, out=None, lse=None):
+    """Causal attention of a prompt's tokens q [tokens, q_heads, head_dim] over the cache that holds their keys and values already;
+    with a window the last `window` slots and the first `sinks`. Returns (out, lse): lse fp32 [tokens, q_heads]."""
+    _need(cu_seqlens, "cu_seqlens", torch.int32, 1)
+    if cu_seqlens.shape[0] != cache.batch + 1:
+        raise ValueError("cu_seqlens must have batch + 1 entries")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    lse = _lse_of(q, lse)
+    check(_lib.lib().b2_attention_paged(cache.struct, _heads_view(q, cache, "q"), _heads_view(out, cache, "out"), lse.data_ptr(),
+                                        cu_seqlens.data_ptr(), max_q, scale, window, sinks, _raw_stream()))
+    return out, lse
+
+
+def attention_paged_decode_workspace_bytes(cache, q_heads, max_len=0, window=0, sinks=0, weights=False) -> int:
+    n = _lib.lib().b2_attention_paged_decode_workspace_bytes(cache.struct, q_heads, max_len, window, sinks, int(weights))
+    if n == 0:
+        check(-1)
+    return n
+
+
+def attention_paged_decode(q, cache, scale, max_len=0, window=0, sinks=0, weights=None, weights_out=None, out=None, lse=None, workspace=None):
+    """Attention of one new token per sequence, q [batch, q_heads, head_dim], split over the cache's length. With `weights` (fp32 [batch,
+    kv_heads, slots]) the attention each slot got is added to them (in weights_out, or in place). Returns (out, lse)."""
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    lse = _lse_of(q, lse)
+    ld = 0
+    if weights is not None:
+        weights_out = weights if weights_out is None else weights_out
+        _need(weights, "weights", torch.float32, 3)
+        if weights.shape[:2] != (cache.batch, cache.kv_heads) or not weights.is_contiguous() or weights_out.shape != weights.shape or \
+                weights_out.dtype != torch.float32 or not weights_out.is_contiguous():
+            raise ValueError("weights and weights_out must be contiguous fp32 [batch, kv_heads, slots] tensors of one shape")
+        ld = weights.shape[2]
+    if workspace is None:
+        workspace = torch.empty(attention_paged_decode_workspace_bytes(cache, q.shape[1], max_len, window, sinks, weights is not None),
+                                dtype=torch.uint8, device=q.device)
+    check(_lib.lib().b2_attention_paged_decode(cache.struct, _heads_view(q, cache, "q"), _heads_view(out, cache, "out"), lse.data_ptr(), max_len, scale,
+                                               window, sinks, _at(weights), _at(weights_out), ld, workspace.data_ptr(), workspace.numel(), _raw_stream()))
+    return out, lse
+
+
+def kv_evict(cache, weights, table_out, budget, sinks=0, recent=0, kept=None, lens_out=None, weights_out=None):
+    """Sequences of more than `budget` slots keep their first `sinks`, their last `recent` and, of the rest, the slots of most weight
+    (fp32 [batch, kv_heads, slots]), for each key head by itself; what is kept moves in order to the pages of table_out. Returns
+    (kept int32 [batch, kv_heads, budget], lens int32 [batch]); weights_out receives the weights of what is kept."""
+    if budget <= 0:
+        raise ValueError("budget must be positive")
+    _need(weights, "weights", torch.float32, 3)
+    _need(table_out, "table_out", torch.int32, 2)
+    if weights.shape[:2] != (cache.batch, cache.kv_heads) or not weights.is_contiguous() or table_out.shape[0] != cache.batch:
+        raise ValueError("weights must be contiguous [batch, kv_heads, slots], table_out [batch, pages]")
+    if weights_out is not None and (weights_out.dtype != torch.float32 or weights_out.dim() != 3 or weights_out.shape[:2] != weights.shape[:2] or
+                                    not weights_out.is_contiguous()):
+        raise ValueError("weights_out must be a contiguous fp32 [batch, kv_heads, slots] tensor")
+    kept = torch.empty((cache.batch, cache.kv_heads, budget), dtype=torch.int32, device=weights.device) if kept is None else kept
+    lens_out = torch.empty(cache.batch, dtype=torch.int32, device=weights.device) if lens_out is None else lens_out
+    if kept.dtype != torch.int32 or kept.shape != (cache.batch, cache.kv_heads, budget) or not kept.is_contiguous() or \
+            lens_out.dtype != torch.int32 or lens_out.shape != (cache.batch,) or not lens_out.is_contiguous():
+        raise ValueError("kept must be a contiguous int32 [batch, kv_heads, budget] tensor, lens_out int32 [batch]")
+    check(_lib.lib().b2_kv_evict(cache.struct, weights.data_ptr(), weights.shape[2], sinks, recent, budget, table_out.data_ptr(),
+                                 max(table_out.stride(0), table_out.shape[1]), table_out.shape[1], kept.data_ptr(), lens_out.data_ptr(), _at(weights_out),
+                                 0 if weights_out is None else weights_out.shape[2], _raw_stream()))
+    return kept, lens_out
+
+
+def paged_cache_status(clear=False) -> int:
+    """Bits that the kernels on paged caches raised (b2_paged_cache_status): 0 when every length, page and position was in bounds."""
+    v = C.c_uint(0)
+    check(_lib.lib().b2_paged_cache_status(C.byref(v), int(clear)))
+    return int(v.value)
+
+
 # ------------------------------------------------------------------------------------------------ weight ingestion
 
 class _Loaded:
