@@ -35,11 +35,9 @@ int check_paged_cache(const char* op, const b2_paged_cache* c, PagedArgs* a);
 int paged_status_word(const char* op, PagedArgs* a);
 // Where a call may write or read rows of `row` elements: 16-byte aligned, strides in multiples of 8 elements.
 inline bool rows_ok(const void* p, std::int64_t row, std::int64_t head) { return p != nullptr && aligned_to(p, 16) && row % 8 == 0 && head % 8 == 0; }
-// cuTensorMapEncodeTiled for a pool of pages of 16-bit elements, [pages, heads, rows, head_dim]: boxes of box_rows rows of 64
-// elements, 128-byte swizzle. Returns false (and sets the last error) on failure.
-bool make_tensor_map_pages(CUtensorMap* map, const void* base, int head_dim, int page_size, int heads, std::int64_t pages,
-                           std::int64_t row_stride, std::int64_t head_stride, std::int64_t page_stride, int box_rows, const char* op);
-
+// cuTensorMapEncodeTiled for the cache's keys or values, [pages, heads, rows, head_dim]: boxes of box_rows rows of 64 elements,
+// 128-byte swizzle. Returns false (and sets the last error) on failure.
+bool make_tensor_map_pages(CUtensorMap* map, const b2_paged_cache* c, bool values, int box_rows, const char* op);
 // A window that reaches every slot is none; sinks past the last slot are all slots.
 int check_window(const char* op, const PagedArgs& c, int* window, int* sinks);
 

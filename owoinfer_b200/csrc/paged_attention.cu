@@ -42,20 +42,6 @@ constexpr int kPartBytes = kTile * 128;
 __device__ __forceinline__ std::uint64_t value_desc(std::uint32_t smem_addr) {
   return (umma_desc_sw128(smem_addr) & ~(static_cast<std::uint64_t>(0x3FFF) << 16)) | static_cast<std::uint64_t>(kPartBytes >> 4) << 16;
 }
-__device__ __forceinline__ void tma_load_4d(std::uint32_t dst, const CUtensorMap* map, std::uint32_t bar, int c0, int c1, int c2, int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      ::"r"(dst), "l"(reinterpret_cast<std::uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
-}
-__device__ __forceinline__ uint4 ld_shared(std::uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ void st_shared(std::uint32_t addr, const uint4& v) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
 // The halves of a word whose exponent is all ones (infinities and NaN).
 template <typename T>
 __device__ __forceinline__ std::uint32_t nonfinite_halves(std::uint32_t w) {
@@ -519,12 +505,7 @@ int b2_attention_paged(const b2_paged_cache* cache, const b2_view3* q, const b2_
   a.scale_log2 = scale * 1.4426950408889634f, a.window = window, a.sinks = sinks;
   CUtensorMap map_k, map_v;
   const int box = std::min(cache->page_size, kTile);
-  for (const bool keys : {true, false}) {
-    if (!make_tensor_map_pages(keys ? &map_k : &map_v, keys ? cache->k : cache->v, cache->head_dim, cache->page_size, cache->kv_heads, cache->num_pages,
-                               cache->row_stride, cache->head_stride, cache->page_stride, box, op)) {
-      return B2_ERR_CUDA;
-    }
-  }
+  if (!make_tensor_map_pages(&map_k, cache, false, box, op) || !make_tensor_map_pages(&map_v, cache, true, box, op)) return B2_ERR_CUDA;
   if (const int rc = paged_status_word(op, &a.c)) return rc;
   const cudaStream_t st = as_stream(stream);
   const bool wide = cache->head_dim == 128;

@@ -411,8 +411,7 @@ int paged_status_word(const char* op, PagedArgs* a) {
   return B2_OK;
 }
 
-bool make_tensor_map_pages(CUtensorMap* map, const void* base, int head_dim, int page_size, int heads, std::int64_t pages,
-                           std::int64_t row_stride, std::int64_t head_stride, std::int64_t page_stride, int box_rows, const char* op) {
+bool make_tensor_map_pages(CUtensorMap* map, const b2_paged_cache* c, bool values, int box_rows, const char* op) {
   static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -427,10 +426,10 @@ bool make_tensor_map_pages(CUtensorMap* map, const void* base, int head_dim, int
     return false;
   }
   const auto u = [](std::int64_t v) { return static_cast<cuuint64_t>(v); };
-  const cuuint64_t dims[4] = {u(head_dim), u(page_size), u(heads), u(pages)};
-  const cuuint64_t strides[3] = {u(row_stride) * 2, u(head_stride) * 2, u(page_stride) * 2};
+  const cuuint64_t dims[4] = {u(c->head_dim), u(c->page_size), u(c->kv_heads), u(c->num_pages)};
+  const cuuint64_t strides[3] = {u(c->row_stride) * 2, u(c->head_stride) * 2, u(c->page_stride) * 2};
   const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1}, elem[4] = {1, 1, 1, 1};
-  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, elem,
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, values ? c->v : c->k, dims, strides, box, elem,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) return true;

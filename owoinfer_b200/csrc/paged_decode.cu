@@ -13,9 +13,10 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kKeys = 16;       // slots of a step of a warp: a page holds a multiple of it
-constexpr int kStages = 3;      // steps a warp has in flight
+constexpr int kStages = 2;      // steps of a warp in shared memory: the one it works on and the one on its way
 constexpr int kRows = 16;       // query heads of a CTA: the rows of an MMA
 constexpr int kJoinThreads = 256;
+constexpr int kJoinSlots = 4;
 constexpr int kMostGroup = 4096;  // (a float each in shared memory)
 
 struct DecodeArgs {
@@ -53,9 +54,6 @@ __device__ __forceinline__ bool sees(const DecodeArgs& a, int len, int slot) {
   return slot < len && (a.window == 0 || slot < a.sinks || slot >= len - a.window);
 }
 
-__device__ __forceinline__ void copy16(std::uint32_t dst, const void* src, bool there) {  // zeros where it is not
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void ldsm4(std::uint32_t addr, std::uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -79,58 +77,83 @@ __device__ __forceinline__ void mma16<__half>(float (&d)[4], const std::uint32_t
 // keeps its relative precision however large it is (fp16: up to 2^8 of 2^16).
 constexpr float kRaise = 8.0f;
 
-// A CTA per (part of the cache, key head and block of 16 query heads, sequence). Its warps work apart: each copies its own steps
-// of 16 slots (K and V, 16 bytes a lane, kStages ahead) and keeps its own maxima, sums and output rows in registers; they meet at the
-// end. Q·K^T and P·V are 16-row MMAs with the group's query heads as rows: the cache is read once for all of them, and at one
+// A CTA per (part of the cache, key head and block of 16 query heads, sequence). Its warps work apart: each has TMA bring its own steps
+// of 16 slots and keeps its own maxima, sums and output rows in registers; they meet at the end. Q·K^T and P·V are 16-row MMAs with the group's query heads as rows: the cache is read once for all of them, and at one
 // byte to every 2 group multiply-adds the memory is what bounds it.
 template <typename T, int D, bool kScores>
-__global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(kThreads, 3)
+decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const DecodeArgs a) {
   dependents_may_start();
-  extern __shared__ __align__(128) std::uint8_t smem[];
-  constexpr int kRowBytes = D * 2, kChunks = D / 8, kStageBytes = 2 * kKeys * kRowBytes;
+  extern __shared__ std::uint8_t smem_raw[];
+  __shared__ __align__(8) std::uint64_t s_full[kWarps][kStages];
+  __shared__ int s_abort;
+  // A step in shared memory: K, then V, each D / 64 parts of 16 rows of 128 bytes with the 128-byte swizzle.
+  constexpr int kParts = D / 64, kPartBytes = kKeys * 128, kHalfBytes = kParts * kPartBytes, kStageBytes = 2 * kHalfBytes;
   constexpr bool kTwoParts = std::is_same<T, __nv_bfloat16>::value;
   const int warp = static_cast<int>(threadIdx.x) / 32, lane = static_cast<int>(threadIdx.x) % 32;
   const int blocks = (a.group + kRows - 1) / kRows;
   const int split = blockIdx.x, h = blockIdx.y / blocks, g0 = (blockIdx.y % blocks) * kRows, b = blockIdx.z;
   const int rows = min(kRows, a.group - g0), q_head0 = h * a.group + g0;
+  if (threadIdx.x == 0) s_abort = 0;
+  // Pages of 32 steps at a time, a lane each. Without a window a step's slots do not go by the length, so the first 32 entries of the block
+  // table are on their way along with it.
+  const std::int32_t* const table = a.c.table + b * a.c.table_ld;
+  const int early_slot = (split * a.chunk + warp + lane * kWarps) * kKeys;
+  int entry = a.window == 0 && early_slot < a.c.most ? table[early_slot >> a.c.page_shift] : -1;
   const int len = paged_len(a.c, b);
   const Steps steps(a, len);
   const int begin = split * a.chunk, end = min(steps.count, begin + a.chunk);
   // (Part 0 of an empty sequence goes on: it writes the zeros, or the empty part that the join finds.)
   if (begin >= end && split > 0) return;
   const int mine = begin + warp < end ? (end - begin - warp + kWarps - 1) / kWarps : 0;  // this warp's steps
-
-  const std::uint32_t ring = smem_u32(smem) + static_cast<std::uint32_t>(warp) * (kStages * kStageBytes);
-  // Pages of 32 steps at a time, a lane each, the next 32 fetched ahead.
+  const auto checked = [&](int page, int i) {
+    if (i >= mine) return -1;
+    if (page < 0 || page >= a.c.num_pages) {
+      atomicOr(a.c.status, kPagedBadPage);
+      return -1;
+    }
+    return page;
+  };
   const auto fetch_pages = [&](int n) {
     const int i = n + lane;
-    return i < mine ? paged_page(a.c, b, steps.slot(begin + warp + i * kWarps)) : -1;
+    return i < mine ? checked(table[steps.slot(begin + warp + i * kWarps) >> a.c.page_shift], i) : -1;
   };
-  int pages = fetch_pages(0), pages_next = fetch_pages(32);
-  const auto issue = [&](int n) {  // step n of this warp into its stage
-    if (n < mine) {
-      if (n > 0 && n % 32 == 0) {
-        pages = pages_next;
-        pages_next = fetch_pages(n + 32);
-      }
-      const int page = __shfl_sync(0xffffffffu, pages, n % 32), slot0 = steps.slot(begin + warp + n * kWarps);
-      const std::uint32_t stage = ring + static_cast<std::uint32_t>(n % kStages) * kStageBytes;
-      const int c = lane % kChunks;
-      const std::int64_t from = paged_row(a.c, max(page, 0), h, slot0) + c * 8;
+  int pages = a.window == 0 ? checked(entry, lane) : fetch_pages(0), pages_next = fetch_pages(32);
+
+  std::uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const std::uint32_t ring = smem_u32(smem) + static_cast<std::uint32_t>(warp) * (kStages * kStageBytes);
+  const auto bar = [&](int n) { return smem_u32(&s_full[warp][n % kStages]); };
+  if (lane == 0) {  // (a warp's barriers are its own: no other waits for them)
 #pragma unroll
-      for (int i = 0; i < kKeys * kChunks / 32; ++i) {
-        const int r = i * (32 / kChunks) + lane / kChunks;
-        const bool there = page >= 0 && sees(a, len, slot0 + r);
-        const std::int64_t at = from + r * a.c.row_stride;
-        const std::uint32_t to = stage + r * kRowBytes + ((c ^ (r & 7)) << 4);
-        copy16(to, there ? static_cast<const T*>(a.c.k) + at : a.q, there);
-        copy16(to + kKeys * kRowBytes, there ? static_cast<const T*>(a.c.v) + at : a.q, there);
+    for (int i = 0; i < kStages; ++i) mbar_init(bar(i), 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  const auto issue = [&](int n) {  // step n of this warp into its stage
+    if (n >= mine) return;
+    if (n > 0 && n % 32 == 0) {
+      pages = pages_next;
+      pages_next = fetch_pages(n + 32);
+    }
+    const int page = __shfl_sync(0xffffffffu, pages, n % 32);
+    const std::uint32_t stage = ring + static_cast<std::uint32_t>(n % kStages) * kStageBytes;
+    if (page < 0) {  // a page outside the pool reads as zeros
+      for (int i = lane; i < kStageBytes / 16; i += 32) st_shared(stage + i * 16, make_uint4(0, 0, 0, 0));
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(n));
+    } else if (lane == 0) {
+      const int row = steps.slot(begin + warp + n * kWarps) & ((1 << a.c.page_shift) - 1);
+      mbar_expect_tx(bar(n), kStageBytes);
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        tma_load_4d(stage + i * kPartBytes, &map_k, bar(n), i * 64, row, h, page);
+        tma_load_4d(stage + kHalfBytes + i * kPartBytes, &map_v, bar(n), i * 64, row, h, page);
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int n = 0; n < kStages - 1; ++n) issue(n);
+  for (int n = 0; n < kStages; ++n) issue(n);
 
   // Q as the A operand: rows lane / 4 and + 8 (zeros past the group), two neighbouring channels to a register.
   std::uint32_t qf[D / 16][4];
@@ -148,11 +171,18 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeArgs a) {
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
   for (int n = 0; n < mine; ++n) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    __syncwarp();  // this step's rows are there for every lane, and the step before it is read
-    issue(n + kStages - 1);
-    const std::uint32_t k_rows = ring + static_cast<std::uint32_t>(n % kStages) * kStageBytes, v_rows = k_rows + kKeys * kRowBytes;
+    const bool got = wait_bar(bar(n), n / kStages & 1u, &s_abort);
+    if (__any_sync(0xffffffffu, !got)) break;
+    const std::uint32_t k_rows = ring + static_cast<std::uint32_t>(n % kStages) * kStageBytes, v_rows = k_rows + kHalfBytes;
     const int slot0 = steps.slot(begin + warp + n * kWarps);
+    const bool all = sees(a, len, slot0) && sees(a, len, slot0 + kKeys - 1) && (a.window == 0 || slot0 + kKeys <= a.sinks || slot0 >= len - a.window);
+    if (!all) {  // 0 times what a hidden slot of V holds has to be 0
+      for (int i = lane; i < kKeys * kParts * 8; i += 32) {
+        if (!sees(a, len, slot0 + i / 8 % kKeys)) st_shared(v_rows + i * 16, make_uint4(0, 0, 0, 0));
+      }
+      fence_proxy_async_smem();  // (ahead of the TMA that fills the stage next)
+      __syncwarp();
+    }
 
     float s[2][4] = {};  // slots 0..7 and 8..15 of the step
     {
@@ -160,14 +190,13 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeArgs a) {
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
         std::uint32_t kf[4];
-        ldsm4(k_rows + r * kRowBytes + (((2 * d + half) ^ (r & 7)) << 4), kf);
+        ldsm4(k_rows + d / 4 * kPartBytes + r * 128 + (((2 * d + half) % 8 ^ (r & 7)) << 4), kf);
         mma16<T>(s[0], qf[d], kf[0], kf[1]);
         mma16<T>(s[1], qf[d], kf[2], kf[3]);
       }
     }
     // In binades; what is not seen is minus infinity.
     const int key = slot0 + (lane % 4) * 2;
-    const bool all = sees(a, len, slot0) && sees(a, len, slot0 + kKeys - 1) && (a.window == 0 || slot0 + kKeys <= a.sinks || slot0 >= len - a.window);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -235,7 +264,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeArgs a) {
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) {
       std::uint32_t vf[4];
-      ldsm4_trans(v_rows + r * kRowBytes + (((2 * d + half) ^ (r & 7)) << 4), vf);
+      ldsm4_trans(v_rows + d / 4 * kPartBytes + r * 128 + (((2 * d + half) % 8 ^ (r & 7)) << 4), vf);
       mma16<T>(o[2 * d], hi, vf[0], vf[1]);
       mma16<T>(o[2 * d + 1], hi, vf[2], vf[3]);
       if constexpr (kTwoParts) {
@@ -243,8 +272,9 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeArgs a) {
         mma16<T>(o[2 * d + 1], lo, vf[2], vf[3]);
       }
     }
+    __syncwarp();  // the stage is read
+    issue(n + kStages);
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
@@ -253,6 +283,13 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeArgs a) {
 
   // The warps' parts meet in the rings' place.
   __syncthreads();
+  if (s_abort != 0) {  // a wait expired: give the copies on their way time to land, and leave
+    if (threadIdx.x == 0) atomicOr(a.c.status, kPagedWait);
+    const std::uint64_t t0 = global_ns();
+    while (global_ns() - t0 < 2000000ull) {
+    }
+    return;
+  }
   float* s_o = reinterpret_cast<float*>(smem);           // [kWarps][kRows][D + 4]
   constexpr int kLd = D + 4;
   float* s_ml = s_o + kWarps * kRows * kLd;              // [kWarps][kRows][2]
@@ -292,75 +329,116 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeArgs a) {
   }
 }
 
-// The parts of a (sequence, key head) joined: the outputs of query heads x, x + gridDim.x, ... of its group, and what the slots of the
-// x-th range got. Every CTA works out the group's maxima and sums from the parts' for itself.
+// The maximum and the logarithm of the sum of all parts of a query head, in binades (infinity where nothing is seen). Whole warps.
+__device__ __forceinline__ float joined_lse(const float2* ml, int parts, int lane) {
+  float mm = -INFINITY;
+  for (int i = lane; i < parts; i += 32) mm = fmaxf(mm, ml[i].x);
+#pragma unroll
+  for (int w = 16; w > 0; w /= 2) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, w));
+  float ll = 0.f;
+  for (int i = lane; i < parts; i += 32) ll += ml[i].y == 0.f ? 0.f : ml[i].y * ex2(ml[i].x - mm);
+#pragma unroll
+  for (int w = 16; w > 0; w /= 2) ll += __shfl_xor_sync(0xffffffffu, ll, w);
+  return ll == 0.f ? INFINITY : mm + log2f(ll);
+}
+
+// The parts of a (sequence, key head) joined: the first CTAs have its query heads, the others ranges of its slots.
 template <typename T, int D, bool kScores>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a) {
-  extern __shared__ __align__(16) float s_lse[];  // [group] log2 of the sum of all weights, or infinity where nothing is seen
-  __shared__ __align__(16) float s_sum[kJoinThreads * 4];
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a, int head_ctas) {
+  extern __shared__ __align__(16) float s_lse[];  // [group]
+  __shared__ __align__(16) float4 s_sum[kJoinThreads];
+  __shared__ float2 s_ml[kJoinThreads];
   const int h = blockIdx.y, b = blockIdx.z, warp = static_cast<int>(threadIdx.x) / 32, lane = static_cast<int>(threadIdx.x) % 32;
-  wait_for_predecessors();
-  const int len = paged_len(a.c, b);
+  const int len = paged_len(a.c, b);  // (no kernel of the call writes the lengths: read ahead of the wait)
   const Steps steps(a, len);
   const int parts = max(1, (steps.count + a.chunk - 1) / a.chunk);
   const std::int64_t head0 = static_cast<std::int64_t>(b) * a.q_heads + h * a.group;
-  for (int g = warp; g < a.group; g += kJoinThreads / 32) {
-    const float2* ml = a.part_ml + (head0 + g) * a.splits;
-    float mm = -INFINITY;
-    for (int i = lane; i < parts; i += 32) mm = fmaxf(mm, ml[i].x);
-#pragma unroll
-    for (int w = 16; w > 0; w /= 2) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, w));
-    float ll = 0.f;
-    for (int i = lane; i < parts; i += 32) ll += ml[i].y == 0.f ? 0.f : ml[i].y * ex2(ml[i].x - mm);
-#pragma unroll
-    for (int w = 16; w > 0; w /= 2) ll += __shfl_xor_sync(0xffffffffu, ll, w);
-    if (lane == 0) s_lse[g] = ll == 0.f ? INFINITY : mm + log2f(ll);
-  }
-  __syncthreads();
 
-  constexpr int kQuads = D / 4, kSlices = kJoinThreads / kQuads;  // threads to a row, rows of the parts at a time
-  const int quad = static_cast<int>(threadIdx.x) % kQuads, slice = static_cast<int>(threadIdx.x) / kQuads;
-  for (int g = blockIdx.x; g < a.group; g += gridDim.x) {
-    const float lse2 = s_lse[g];
-    const float2* ml = a.part_ml + (head0 + g) * a.splits;
-    const float* part = a.part_o + (head0 + g) * a.splits * D + quad * 4;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = slice; i < parts; i += kSlices) {
-      const float2 of = ml[i];
-      const float f = of.y == 0.f ? 0.f : ex2(of.x - lse2);
-      const float4 x = *reinterpret_cast<const float4*>(part + static_cast<std::int64_t>(i) * D);
-      sum.x = fmaf(f, x.x, sum.x), sum.y = fmaf(f, x.y, sum.y), sum.z = fmaf(f, x.z, sum.z), sum.w = fmaf(f, x.w, sum.w);
-    }
-    __syncthreads();  // (the sums of the head before are read)
-    *reinterpret_cast<float4*>(s_sum + 4 * threadIdx.x) = sum;
-    __syncthreads();
-    if (slice == 0) {
-      for (int i = 1; i < kSlices; ++i) {
-        const float4 x = *reinterpret_cast<const float4*>(s_sum + 4 * (i * kQuads + quad));
-        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+  if (static_cast<int>(blockIdx.x) < head_ctas) {
+    // Four channels a thread, a slice of the parts each: one pass with a running maximum, so that no load waits for another.
+    constexpr int kQuads = D / 4, kSlices = kJoinThreads / kQuads;
+    const int quad = static_cast<int>(threadIdx.x) % kQuads, slice = static_cast<int>(threadIdx.x) / kQuads;
+    wait_for_predecessors();
+    for (int g = blockIdx.x; g < a.group; g += head_ctas) {
+      const float2* ml = a.part_ml + (head0 + g) * a.splits;
+      const float* part = a.part_o + (head0 + g) * a.splits * D + quad * 4;
+      float m = -INFINITY, l = 0.f;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      const auto add = [&](float mi, float li, const float4& x) {
+        if (li == 0.f) return;  // nothing seen
+        const float top = fmaxf(m, mi), f = ex2(mi - top), keep = l == 0.f ? 0.f : ex2(m - top);
+        m = top, l = fmaf(f, li, keep * l);
+        sum.x = fmaf(f, x.x, keep * sum.x), sum.y = fmaf(f, x.y, keep * sum.y);
+        sum.z = fmaf(f, x.z, keep * sum.z), sum.w = fmaf(f, x.w, keep * sum.w);
+      };
+      for (int i0 = slice; i0 < parts; i0 += 4 * kSlices) {
+        float2 of[4];
+        float4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = i0 + i * kSlices;
+          of[i] = at < parts ? ml[at] : make_float2(0.f, 0.f);
+          if (at < parts) x[i] = *reinterpret_cast<const float4*>(part + static_cast<std::int64_t>(at) * D);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) add(of[i].x, of[i].y, x[i]);
       }
-      T* out = static_cast<T*>(a.out) + b * a.o_row + (h * a.group + g) * a.o_head + quad * 4;
-      *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(sum.x, sum.y), pack16<T>(sum.z, sum.w));
-      if (quad == 0 && a.lse != nullptr) a.lse[head0 + g] = lse2 == INFINITY ? -INFINITY : lse2 * 0.6931471805599453f;
+      __syncthreads();  // (the slices of the head before are read)
+      s_sum[threadIdx.x] = sum, s_ml[threadIdx.x] = make_float2(m, l);
+      __syncthreads();
+      if (slice == 0) {
+        for (int i = 1; i < min(kSlices, parts); ++i) add(s_ml[i * kQuads + quad].x, s_ml[i * kQuads + quad].y, s_sum[i * kQuads + quad]);
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        T* out = static_cast<T*>(a.out) + b * a.o_row + (h * a.group + g) * a.o_head + quad * 4;
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(sum.x * inv, sum.y * inv), pack16<T>(sum.z * inv, sum.w * inv));
+        if (quad == 0 && a.lse != nullptr) a.lse[head0 + g] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      }
     }
+    return;
   }
 
   if constexpr (kScores) {
+    // kJoinSlots slots of a thread at a time, a CTA's width apart: their loads do not wait for one another.
+    constexpr int kRange = kJoinThreads * kJoinSlots;
+    const int first = (static_cast<int>(blockIdx.x) - head_ctas) * kRange;
+    if (first >= len) return;
+    wait_for_predecessors();
+    for (int g = warp; g < a.group; g += kJoinThreads / 32) {
+      const float lse2 = joined_lse(a.part_ml + (head0 + g) * a.splits, parts, lane);
+      if (lane == 0) s_lse[g] = lse2;
+    }
+    __syncthreads();
     const std::int64_t row = (static_cast<std::int64_t>(b) * a.c.kv_heads + h) * a.weights_ld;
-    for (int j = static_cast<int>(blockIdx.x) * kJoinThreads + static_cast<int>(threadIdx.x); j < len; j += gridDim.x * kJoinThreads) {
-      float sum = j < len - 1 ? a.weights[row + j] : 0.f;
-      if (sees(a, len, j)) {
-        const float* s = a.scores + head0 * a.scores_ld + j;
-        float got = 0.f;
-        for (int g = 0; g < a.group; ++g) got += ex2(s[g * a.scores_ld] - s_lse[g]);
-        sum += got;
+    for (int j0 = first + static_cast<int>(threadIdx.x); j0 < len; j0 += (static_cast<int>(gridDim.x) - head_ctas) * kRange) {
+      float sum[kJoinSlots], got[kJoinSlots] = {};
+      bool seen[kJoinSlots];
+#pragma unroll
+      for (int i = 0; i < kJoinSlots; ++i) {
+        const int j = j0 + i * kJoinThreads;
+        seen[i] = sees(a, len, j);
+        sum[i] = j < len - 1 ? a.weights[row + j] : 0.f;
       }
-      a.weights_out[row + j] = sum;
+      const float* s = a.scores + head0 * a.scores_ld + j0;
+#pragma unroll 4
+      for (int g = 0; g < a.group; ++g) {
+#pragma unroll
+        for (int i = 0; i < kJoinSlots; ++i) {
+          if (seen[i]) got[i] += ex2(s[g * a.scores_ld + i * kJoinThreads] - s_lse[g]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kJoinSlots; ++i) {
+        if (j0 + i * kJoinThreads < len) a.weights_out[row + j0 + i * kJoinThreads] = sum[i] + got[i];
+      }
     }
   }
 }
 
-constexpr int kTargetCtas = 4;  // CTAs per SM that a call is cut into, where it is long enough
+// How a call is cut into CTAs, by their number per SM, of which three fit at a time. One sequence: two equal CTAs per SM (131001
+// slots, 4 key heads: 53 us; three per SM 58, six 76). Several, whose lengths differ: eighteen, handed out as SMs come free (64 of up to 8101, 8
+// key heads: 196 us; three per SM 233), but of kLongEnough steps at least, since each has its start and its part to join
+// (4 of up to 30001: 76 us; as eighteen per SM 79).
+constexpr int kOneSequence = 2, kSeveral = 18, kLongEnough = 32, kShortest = kWarps;
 
 struct Plan {
   int chunk, splits;
@@ -374,9 +452,10 @@ Plan plan(const PagedArgs& c, int q_heads, int head_dim, int window, int sinks, 
   const std::int64_t group = q_heads / c.kv_heads, units = std::max<std::int64_t>(1, c.batch * c.kv_heads * ((group + kRows - 1) / kRows));
   std::int64_t steps = p.scores_ld / kKeys;
   if (window > 0) steps = std::min<std::int64_t>(steps, (static_cast<std::int64_t>(window) + kKeys - 1) / kKeys + 1 + (static_cast<std::int64_t>(sinks) + kKeys - 1) / kKeys);
-  const std::int64_t target = static_cast<std::int64_t>(sm_count()) * kTargetCtas;
-  std::int64_t chunk = (steps * units + target - 1) / target;
-  chunk = std::max<std::int64_t>((chunk + kWarps - 1) / kWarps * kWarps, 2 * kWarps);
+  const std::int64_t ctas = static_cast<std::int64_t>(sm_count()) * (c.batch <= 1 ? kOneSequence : kSeveral);
+  std::int64_t chunk = (steps * units + ctas - 1) / ctas;
+  if (c.batch > 1) chunk = std::max<std::int64_t>(chunk, kLongEnough);
+  chunk = std::max<std::int64_t>(chunk, kShortest);
   p.chunk = static_cast<int>(std::min<std::int64_t>(chunk, INT_MAX / 2));
   p.splits = static_cast<int>(std::max<std::int64_t>(1, (steps + p.chunk - 1) / p.chunk));
   p.parts = p.splits > 1 || weights;
@@ -402,9 +481,9 @@ int check(const char* op, const b2_paged_cache* cache, PagedArgs* c, int q_heads
 }
 
 template <typename T, int D, bool kScores>
-int launch(const char* op, const DecodeArgs& a, const Plan& p, cudaStream_t st) {
+int launch(const char* op, const DecodeArgs& a, const Plan& p, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t st) {
   constexpr int ring = kWarps * kStages * 2 * kKeys * D * 2, meet = kWarps * kRows * (D + 4 + 2) * 4;
-  constexpr int smem = ring > meet ? ring : meet;
+  constexpr int smem = (ring > meet ? ring : meet) + 1024;  // and what aligns it
   const auto kernel = decode_kernel<T, D, kScores>;
   if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) {
     cudaGetLastError();
@@ -413,11 +492,11 @@ int launch(const char* op, const DecodeArgs& a, const Plan& p, cudaStream_t st) 
   const LaunchChain chain(st);
   const unsigned blocks = static_cast<unsigned>((a.group + kRows - 1) / kRows), batch = static_cast<unsigned>(a.c.batch);
   const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.c.kv_heads) * blocks, batch);
-  if (const int rc = enqueue(op, kernel, grid, kThreads, smem, st, 1, a)) return rc;
+  if (const int rc = enqueue(op, kernel, grid, kThreads, smem, st, 1, map_k, map_v, a)) return rc;
   if (!p.parts) return B2_OK;
-  const int slices = std::max(std::min(a.group, 64), kScores ? std::min((a.c.most + 1023) / 1024, 1 << 20) : 1);
-  return enqueue(op, join_kernel<T, D, kScores>, dim3(static_cast<unsigned>(slices), static_cast<unsigned>(a.c.kv_heads), batch), kJoinThreads,
-                 static_cast<std::size_t>(a.group) * 4, st, 1, a);
+  const int head_ctas = std::min(a.group, 64), range = kJoinThreads * kJoinSlots, slot_ctas = kScores ? (a.c.most + range - 1) / range : 0;
+  return enqueue(op, join_kernel<T, D, kScores>, dim3(static_cast<unsigned>(head_ctas + slot_ctas), static_cast<unsigned>(a.c.kv_heads), batch), kJoinThreads,
+                 kScores ? static_cast<std::size_t>(a.group) * 4 : 0, st, 1, a, head_ctas);
 }
 
 }  // namespace
@@ -467,15 +546,18 @@ int b2_attention_paged_decode(const b2_paged_cache* cache, const b2_view3* q, co
   a.weights = weights, a.weights_out = weights_out, a.weights_ld = weights_ld;
   const cudaStream_t st = as_stream(stream);
   if (const int rc = paged_status_word(op, &a.c)) return rc;
+  if (cache->num_pages == 0) return fail_invalid(op, "the pool has no pages");
+  CUtensorMap map_k, map_v;
+  if (!make_tensor_map_pages(&map_k, cache, false, kKeys, op) || !make_tensor_map_pages(&map_v, cache, true, kKeys, op)) return B2_ERR_CUDA;
   const bool wide = cache->head_dim == 128;
   if (cache->dtype == B2_DTYPE_BF16) {
     using T = __nv_bfloat16;
-    if (scores) return wide ? launch<T, 128, true>(op, a, p, st) : launch<T, 64, true>(op, a, p, st);
-    return wide ? launch<T, 128, false>(op, a, p, st) : launch<T, 64, false>(op, a, p, st);
+    if (scores) return wide ? launch<T, 128, true>(op, a, p, map_k, map_v, st) : launch<T, 64, true>(op, a, p, map_k, map_v, st);
+    return wide ? launch<T, 128, false>(op, a, p, map_k, map_v, st) : launch<T, 64, false>(op, a, p, map_k, map_v, st);
   }
   using T = __half;
-  if (scores) return wide ? launch<T, 128, true>(op, a, p, st) : launch<T, 64, true>(op, a, p, st);
-  return wide ? launch<T, 128, false>(op, a, p, st) : launch<T, 64, false>(op, a, p, st);
+  if (scores) return wide ? launch<T, 128, true>(op, a, p, map_k, map_v, st) : launch<T, 64, true>(op, a, p, map_k, map_v, st);
+  return wide ? launch<T, 128, false>(op, a, p, map_k, map_v, st) : launch<T, 64, false>(op, a, p, map_k, map_v, st);
 }
 
 }  // extern "C"

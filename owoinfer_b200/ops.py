@@ -669,6 +669,10 @@ def dit_prefill_references(model, latents, time_vector, tier=TIER_INT8):
 # ------------------------------------------------------------------------------------------------ paged key-value cache
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_PAGED_BYTES = C.sizeof(_lib.PagedCache)
+
+# (A single token's kernels take a few microseconds, so what a call does on the host is a good part of it: the checks below
+# are written for their number of tensor queries, and the structs filled in one go.)
 
 
 def _raw_stream() -> int:
@@ -679,9 +683,23 @@ def _at(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _need(t, name, dtype, dim):
-    if t.dtype != dtype or t.dim() != dim or (dim and t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{name} must be a {dtype} tensor of {dim} dimensions, the last one contiguous")
+def _rows(t, name, dtype):
+    """(rows, row stride) of a matrix of `dtype` whose rows are contiguous."""
+    if t.dtype != dtype or t.dim() != 2:
+        raise ValueError(f"{name} must be a {dtype} matrix")
+    rows, width = t.shape
+    if t.is_contiguous():
+        return rows, width
+    stride, inner = t.stride()
+    if inner != 1 and width > 1:
+        raise ValueError(f"the rows of {name} must be contiguous")
+    return rows, max(stride, width)
+
+
+def _vector(t, name, count):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != count or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {count} entries")
+    return t.data_ptr()
 
 
 class PagedCache:
@@ -690,59 +708,61 @@ class PagedCache:
     contents may change between calls (lengths that grow, pages that are added) without a new handle."""
 
     def __init__(self, k, v, block_table, seq_lens):
-        if k.dtype not in _DTYPES or k.dtype != v.dtype or k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.stride(3) != 1:
+        shape, strides = k.shape, k.stride()
+        dtype = k.dtype
+        code = _DTYPES.get(dtype)
+        if code is None or dtype != v.dtype or len(shape) != 4 or shape != v.shape or strides != v.stride() or strides[3] != 1:
             raise ValueError("k and v must be bf16 or fp16 pools [pages, kv_heads, page_size, head_dim] of the same strides, head_dim contiguous")
-        _need(block_table, "block_table", torch.int32, 2)
-        _need(seq_lens, "seq_lens", torch.int32, 1)
-        if block_table.shape[0] != seq_lens.shape[0]:
-            raise ValueError("block_table and seq_lens must have a row for every sequence")
-        self.k, self.v, self.block_table, self.seq_lens, self.dtype = k, v, block_table, seq_lens, k.dtype
-        pages, heads, page, dim = k.shape
-        page_stride, head_stride, row_stride, _ = k.stride()
-        batch, width = block_table.shape
-        self.batch, self.kv_heads, self.page_size, self.head_dim, self.slots = batch, heads, page, dim, width * page
-        self.struct = _lib.PagedCache(C.sizeof(_lib.PagedCache), k.data_ptr(), v.data_ptr(), page_stride, head_stride, row_stride, pages,
-                                      _DTYPES[k.dtype], heads, page, dim, block_table.data_ptr(), max(block_table.stride(0), width), width,
-                                      seq_lens.data_ptr(), batch)
+        batch, ld = _rows(block_table, "block_table", torch.int32)
+        self.k, self.v, self.block_table, self.seq_lens, self.dtype = k, v, block_table, seq_lens, dtype
+        pages, self.kv_heads, self.page_size, self.head_dim = shape
+        width = block_table.numel() // batch if batch else 0
+        self.batch, self.slots = batch, width * self.page_size
+        self.struct = _lib.PagedCache(_PAGED_BYTES, k.data_ptr(), v.data_ptr(), strides[0], strides[1], strides[2], pages, code, self.kv_heads,
+                                      self.page_size, self.head_dim, block_table.data_ptr(), ld, width, _vector(seq_lens, "seq_lens", batch), batch)
 
 
 def _heads_view(t, cache, name):
-    if t.dim() != 3 or t.dtype != cache.dtype or t.shape[2] != cache.head_dim or t.stride(2) != 1:
-        raise ValueError(f"{name} must be a [tokens, heads, head_dim] view of the cache's dtype and head_dim, head_dim contiguous")
-    return _view3(t)
+    if t.dim() != 3 or t.dtype != cache.dtype:
+        raise ValueError(f"{name} must be a [tokens, heads, head_dim] view of the cache's dtype")
+    tokens, heads, dim = t.shape
+    row, head, inner = t.stride()
+    if dim != cache.head_dim or inner != 1:
+        raise ValueError(f"{name} must have the cache's head_dim, contiguous")
+    return _lib.View3(t.data_ptr(), tokens, heads, row, head)
 
 
 def qk_norm_rope_append(qkv, cache, cu_seqlens, q_norm, k_norm, rope, positions=None, eps=1e-6, interleaved=False, out=None):
     """qkv [tokens, (q_heads + 2 kv_heads) * head_dim]: per-head RMS norm of queries and keys (None: none), rotation by the fp32 table
     rope [positions, rot_dim] (sin | cos; None: none), keys and values into the cache's last slots. Returns the queries
     [tokens, q_heads, head_dim] (into `out` when given; qkv's own query part will do)."""
-    _need(qkv, "qkv", cache.dtype, 2)
-    _need(cu_seqlens, "cu_seqlens", torch.int32, 1)
-    tokens, width = qkv.shape
-    heads, rest = divmod(width, cache.head_dim)
+    tokens, ld = _rows(qkv, "qkv", cache.dtype)
+    dim = cache.head_dim
+    heads, rest = divmod(qkv.shape[1], dim)
     q_heads = heads - 2 * cache.kv_heads
-    if rest or q_heads <= 0 or cu_seqlens.shape[0] != cache.batch + 1:
-        raise ValueError("qkv must have q_heads + 2 kv_heads heads, cu_seqlens batch + 1 entries")
+    if rest or q_heads <= 0:
+        raise ValueError("qkv must have q_heads + 2 kv_heads heads")
     for norm in (q_norm, k_norm):
-        if norm is not None and (norm.dtype != cache.dtype or norm.shape != (cache.head_dim,) or not norm.is_contiguous()):
+        if norm is not None and (norm.dtype != cache.dtype or norm.dim() != 1 or norm.numel() != dim or not norm.is_contiguous()):
             raise ValueError("q_norm and k_norm must be contiguous [head_dim] tensors of the cache's dtype")
-    if rope is not None and (rope.dtype != torch.float32 or rope.dim() != 2 or not rope.is_contiguous()):
-        raise ValueError("rope must be a contiguous fp32 table [positions, rot_dim]")
-    if positions is not None and (positions.dtype != torch.int32 or positions.shape != (tokens,) or not positions.is_contiguous()):
-        raise ValueError("positions must be a contiguous int32 tensor with one entry per token")
-    out = torch.empty((tokens, q_heads, cache.head_dim), dtype=cache.dtype, device=qkv.device) if out is None else out
-    if out.dtype != cache.dtype or out.shape != (tokens, q_heads, cache.head_dim) or out.stride(2) != 1:
-        raise ValueError("out must be a [tokens, q_heads, head_dim] view of the cache's dtype, head_dim contiguous")
-    rows, rot = (0, 0) if rope is None else rope.shape
-    check(_lib.lib().b2_qk_norm_rope_append(cache.struct, qkv.data_ptr(), _ld(qkv), tokens, q_heads, cu_seqlens.data_ptr(), _at(positions), _at(q_norm),
-                                            _at(k_norm), eps, _at(rope), rows, rot, int(interleaved), out.data_ptr(), out.stride(0), out.stride(1),
-                                            _raw_stream()))
+    rows = rot = 0
+    if rope is not None:
+        if rope.dtype != torch.float32 or rope.dim() != 2 or not rope.is_contiguous():
+            raise ValueError("rope must be a contiguous fp32 table [positions, rot_dim]")
+        rows, rot = rope.shape
+    out = torch.empty((tokens, q_heads, dim), dtype=cache.dtype, device=qkv.device) if out is None else out
+    view = _heads_view(out, cache, "out")
+    if view.tokens != tokens or view.heads != q_heads:
+        raise ValueError("out must be a [tokens, q_heads, head_dim] view")
+    check(_lib.lib().b2_qk_norm_rope_append(cache.struct, qkv.data_ptr(), ld, tokens, q_heads, _vector(cu_seqlens, "cu_seqlens", cache.batch + 1),
+                                            0 if positions is None else _vector(positions, "positions", tokens), _at(q_norm), _at(k_norm), eps,
+                                            _at(rope), rows, rot, interleaved, view.data, view.row_stride, view.head_stride, _raw_stream()))
     return out
 
 
-def _lse_of(q, lse):
+def _lse_of(view, q, lse):
     if lse is None:
-        return torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        return torch.empty((view.tokens, view.heads), dtype=torch.float32, device=q.device)
     if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous():
         raise ValueError("lse must be a contiguous fp32 [tokens, q_heads] tensor")
     return lse
@@ -751,18 +771,16 @@ def _lse_of(q, lse):
 def attention_paged(q, cache, cu_seqlens, max_q, scale, window=0, sinks=0, out=None, lse=None):
     """Causal attention of a prompt's tokens q [tokens, q_heads, head_dim] over the cache that holds their keys and values already;
     with a window the last `window` slots and the first `sinks`. Returns (out, lse): lse fp32 [tokens, q_heads]."""
-    _need(cu_seqlens, "cu_seqlens", torch.int32, 1)
-    if cu_seqlens.shape[0] != cache.batch + 1:
-        raise ValueError("cu_seqlens must have batch + 1 entries")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    lse = _lse_of(q, lse)
-    check(_lib.lib().b2_attention_paged(cache.struct, _heads_view(q, cache, "q"), _heads_view(out, cache, "out"), lse.data_ptr(),
-                                        cu_seqlens.data_ptr(), max_q, scale, window, sinks, _raw_stream()))
+    view = _heads_view(q, cache, "q")
+    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    lse = _lse_of(view, q, lse)
+    check(_lib.lib().b2_attention_paged(cache.struct, view, _heads_view(out, cache, "out"), lse.data_ptr(), _vector(cu_seqlens, "cu_seqlens", cache.batch + 1),
+                                        max_q, scale, window, sinks, _raw_stream()))
     return out, lse
 
 
 def attention_paged_decode_workspace_bytes(cache, q_heads, max_len=0, window=0, sinks=0, weights=False) -> int:
-    n = _lib.lib().b2_attention_paged_decode_workspace_bytes(cache.struct, q_heads, max_len, window, sinks, int(weights))
+    n = _lib.lib().b2_attention_paged_decode_workspace_bytes(cache.struct, q_heads, max_len, window, sinks, weights)
     if n == 0:
         check(-1)
     return n
@@ -771,22 +789,31 @@ def attention_paged_decode_workspace_bytes(cache, q_heads, max_len=0, window=0, 
 def attention_paged_decode(q, cache, scale, max_len=0, window=0, sinks=0, weights=None, weights_out=None, out=None, lse=None, workspace=None):
     """Attention of one new token per sequence, q [batch, q_heads, head_dim], split over the cache's length. With `weights` (fp32 [batch,
     kv_heads, slots]) the attention each slot got is added to them (in weights_out, or in place). Returns (out, lse)."""
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    lse = _lse_of(q, lse)
+    view = _heads_view(q, cache, "q")
+    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    lse = _lse_of(view, q, lse)
     ld = 0
     if weights is not None:
         weights_out = weights if weights_out is None else weights_out
-        _need(weights, "weights", torch.float32, 3)
-        if weights.shape[:2] != (cache.batch, cache.kv_heads) or not weights.is_contiguous() or weights_out.shape != weights.shape or \
-                weights_out.dtype != torch.float32 or not weights_out.is_contiguous():
-            raise ValueError("weights and weights_out must be contiguous fp32 [batch, kv_heads, slots] tensors of one shape")
-        ld = weights.shape[2]
+        ld = _slots_of(weights, cache, "weights")
+        if weights_out is not weights and _slots_of(weights_out, cache, "weights_out") != ld:
+            raise ValueError("weights and weights_out must have the same shape")
     if workspace is None:
-        workspace = torch.empty(attention_paged_decode_workspace_bytes(cache, q.shape[1], max_len, window, sinks, weights is not None),
+        workspace = torch.empty(attention_paged_decode_workspace_bytes(cache, view.heads, max_len, window, sinks, weights is not None),
                                 dtype=torch.uint8, device=q.device)
-    check(_lib.lib().b2_attention_paged_decode(cache.struct, _heads_view(q, cache, "q"), _heads_view(out, cache, "out"), lse.data_ptr(), max_len, scale,
-                                               window, sinks, _at(weights), _at(weights_out), ld, workspace.data_ptr(), workspace.numel(), _raw_stream()))
+    check(_lib.lib().b2_attention_paged_decode(cache.struct, view, _heads_view(out, cache, "out"), lse.data_ptr(), max_len, scale, window, sinks,
+                                               _at(weights), _at(weights_out), ld, workspace.data_ptr(), workspace.numel(), _raw_stream()))
     return out, lse
+
+
+def _slots_of(t, cache, name):
+    """Slots of a contiguous fp32 [batch, kv_heads, slots] tensor."""
+    if t.dtype != torch.float32 or t.dim() != 3 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous fp32 [batch, kv_heads, slots] tensor")
+    batch, heads, slots = t.shape
+    if batch != cache.batch or heads != cache.kv_heads:
+        raise ValueError(f"{name} must have a row for each sequence and key head")
+    return slots
 
 
 def kv_evict(cache, weights, table_out, budget, sinks=0, recent=0, kept=None, lens_out=None, weights_out=None):
@@ -795,21 +822,17 @@ def kv_evict(cache, weights, table_out, budget, sinks=0, recent=0, kept=None, le
     (kept int32 [batch, kv_heads, budget], lens int32 [batch]); weights_out receives the weights of what is kept."""
     if budget <= 0:
         raise ValueError("budget must be positive")
-    _need(weights, "weights", torch.float32, 3)
-    _need(table_out, "table_out", torch.int32, 2)
-    if weights.shape[:2] != (cache.batch, cache.kv_heads) or not weights.is_contiguous() or table_out.shape[0] != cache.batch:
-        raise ValueError("weights must be contiguous [batch, kv_heads, slots], table_out [batch, pages]")
-    if weights_out is not None and (weights_out.dtype != torch.float32 or weights_out.dim() != 3 or weights_out.shape[:2] != weights.shape[:2] or
-                                    not weights_out.is_contiguous()):
-        raise ValueError("weights_out must be a contiguous fp32 [batch, kv_heads, slots] tensor")
+    slots = _slots_of(weights, cache, "weights")
+    rows_out, ld_out = _rows(table_out, "table_out", torch.int32)
+    if rows_out != cache.batch:
+        raise ValueError("table_out must have a row for every sequence")
+    slots_out = 0 if weights_out is None else _slots_of(weights_out, cache, "weights_out")
     kept = torch.empty((cache.batch, cache.kv_heads, budget), dtype=torch.int32, device=weights.device) if kept is None else kept
-    lens_out = torch.empty(cache.batch, dtype=torch.int32, device=weights.device) if lens_out is None else lens_out
-    if kept.dtype != torch.int32 or kept.shape != (cache.batch, cache.kv_heads, budget) or not kept.is_contiguous() or \
-            lens_out.dtype != torch.int32 or lens_out.shape != (cache.batch,) or not lens_out.is_contiguous():
-        raise ValueError("kept must be a contiguous int32 [batch, kv_heads, budget] tensor, lens_out int32 [batch]")
-    check(_lib.lib().b2_kv_evict(cache.struct, weights.data_ptr(), weights.shape[2], sinks, recent, budget, table_out.data_ptr(),
-                                 max(table_out.stride(0), table_out.shape[1]), table_out.shape[1], kept.data_ptr(), lens_out.data_ptr(), _at(weights_out),
-                                 0 if weights_out is None else weights_out.shape[2], _raw_stream()))
+    lens_out = torch.empty_like(cache.seq_lens) if lens_out is None else lens_out
+    if kept.dtype != torch.int32 or kept.shape != (cache.batch, cache.kv_heads, budget) or not kept.is_contiguous():
+        raise ValueError("kept must be a contiguous int32 [batch, kv_heads, budget] tensor")
+    check(_lib.lib().b2_kv_evict(cache.struct, weights.data_ptr(), slots, sinks, recent, budget, table_out.data_ptr(), ld_out, table_out.shape[1],
+                                 kept.data_ptr(), _vector(lens_out, "lens_out", cache.batch), _at(weights_out), slots_out, _raw_stream()))
     return kept, lens_out
 
 
