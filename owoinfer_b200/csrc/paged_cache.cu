@@ -6,6 +6,7 @@
 #include <cmath>
 #include <mutex>
 
+#include "attention.cuh"
 #include "paged.cuh"
 
 namespace b2 {
@@ -29,37 +30,102 @@ struct AppendArgs {
   void* q_out;
   std::int64_t q_row, q_head;
   float eps;
-  int q_heads, half, chunks;  // half: rotated pairs; chunks: groups of kHeads heads of a token
+  int q_heads, half;          // half: rotated pairs
+  std::int64_t padded;        // tokens, up to a whole number of warps
+  int chunks, chunk_heads;    // a token's heads are cut into chunks of chunk_heads, each for one group of lanes
 };
 
-constexpr int kAppendHeads = 4;  // heads a group of lanes works on at a time, their loads issued together
-constexpr int kAppendThreads = 256;
+constexpr int kAppendHeads = 4;  // heads a group of lanes loads at a time
+constexpr int kAppendThreads = 128;
 
-// One group of D / 8 lanes (8 channels each) per (token, four heads): the sum of squares is a butterfly within the group, and
-// the other element of a rotation pair is in the same lane (interleaved) or half a rotation's lanes away.
+// A lane's 8 channels of a head: the first elements of four rotation pairs and the second ones, so that norm, rotation and rounding
+// need no other lane (the sum of squares apart). Pairs (i, i + half): two pieces of 4 channels; pairs (2 i, 2 i + 1), and the
+// channels that are not rotated: one piece of 8.
+template <bool kInterleaved>
+struct Pieces {
+  int first, second;  // channels of the pieces
+  __device__ __forceinline__ Pieces(int lane, int half) {
+    const bool turns = lane * 8 < 2 * half;
+    first = !kInterleaved && turns ? lane * 4 : lane * 8;
+    second = !kInterleaved && turns ? half + lane * 4 : lane * 8 + 4;
+  }
+  template <typename T>
+  __device__ __forceinline__ uint4 load(const T* row) const {
+    if constexpr (kInterleaved) return __ldcs(reinterpret_cast<const uint4*>(row + first));
+    const uint2 x = __ldcs(reinterpret_cast<const uint2*>(row + first)), y = __ldcs(reinterpret_cast<const uint2*>(row + second));
+    return make_uint4(x.x, x.y, y.x, y.y);
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* row, const uint4& v) const {
+    if constexpr (kInterleaved) {
+      *reinterpret_cast<uint4*>(row + first) = v;
+    } else {
+      *reinterpret_cast<uint2*>(row + first) = make_uint2(v.x, v.y);
+      *reinterpret_cast<uint2*>(row + second) = make_uint2(v.z, v.w);
+    }
+  }
+  // The pieces' values as the (a, b) of the four rotation pairs, two pairs to a packed pair of fp32, and back.
+  template <typename T>
+  __device__ __forceinline__ static void split(const uint4& v, std::uint64_t (&a)[2], std::uint64_t (&b)[2]) {
+    float x[8];
+    load8<T>(v, x);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      a[i] = kInterleaved ? pack2(x[4 * i], x[4 * i + 2]) : pack2(x[2 * i], x[2 * i + 1]);
+      b[i] = kInterleaved ? pack2(x[4 * i + 1], x[4 * i + 3]) : pack2(x[4 + 2 * i], x[5 + 2 * i]);
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ static uint4 merge(const std::uint64_t (&pa)[2], const std::uint64_t (&pb)[2]) {
+    float a[4], b[4];
+    unpack2(pa[0], a[0], a[1]), unpack2(pa[1], a[2], a[3]);
+    unpack2(pb[0], b[0], b[1]), unpack2(pb[1], b[2], b[3]);
+    if constexpr (kInterleaved) return make_uint4(pack16<T>(a[0], b[0]), pack16<T>(a[1], b[1]), pack16<T>(a[2], b[2]), pack16<T>(a[3], b[3]));
+    return make_uint4(pack16<T>(a[0], a[1]), pack16<T>(a[2], a[3]), pack16<T>(b[0], b[1]), pack16<T>(b[2], b[3]));
+  }
+};
+
+// A group of D / 8 lanes per (token, chunk of its heads). What a token needs once (its sequence, slot, page and angles: four loads one
+// after the other) is found while its first heads are on their way; the norm's weights are folded into the angles once per token, so that a
+// head costs its loads, a sum of squares over the group, four multiplications or additions a pair, the factor and the rounding.
+// With a lane holding 8 neighbouring channels (the other half of a pair 8 shuffles away) and addresses worked out per head it was 230 instructions
+// per head and warp, and the issue rate bound it at half the memory's.
 template <typename T, int D, bool kInterleaved>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
   constexpr int kLanes = D / 8;
   const int lane = static_cast<int>(threadIdx.x) % kLanes;
-  const unsigned group_mask = (kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1u)) << (threadIdx.x % 32 / kLanes * kLanes);
+  // A warp's groups have neighbouring tokens and the same heads, so that every branch below that a shuffle depends on is the warp's; a
+  // group without a token goes along.
   const std::int64_t unit = (static_cast<std::int64_t>(blockIdx.x) * kAppendThreads + threadIdx.x) / kLanes;
-  const std::int64_t token = unit / a.chunks;
-  if (token >= a.tokens) return;
-  const int head0 = static_cast<int>(unit - token * a.chunks) * kAppendHeads, heads = a.q_heads + 2 * a.c.kv_heads;
+  const std::int64_t chunk = unit / a.padded, at_token = unit - chunk * a.padded;
+  if (chunk >= a.chunks) return;  // (padded is a multiple of a warp's groups)
+  const bool there = at_token < a.tokens;
+  const std::int64_t token = there ? at_token : a.tokens - 1;
+  const int head0 = static_cast<int>(chunk) * a.chunk_heads;
+  const Pieces<kInterleaved> pieces(lane, a.half);
+  const T* row = static_cast<const T*>(a.qkv) + token * a.ld;
 
-  uint4 raw[kAppendHeads];
-  const T* row = static_cast<const T*>(a.qkv) + token * a.ld + lane * 8;
+  const int last = min(head0 + a.chunk_heads, a.q_heads + 2 * a.c.kv_heads);
+  uint4 raw[kAppendHeads], next[kAppendHeads];
+  const auto load = [&](int from) {
 #pragma unroll
-  for (int i = 0; i < kAppendHeads; ++i) {
-    if (head0 + i < heads) raw[i] = *reinterpret_cast<const uint4*>(row + static_cast<std::int64_t>(head0 + i) * D);
-  }
+    for (int i = 0; i < kAppendHeads; ++i) {
+      if (from + i < last) next[i] = pieces.load(row + (from + i) * D);
+    }
+  };
+  const auto take = [&](int then) {  // the heads that were on their way; those from `then` on take their place
+#pragma unroll
+    for (int i = 0; i < kAppendHeads; ++i) raw[i] = next[i];
+    load(then);
+  };
+  load(head0);
 
   // The sequence of this token: the lanes of the group try kLanes places of cu_seqlens at a time.
   int lo = 0, hi = a.c.batch;  // cu[lo] <= token < cu[hi] (what lies outside shows up below)
-  while (hi - lo > 1) {
-    const int step = (hi - lo + kLanes - 1) / kLanes, at = lo + (lane + 1) * step;
-    const bool below = at < hi && a.cu[at] <= token;
-    const int n = __popc(__ballot_sync(group_mask, below) & group_mask);
+  while (__any_sync(0xffffffffu, hi - lo > 1)) {
+    const int step = max(1, (hi - lo + kLanes - 1) / kLanes), at = lo + (lane + 1) * step;
+    const unsigned below = __ballot_sync(0xffffffffu, at < hi && a.cu[at] <= token) >> (threadIdx.x % 32 / kLanes * kLanes);
+    const int n = __popc(below & ((1u << kLanes) - 1u));
     hi = min(hi, lo + (n + 1) * step);
     lo += n * step;
   }
@@ -68,86 +134,83 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
   paged_tokens(a.c, a.cu, b, a.tokens, first, n);
   const int slot = paged_len(a.c, b) - n + static_cast<int>(token - first);
   const bool in_sequence = token >= first && token < first + n;
-  if (!in_sequence || slot < 0) {
-    atomicOr(a.c.status, kPagedBadTokens);
-    if (!in_sequence) return;
-  }
+  if (!in_sequence || slot < 0) atomicOr(a.c.status, kPagedBadTokens);
+  const int page = !there || !in_sequence || slot < 0 ? -1 : paged_page(a.c, b, slot);
+  const bool stores = there && in_sequence;
 
-  float sn[8], cs[8];
-  // Which pair of the rotation this lane's first channel belongs to; lanes past the rotation keep their values.
+  // sin and cos of this lane's pairs; 0 and 1 past the rotation.
   const bool turns = lane * 8 < 2 * a.half;
+  std::uint64_t sn[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)}, cs[2] = {pack2(1.f, 1.f), pack2(1.f, 1.f)};
   if (turns) {
     std::int64_t position = a.positions != nullptr ? a.positions[token] : max(slot, 0);
     if (position < 0 || position >= a.rope_rows) {
-      atomicOr(a.c.status, kPagedBadPosition);
+      if (in_sequence) atomicOr(a.c.status, kPagedBadPosition);
       position = position < 0 ? 0 : a.rope_rows - 1;
     }
-    const float* t = a.rope + position * (2 * a.half);
-    if constexpr (kInterleaved) {
-      const float4 s4 = *reinterpret_cast<const float4*>(t + lane * 4), c4 = *reinterpret_cast<const float4*>(t + a.half + lane * 4);
-      sn[0] = sn[1] = s4.x, sn[2] = sn[3] = s4.y, sn[4] = sn[5] = s4.z, sn[6] = sn[7] = s4.w;
-      cs[0] = cs[1] = c4.x, cs[2] = cs[3] = c4.y, cs[4] = cs[5] = c4.z, cs[6] = cs[7] = c4.w;
-    } else {
-      const int pair = lane * 8 < a.half ? lane * 8 : lane * 8 - a.half;
-#pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        const float4 s4 = *reinterpret_cast<const float4*>(t + pair + i), c4 = *reinterpret_cast<const float4*>(t + a.half + pair + i);
-        sn[i] = s4.x, sn[i + 1] = s4.y, sn[i + 2] = s4.z, sn[i + 3] = s4.w;
-        cs[i] = c4.x, cs[i + 1] = c4.y, cs[i + 2] = c4.z, cs[i + 3] = c4.w;
-      }
-    }
+    const float* t = a.rope + position * (2 * a.half) + lane * 4;
+    const float4 s4 = *reinterpret_cast<const float4*>(t), c4 = *reinterpret_cast<const float4*>(t + a.half);
+    sn[0] = pack2(s4.x, s4.y), sn[1] = pack2(s4.z, s4.w);
+    cs[0] = pack2(c4.x, c4.y), cs[1] = pack2(c4.z, c4.w);
   }
-  const int page = slot < 0 ? -1 : paged_page(a.c, b, slot);
-  const int away = a.half / 8, partner = !turns ? lane : lane < away ? lane + away : lane - away;
 
+  // Heads [from, to) normalised and rotated; head `from` goes to `out`, the next ones `step` elements apart (nullptr: nowhere).
+  const auto rotate = [&](int from, int to, const void* norm, T* out, std::int64_t step) {
+    std::uint64_t ac[2], as[2], bc[2], bs[2];  // weight times cos and sin (bs: minus), for the first and the second of a pair
+    {
+      std::uint64_t wa[2] = {pack2(1.f, 1.f), pack2(1.f, 1.f)}, wb[2] = {wa[0], wa[0]};
+      if (norm != nullptr) Pieces<kInterleaved>::template split<T>(pieces.load(static_cast<const T*>(norm)), wa, wb);
+      const std::uint64_t minus = pack2(-1.f, -1.f);
 #pragma unroll
-  for (int i = 0; i < kAppendHeads; ++i) {
-    const int head = head0 + i;
-    if (head >= heads) break;
-    if (head >= a.q_heads + a.c.kv_heads) {
-      if (page >= 0) {
-        T* v = static_cast<T*>(a.c.v) + paged_row(a.c, page, head - a.q_heads - a.c.kv_heads, slot) + lane * 8;
-        *reinterpret_cast<uint4*>(v) = raw[i];
-      }
-      continue;
+      for (int i = 0; i < 2; ++i) ac[i] = mul2(wa[i], cs[i]), as[i] = mul2(wa[i], sn[i]), bc[i] = mul2(wb[i], cs[i]), bs[i] = mul2(mul2(wb[i], sn[i]), minus);
     }
-    const bool is_q = head < a.q_heads;
-    float x[8];
-    load8<T>(raw[i], x);
-    if (a.q_norm != nullptr) {
-      float sum = 0.f;
+    for (; from < to; from += kAppendHeads) {
+      take(min(from + kAppendHeads, to));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
+      for (int i = 0; i < kAppendHeads; ++i) {
+        if (from + i >= to) break;
+        std::uint64_t x[2], y[2], u[2], v[2];
+        Pieces<kInterleaved>::template split<T>(raw[i], x, y);
+        float r = 1.0f;
+        if (norm != nullptr) {
+          float even, odd;
+          unpack2(fma2(y[1], y[1], fma2(x[1], x[1], fma2(y[0], y[0], mul2(x[0], x[0])))), even, odd);
+          float sum = even + odd;
 #pragma unroll
-      for (int m = kLanes / 2; m > 0; m /= 2) sum += __shfl_xor_sync(group_mask, sum, m);
-      const float r = rsqrtf(sum * (1.0f / D) + a.eps);
-      float w[8];
-      load8<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(is_q ? a.q_norm : a.k_norm) + lane * 8)), w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = x[j] * r * w[j];
-    }
-    if (a.half > 0) {
-      if constexpr (kInterleaved) {
-        if (turns) {
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            const float u = x[j], v = x[j + 1];
-            x[j] = u * cs[j] - v * sn[j];
-            x[j + 1] = v * cs[j] + u * sn[j];
-          }
+          for (int m = kLanes / 2; m > 0; m /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+          r = rsqrtf(sum * (1.0f / D) + a.eps);
         }
-      } else {
+        const std::uint64_t r2 = pack2(r, r);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float other = __shfl_sync(group_mask, x[j], partner, kLanes);
-          if (turns) x[j] = lane < away ? x[j] * cs[j] - other * sn[j] : x[j] * cs[j] + other * sn[j];
+        for (int j = 0; j < 2; ++j) {
+          u[j] = mul2(x[j], ac[j]), v[j] = mul2(y[j], bc[j]);
+          if (turns) u[j] = fma2(y[j], bs[j], u[j]), v[j] = fma2(x[j], as[j], v[j]);
+          u[j] = mul2(u[j], r2), v[j] = mul2(v[j], r2);
+        }
+        if (out != nullptr) {
+          pieces.store(out, Pieces<kInterleaved>::template merge<T>(u, v));
+          out += step;
         }
       }
     }
-    if (is_q) {
-      *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + token * a.q_row + head * a.q_head + lane * 8) = store8<T>(x);
-    } else if (page >= 0) {
-      *reinterpret_cast<uint4*>(static_cast<T*>(a.c.k) + paged_row(a.c, page, head - a.q_heads, slot) + lane * 8) = store8<T>(x);
+  };
+  const int q_end = min(a.q_heads, last);
+  if (head0 < q_end) rotate(head0, q_end, a.q_norm, stores ? static_cast<T*>(a.q_out) + token * a.q_row + head0 * a.q_head : nullptr, a.q_head);
+  const int k_begin = max(head0, a.q_heads), k_end = min(a.q_heads + a.c.kv_heads, last);
+  if (k_begin < k_end) {
+    T* out = page < 0 ? nullptr : static_cast<T*>(a.c.k) + paged_row(a.c, page, k_begin - a.q_heads, slot);
+    rotate(k_begin, k_end, a.k_norm, out, a.c.head_stride);
+  }
+  const int v_begin = max(head0, a.q_heads + a.c.kv_heads), v_end = min(a.q_heads + 2 * a.c.kv_heads, last);
+  if (v_begin < v_end && page >= 0) {
+    T* out = static_cast<T*>(a.c.v) + paged_row(a.c, page, v_begin - a.q_heads - a.c.kv_heads, slot);
+    for (int from = v_begin; from < v_end; from += kAppendHeads) {
+      take(min(from + kAppendHeads, v_end));
+#pragma unroll
+      for (int i = 0; i < kAppendHeads; ++i) {
+        if (from + i >= v_end) break;
+        pieces.store(out, raw[i]);
+        out += a.c.head_stride;
+      }
     }
   }
 }
@@ -168,10 +231,11 @@ struct EvictArgs {
   int sinks, recent, budget;
 };
 
-constexpr int kSelectThreads = 512;
-constexpr int kSelectItems = 16;  // consecutive slots of a thread in a round
+constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32;
+constexpr int kSelectItems = 16;  // slots of a thread in a round: a warp has 32 * kSelectItems neighbouring ones, a lane every 32nd
 constexpr int kSelectRound = kSelectThreads * kSelectItems;
 constexpr int kMostSelectCtas = 8;
+constexpr int kBins = 2048, kThreadBins = kBins / kSelectThreads;
 
 // The order of the weights as the order of unsigned numbers: -0 counts as 0, NaN comes below everything.
 __device__ __forceinline__ unsigned weight_key(float w) {
@@ -179,21 +243,48 @@ __device__ __forceinline__ unsigned weight_key(float w) {
   const unsigned u = __float_as_uint(w + 0.0f);
   return (u & 0x80000000u) != 0u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ unsigned ld_cluster_u32(std::uint32_t addr) {
-  unsigned v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ uint4 ld_cluster_v4(std::uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ uint2 ld_cluster_v2(std::uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+// Sum of `v` over the CTA's threads before this one, and over all of them. Two barriers; s_warp is free again behind the next one.
+__device__ __forceinline__ unsigned sum_before(unsigned v, unsigned (&s_warp)[kSelectWarps], int warp, int lane, unsigned& total) {
+  unsigned upto = v;
+#pragma unroll
+  for (int m = 1; m < 32; m *= 2) {
+    const unsigned o = __shfl_up_sync(0xffffffffu, upto, m);
+    if (lane >= m) upto += o;
+  }
+  __syncthreads();
+  if (lane == 31) s_warp[warp] = upto;
+  __syncthreads();
+  unsigned before = upto - v;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < kSelectWarps; ++i) {
+    const unsigned n = s_warp[i];
+    before += i < warp ? n : 0u;
+    total += n;
+  }
+  return before;
+}
 
-// A cluster per (sequence, key head), each CTA with its share of the slots between the first and the last ones. The weight of
-// the last slot that stays is found bit by bit from the top (8 at a time, a histogram over the cluster for each byte); then
-// every CTA counts what stays in its share, and writes it behind what the CTAs before it keep.
+// A cluster per (sequence, key head), each CTA with its share of the slots between the first and the last ones, which stays in registers
+// (up to kSelectRound slots a CTA: 65536 a head; more are read again for every pass). The weight of the last slot that stays is found from the top
+// bits down, 11, 11 and 10 of them: a histogram over the cluster, and the bin in which the running count from above reaches what
+// may stay. (Bytes put the weights of a cache into a dozen bins of the first histogram, and a warp's additions to one word wait for one another:
+// 16384 slots took 25 us.) Then every CTA counts what stays of its share, and writes it behind what the CTAs before it keep.
 __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs a) {
   dependents_may_start();
-  __shared__ unsigned s_hist[2][256];
-  __shared__ unsigned s_total[256];
-  __shared__ unsigned s_warp[2][kSelectThreads / 32];
-  __shared__ unsigned s_count[2];
+  __shared__ __align__(16) unsigned s_hist[2][kBins];
+  __shared__ unsigned s_warp[kSelectWarps];
+  __shared__ __align__(8) uint2 s_count;
   __shared__ unsigned s_pick[2];
   const int ctas = gridDim.x, rank = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
@@ -217,106 +308,109 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs 
   }
   const int room = a.budget - a.sinks - a.recent;
   if (room == 0) return;
-  // This CTA's share, a multiple of 4 slots.
-  const int middle = len - a.recent - a.sinks;
-  const int share = ((middle + ctas - 1) / ctas + 3) / 4 * 4;
+  const int middle = len - a.recent - a.sinks, share = (middle + ctas - 1) / ctas;
   const int begin = a.sinks + min(middle, rank * share), end = a.sinks + min(middle, (rank + 1) * share);
+  const int rounds = max(1, (share + kSelectRound - 1) / kSelectRound);
+
+  float mine[kSelectItems];
+  const auto slot_of = [&](int round, int i) { return begin + round * kSelectRound + (warp * kSelectItems + i) * 32 + lane; };
+  const auto load = [&](int round) {
+#pragma unroll
+    for (int i = 0; i < kSelectItems; ++i) {
+      const int slot = slot_of(round, i);
+      mine[i] = slot < end ? w[slot] : 0.f;
+    }
+  };
+  if (rounds == 1) load(0);
 
   unsigned prefix = 0, wanted = static_cast<unsigned>(room);  // of the slots whose upper bits are `prefix`, how many stay
-  for (int pass = 0; pass < 4; ++pass) {
-    const int shift = 24 - 8 * pass;
-    unsigned(&hist)[256] = s_hist[pass & 1];
-    for (int i = tid; i < 256; i += kSelectThreads) hist[i] = 0;
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, above_shift = pass == 0 ? 32 : pass == 1 ? 21 : 10;
+    const unsigned mask = pass == 2 ? 1023u : 2047u;
+    unsigned(&hist)[kBins] = s_hist[pass & 1];
+    *reinterpret_cast<uint4*>(&hist[tid * kThreadBins]) = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (int i = begin + tid; i < end; i += kSelectThreads) {
-      const unsigned key = weight_key(w[i]);
-      if (pass == 0 || key >> (shift + 8) == prefix) atomicAdd(&hist[key >> shift & 255u], 1u);
+    for (int round = 0; round < rounds; ++round) {
+      if (rounds > 1) load(round);
+#pragma unroll
+      for (int i = 0; i < kSelectItems; ++i) {
+        const unsigned key = weight_key(mine[i]);
+        if (slot_of(round, i) < end && (pass == 0 || key >> above_shift == prefix)) atomicAdd(&hist[key >> shift & mask], 1u);
+      }
     }
     // (The other half of s_hist is cleared for the next pass only after this barrier: by then every CTA has read it.)
     cluster_sync_all();
-    if (tid < 256) {
-      unsigned sum = 0;
-      for (int c = 0; c < ctas; ++c) sum += ld_cluster_u32(map_to_cta(smem_u32(&hist[tid]), c));
-      s_total[tid] = sum;
+    uint4 bins = make_uint4(0, 0, 0, 0);  // this thread's bins, the largest ones thread 0's
+    const int bin0 = kBins - (tid + 1) * kThreadBins;
+    for (int c = 0; c < ctas; ++c) {
+      const uint4 x = ld_cluster_v4(map_to_cta(smem_u32(&hist[bin0]), c));
+      bins.x += x.x, bins.y += x.y, bins.z += x.z, bins.w += x.w;
+    }
+    unsigned total;
+    unsigned before = sum_before(bins.x + bins.y + bins.z + bins.w, s_warp, warp, lane, total);
+    const unsigned n[kThreadBins] = {bins.w, bins.z, bins.y, bins.x};
+#pragma unroll
+    for (int i = 0; i < kThreadBins; ++i) {
+      if (before < wanted && before + n[i] >= wanted) s_pick[0] = static_cast<unsigned>(bin0 + kThreadBins - 1 - i), s_pick[1] = wanted - before;
+      before += n[i];
     }
     __syncthreads();
-    if (warp == 0) {  // from the largest byte down: where the running count reaches what is wanted
-      unsigned mine = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mine += s_total[255 - lane * 8 - i];
-      unsigned upto = mine;
-#pragma unroll
-      for (int m = 1; m < 32; m *= 2) {
-        const unsigned o = __shfl_up_sync(0xffffffffu, upto, m);
-        if (lane >= m) upto += o;
-      }
-      unsigned before = upto - mine;
-      if (before < wanted && upto >= wanted) {
-        for (int i = 0; i < 8; ++i) {
-          const unsigned n = s_total[255 - lane * 8 - i];
-          if (before + n >= wanted) {
-            s_pick[0] = static_cast<unsigned>(255 - lane * 8 - i), s_pick[1] = wanted - before;
-            break;
-          }
-          before += n;
-        }
-      }
-    }
-    __syncthreads();
-    prefix = prefix << 8 | s_pick[0];
+    prefix = prefix << (pass == 2 ? 10 : 11) | s_pick[0];
     wanted = s_pick[1];
   }
 
-  // `prefix` is the key of the last one that stays, and `wanted` of its equals stay. Counts of this CTA's share: above, equal.
-  unsigned above = 0, equal = 0;
-  for (int i = begin + tid; i < end; i += kSelectThreads) {
-    const unsigned key = weight_key(w[i]);
-    above += key > prefix, equal += key == prefix;
-  }
-  if (tid < 2) s_count[tid] = 0;
-  __syncthreads();
-  above = __reduce_add_sync(0xffffffffu, above), equal = __reduce_add_sync(0xffffffffu, equal);
-  if (lane == 0) atomicAdd(&s_count[0], above), atomicAdd(&s_count[1], equal);
-  cluster_sync_all();
+  // `prefix` is the key of the last one that stays, and `wanted` of its equals stay. What lies above it and level with it in the shares ahead.
   unsigned above_before = 0, equal_before = 0;
-  for (int c = 0; c < rank; ++c) {
-    above_before += ld_cluster_u32(map_to_cta(smem_u32(&s_count[0]), c));
-    equal_before += ld_cluster_u32(map_to_cta(smem_u32(&s_count[1]), c));
-  }
-  cluster_sync_all();  // nobody reads another CTA's shared memory from here on
-
-  for (int at = begin; at < end; at += kSelectRound) {
-    const int mine = at + tid * kSelectItems;
-    unsigned key[kSelectItems], n_above = 0, n_equal = 0;
+  if (ctas > 1) {
+    unsigned above = 0, equal = 0;
+    for (int round = 0; round < rounds; ++round) {
+      if (rounds > 1) load(round);
 #pragma unroll
-    for (int i = 0; i < kSelectItems; ++i) {
-      key[i] = mine + i < end ? weight_key(w[mine + i]) : 0u;
-      n_above += mine + i < end && key[i] > prefix, n_equal += mine + i < end && key[i] == prefix;
-    }
-    unsigned upto_above = n_above, upto_equal = n_equal;
-#pragma unroll
-    for (int m = 1; m < 32; m *= 2) {
-      const unsigned oa = __shfl_up_sync(0xffffffffu, upto_above, m), oe = __shfl_up_sync(0xffffffffu, upto_equal, m);
-      if (lane >= m) upto_above += oa, upto_equal += oe;
-    }
-    __syncthreads();  // (s_warp of the round before is read)
-    if (lane == 31) s_warp[0][warp] = upto_above, s_warp[1][warp] = upto_equal;
-    __syncthreads();
-    unsigned ra = above_before + upto_above - n_above, re = equal_before + upto_equal - n_equal;
-    for (int i = 0; i < kSelectThreads / 32; ++i) {
-      if (i < warp) ra += s_warp[0][i], re += s_warp[1][i];
-      above_before += s_warp[0][i], equal_before += s_warp[1][i];
-    }
-#pragma unroll
-    for (int i = 0; i < kSelectItems; ++i) {
-      if (mine + i >= end) break;
-      const bool up = key[i] > prefix, level = key[i] == prefix;
-      if (up || (level && re < wanted)) {
-        const unsigned to = static_cast<unsigned>(a.sinks) + ra + min(re, wanted);
-        kept[to] = mine + i;
-        if (w_out != nullptr) w_out[to] = w[mine + i];
+      for (int i = 0; i < kSelectItems; ++i) {
+        const unsigned key = weight_key(mine[i]);
+        const bool there = slot_of(round, i) < end;
+        above += there && key > prefix, equal += there && key == prefix;
       }
-      ra += up, re += level;
+    }
+    unsigned all_above, all_equal;
+    sum_before(above, s_warp, warp, lane, all_above);
+    sum_before(equal, s_warp, warp, lane, all_equal);
+    if (tid == 0) s_count = make_uint2(all_above, all_equal);
+    cluster_sync_all();
+    for (int c = 0; c < rank; ++c) {
+      const uint2 x = ld_cluster_v2(map_to_cta(smem_u32(&s_count), c));
+      above_before += x.x, equal_before += x.y;
+    }
+    cluster_sync_all();  // nobody reads another CTA's shared memory from here on
+  }
+
+  const unsigned lower = (1u << lane) - 1u;
+  for (int round = 0; round < rounds; ++round) {
+    if (rounds > 1) load(round);
+    unsigned above[kSelectItems], equal[kSelectItems], n_above = 0, n_equal = 0;  // of 32 slots side by side, a bit each
+#pragma unroll
+    for (int i = 0; i < kSelectItems; ++i) {
+      const unsigned key = weight_key(mine[i]);
+      const bool there = slot_of(round, i) < end;
+      above[i] = __ballot_sync(0xffffffffu, there && key > prefix), equal[i] = __ballot_sync(0xffffffffu, there && key == prefix);
+      n_above += __popc(above[i]), n_equal += __popc(equal[i]);
+    }
+    // (A lane's share of its warp's counts, so that the sums over threads are those over warps.)
+    unsigned all_above, all_equal;
+    unsigned ra = sum_before(lane == 0 ? n_above : 0u, s_warp, warp, lane, all_above);
+    unsigned re = sum_before(lane == 0 ? n_equal : 0u, s_warp, warp, lane, all_equal);
+    ra = above_before + __shfl_sync(0xffffffffu, ra, 0), re = equal_before + __shfl_sync(0xffffffffu, re, 0);
+    above_before += all_above, equal_before += all_equal;
+#pragma unroll
+    for (int i = 0; i < kSelectItems; ++i) {
+      const unsigned mine_above = ra + __popc(above[i] & lower), mine_equal = re + __popc(equal[i] & lower);
+      if ((above[i] >> lane & 1u) != 0u || ((equal[i] >> lane & 1u) != 0u && mine_equal < wanted)) {
+        const unsigned to = static_cast<unsigned>(a.sinks) + mine_above + min(mine_equal, wanted);
+        kept[to] = slot_of(round, i);
+        if (w_out != nullptr) w_out[to] = mine[i];
+      }
+      ra += __popc(above[i]), re += __popc(equal[i]);
     }
   }
 }
@@ -360,7 +454,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictArgs a) {
 
 template <typename T, int D>
 int launch_append(const char* op, const AppendArgs& a, bool interleaved, cudaStream_t st) {
-  const std::int64_t units = a.tokens * a.chunks, per_block = kAppendThreads / (D / 8);
+  const std::int64_t units = a.padded * a.chunks, per_block = kAppendThreads / (D / 8);
   const auto kernel = interleaved ? append_kernel<T, D, true> : append_kernel<T, D, false>;
   return enqueue(op, kernel, dim3(static_cast<unsigned>((units + per_block - 1) / per_block)), kAppendThreads, 0, st, 1, a);
 }
@@ -464,8 +558,14 @@ int b2_qk_norm_rope_append(const b2_paged_cache* cache, const void* qkv, int64_t
   a.qkv = qkv, a.ld = ld, a.tokens = tokens, a.cu = cu_seqlens, a.positions = positions, a.q_norm = q_norm, a.k_norm = k_norm;
   a.rope = rope, a.rope_rows = rope_rows, a.q_out = q_out, a.q_row = q_row_stride, a.q_head = q_head_stride, a.eps = eps;
   a.q_heads = q_heads, a.half = rot_dim / 2;
-  a.chunks = static_cast<int>((heads + kAppendHeads - 1) / kAppendHeads);
-  if (tokens * a.chunks > INT_MAX) return fail_invalid(op, "too many tokens for one call");
+  // Few tokens: four heads to a group of lanes, so that the whole GPU works. From 16 tokens per SM on all of a token's heads, so that what
+  // a token needs is found once (32 / 8 heads of 128: 9000 tokens 47 us, with four heads 66; 4000 25 against 32; 2300 both 21; 1500 23
+  // against 14).
+  const bool whole = tokens >= 16 * static_cast<std::int64_t>(sm_count());
+  a.chunk_heads = whole ? static_cast<int>(heads) : kAppendHeads;
+  a.chunks = static_cast<int>((heads + a.chunk_heads - 1) / a.chunk_heads);
+  a.padded = (tokens + 3) / 4 * 4;
+  if (a.padded * a.chunks > INT_MAX) return fail_invalid(op, "too many tokens for one call");
   if (const int rc = paged_status_word(op, &a.c)) return rc;
   const bool wide = cache->head_dim == 128;
   if (cache->dtype == B2_DTYPE_BF16) {
