@@ -231,8 +231,8 @@ struct EvictArgs {
   int sinks, recent, budget;
 };
 
-constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32;
-constexpr int kSelectItems = 16;  // slots of a thread in a round: a warp has 32 * kSelectItems neighbouring ones, a lane every 32nd
+constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
+constexpr int kSelectItems = 8;  // most slots of a thread in a round: a warp has neighbouring ones, a lane every 32nd of them
 constexpr int kSelectRound = kSelectThreads * kSelectItems;
 constexpr int kMostSelectCtas = 8;
 constexpr int kBins = 2048, kThreadBins = kBins / kSelectThreads;
@@ -242,11 +242,6 @@ __device__ __forceinline__ unsigned weight_key(float w) {
   if (isnan(w)) return 0u;
   const unsigned u = __float_as_uint(w + 0.0f);
   return (u & 0x80000000u) != 0u ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ uint4 ld_cluster_v4(std::uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
 }
 __device__ __forceinline__ uint2 ld_cluster_v2(std::uint32_t addr) {
   uint2 v;
@@ -264,22 +259,24 @@ __device__ __forceinline__ unsigned sum_before(unsigned v, unsigned (&s_warp)[kS
   __syncthreads();
   if (lane == 31) s_warp[warp] = upto;
   __syncthreads();
-  unsigned before = upto - v;
-  total = 0;
+  const unsigned mine = lane < kSelectWarps ? s_warp[lane] : 0u;
+  unsigned warps = mine;  // of the warps up to this lane's
 #pragma unroll
-  for (int i = 0; i < kSelectWarps; ++i) {
-    const unsigned n = s_warp[i];
-    before += i < warp ? n : 0u;
-    total += n;
+  for (int m = 1; m < kSelectWarps; m *= 2) {
+    const unsigned o = __shfl_up_sync(0xffffffffu, warps, m);
+    if (lane >= m) warps += o;
   }
-  return before;
+  total = __shfl_sync(0xffffffffu, warps, kSelectWarps - 1);
+  return __shfl_sync(0xffffffffu, warps - mine, warp) + upto - v;
 }
 
-// A cluster per (sequence, key head), each CTA with its share of the slots between the first and the last ones, which stays in registers
-// (up to kSelectRound slots a CTA: 65536 a head; more are read again for every pass). The weight of the last slot that stays is found from the top
-// bits down, 11, 11 and 10 of them: a histogram over the cluster, and the bin in which the running count from above reaches what
-// may stay. (Bytes put the weights of a cache into a dozen bins of the first histogram, and a warp's additions to one word wait for one another:
-// 16384 slots took 25 us.) Then every CTA counts what stays of its share, and writes it behind what the CTAs before it keep.
+// A CTA per (sequence, key head), or a cluster of up to 8 where a head can have more than kSelectRound slots (16384 slots of 64 heads: 64 us for
+// the call with two CTAs a head, 66 with one of twice the slots a thread, 76 with four: what a cluster waits for is more than what it shares). A
+// CTA's share of the slots between the first and the last ones stays in registers (past 65536 slots a head it is read again for every pass).
+// The weight of the last slot that stays is found from the top bits down, 11, 11 and 10 of them: a histogram over the cluster, and the bin in
+// which the running count from above reaches what may stay. (Bytes put the weights of a cache into a dozen bins of the first
+// histogram, where a warp's additions to one word wait for one another.) Then every CTA counts what stays of its share, and
+// writes it behind what the CTAs before it keep. Bound by the latency of its dozen steps between barriers, not by the weights' bytes.
 __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs a) {
   dependents_may_start();
   __shared__ __align__(16) unsigned s_hist[2][kBins];
@@ -311,12 +308,14 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs 
   const int middle = len - a.recent - a.sinks, share = (middle + ctas - 1) / ctas;
   const int begin = a.sinks + min(middle, rank * share), end = a.sinks + min(middle, (rank + 1) * share);
   const int rounds = max(1, (share + kSelectRound - 1) / kSelectRound);
+  const int items = rounds > 1 ? kSelectItems : (share + kSelectThreads - 1) / kSelectThreads;  // of a thread in a round
 
   float mine[kSelectItems];
-  const auto slot_of = [&](int round, int i) { return begin + round * kSelectRound + (warp * kSelectItems + i) * 32 + lane; };
+  const auto slot_of = [&](int round, int i) { return begin + round * kSelectRound + (warp * items + i) * 32 + lane; };
   const auto load = [&](int round) {
 #pragma unroll
     for (int i = 0; i < kSelectItems; ++i) {
+      if (i >= items) break;
       const int slot = slot_of(round, i);
       mine[i] = slot < end ? w[slot] : 0.f;
     }
@@ -329,27 +328,34 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs 
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, above_shift = pass == 0 ? 32 : pass == 1 ? 21 : 10;
     const unsigned mask = pass == 2 ? 1023u : 2047u;
     unsigned(&hist)[kBins] = s_hist[pass & 1];
-    *reinterpret_cast<uint4*>(&hist[tid * kThreadBins]) = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint2*>(&hist[tid * kThreadBins]) = make_uint2(0, 0);
     __syncthreads();
     for (int round = 0; round < rounds; ++round) {
       if (rounds > 1) load(round);
 #pragma unroll
       for (int i = 0; i < kSelectItems; ++i) {
+        if (i >= items) break;
         const unsigned key = weight_key(mine[i]);
         if (slot_of(round, i) < end && (pass == 0 || key >> above_shift == prefix)) atomicAdd(&hist[key >> shift & mask], 1u);
       }
     }
     // (The other half of s_hist is cleared for the next pass only after this barrier: by then every CTA has read it.)
-    cluster_sync_all();
-    uint4 bins = make_uint4(0, 0, 0, 0);  // this thread's bins, the largest ones thread 0's
+    uint2 bins;  // this thread's bins, the largest ones thread 0's
     const int bin0 = kBins - (tid + 1) * kThreadBins;
-    for (int c = 0; c < ctas; ++c) {
-      const uint4 x = ld_cluster_v4(map_to_cta(smem_u32(&hist[bin0]), c));
-      bins.x += x.x, bins.y += x.y, bins.z += x.z, bins.w += x.w;
+    if (ctas == 1) {
+      __syncthreads();
+      bins = *reinterpret_cast<const uint2*>(&hist[bin0]);
+    } else {
+      cluster_sync_all();
+      bins = make_uint2(0, 0);
+      for (int c = 0; c < ctas; ++c) {
+        const uint2 x = ld_cluster_v2(map_to_cta(smem_u32(&hist[bin0]), c));
+        bins.x += x.x, bins.y += x.y;
+      }
     }
     unsigned total;
-    unsigned before = sum_before(bins.x + bins.y + bins.z + bins.w, s_warp, warp, lane, total);
-    const unsigned n[kThreadBins] = {bins.w, bins.z, bins.y, bins.x};
+    unsigned before = sum_before(bins.x + bins.y, s_warp, warp, lane, total);
+    const unsigned n[kThreadBins] = {bins.y, bins.x};
 #pragma unroll
     for (int i = 0; i < kThreadBins; ++i) {
       if (before < wanted && before + n[i] >= wanted) s_pick[0] = static_cast<unsigned>(bin0 + kThreadBins - 1 - i), s_pick[1] = wanted - before;
@@ -368,6 +374,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs 
       if (rounds > 1) load(round);
 #pragma unroll
       for (int i = 0; i < kSelectItems; ++i) {
+        if (i >= items) break;
         const unsigned key = weight_key(mine[i]);
         const bool there = slot_of(round, i) < end;
         above += there && key > prefix, equal += there && key == prefix;
@@ -388,13 +395,18 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs 
   const unsigned lower = (1u << lane) - 1u;
   for (int round = 0; round < rounds; ++round) {
     if (rounds > 1) load(round);
-    unsigned above[kSelectItems], equal[kSelectItems], n_above = 0, n_equal = 0;  // of 32 slots side by side, a bit each
-#pragma unroll
-    for (int i = 0; i < kSelectItems; ++i) {
+    // Of 32 slots side by side a bit each: above, level.
+    const auto compare = [&](int i, unsigned& above, unsigned& equal) {
       const unsigned key = weight_key(mine[i]);
       const bool there = slot_of(round, i) < end;
-      above[i] = __ballot_sync(0xffffffffu, there && key > prefix), equal[i] = __ballot_sync(0xffffffffu, there && key == prefix);
-      n_above += __popc(above[i]), n_equal += __popc(equal[i]);
+      above = __ballot_sync(0xffffffffu, there && key > prefix), equal = __ballot_sync(0xffffffffu, there && key == prefix);
+    };
+    unsigned n_above = 0, n_equal = 0, above, equal;
+#pragma unroll
+    for (int i = 0; i < kSelectItems; ++i) {
+      if (i >= items) break;
+      compare(i, above, equal);
+      n_above += __popc(above), n_equal += __popc(equal);
     }
     // (A lane's share of its warp's counts, so that the sums over threads are those over warps.)
     unsigned all_above, all_equal;
@@ -404,13 +416,15 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs 
     above_before += all_above, equal_before += all_equal;
 #pragma unroll
     for (int i = 0; i < kSelectItems; ++i) {
-      const unsigned mine_above = ra + __popc(above[i] & lower), mine_equal = re + __popc(equal[i] & lower);
-      if ((above[i] >> lane & 1u) != 0u || ((equal[i] >> lane & 1u) != 0u && mine_equal < wanted)) {
+      if (i >= items) break;
+      compare(i, above, equal);
+      const unsigned mine_above = ra + __popc(above & lower), mine_equal = re + __popc(equal & lower);
+      if ((above >> lane & 1u) != 0u || ((equal >> lane & 1u) != 0u && mine_equal < wanted)) {
         const unsigned to = static_cast<unsigned>(a.sinks) + mine_above + min(mine_equal, wanted);
         kept[to] = slot_of(round, i);
         if (w_out != nullptr) w_out[to] = mine[i];
       }
-      ra += __popc(above[i]), re += __popc(equal[i]);
+      ra += __popc(above), re += __popc(equal);
     }
   }
 }
