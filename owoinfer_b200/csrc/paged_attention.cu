@@ -28,7 +28,7 @@ struct PromptArgs {
 
 template <typename T, int D, int kTiles>
 struct Shape {
-  static constexpr int kThreads = 64 + 128 * kTiles;  // TMA warp, MMA warp, a softmax thread per query row
+  static constexpr int kThreads = 128 + 128 * kTiles;  // a warpgroup of TMA warp, MMA warp and two that sleep; a softmax thread per query row
   static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kStages = D == 128 ? 5 : 8;
   static constexpr int kSmem = kTileBytes * (kTiles + kStages) + 1024;  // Q, the ring of K and V tiles, alignment slack
@@ -145,7 +145,10 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     return !__any_sync(0xffffffffu, !ok);
   };
 
-  if (warp == 0) {
+  // 168 registers a thread (65536 over 384, in eights) become 208 for the softmax and 88 for the others.
+  if (warp < 4) {
+   if constexpr (kTiles == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+   if (warp == 0) {
     // Item 2 j is K of tile j, item 2 j + 1 its V. A lane per (box of a page's rows, part).
     constexpr int kParts = D / 64;
     const int box_rows = min(1 << a.c.page_shift, kTile), boxes = kTile / box_rows * kParts;
@@ -179,7 +182,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       page = next;
     }
     __syncwarp();
-  } else if (warp == 1) {
+   } else if (warp == 1) {
     // The whole warp walks the loop (uniform control flow, every lane takes the waits); one elected lane issues.
     constexpr int kFormat = kHalf ? 0 : 1;
     constexpr std::uint32_t idesc_qk = umma_idesc(/*f32*/ 1, kFormat, kFormat, 0, 0, kTile, kTile);
@@ -237,13 +240,15 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         __syncwarp();
       }
     }
+   }
   } else {
-    const int i = (warp - 2) / 4, quarter = warp & 3;  // a warp may touch TMEM lanes [32 (warp % 4), +32)
+    if constexpr (kTiles == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int i = (warp - 4) / 4, quarter = warp & 3;  // a warp may touch TMEM lanes [32 (warp % 4), +32)
     const int r_local = quarter * 32 + lane, row = row0 + i * kTile + r_local;
     const std::uint32_t lane_off = static_cast<std::uint32_t>(quarter * 32) << 16;
     const bool live = row < rows;
     // Q: 16 bytes a thread, a row's chunks side by side; zeros past the last row.
-    for (int at = static_cast<int>(threadIdx.x) - 64; at < kTiles * kTile * (D / 8); at += 128 * kTiles) {
+    for (int at = static_cast<int>(threadIdx.x) - 128; at < kTiles * kTile * (D / 8); at += 128 * kTiles) {
       const int r = at / (D / 8), c = at % (D / 8), of = row0 + r;
       uint4 v = make_uint4(0, 0, 0, 0);
       if (of < rows) {
@@ -337,14 +342,15 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         unpack2(sum_b, s2, s3);
         sum = (s0 + s1) + (s2 + s3);
       };
-      const auto any_pass = [&]() {
-        if (masked) pass(std::true_type{});
-        else pass(std::false_type{});
-      };
-      any_pass();
-      // Over the limit, or NaN (once: a row that has become NaN stays so).
-      const bool over = !(sum <= kLimit) && l == l;
-      if (__any_sync(0xffffffffu, over)) {
+      for (bool again = false;; again = true) {
+        if (masked) {
+          pass(std::true_type{});
+        } else {
+          pass(std::false_type{});
+        }
+        // Over the limit, or NaN (a row that has become NaN stays so).
+        const bool over = !(sum <= kLimit) && l == l;
+        if (again || !__any_sync(0xffffffffu, over)) break;
         const float top = tile_max();
         float alpha = 1.0f;
         if (over && top - kShift > m) {
@@ -359,8 +365,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
           tc_fence_after();
           rescale_o(alpha);
         }
-        any_pass();
       }
+      if (dead) break;
       l += sum;
       {
         const std::uint32_t(&lower)[32] = *reinterpret_cast<const std::uint32_t(*)[32]>(&pw[0]);
