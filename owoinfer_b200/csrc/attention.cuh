@@ -27,6 +27,20 @@ __device__ __forceinline__ bool wait_bar(std::uint32_t bar, std::uint32_t parity
   }
 }
 
+// The same for a whole converged warp with one answer, in as little code as that takes.
+__device__ __forceinline__ bool warp_wait_bar(std::uint32_t bar, std::uint32_t parity, volatile int* abort_word) {
+  if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
+  const std::uint64_t t0 = global_ns();
+#pragma unroll 1
+  while (!__all_sync(0xffffffffu, mbar_try_wait_hint(bar, parity))) {
+    if (__any_sync(0xffffffffu, *abort_word != 0 || global_ns() - t0 > 200000000ull)) {
+      *abort_word = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
 // The same for a role with slack (the TMA and MMA warps share their scheduler with softmax warps): sleeps between tests so
 // that waiting costs next to no issue slots.
 template <int kSleepNs>
@@ -107,11 +121,49 @@ __device__ __forceinline__ void umma_f16_ts(std::uint32_t d_tmem, std::uint32_t 
       ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// Both for a CTA pair (see umma_i8_pair): 128 rows of A and of D in each CTA, half of B's N in each; issued by the pair's leader only.
+__device__ __forceinline__ void umma_f16_pair(std::uint32_t d_tmem, std::uint64_t a_desc, std::uint64_t b_desc,
+                                              std::uint32_t idesc, std::uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts_pair(std::uint32_t d_tmem, std::uint32_t a_tmem, std::uint64_t b_desc,
+                                                 std::uint32_t idesc, std::uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrive on an mbarrier of a CTA of the cluster for what tcgen05 fences order, tensor memory that is read or written: ordinary
+// memory goes along at CTA scope only. (With release.cluster every such arrival waits some 900 clocks for the warp's other accesses.)
+__device__ __forceinline__ void mbar_arrive_tensor(std::uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // 4-D tiled TMA load global -> shared, completion on an mbarrier of this CTA.
 __device__ __forceinline__ void tma_load_4d(std::uint32_t dst, const CUtensorMap* map, std::uint32_t bar, int c0, int c1, int c2, int c3) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
       ::"r"(dst), "l"(reinterpret_cast<std::uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(std::uint32_t dst, const CUtensorMap* map, std::uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<std::uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+// The same with completion on an mbarrier that may live in the peer CTA of the pair (shared::cluster address).
+__device__ __forceinline__ void tma_load_4d_pair(std::uint32_t dst, const CUtensorMap* map, std::uint32_t bar_cluster_addr, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<std::uint64_t>(map)), "r"(bar_cluster_addr), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
 __device__ __forceinline__ uint4 ld_shared(std::uint32_t addr) {

@@ -35,9 +35,11 @@ int check_paged_cache(const char* op, const b2_paged_cache* c, PagedArgs* a);
 int paged_status_word(const char* op, PagedArgs* a);
 // Where a call may write or read rows of `row` elements: 16-byte aligned, strides in multiples of 8 elements.
 inline bool rows_ok(const void* p, std::int64_t row, std::int64_t head) { return p != nullptr && aligned_to(p, 16) && row % 8 == 0 && head % 8 == 0; }
-// cuTensorMapEncodeTiled for the cache's keys or values, [pages, heads, rows, head_dim]: boxes of box_rows rows of 64 elements,
-// 128-byte swizzle. Returns false (and sets the last error) on failure.
-bool make_tensor_map_pages(CUtensorMap* map, const b2_paged_cache* c, bool values, int box_rows, const char* op);
+// cuTensorMapEncodeTiled for the cache's keys or values, [pages, heads, rows, head_dim]: boxes of box_rows rows of box_columns
+// elements, 64 with the 128-byte swizzle or 32 with the 64-byte one. Returns false (and sets the last error) on failure.
+bool make_tensor_map_pages(CUtensorMap* map, const b2_paged_cache* c, bool values, int box_rows, int box_columns, const char* op);
+// The same for a view [tokens, heads, head_dim] of 16-bit elements: boxes of 64 elements of box_heads heads of box_tokens tokens.
+bool make_tensor_map_rows(CUtensorMap* map, const b2_view3* v, int head_dim, int box_heads, int box_tokens, const char* op);
 // A window that reaches every slot is none; sinks past the last slot are all slots.
 int check_window(const char* op, const PagedArgs& c, int* window, int* sinks);
 

@@ -519,7 +519,9 @@ int paged_status_word(const char* op, PagedArgs* a) {
   return B2_OK;
 }
 
-bool make_tensor_map_pages(CUtensorMap* map, const b2_paged_cache* c, bool values, int box_rows, const char* op) {
+namespace {
+// A map of 16-bit elements: sizes and boxes from the inner dimension out, strides of the outer ones in elements.
+bool encode_map(CUtensorMap* map, const void* base, int rank, const std::int64_t* sizes, const std::int64_t* strides, const int* box, bool narrow, const char* op) {
   static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -533,16 +535,29 @@ bool make_tensor_map_pages(CUtensorMap* map, const b2_paged_cache* c, bool value
     fail_status(B2_ERR_CUDA, op, "cuTensorMapEncodeTiled is not available from this driver");
     return false;
   }
-  const auto u = [](std::int64_t v) { return static_cast<cuuint64_t>(v); };
-  const cuuint64_t dims[4] = {u(c->head_dim), u(c->page_size), u(c->kv_heads), u(c->num_pages)};
-  const cuuint64_t strides[3] = {u(c->row_stride) * 2, u(c->head_stride) * 2, u(c->page_stride) * 2};
-  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1}, elem[4] = {1, 1, 1, 1};
-  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, values ? c->v : c->k, dims, strides, box, elem,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  cuuint64_t dims[4], bytes[3];
+  cuuint32_t boxes[4], elem[4];
+  for (int i = 0; i < rank; ++i) dims[i] = static_cast<cuuint64_t>(sizes[i]), boxes[i] = static_cast<cuuint32_t>(box[i]), elem[i] = 1;
+  for (int i = 0; i + 1 < rank; ++i) bytes[i] = static_cast<cuuint64_t>(strides[i]) * 2;
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, bytes, boxes, elem,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) return true;
-  fail_status(B2_ERR_CUDA, op, "cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(r)) + " for the pages' pool");
+  fail_status(B2_ERR_CUDA, op, "cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(r)));
   return false;
+}
+}  // namespace
+
+bool make_tensor_map_pages(CUtensorMap* map, const b2_paged_cache* c, bool values, int box_rows, int box_columns, const char* op) {
+  const std::int64_t sizes[4] = {c->head_dim, c->page_size, c->kv_heads, c->num_pages}, strides[3] = {c->row_stride, c->head_stride, c->page_stride};
+  const int box[4] = {box_columns, box_rows, 1, 1};
+  return encode_map(map, values ? c->v : c->k, 4, sizes, strides, box, box_columns == 32, op);
+}
+
+bool make_tensor_map_rows(CUtensorMap* map, const b2_view3* v, int head_dim, int box_heads, int box_tokens, const char* op) {
+  const std::int64_t sizes[3] = {head_dim, v->heads, v->tokens}, strides[2] = {v->head_stride, v->row_stride};
+  const int box[3] = {64, box_heads, box_tokens};
+  return encode_map(map, v->data, 3, sizes, strides, box, false, op);
 }
 
 }  // namespace b2

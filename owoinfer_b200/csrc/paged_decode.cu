@@ -548,7 +548,7 @@ int b2_attention_paged_decode(const b2_paged_cache* cache, const b2_view3* q, co
   if (const int rc = paged_status_word(op, &a.c)) return rc;
   if (cache->num_pages == 0) return fail_invalid(op, "the pool has no pages");
   CUtensorMap map_k, map_v;
-  if (!make_tensor_map_pages(&map_k, cache, false, kKeys, op) || !make_tensor_map_pages(&map_v, cache, true, kKeys, op)) return B2_ERR_CUDA;
+  if (!make_tensor_map_pages(&map_k, cache, false, kKeys, 64, op) || !make_tensor_map_pages(&map_v, cache, true, kKeys, 64, op)) return B2_ERR_CUDA;
   const bool wide = cache->head_dim == 128;
   if (cache->dtype == B2_DTYPE_BF16) {
     using T = __nv_bfloat16;
