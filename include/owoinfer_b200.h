@@ -711,9 +711,12 @@ int b2_qk_norm_rope_append(const b2_paged_cache* cache, const void* qkv, int64_t
  * j <= p). out = softmax(scale * q k^T) v; lse (fp32 [tokens, q_heads], or NULL) = log sum exp(scale * q k^T). A token that
  * sees nothing (a cache shorter than the call's tokens) gets zeros and -infinity. q, out: views of one dtype [tokens,
  * q_heads, head_dim]; max_q: no sequence has more tokens in the call. Keys and values of slots that a token does not see do
- * not reach its output, NaN and infinities included. */
+ * not reach its output, NaN and infinities included.
+ * workspace: b2_attention_paged_workspace_bytes() of the same arguments, 256-byte aligned (few tokens over a long cache: parts of the
+ * keys are worked on apart and joined; 256 where none is needed, and then NULL will do). Nothing is kept in it. */
+size_t b2_attention_paged_workspace_bytes(const b2_paged_cache* cache, int64_t tokens, int q_heads, int max_q, int window, int sinks);
 int b2_attention_paged(const b2_paged_cache* cache, const b2_view3* q, const b2_view3* out, float* lse, const int32_t* cu_seqlens,
-                       int max_q, float scale, int window, int sinks, void* stream);
+                       int max_q, float scale, int window, int sinks, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The same for one token per sequence (token b of q and out is sequence b's newest, at slot seq_len - 1), the cache's length
  * split over the GPU and joined. With weights_out != NULL the attention each slot got is added up besides:

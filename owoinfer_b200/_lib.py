@@ -24,7 +24,7 @@ EXPORTS = [
     "b2_dit_file_open_expanded", "b2_silu_bf16", "b2_time_modulation_bf16_workspace_bytes", "b2_time_modulation_bf16",
     "b2_dit_graphs_create", "b2_dit_graphs_clear", "b2_dit_graphs_destroy", "b2_dit_graphs_stats", "b2_dit_forward_graphed",
     "b2_dit_file_open", "b2_dit_file_get_info", "b2_dit_file_model", "b2_dit_file_time_embedding", "b2_dit_file_time_mlp_bf16", "b2_dit_file_close",
-    "b2_qk_norm_rope_append", "b2_attention_paged", "b2_attention_paged_decode_workspace_bytes", "b2_attention_paged_decode",
+    "b2_qk_norm_rope_append", "b2_attention_paged", "b2_attention_paged_workspace_bytes", "b2_attention_paged_decode_workspace_bytes", "b2_attention_paged_decode",
     "b2_kv_evict", "b2_paged_cache_status",
 ]
 
@@ -186,7 +186,9 @@ def lib() -> C.CDLL:
         l.b2_block_quant_sp_workspace_bytes.argtypes = [C.POINTER(SpRun), C.c_int]
         cache, view, p, i, n = C.POINTER(PagedCache), C.POINTER(View3), C.c_void_p, C.c_int, C.c_int64
         l.b2_qk_norm_rope_append.argtypes = [cache, p, n, n, i, p, p, p, p, C.c_float, p, n, i, i, p, n, n, p]
-        l.b2_attention_paged.argtypes = [cache, view, view, p, p, i, C.c_float, i, i, p]
+        l.b2_attention_paged_workspace_bytes.restype = C.c_size_t
+        l.b2_attention_paged_workspace_bytes.argtypes = [cache, n, i, i, i, i]
+        l.b2_attention_paged.argtypes = [cache, view, view, p, p, i, C.c_float, i, i, p, C.c_size_t, p]
         l.b2_attention_paged_decode_workspace_bytes.restype = C.c_size_t
         l.b2_attention_paged_decode_workspace_bytes.argtypes = [cache, i, i, i, i, i]
         l.b2_attention_paged_decode.argtypes = [cache, view, view, p, i, C.c_float, i, i, p, p, n, p, C.c_size_t, p]

@@ -25,7 +25,10 @@ struct PromptArgs {
   float scale_log2;  // scale * log2(e)
   int window, sinks;
   int q_tma;         // a box of the map of q is whole tokens (the group divides 128)
-  int tiles, works;  // 256-row tiles of the longest sequence; times sequences and key heads
+  int tiles, splits, works;  // 256-row tiles of the longest sequence; parts of each one's keys; all of them, for all sequences and key heads
+  // Of a part, by [part, token, query head]: maximum and sum; O before the division.
+  float2* part_ml;
+  float* part_o;
 };
 
 template <int D>
@@ -107,9 +110,10 @@ struct __align__(16) Work {
   int h, b, first_token, n, len;
   int row0, row_last;  // rows of the sequence: (token, query head of the group)
   int p_lo, p_hi;      // slots of the first and the last token
-  int from, sink_tiles, count;  // count 0: no row sees a key
+  int from, sink_tiles, part, first_tile, count;  // a part has some of the key tiles; count 0: none
   __device__ __forceinline__ void set(const PromptArgs& a, int id, int first, int tokens, int slots) {
     const int heads = a.c.kv_heads;
+    part = id % a.splits, id /= a.splits;
     h = id % heads, b = id / heads % a.c.batch;
     first_token = first, n = tokens, len = slots;
     row0 = (a.tiles - 1 - id / heads / a.c.batch) * (2 * kTile);
@@ -117,9 +121,13 @@ struct __align__(16) Work {
     p_lo = len - n + row0 / a.group, p_hi = len - n + row_last / a.group;
     from = a.window > 0 && max(p_lo, 0) - a.window + 1 > 0 ? (max(p_lo, 0) - a.window + 1) / kTile : 0;
     sink_tiles = min((min(a.sinks, p_hi + 1) + kTile - 1) / kTile, from);
-    count = p_hi < 0 ? 0 : sink_tiles + p_hi / kTile + 1 - from;
+    const long long all = p_hi < 0 ? 0 : sink_tiles + p_hi / kTile + 1 - from;
+    first_tile = static_cast<int>(part * all / a.splits), count = static_cast<int>((part + 1) * all / a.splits) - first_tile;
   }
-  __device__ __forceinline__ int slot(int j) const { return (j < sink_tiles ? j : j - sink_tiles + from) * kTile; }
+  __device__ __forceinline__ int slot(int j) const {
+    j += first_tile;
+    return (j < sink_tiles ? j : j - sink_tiles + from) * kTile;
+  }
   // Whether every row from slot lo to slot hi sees all of a tile.
   __device__ __forceinline__ static bool all_seen(const PromptArgs& a, int slot0, int lo, int hi) {
     return slot0 + kTile - 1 <= lo && (a.window == 0 || slot0 + kTile <= a.sinks || slot0 > hi - a.window);
@@ -145,14 +153,14 @@ struct Walk {
       bool mine = mine_id < a.works;
       if (mine) {
         id = static_cast<int>(mine_id);
-        const int b = id / a.c.kv_heads % a.c.batch;
+        const int tile_id = id / a.splits / a.c.kv_heads, b = tile_id % a.c.batch;
         paged_tokens(a.c, a.cu, b, a.tokens, first, n);
         if (n > a.max_q) {
           atomicOr(a.c.status, kPagedBadTokens);
           n = a.max_q;
         }
         len = paged_len(a.c, b);
-        mine = (a.tiles - 1 - id / a.c.kv_heads / a.c.batch) * (2 * kTile) < n * a.group;
+        mine = (a.tiles - 1 - tile_id / a.c.batch) * (2 * kTile) < n * a.group;
       }
       left = __ballot_sync(0xffffffffu, mine);
       round += 32;
@@ -204,8 +212,8 @@ struct Tiles {
 
 // What infinities and NaN of V that some row does not see did not reach (see the V warp), for one row that has been stored: channels
 // [from, to) of `out`.
-template <typename T>
-__device__ __forceinline__ void add_nonfinite(const PromptArgs& a, const Work& w, int p, T* out, int from, int to) {
+template <typename T, typename Out>
+__device__ __forceinline__ void add_nonfinite(const PromptArgs& a, const Work& w, int p, Out* out, int from, int to) {
 #pragma unroll 1
   for (int j = 0; j < w.count; ++j) {
     const int slot0 = w.slot(j);
@@ -219,7 +227,7 @@ __device__ __forceinline__ void add_nonfinite(const PromptArgs& a, const Work& w
 #pragma unroll 1
       for (int d = from; d < to; ++d) {
         const float x = to_float(v[d]);
-        if (!isfinite(x)) out[d] = static_cast<T>(to_float(out[d]) + x);
+        if (!isfinite(x)) out[d] = static_cast<Out>(static_cast<float>(out[d]) + x);
       }
     }
   }
@@ -482,11 +490,15 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       bool more = has_work;
       for (int at = 0;; ++at) {
         for (; more && w.count == 0; more = walk.next(a, lane, w)) {
-          // Nothing to see for any row: their zeros, and no place in the list.
+          // Nothing to see for any row: their zeros (or an empty part), and no place in the list.
           for (int i = lane; i < kTile * kChunks; i += 32) {
             const int row = w.row0 + static_cast<int>(rank) * kTile + i / kChunks, token = row / a.group;
             if (row > w.row_last) break;
             const int head = w.h * a.group + row - token * a.group;
+            if (a.splits > 1) {
+              if (i % kChunks == 0) a.part_ml[(w.part * a.tokens + w.first_token + token) * a.q_heads + head] = make_float2(-INFINITY, 0.f);
+              continue;
+            }
             *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<std::int64_t>(w.first_token + token) * a.o_row + head * a.o_head + i % kChunks * 8) = make_uint4(0, 0, 0, 0);
             if (i % kChunks == 0 && a.lse != nullptr) a.lse[static_cast<std::int64_t>(w.first_token + token) * a.q_heads + head] = -INFINITY;
           }
@@ -693,35 +705,50 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_tensor(at_leader(s_o_free));
-      // 32 channels of the warp's rows at a time through shared memory, so that four lanes store 64 bytes of a row: a lane storing its own row
-      // touches 32 lines an instruction, and the eight warps kept each other waiting for 4500 clocks a work.
-      {
-        std::uint32_t at = smem_u32(&s_out[warp - 4][0]);
-        const int sub = lane >> 2, piece = lane & 3;
+      // The warp's rows, 64 bytes of each at a time, through shared memory, so that four lanes store them: a lane storing its own row touches 32
+      // lines an instruction, and the eight warps kept each other waiting for 4500 clocks a work.
+      const std::uint32_t at = smem_u32(&s_out[warp - 4][0]);
+      const auto put = [&](int e, const uint4& v) { st_shared(at + lane * 64 + ((e ^ (lane >> 1 & 3)) << 4), v); };
+      const auto store = [&](void* row_at, int byte) {
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int of = (lane >> 2) + 8 * e;  // row of the warp
+          const std::uint64_t to = __shfl_sync(0xffffffffu, reinterpret_cast<std::uint64_t>(row_at), of);
+          const uint4 v = ld_shared(at + of * 64 + (((lane & 3) ^ (of >> 1 & 3)) << 4));
+          if (w.row0 + static_cast<int>(rank) * kTile + quarter * 32 + of <= w.row_last) *reinterpret_cast<uint4*>(reinterpret_cast<std::uint8_t*>(to) + byte + (lane & 3) * 16) = v;
+        }
+        __syncwarp();
+      };
+      if (__builtin_expect(a.splits > 1, 0)) {
+        const std::int64_t part_at = static_cast<std::int64_t>(w.part) * a.tokens * a.q_heads + lse_at;
+        float* const part_o = a.part_o + part_at * D;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) put(e, make_uint4(x[i * 16 + e * 4], x[i * 16 + e * 4 + 1], x[i * 16 + e * 4 + 2], x[i * 16 + e * 4 + 3]));
+          store(part_o, (group * (D / 2) + i * 16) * 4);
+        }
+        if (live) {
+          if (repair) add_nonfinite<T>(a, w, p, part_o, group * (D / 2), (group + 1) * (D / 2));
+          if (group == 0) a.part_ml[part_at] = make_float2(m, empty ? 0.f : l);
+        }
+      } else {
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
-          __syncwarp();
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float o[8];
 #pragma unroll
             for (int f = 0; f < 8; ++f) o[f] = __uint_as_float(x[i * 32 + e * 8 + f]) * inv;
-            st_shared(at + lane * 64 + ((e ^ (lane >> 1 & 3)) << 4), store8<T>(o));
+            put(e, store8<T>(o));
           }
-          __syncwarp();
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int of = sub + 8 * e;  // row of the warp
-            const std::uint64_t to = __shfl_sync(0xffffffffu, reinterpret_cast<std::uint64_t>(out), of);
-            const uint4 v = ld_shared(at + of * 64 + ((piece ^ (of >> 1 & 3)) << 4));
-            if (w.row0 + static_cast<int>(rank) * kTile + quarter * 32 + of <= w.row_last) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(to) + group * (D / 2) + i * 32 + piece * 8) = v;
-          }
+          store(out, (group * (D / 2) + i * 32) * 2);
         }
-        __syncwarp();
-      }
-      if (live) {
-        if (repair) add_nonfinite(a, w, p, out, group * (D / 2), (group + 1) * (D / 2));
-        if (group == 0 && a.lse != nullptr) a.lse[lse_at] = empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        if (live) {
+          if (repair) add_nonfinite<T>(a, w, p, out, group * (D / 2), (group + 1) * (D / 2));
+          if (group == 0 && a.lse != nullptr) a.lse[lse_at] = empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&s_left[place]));
@@ -744,6 +771,68 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   }
 }
 
+constexpr int kJoinWarps = 8;
+
+// The parts of a row's keys joined, a warp per row: blockIdx.x is (tile, sequence, key head), blockIdx.y its rows.
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kJoinWarps) prompt_join_kernel(const PromptArgs a) {
+  constexpr int kEach = D / 32;  // channels of a lane
+  const int lane = static_cast<int>(threadIdx.x) & 31, id = blockIdx.x, h = id % a.c.kv_heads, b = id / a.c.kv_heads % a.c.batch;
+  int first, n;  // (no kernel of the call writes cu_seqlens: read ahead of the wait)
+  paged_tokens(a.c, a.cu, b, a.tokens, first, n);
+  const int row = (a.tiles - 1 - id / a.c.kv_heads / a.c.batch) * (2 * kTile) + static_cast<int>(blockIdx.y) * kJoinWarps + static_cast<int>(threadIdx.x) / 32;
+  if (row >= min(n, a.max_q) * a.group) return;
+  const int token = first + row / a.group, head = h * a.group + row % a.group;
+  const std::int64_t at = static_cast<std::int64_t>(token) * a.q_heads + head, step = a.tokens * a.q_heads;
+  wait_for_predecessors();
+  float m = -INFINITY, l = 0.f, o[kEach] = {};
+#pragma unroll 4
+  for (int i = 0; i < a.splits; ++i) {
+    const float2 ml = a.part_ml[i * step + at];
+    if (ml.y == 0.f) continue;  // nothing seen
+    const float* part = a.part_o + (i * step + at) * D + lane * kEach;
+    const float top = fmaxf(m, ml.x), f = ex2(ml.x - top), keep = l == 0.f ? 0.f : ex2(m - top);
+    m = top, l = fmaf(f, ml.y, keep * l);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) o[e] = fmaf(f, part[e], keep * o[e]);
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  std::uint32_t packed[kEach / 2];
+#pragma unroll
+  for (int e = 0; e < kEach; e += 2) packed[e / 2] = pack16<T>(o[e] * inv, o[e + 1] * inv);
+  T* out = static_cast<T*>(a.out) + static_cast<std::int64_t>(token) * a.o_row + head * a.o_head + lane * kEach;
+  if constexpr (kEach == 4) {
+    *reinterpret_cast<uint2*>(out) = make_uint2(packed[0], packed[1]);
+  } else {
+    *reinterpret_cast<std::uint32_t*>(out) = packed[0];
+  }
+  if (lane == 0 && a.lse != nullptr) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// How many parts the keys of 256 rows are cut into: as many as there are pairs without a work, but of kShortestPart tiles each.
+// (509 tokens over 8192 slots, 14 / 2 heads of 64, 28 works for 74 pairs: 74 us in one part, 49 in two.)
+constexpr int kShortestPart = 4;
+struct PromptPlan {
+  int tiles, splits;
+  std::int64_t works;
+  std::size_t ml, total;
+};
+PromptPlan plan(const PagedArgs& c, std::int64_t tokens, int q_heads, int head_dim, int max_q, int window, int sinks) {
+  PromptPlan p{};
+  const std::int64_t tiles = (static_cast<std::int64_t>(max_q) * (q_heads / c.kv_heads) + 2 * kTile - 1) / (2 * kTile), works = tiles * c.batch * c.kv_heads;
+  std::int64_t keys = c.most;
+  if (window > 0) keys = std::min<std::int64_t>(keys, static_cast<std::int64_t>(window) + max_q + sinks);
+  const std::int64_t most = std::max<std::int64_t>(1, keys / (kTile * kShortestPart)), idle = std::max<std::int64_t>(1, sm_count() / 2 / std::max<std::int64_t>(1, works));
+  p.splits = static_cast<int>(std::min(most, idle));
+  p.tiles = static_cast<int>(std::min<std::int64_t>(tiles, INT_MAX)), p.works = works * p.splits;
+  if (p.splits > 1) {
+    const std::size_t rows = static_cast<std::size_t>(tokens) * q_heads * p.splits;
+    p.ml = (rows * sizeof(float2) + 255) / 256 * 256;
+    p.total = p.ml + rows * head_dim * sizeof(float);
+  }
+  return p;
+}
+
 template <typename T, int D>
 int launch(const char* op, const PromptArgs& a, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t st) {
   using S = Shape<D>;
@@ -752,9 +841,19 @@ int launch(const char* op, const PromptArgs& a, const CUtensorMap& map_q, const 
     cudaGetLastError();
     return fail_cuda(op, e);
   }
+  const LaunchChain chain(st);
   // As many pairs as fit at once, or as there are works.
   const unsigned pairs = static_cast<unsigned>(std::max(1, std::min(sm_count() / 2, a.works)));
-  return enqueue(op, kernel, dim3(2 * pairs), S::kThreads, S::kSmem, st, 2, map_q, map_k, map_v, a);
+  if (const int rc = enqueue(op, kernel, dim3(2 * pairs), S::kThreads, S::kSmem, st, 2, map_q, map_k, map_v, a)) return rc;
+  if (a.splits == 1) return B2_OK;
+  return enqueue(op, prompt_join_kernel<T, D>, dim3(static_cast<unsigned>(a.works / a.splits), 2 * kTile / kJoinWarps), 32 * kJoinWarps, 0, st, 1, a);
+}
+
+int check(const char* op, const b2_paged_cache* cache, PagedArgs* c, std::int64_t tokens, std::int64_t q_heads, int max_q, int* window, int* sinks) {
+  if (const int rc = check_paged_cache(op, cache, c)) return rc;
+  if (q_heads <= 0 || q_heads > 65535 || q_heads % cache->kv_heads != 0) return fail_invalid(op, "q must have a multiple of kv_heads heads, at most 65535");
+  if (tokens < 0 || tokens > INT_MAX || max_q < 0) return fail_invalid(op, "tokens and max_q must not be negative");
+  return check_window(op, *c, window, sinks);
 }
 
 }  // namespace
@@ -764,18 +863,22 @@ using namespace b2;
 
 extern "C" {
 
+size_t b2_attention_paged_workspace_bytes(const b2_paged_cache* cache, int64_t tokens, int q_heads, int max_q, int window, int sinks) {
+  PagedArgs c{};
+  if (check("attention_paged", cache, &c, tokens, q_heads, max_q, &window, &sinks) != B2_OK) return 0;
+  return std::max<std::size_t>(plan(c, tokens, q_heads, cache->head_dim, static_cast<int>(std::min<std::int64_t>(max_q, tokens)), window, sinks).total, 256);
+}
+
 int b2_attention_paged(const b2_paged_cache* cache, const b2_view3* q, const b2_view3* out, float* lse, const int32_t* cu_seqlens,
-                       int max_q, float scale, int window, int sinks, void* stream) {
+                       int max_q, float scale, int window, int sinks, void* workspace, size_t workspace_bytes, void* stream) {
   constexpr const char* op = "attention_paged";
   PromptArgs a{};
   if (q == nullptr || out == nullptr) return fail_invalid(op, "null q or out");
-  if (const int rc = check_paged_cache(op, cache, &a.c)) return rc;
-  if (q->heads <= 0 || q->heads > 65535 || q->heads % cache->kv_heads != 0) return fail_invalid(op, "q must have a multiple of kv_heads heads, at most 65535");
-  if (q->tokens < 0 || q->tokens > INT_MAX || out->tokens != q->tokens || out->heads != q->heads) return fail_invalid(op, "q and out must have the same tokens and heads");
+  if (const int rc = check(op, cache, &a.c, q->tokens, q->heads, max_q, &window, &sinks)) return rc;
+  if (out->tokens != q->tokens || out->heads != q->heads) return fail_invalid(op, "q and out must have the same tokens and heads");
   if (!std::isfinite(scale) || !(scale > 0.0f)) return fail_invalid(op, "scale must be finite and positive");
-  if (const int rc = check_window(op, a.c, &window, &sinks)) return rc;
-  if (max_q < 0) return fail_invalid(op, "max_q must not be negative");
-  if (q->tokens == 0 || cache->batch == 0 || max_q == 0) return q->tokens == 0 ? B2_OK : fail_invalid(op, "tokens without a sequence, or max_q 0");
+  if (q->tokens == 0) return B2_OK;
+  if (cache->batch == 0 || max_q == 0) return fail_invalid(op, "tokens without a sequence, or max_q 0");
   if (cu_seqlens == nullptr) return fail_invalid(op, "null cu_seqlens");
   if (!rows_ok(q->data, q->row_stride, q->head_stride) || !rows_ok(out->data, out->row_stride, out->head_stride)) {
     return fail_invalid(op, "q and out need a 16-byte aligned base and strides that are multiples of 8");
@@ -786,14 +889,20 @@ int b2_attention_paged(const b2_paged_cache* cache, const b2_view3* q, const b2_
   a.q_heads = static_cast<int>(q->heads), a.group = a.q_heads / cache->kv_heads;
   a.max_q = static_cast<int>(std::min<std::int64_t>(max_q, q->tokens));
   if (q->tokens * a.group > INT_MAX / 2) return fail_invalid(op, "too many tokens for one call");
-  const std::int64_t tiles = (static_cast<std::int64_t>(a.max_q) * a.group + 2 * kTile - 1) / (2 * kTile), works = tiles * cache->batch * cache->kv_heads;
-  if (works > INT_MAX / 2) return fail_invalid(op, "too many tokens for one call");
-  a.tiles = static_cast<int>(tiles), a.works = static_cast<int>(works);
+  const PromptPlan p = plan(a.c, a.tokens, a.q_heads, cache->head_dim, a.max_q, window, sinks);
+  if (p.works > INT_MAX / 2) return fail_invalid(op, "too many tokens for one call");
+  a.tiles = p.tiles, a.splits = p.splits, a.works = static_cast<int>(p.works);
+  if (p.splits > 1) {
+    if (workspace == nullptr || !aligned_to(workspace, 256) || workspace_bytes < p.total) {
+      return fail_invalid(op, "workspace is too small or not 256-byte aligned (b2_attention_paged_workspace_bytes)");
+    }
+    a.part_ml = static_cast<float2*>(workspace), a.part_o = reinterpret_cast<float*>(static_cast<std::uint8_t*>(workspace) + p.ml);
+  }
   a.scale_log2 = scale * 1.4426950408889634f, a.window = window, a.sinks = sinks;
-  CUtensorMap map_q{}, map_k, map_v;
   a.q_tma = kTile % a.group == 0 && q->row_stride > 0 && q->head_stride > 0;
-  if (a.q_tma != 0 && !make_tensor_map_rows(&map_q, q, cache->head_dim, a.group, kTile / a.group, op)) return B2_ERR_CUDA;
-  if (!make_tensor_map_pages(&map_k, cache, false, std::min(cache->page_size, kTile / 2), 64, op) ||
+  CUtensorMap map_q{}, map_k, map_v;
+  if ((a.q_tma != 0 && !make_tensor_map_rows(&map_q, q, cache->head_dim, a.group, kTile / a.group, op)) ||
+      !make_tensor_map_pages(&map_k, cache, false, std::min(cache->page_size, kTile / 2), 64, op) ||
       !make_tensor_map_pages(&map_v, cache, true, std::min(cache->page_size, kTile), cache->head_dim / 2, op)) {
     return B2_ERR_CUDA;
   }

@@ -768,14 +768,24 @@ def _lse_of(view, q, lse):
     return lse
 
 
-def attention_paged(q, cache, cu_seqlens, max_q, scale, window=0, sinks=0, out=None, lse=None):
+def attention_paged_workspace_bytes(cache, tokens, q_heads, max_q, window=0, sinks=0) -> int:
+    n = _lib.lib().b2_attention_paged_workspace_bytes(cache.struct, tokens, q_heads, max_q, window, sinks)
+    if n == 0:
+        check(-1)
+    return n
+
+
+def attention_paged(q, cache, cu_seqlens, max_q, scale, window=0, sinks=0, out=None, lse=None, workspace=None):
     """Causal attention of a prompt's tokens q [tokens, q_heads, head_dim] over the cache that holds their keys and values already;
     with a window the last `window` slots and the first `sinks`. Returns (out, lse): lse fp32 [tokens, q_heads]."""
     view = _heads_view(q, cache, "q")
     out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
     lse = _lse_of(view, q, lse)
+    if workspace is None:
+        need = attention_paged_workspace_bytes(cache, view.tokens, view.heads, max_q, window, sinks)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 256 else None  # (256: none is used)
     check(_lib.lib().b2_attention_paged(cache.struct, view, _heads_view(out, cache, "out"), lse.data_ptr(), _vector(cu_seqlens, "cu_seqlens", cache.batch + 1),
-                                        max_q, scale, window, sinks, _raw_stream()))
+                                        max_q, scale, window, sinks, _at(workspace), 0 if workspace is None else workspace.numel(), _raw_stream()))
     return out, lse
 
 

@@ -234,6 +234,28 @@ def test_prompt(lens, new, hq, hk, d, page, dtype, window, sinks, outside):
     assert torch.equal(again.view(torch.int16), got.contiguous().view(torch.int16))
 
 
+@pytest.mark.parametrize("lens,new,hq,hk,d,page,dtype,window,sinks", [
+    ([5000], [1], 8, 1, 128, 16, BF16, 0, 0),
+    ([6000, 0, 700], [3, 0, 300], 10, 2, 64, 64, F16, 0, 0),
+    ([6000, 5], [300, 9], 4, 1, 128, 32, BF16, 0, 0),         # a short sequence has parts without keys, and tokens that see nothing
+    ([9000], [130], 7, 1, 128, 128, BF16, 2500, 700),
+])
+@pytest.mark.parametrize("bad", [0.5, math.nan, math.inf])
+def test_prompt_over_a_long_cache(lens, new, hq, hk, d, page, dtype, window, sinks, bad):
+    """Few tokens over many slots: the keys are cut into parts that are worked on apart."""
+    cache = make_cache(lens, hk, d, page, dtype, fill=math.nan)
+    assert ops.attention_paged_workspace_bytes(cache, sum(new), hq, max(new), window, sinks) > 256
+    for slot in (lens[0] - 1, lens[0] - 2, lens[0] - 140):  # near the causal edge, where some rows do not see them
+        if slot < lens[0] - new[0] + 1 or bad == 0.5:
+            continue
+        cache.v[cache.block_table[0, slot // page].item(), 0, slot % page, 3] = bad
+    q = (2.0 * torch.randn((sum(new), hq, d), generator=torch.Generator().manual_seed(5))).to(dtype).cuda()
+    got, lse = ops.attention_paged(q, cache, cu_of(new), max(new), d ** -0.5, window=window, sinks=sinks)
+    check_prompt(cache, q, new, window, sinks, d ** -0.5, got, lse, dtype)
+    again, _ = ops.attention_paged(q, cache, cu_of(new), max(new), d ** -0.5, window=window, sinks=sinks)
+    assert torch.equal(again.view(torch.int16), got.view(torch.int16)) and ops.paged_cache_status() == 0
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("steep", [3.0, 30.0])
 def test_prompt_with_scores_that_rise(dtype, steep):

@@ -24,8 +24,8 @@ def append(c=None, qkv=A, ld=1024, tokens=1, q_heads=4, cu=A, q_norm=A, k_norm=A
     return _lib.lib().b2_qk_norm_rope_append(c or cache(), qkv, ld, tokens, q_heads, cu, None, q_norm, k_norm, eps, rope, rows, rot, 0, q_out, q_row, q_head, None)
 
 
-def prompt(c=None, q=None, out=None, cu=A, max_q=1, scale=0.1, window=0, sinks=0):
-    return _lib.lib().b2_attention_paged(c or cache(), q or view(), out or view(), None, cu, max_q, scale, window, sinks, None)
+def prompt(c=None, q=None, out=None, cu=A, max_q=1, scale=0.1, window=0, sinks=0, ws=A, ws_bytes=1 << 30):
+    return _lib.lib().b2_attention_paged(c or cache(), q or view(), out or view(), None, cu, max_q, scale, window, sinks, ws, ws_bytes, None)
 
 
 def decode(c=None, q=None, out=None, max_len=0, scale=0.1, window=0, sinks=0, weights=None, weights_out=None, ld=64, ws=A, ws_bytes=1 << 30):
@@ -63,6 +63,8 @@ def test_bad_caches(call, over, word):
     (prompt, dict(scale=float("inf")), "scale"), (prompt, dict(window=-1), "window"), (prompt, dict(sinks=-1), "sinks"), (prompt, dict(max_q=-1), "max_q"),
     (prompt, dict(max_q=0), "max_q"), (prompt, dict(cu=None), "cu_seqlens"), (prompt, dict(q=view(data=A + 2)), "aligned"), (prompt, dict(out=view(row=516)), "multiples of 8"),
     (prompt, dict(c=cache(num_pages=0, k=0, v=0)), "no pages"),
+    (prompt, dict(c=cache(table_width=4096, table_ld=4096), ws=None), "workspace"), (prompt, dict(c=cache(table_width=4096, table_ld=4096), ws=A + 16), "workspace"),
+    (prompt, dict(c=cache(table_width=4096, table_ld=4096), ws_bytes=512), "workspace"),
     (decode, dict(q=view(tokens=2)), "one token"), (decode, dict(q=view(heads=5), out=view(heads=5)), "multiple of kv_heads"), (decode, dict(scale=-1.0), "scale"),
     (decode, dict(window=-2), "window"), (decode, dict(max_len=65), "max_len"), (decode, dict(max_len=-1), "max_len"), (decode, dict(weights=A), "both or neither"),
     (decode, dict(weights=A, weights_out=A, ld=63), "every slot"), (decode, dict(weights=A, weights_out=A, ws=None), "workspace"),
@@ -93,6 +95,14 @@ def test_workspace_sizes():
     assert size(long, max_len=100000) == 0 and size(long, heads=5) == 0
     assert 0 < size(cache()) <= size(long, window=64) <= size(long) < size(long, weights=1)
     assert size(long, max_len=1000) < size(long) and size(long, max_len=1000, weights=1) < size(long, weights=1)
+
+
+def test_workspace_sizes_of_prompts():
+    size = lambda c, tokens=1, heads=4, max_q=1, window=0: _lib.lib().b2_attention_paged_workspace_bytes(c, tokens, heads, max_q, window, 0)  # noqa: E731
+    long = cache(table_width=4096, table_ld=4096)
+    assert size(cache()) == 256 and size(long, tokens=100000, max_q=100000) == 256  # nothing to cut, enough tokens
+    assert size(long) > size(long, window=2000) > 256
+    assert size(long, heads=5) == 0 and size(long, tokens=-1) == 0 and size(long, window=-1) == 0
 
 
 def test_python_side_refusals():
