@@ -4,6 +4,8 @@
 
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace b2 {
@@ -35,6 +37,18 @@ int check_paged_cache(const char* op, const b2_paged_cache* c, PagedArgs* a);
 int paged_status_word(const char* op, PagedArgs* a);
 // Where a call may write or read rows of `row` elements: 16-byte aligned, strides in multiples of 8 elements.
 inline bool rows_ok(const void* p, std::int64_t row, std::int64_t head) { return p != nullptr && aligned_to(p, 16) && row % 8 == 0 && head % 8 == 0; }
+// A kernel's dynamic shared memory, set once per device (`done`: a static of the caller's, a bit for each device).
+template <typename Kernel>
+int allow_shared(const char* op, Kernel kernel, int bytes, std::atomic<std::uint64_t>& done) {
+  int device = 0;
+  if (cudaGetDevice(&device) == cudaSuccess && device < 64 && (done.load(std::memory_order_relaxed) >> device & 1u) != 0u) return B2_OK;
+  if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); e != cudaSuccess) {
+    cudaGetLastError();
+    return fail_cuda(op, e);
+  }
+  if (device < 64) done.fetch_or(1ull << device, std::memory_order_relaxed);
+  return B2_OK;
+}
 // cuTensorMapEncodeTiled for the cache's keys or values, [pages, heads, rows, head_dim]: boxes of box_rows rows of box_columns
 // elements, 64 with the 128-byte swizzle or 32 with the 64-byte one. Returns false (and sets the last error) on failure.
 bool make_tensor_map_pages(CUtensorMap* map, const b2_paged_cache* c, bool values, int box_rows, int box_columns, const char* op);

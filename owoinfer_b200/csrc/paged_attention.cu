@@ -837,10 +837,8 @@ template <typename T, int D>
 int launch(const char* op, const PromptArgs& a, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t st) {
   using S = Shape<D>;
   const auto kernel = prompt_kernel<T, D>;
-  if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem); e != cudaSuccess) {
-    cudaGetLastError();
-    return fail_cuda(op, e);
-  }
+  static std::atomic<std::uint64_t> allowed{0};
+  if (const int rc = allow_shared(op, kernel, S::kSmem, allowed)) return rc;
   const LaunchChain chain(st);
   // As many pairs as fit at once, or as there are works.
   const unsigned pairs = static_cast<unsigned>(std::max(1, std::min(sm_count() / 2, a.works)));

@@ -510,12 +510,18 @@ int check_window(const char* op, const PagedArgs& c, int* window, int* sinks) {
 }
 
 int paged_status_word(const char* op, PagedArgs* a) {
+  static std::atomic<unsigned*> cached[64] = {};  // by device
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) device = 64;
+  a->status = device < 64 ? cached[device].load(std::memory_order_relaxed) : nullptr;
+  if (a->status != nullptr) return B2_OK;
   void* word = nullptr;
   if (const cudaError_t e = cudaGetSymbolAddress(&word, g_paged_status); e != cudaSuccess) {
     cudaGetLastError();
     return fail_cuda(op, e);
   }
   a->status = static_cast<unsigned*>(word);
+  if (device < 64) cached[device].store(a->status, std::memory_order_relaxed);
   return B2_OK;
 }
 

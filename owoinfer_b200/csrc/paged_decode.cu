@@ -3,7 +3,6 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
-#include <type_traits>
 
 #include "attention.cuh"
 #include "paged.cuh"
@@ -89,7 +88,6 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
   __shared__ int s_abort;
   // A step in shared memory: K, then V, each D / 64 parts of 16 rows of 128 bytes with the 128-byte swizzle.
   constexpr int kParts = D / 64, kPartBytes = kKeys * 128, kHalfBytes = kParts * kPartBytes, kStageBytes = 2 * kHalfBytes;
-  constexpr bool kTwoParts = std::is_same<T, __nv_bfloat16>::value;
   const int warp = static_cast<int>(threadIdx.x) / 32, lane = static_cast<int>(threadIdx.x) % 32;
   const int blocks = (a.group + kRows - 1) / kRows;
   const int split = blockIdx.x, h = blockIdx.y / blocks, g0 = (blockIdx.y % blocks) * kRows, b = blockIdx.z;
@@ -244,8 +242,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         l[i >> 1] += p[t][i];
       }
     }
-    // P for the tensor core. bf16 keeps 8 bits of it, so the 8 bits that this leaves go in as a second operand: P·V is then as exact as
-    // the values are, for 16 more MMAs in a kernel that waits for memory. fp16's 11 bits stand alone.
+    // P for the tensor core. What its rounding to 8 (11) bits leaves goes in as a second operand: P·V is then as exact as the values
+    // are, for 16 more MMAs in a kernel that waits for memory.
     std::uint32_t hi[4], lo[4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -253,11 +251,9 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       for (int i = 0; i < 2; ++i) {
         const float x = p[t][2 * i], y = p[t][2 * i + 1];
         hi[2 * t + i] = pack16<T>(x, y);
-        if constexpr (kTwoParts) {
-          float xh, yh;
-          unpack16<T>(hi[2 * t + i], xh, yh);
-          lo[2 * t + i] = pack16<T>(x - xh, y - yh);
-        }
+        float xh, yh;
+        unpack16<T>(hi[2 * t + i], xh, yh);
+        lo[2 * t + i] = pack16<T>(x - xh, y - yh);
       }
     }
     const int r = (lane >> 3 & 1) * 8 + lane % 8, half = lane >> 4;
@@ -267,10 +263,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       ldsm4_trans(v_rows + d / 4 * kPartBytes + r * 128 + (((2 * d + half) % 8 ^ (r & 7)) << 4), vf);
       mma16<T>(o[2 * d], hi, vf[0], vf[1]);
       mma16<T>(o[2 * d + 1], hi, vf[2], vf[3]);
-      if constexpr (kTwoParts) {
-        mma16<T>(o[2 * d], lo, vf[0], vf[1]);
-        mma16<T>(o[2 * d + 1], lo, vf[2], vf[3]);
-      }
+      mma16<T>(o[2 * d], lo, vf[0], vf[1]);
+      mma16<T>(o[2 * d + 1], lo, vf[2], vf[3]);
     }
     __syncwarp();  // the stage is read
     issue(n + kStages);
@@ -485,10 +479,8 @@ int launch(const char* op, const DecodeArgs& a, const Plan& p, const CUtensorMap
   constexpr int ring = kWarps * kStages * 2 * kKeys * D * 2, meet = kWarps * kRows * (D + 4 + 2) * 4;
   constexpr int smem = (ring > meet ? ring : meet) + 1024;  // and what aligns it
   const auto kernel = decode_kernel<T, D, kScores>;
-  if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) {
-    cudaGetLastError();
-    return fail_cuda(op, e);
-  }
+  static std::atomic<std::uint64_t> allowed{0};
+  if (const int rc = allow_shared(op, kernel, smem, allowed)) return rc;
   const LaunchChain chain(st);
   const unsigned blocks = static_cast<unsigned>((a.group + kRows - 1) / kRows), batch = static_cast<unsigned>(a.c.batch);
   const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.c.kv_heads) * blocks, batch);

@@ -8,6 +8,7 @@ memory and streams only. Invalid arguments raise ValueError (the reference throw
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 import torch
@@ -675,8 +676,28 @@ _PAGED_BYTES = C.sizeof(_lib.PagedCache)
 # are written for their number of tensor queries, and the structs filled in one go.)
 
 
+try:  # (private names, which another torch may not have)
+    _get_device, _get_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+except AttributeError:
+    _get_device = _get_stream = None
+
+
 def _raw_stream() -> int:
-    return _stream().value or 0
+    """The current stream's handle as an int; for calls on tensors that are on the GPU already."""
+    return torch.cuda.current_stream().cuda_stream if _get_stream is None else _get_stream(_get_device())
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_need(call, *shape):
+    """Bytes of workspace by the C function `call`, which looks at sizes only: the struct has addresses that nothing follows."""
+    batch, kv_heads, page_size, head_dim, slots, dtype = shape[:6]
+    dims = page_size * head_dim
+    cache = _lib.PagedCache(_PAGED_BYTES, 256, 256, kv_heads * dims, dims, head_dim, 1, _DTYPES[dtype], kv_heads, page_size, head_dim, 256, slots // page_size,
+                            slots // page_size, 256, batch)
+    n = getattr(_lib.lib(), call)(cache, *shape[6:])
+    if n == 0:
+        check(-1)
+    return n
 
 
 def _at(t) -> int:
@@ -718,6 +739,7 @@ class PagedCache:
         pages, self.kv_heads, self.page_size, self.head_dim = shape
         width = block_table.numel() // batch if batch else 0
         self.batch, self.slots = batch, width * self.page_size
+        self._sizes = (batch, self.kv_heads, self.page_size, self.head_dim, self.slots, dtype)
         self.struct = _lib.PagedCache(_PAGED_BYTES, k.data_ptr(), v.data_ptr(), strides[0], strides[1], strides[2], pages, code, self.kv_heads,
                                       self.page_size, self.head_dim, block_table.data_ptr(), ld, width, _vector(seq_lens, "seq_lens", batch), batch)
 
@@ -760,48 +782,42 @@ def qk_norm_rope_append(qkv, cache, cu_seqlens, q_norm, k_norm, rope, positions=
     return out
 
 
-def _lse_of(view, q, lse):
+def _lse_of(q, lse):
     if lse is None:
-        return torch.empty((view.tokens, view.heads), dtype=torch.float32, device=q.device)
+        return q.new_empty(q.shape[:2], dtype=torch.float32)
     if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous():
         raise ValueError("lse must be a contiguous fp32 [tokens, q_heads] tensor")
     return lse
 
 
 def attention_paged_workspace_bytes(cache, tokens, q_heads, max_q, window=0, sinks=0) -> int:
-    n = _lib.lib().b2_attention_paged_workspace_bytes(cache.struct, tokens, q_heads, max_q, window, sinks)
-    if n == 0:
-        check(-1)
-    return n
+    return _workspace_need("b2_attention_paged_workspace_bytes", *cache._sizes, tokens, q_heads, max_q, window, sinks)
 
 
 def attention_paged(q, cache, cu_seqlens, max_q, scale, window=0, sinks=0, out=None, lse=None, workspace=None):
     """Causal attention of a prompt's tokens q [tokens, q_heads, head_dim] over the cache that holds their keys and values already;
     with a window the last `window` slots and the first `sinks`. Returns (out, lse): lse fp32 [tokens, q_heads]."""
     view = _heads_view(q, cache, "q")
-    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
-    lse = _lse_of(view, q, lse)
+    out = q.new_empty(q.shape) if out is None else out
+    lse = _lse_of(q, lse)
     if workspace is None:
-        need = attention_paged_workspace_bytes(cache, view.tokens, view.heads, max_q, window, sinks)
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 256 else None  # (256: none is used)
+        need = attention_paged_workspace_bytes(cache, *q.shape[:2], max_q, window, sinks)
+        workspace = q.new_empty(need, dtype=torch.uint8) if need > 256 else None  # (256: none is used)
     check(_lib.lib().b2_attention_paged(cache.struct, view, _heads_view(out, cache, "out"), lse.data_ptr(), _vector(cu_seqlens, "cu_seqlens", cache.batch + 1),
                                         max_q, scale, window, sinks, _at(workspace), 0 if workspace is None else workspace.numel(), _raw_stream()))
     return out, lse
 
 
 def attention_paged_decode_workspace_bytes(cache, q_heads, max_len=0, window=0, sinks=0, weights=False) -> int:
-    n = _lib.lib().b2_attention_paged_decode_workspace_bytes(cache.struct, q_heads, max_len, window, sinks, weights)
-    if n == 0:
-        check(-1)
-    return n
+    return _workspace_need("b2_attention_paged_decode_workspace_bytes", *cache._sizes, q_heads, max_len, window, sinks, weights)
 
 
 def attention_paged_decode(q, cache, scale, max_len=0, window=0, sinks=0, weights=None, weights_out=None, out=None, lse=None, workspace=None):
     """Attention of one new token per sequence, q [batch, q_heads, head_dim], split over the cache's length. With `weights` (fp32 [batch,
     kv_heads, slots]) the attention each slot got is added to them (in weights_out, or in place). Returns (out, lse)."""
     view = _heads_view(q, cache, "q")
-    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
-    lse = _lse_of(view, q, lse)
+    out = q.new_empty(q.shape) if out is None else out
+    lse = _lse_of(q, lse)
     ld = 0
     if weights is not None:
         weights_out = weights if weights_out is None else weights_out
@@ -809,8 +825,7 @@ def attention_paged_decode(q, cache, scale, max_len=0, window=0, sinks=0, weight
         if weights_out is not weights and _slots_of(weights_out, cache, "weights_out") != ld:
             raise ValueError("weights and weights_out must have the same shape")
     if workspace is None:
-        workspace = torch.empty(attention_paged_decode_workspace_bytes(cache, view.heads, max_len, window, sinks, weights is not None),
-                                dtype=torch.uint8, device=q.device)
+        workspace = q.new_empty(attention_paged_decode_workspace_bytes(cache, q.shape[1], max_len, window, sinks, weights is not None), dtype=torch.uint8)
     check(_lib.lib().b2_attention_paged_decode(cache.struct, view, _heads_view(out, cache, "out"), lse.data_ptr(), max_len, scale, window, sinks,
                                                _at(weights), _at(weights_out), ld, workspace.data_ptr(), workspace.numel(), _raw_stream()))
     return out, lse
@@ -837,7 +852,7 @@ def kv_evict(cache, weights, table_out, budget, sinks=0, recent=0, kept=None, le
     if rows_out != cache.batch:
         raise ValueError("table_out must have a row for every sequence")
     slots_out = 0 if weights_out is None else _slots_of(weights_out, cache, "weights_out")
-    kept = torch.empty((cache.batch, cache.kv_heads, budget), dtype=torch.int32, device=weights.device) if kept is None else kept
+    kept = cache.seq_lens.new_empty((cache.batch, cache.kv_heads, budget)) if kept is None else kept
     lens_out = torch.empty_like(cache.seq_lens) if lens_out is None else lens_out
     if kept.dtype != torch.int32 or kept.shape != (cache.batch, cache.kv_heads, budget) or not kept.is_contiguous():
         raise ValueError("kept must be a contiguous int32 [batch, kv_heads, budget] tensor")
