@@ -713,7 +713,7 @@ int b2_qk_norm_rope_append(const b2_paged_cache* cache, const void* qkv, int64_t
  * q_heads, head_dim]; max_q: no sequence has more tokens in the call. Keys and values of slots that a token does not see do
  * not reach its output, NaN and infinities included.
  * workspace: b2_attention_paged_workspace_bytes() of the same arguments, 256-byte aligned (few tokens over a long cache: parts of the
- * keys are worked on apart and joined; 256 where none is needed, and then NULL will do). Nothing is kept in it. */
+ * keys are worked on apart and joined; 256 where none is needed, and then NULL with 0 bytes will do). Nothing is kept in it. */
 size_t b2_attention_paged_workspace_bytes(const b2_paged_cache* cache, int64_t tokens, int q_heads, int max_q, int window, int sinks);
 int b2_attention_paged(const b2_paged_cache* cache, const b2_view3* q, const b2_view3* out, float* lse, const int32_t* cu_seqlens,
                        int max_q, float scale, int window, int sinks, void* workspace, size_t workspace_bytes, void* stream);
@@ -724,8 +724,8 @@ int b2_attention_paged(const b2_paged_cache* cache, const b2_view3* q, const b2_
  * for every slot j < seq_len; the others are left alone. weights, weights_out: device fp32, [batch, kv_heads, slots] with
  * rows weights_ld apart (at least max_len, or the table's slots), the same buffer or two that do not overlap.
  * max_len: no sequence is longer (0: as long as the block table allows); the split goes by it.
- * workspace: b2_attention_paged_decode_workspace_bytes() of the same arguments (with_weights: whether weights_out is given), 256-byte aligned;
- * nothing in it needs clearing and nothing is kept in it. */
+ * workspace: b2_attention_paged_decode_workspace_bytes() of the same arguments (with_weights: whether weights_out is given), 256-byte aligned
+ * (256 where none is needed, and then NULL with 0 bytes will do); nothing in it needs clearing and nothing is kept in it. */
 size_t b2_attention_paged_decode_workspace_bytes(const b2_paged_cache* cache, int q_heads, int max_len, int window, int sinks,
                                                  int with_weights);
 int b2_attention_paged_decode(const b2_paged_cache* cache, const b2_view3* q, const b2_view3* out, float* lse, int max_len,

@@ -4,6 +4,7 @@
 
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
@@ -56,6 +57,12 @@ bool make_tensor_map_pages(CUtensorMap* map, const b2_paged_cache* c, bool value
 bool make_tensor_map_rows(CUtensorMap* map, const b2_view3* v, int head_dim, int box_heads, int box_tokens, const char* op);
 // A window that reaches every slot is none; sinks past the last slot are all slots.
 int check_window(const char* op, const PagedArgs& c, int* window, int* sinks);
+// A workspace of `need` bytes. One that is given is looked at even where none is needed: what a caller sized wrongly shows at
+// its first call, whatever that call's lengths.
+inline int check_workspace(const char* op, const void* workspace, std::size_t bytes, std::size_t need) {
+  if (workspace == nullptr ? bytes == 0 && need == 0 : aligned_to(workspace, 256) && bytes >= std::max<std::size_t>(need, 256)) return B2_OK;
+  return fail_invalid(op, "workspace is missing, too small (its _workspace_bytes call has the size) or not 256-byte aligned");
+}
 
 #ifdef __CUDACC__
 // Slots of sequence b, at least 0 and at most what its row of the block table (or the call) allows.

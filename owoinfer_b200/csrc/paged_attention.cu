@@ -890,10 +890,8 @@ int b2_attention_paged(const b2_paged_cache* cache, const b2_view3* q, const b2_
   const PromptPlan p = plan(a.c, a.tokens, a.q_heads, cache->head_dim, a.max_q, window, sinks);
   if (p.works > INT_MAX / 2) return fail_invalid(op, "too many tokens for one call");
   a.tiles = p.tiles, a.splits = p.splits, a.works = static_cast<int>(p.works);
+  if (const int rc = check_workspace(op, workspace, workspace_bytes, p.splits > 1 ? p.total : 0)) return rc;
   if (p.splits > 1) {
-    if (workspace == nullptr || !aligned_to(workspace, 256) || workspace_bytes < p.total) {
-      return fail_invalid(op, "workspace is too small or not 256-byte aligned (b2_attention_paged_workspace_bytes)");
-    }
     a.part_ml = static_cast<float2*>(workspace), a.part_o = reinterpret_cast<float*>(static_cast<std::uint8_t*>(workspace) + p.ml);
   }
   a.scale_log2 = scale * 1.4426950408889634f, a.window = window, a.sinks = sinks;

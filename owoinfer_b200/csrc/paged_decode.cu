@@ -14,6 +14,7 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kKeys = 16;       // slots of a step of a warp: a page holds a multiple of it
 constexpr int kStages = 2;      // steps of a warp in shared memory: the one it works on and the one on its way
 constexpr int kRows = 16;       // query heads of a CTA: the rows of an MMA
+constexpr int kMostCluster = 8, kClusterSteps = 16;  // CTAs that join their parts in shared memory; steps of each at most
 constexpr int kJoinThreads = 256;
 constexpr int kJoinSlots = 4;
 constexpr int kMostGroup = 4096;  // (a float each in shared memory)
@@ -59,6 +60,16 @@ __device__ __forceinline__ void ldsm4(std::uint32_t addr, std::uint32_t (&r)[4])
 __device__ __forceinline__ void ldsm4_trans(std::uint32_t addr, std::uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ float2 ld_cluster_f32x2(std::uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(std::uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 template <typename T>
 __device__ __forceinline__ void mma16(float (&d)[4], const std::uint32_t (&a)[4], std::uint32_t b0, std::uint32_t b1);
 template <>
@@ -76,10 +87,14 @@ __device__ __forceinline__ void mma16<__half>(float (&d)[4], const std::uint32_t
 // keeps its relative precision however large it is (fp16: up to 2^8 of 2^16).
 constexpr float kRaise = 8.0f;
 
-// A CTA per (part of the cache, key head and block of 16 query heads, sequence). Its warps work apart: each has TMA bring its own steps
-// of 16 slots and keeps its own maxima, sums and output rows in registers; they meet at the end. Q·K^T and P·V are 16-row MMAs with the group's query heads as rows: the cache is read once for all of them, and at one
-// byte to every 2 group multiply-adds the memory is what bounds it.
-template <typename T, int D, bool kScores>
+// softmax(scale q·K^T)·V of one query row per head: o = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m), s in binades, m a running
+// reference. A CTA per (part of the cache, key head and block of 16 query heads, sequence). Its warps work apart: each has TMA
+// bring its own steps of 16 slots (whose 16 rows a page holds in one piece) and keeps its own maxima, sums and output rows in
+// registers; they meet at the end. Q·K^T and P·V are 16-row MMAs with the group's query heads as rows: the cache is read once
+// for all of them. At one byte of cache to every group / 2 multiply-adds the memory bounds it; 128-row tensor tiles would be
+// filled to group / 128. 64 sequences of up to 8101 slots, 32 / 8 heads of 128: 194 us, 6.5 TB/s with the join; one of 131001,
+// 16 / 4 heads: 53 us, 5.1 TB/s.
+template <typename T, int D, bool kScores, bool kCluster>
 __global__ void __launch_bounds__(kThreads, 3)
 decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const DecodeArgs a) {
   dependents_may_start();
@@ -101,8 +116,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
   const int len = paged_len(a.c, b);
   const Steps steps(a, len);
   const int begin = split * a.chunk, end = min(steps.count, begin + a.chunk);
-  // (Part 0 of an empty sequence goes on: it writes the zeros, or the empty part that the join finds.)
-  if (begin >= end && split > 0) return;
+  // (Part 0 of an empty sequence goes on: it writes the zeros, or the empty part that the join finds. So does all of a cluster.)
+  if (!kCluster && begin >= end && split > 0) return;
   const int mine = begin + warp < end ? (end - begin - warp + kWarps - 1) / kWarps : 0;  // this warp's steps
   const auto checked = [&](int page, int i) {
     if (i >= mine) return -1;
@@ -119,6 +134,9 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
   int pages = a.window == 0 ? checked(entry, lane) : fetch_pages(0), pages_next = fetch_pages(32);
 
   std::uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  // In a cluster the scores stay here, [rows][chunk * kKeys], behind the rings.
+  float* const own_scores = reinterpret_cast<float*>(smem + kWarps * kStages * kStageBytes);
+  const int own_ld = a.chunk * kKeys;
   const std::uint32_t ring = smem_u32(smem) + static_cast<std::uint32_t>(warp) * (kStages * kStageBytes);
   const auto bar = [&](int n) { return smem_u32(&s_full[warp][n % kStages]); };
   if (lane == 0) {  // (a warp's barriers are its own: no other waits for them)
@@ -208,7 +226,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       for (int i = 0; i < 2; ++i) {
         const int r = lane / 4 + 8 * i;
         if (r < rows) {
-          float* row = a.scores + (static_cast<std::int64_t>(b) * a.q_heads + q_head0 + r) * a.scores_ld + key;
+          float* row = kCluster ? own_scores + r * own_ld + (warp + n * kWarps) * kKeys + (lane % 4) * 2
+                                : a.scores + (static_cast<std::int64_t>(b) * a.q_heads + q_head0 + r) * a.scores_ld + key;
           *reinterpret_cast<float2*>(row) = make_float2(s[0][2 * i], s[0][2 * i + 1]);
           *reinterpret_cast<float2*>(row + 8) = make_float2(s[1][2 * i], s[1][2 * i + 1]);
         }
@@ -277,16 +296,17 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
 
   // The warps' parts meet in the rings' place.
   __syncthreads();
-  if (s_abort != 0) {  // a wait expired: give the copies on their way time to land, and leave
+  if (s_abort != 0) {  // a wait expired: give the copies on their way time to land
     if (threadIdx.x == 0) atomicOr(a.c.status, kPagedWait);
     const std::uint64_t t0 = global_ns();
     while (global_ns() - t0 < 2000000ull) {
     }
-    return;
+    if constexpr (!kCluster) return;
   }
   float* s_o = reinterpret_cast<float*>(smem);           // [kWarps][kRows][D + 4]
   constexpr int kLd = D + 4;
   float* s_ml = s_o + kWarps * kRows * kLd;              // [kWarps][kRows][2]
+  float* s_part = s_ml + kWarps * kRows * 2;             // [kRows][2] of this CTA
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int row = warp * kRows + lane / 4 + 8 * i;
@@ -311,7 +331,10 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       sum.x = fmaf(f, x.x, sum.x), sum.y = fmaf(f, x.y, sum.y), sum.z = fmaf(f, x.z, sum.z), sum.w = fmaf(f, x.w, sum.w);
     }
     const std::int64_t head = static_cast<std::int64_t>(b) * a.q_heads + q_head0 + row;
-    if (a.part_o == nullptr) {
+    if constexpr (kCluster) {
+      *reinterpret_cast<float4*>(s_o + row * kLd + d) = sum;  // (in the place of warp 0's, which only this thread reads)
+      if (d == 0) s_part[2 * row] = mm, s_part[2 * row + 1] = ll;
+    } else if (a.part_o == nullptr) {
       const float inv = ll == 0.f ? 0.f : 1.0f / ll;
       T* out = static_cast<T*>(a.out) + b * a.o_row + (q_head0 + row) * a.o_head + d;
       *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(sum.x * inv, sum.y * inv), pack16<T>(sum.z * inv, sum.w * inv));
@@ -320,6 +343,70 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       *reinterpret_cast<float4*>(a.part_o + (head * a.splits + split) * D + d) = sum;
       if (d == 0) a.part_ml[head * a.splits + split] = make_float2(mm, ll);
     }
+  }
+  if constexpr (kCluster) {
+    // The parts are the cluster's CTAs: each joins some of the output, and adds up what its own slots got.
+    __shared__ float s_lse[kRows];
+    cluster_sync_all();
+    const auto all_parts = [&](int row, float2(&ml)[kMostCluster]) {
+#pragma unroll
+      for (int i = 0; i < kMostCluster; ++i) ml[i] = i < a.splits ? ld_cluster_f32x2(map_to_cta(smem_u32(s_part + 2 * row), static_cast<std::uint32_t>(i))) : make_float2(-INFINITY, 0.f);
+    };
+    const auto sum_of = [&](const float2(&ml)[kMostCluster], float& mm, float& ll) {
+      mm = -INFINITY, ll = 0.f;
+#pragma unroll
+      for (int i = 0; i < kMostCluster; ++i) mm = fmaxf(mm, ml[i].x);
+#pragma unroll
+      for (int i = 0; i < kMostCluster; ++i) ll += ml[i].y == 0.f ? 0.f : ml[i].y * ex2(ml[i].x - mm);
+    };
+    for (int at = split * kThreads + static_cast<int>(threadIdx.x); at < rows * kQuads; at += a.splits * kThreads) {
+      const int row = at / kQuads, d = (at % kQuads) * 4;
+      float2 ml[kMostCluster];
+      float4 x[kMostCluster];
+      all_parts(row, ml);
+#pragma unroll
+      for (int i = 0; i < kMostCluster; ++i) {
+        if (i < a.splits) x[i] = ld_cluster_f32x4(map_to_cta(smem_u32(s_o + row * kLd + d), static_cast<std::uint32_t>(i)));
+      }
+      float mm, ll;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      sum_of(ml, mm, ll);
+#pragma unroll
+      for (int i = 0; i < kMostCluster; ++i) {
+        if (ml[i].y == 0.f) continue;
+        const float f = ex2(ml[i].x - mm);
+        sum.x = fmaf(f, x[i].x, sum.x), sum.y = fmaf(f, x[i].y, sum.y), sum.z = fmaf(f, x[i].z, sum.z), sum.w = fmaf(f, x[i].w, sum.w);
+      }
+      const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+      T* out = static_cast<T*>(a.out) + b * a.o_row + (q_head0 + row) * a.o_head + d;
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(sum.x * inv, sum.y * inv), pack16<T>(sum.z * inv, sum.w * inv));
+      if (d == 0 && a.lse != nullptr) a.lse[static_cast<std::int64_t>(b) * a.q_heads + q_head0 + row] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+    }
+    if constexpr (kScores) {
+      if (static_cast<int>(threadIdx.x) < rows) {
+        float2 ml[kMostCluster];
+        float mm, ll;
+        all_parts(static_cast<int>(threadIdx.x), ml);
+        sum_of(ml, mm, ll);
+        s_lse[threadIdx.x] = ll == 0.f ? INFINITY : mm + log2f(ll);
+      }
+      __syncthreads();
+      const std::int64_t at = (static_cast<std::int64_t>(b) * a.c.kv_heads + h) * a.weights_ld;
+      for (int i = threadIdx.x; i < (end - begin) * kKeys; i += kThreads) {
+        const int slot = steps.slot(begin + i / kKeys) + i % kKeys;
+        if (slot >= len) continue;
+        float got = 0.f;
+        if (sees(a, len, slot)) {
+          for (int g = 0; g < rows; ++g) got += ex2(own_scores[g * own_ld + i] - s_lse[g]);
+        }
+        a.weights_out[at + slot] = (slot < len - 1 ? a.weights[at + slot] : 0.f) + got;
+      }
+      // Slots of steps that the window hides.
+      for (int slot = steps.sinks * kKeys + split * kThreads + static_cast<int>(threadIdx.x); slot < steps.from * kKeys; slot += a.splits * kThreads) {
+        a.weights_out[at + slot] = a.weights[at + slot];
+      }
+    }
+    cluster_sync_all();  // nobody reads another CTA's shared memory from here on
   }
 }
 
@@ -432,13 +519,17 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a, 
 // slots, 4 key heads: 53 us; three per SM 58, six 76). Several, whose lengths differ: eighteen, handed out as SMs come free (64 of up to 8101, 8
 // key heads: 196 us; three per SM 233), but of kLongEnough steps at least, since each has its start and its part to join
 // (4 of up to 30001: 76 us; as eighteen per SM 79).
+// Few short ones, whose clusters all run at once, are joined by the CTAs of a cluster in shared memory: one launch instead of
+// two and no workspace, some 2 us of the host's time. Six of up to 500 slots, 8 key heads: 10.4 us, with the second kernel
+// 16.5; of up to 2000, 16.5 and 19.3; of up to 4000, 24.0 and 22.6, so it ends at kClusterSteps. One sequence has too few CTAs
+// that way sooner (160 slots: 6.9 us and 8.3; 517: 8.3 and 8.3; 1000: 9.8 and 8.3; 2000: 12.4 and 10.3) and ends at half of it.
 constexpr int kOneSequence = 2, kSeveral = 18, kLongEnough = 32, kShortest = kWarps;
 
 struct Plan {
   int chunk, splits;
   std::int64_t scores_ld;
   std::size_t ml, o, scores, total;
-  bool parts;
+  bool parts, cluster;  // parts in the workspace; or in the CTAs of a cluster
 };
 Plan plan(const PagedArgs& c, int q_heads, int head_dim, int window, int sinks, bool weights) {
   Plan p{};
@@ -450,9 +541,11 @@ Plan plan(const PagedArgs& c, int q_heads, int head_dim, int window, int sinks, 
   std::int64_t chunk = (steps * units + ctas - 1) / ctas;
   if (c.batch > 1) chunk = std::max<std::int64_t>(chunk, kLongEnough);
   chunk = std::max<std::int64_t>(chunk, kShortest);
+  p.cluster = group <= kRows && units * kMostCluster <= 3LL * sm_count() && steps <= kMostCluster * (c.batch <= 1 ? kClusterSteps / 2 : kClusterSteps);
+  if (p.cluster) chunk = std::max<std::int64_t>((steps + kMostCluster - 1) / kMostCluster, kShortest);
   p.chunk = static_cast<int>(std::min<std::int64_t>(chunk, INT_MAX / 2));
   p.splits = static_cast<int>(std::max<std::int64_t>(1, (steps + p.chunk - 1) / p.chunk));
-  p.parts = p.splits > 1 || weights;
+  p.parts = !p.cluster && (p.splits > 1 || weights);
   const auto align = [](std::size_t n) { return (n + 255) / 256 * 256; };
   const std::size_t heads = static_cast<std::size_t>(c.batch) * q_heads;
   if (p.parts) {
@@ -476,14 +569,22 @@ int check(const char* op, const b2_paged_cache* cache, PagedArgs* c, int q_heads
 
 template <typename T, int D, bool kScores>
 int launch(const char* op, const DecodeArgs& a, const Plan& p, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t st) {
-  constexpr int ring = kWarps * kStages * 2 * kKeys * D * 2, meet = kWarps * kRows * (D + 4 + 2) * 4;
-  constexpr int smem = (ring > meet ? ring : meet) + 1024;  // and what aligns it
-  const auto kernel = decode_kernel<T, D, kScores>;
-  static std::atomic<std::uint64_t> allowed{0};
-  if (const int rc = allow_shared(op, kernel, smem, allowed)) return rc;
+  constexpr int ring = kWarps * kStages * 2 * kKeys * D * 2, meet = (kWarps * kRows * (D + 4 + 2) + 2 * kRows) * 4;
+  static_assert(meet <= ring);
   const LaunchChain chain(st);
   const unsigned blocks = static_cast<unsigned>((a.group + kRows - 1) / kRows), batch = static_cast<unsigned>(a.c.batch);
   const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.c.kv_heads) * blocks, batch);
+  if (p.cluster) {
+    constexpr int most = ring + 1024 + kRows * kClusterSteps * kKeys * 4;
+    static std::atomic<std::uint64_t> allowed{0};
+    if (const int rc = allow_shared(op, decode_kernel<T, D, kScores, true>, most, allowed)) return rc;
+    const int smem = ring + 1024 + (kScores ? a.group * p.chunk * kKeys * 4 : 0);
+    return enqueue(op, decode_kernel<T, D, kScores, true>, grid, kThreads, static_cast<std::size_t>(smem), st, p.splits, map_k, map_v, a);
+  }
+  constexpr int smem = ring + 1024;  // and what aligns it
+  const auto kernel = decode_kernel<T, D, kScores, false>;
+  static std::atomic<std::uint64_t> allowed{0};
+  if (const int rc = allow_shared(op, kernel, smem, allowed)) return rc;
   if (const int rc = enqueue(op, kernel, grid, kThreads, smem, st, 1, map_k, map_v, a)) return rc;
   if (!p.parts) return B2_OK;
   const int head_ctas = std::min(a.group, 64), range = kJoinThreads * kJoinSlots, slot_ctas = kScores ? (a.c.most + range - 1) / range : 0;
@@ -525,9 +626,7 @@ int b2_attention_paged_decode(const b2_paged_cache* cache, const b2_view3* q, co
   if (static_cast<std::int64_t>(cache->kv_heads) * ((a.group + kRows - 1) / kRows) > 65535) return fail_invalid(op, "too many heads");
   const bool scores = weights != nullptr;
   const Plan p = plan(a.c, a.q_heads, cache->head_dim, window, sinks, scores);
-  if (p.parts && (workspace == nullptr || !aligned_to(workspace, 256) || workspace_bytes < p.total)) {
-    return fail_invalid(op, "workspace is too small or not 256-byte aligned (b2_attention_paged_decode_workspace_bytes)");
-  }
+  if (const int rc = check_workspace(op, workspace, workspace_bytes, p.total)) return rc;
   a.scores_ld = p.scores_ld;
   a.scale_log2 = scale * 1.4426950408889634f, a.window = window, a.sinks = sinks, a.chunk = p.chunk, a.splits = p.splits;
   if (p.parts) {

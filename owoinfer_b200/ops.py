@@ -825,9 +825,10 @@ def attention_paged_decode(q, cache, scale, max_len=0, window=0, sinks=0, weight
         if weights_out is not weights and _slots_of(weights_out, cache, "weights_out") != ld:
             raise ValueError("weights and weights_out must have the same shape")
     if workspace is None:
-        workspace = q.new_empty(attention_paged_decode_workspace_bytes(cache, q.shape[1], max_len, window, sinks, weights is not None), dtype=torch.uint8)
+        need = attention_paged_decode_workspace_bytes(cache, q.shape[1], max_len, window, sinks, weights is not None)
+        workspace = q.new_empty(need, dtype=torch.uint8) if need > 256 else None  # (256: none is used)
     check(_lib.lib().b2_attention_paged_decode(cache.struct, view, _heads_view(out, cache, "out"), lse.data_ptr(), max_len, scale, window, sinks,
-                                               _at(weights), _at(weights_out), ld, workspace.data_ptr(), workspace.numel(), _raw_stream()))
+                                               _at(weights), _at(weights_out), ld, _at(workspace), 0 if workspace is None else workspace.numel(), _raw_stream()))
     return out, lse
 
 
