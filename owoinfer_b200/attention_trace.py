@@ -26,7 +26,7 @@ def build_trace() -> str:
     build.build()
     obj = os.path.join(build.OBJ, "attention_trace.o")
     src = os.path.join(build.CSRC, "attention.cu")
-    if build._stale(obj, [src, os.path.join(build.CSRC, "common.cuh")]):
+    if build._stale(obj, [src, *(os.path.join(build.CSRC, h) for h in build.HEADERS)]):
         subprocess.check_call([build.NVCC, *build.FLAGS, "-DB2_ATTN_TRACE", "-c", src, "-o", obj])
     others = [os.path.join(build.OBJ, s.replace(".cu", ".o")) for s in build.SOURCES if s != "attention.cu"]
     if build._stale(TRACE_LIB, [obj, *others]):
