@@ -74,18 +74,18 @@ __device__ __forceinline__ std::uint32_t seen_mask(int at, int hi, int lo, int f
   return below(hi + 1 - at) & (~below(lo + 1 - at) | below(first - at));
 }
 
-#ifndef B2_FMA_PAIRS
-#define B2_FMA_PAIRS 2
-#endif
-constexpr int kFmaPairs = B2_FMA_PAIRS;
-// 2^x for a pair of x above -126 (below: 2^-126) on the FMA unit, which the softmax leaves half idle while the hardware's exponential, 16 results
+constexpr int kFmaPairs = 2;  // of every 8
+// 2^x for a pair of x on the FMA unit, which the softmax leaves half idle while the hardware's exponential, 16 results
 // a clock and SM, sets its pace: x = n + f with n whole and f in [-1/2, 1/2] (the sum with 1.5 * 2^23 rounds), 2^f by the polynomial
-// of degree 4 with the least largest relative error on that interval (2.6e-6; Remez exchange), n added to its exponent. What is past
+// of degree 4 with the least largest relative error on that interval (2.6e-6; Remez exchange), n added to its exponent. Below
+// -126.5 what is left is a subnormal number, and below -127 one that is 0 in 16 bits: kFloor is the float above -127, where the polynomial is
+// just above 1 and the exponent's field just empty. (2^-126 for what is not seen, times the largest bf16, would be 4.) What is past
 // 127 or NaN gives nonsense: the caller looks at the largest x.
 __device__ __forceinline__ void exp2_fma(std::uint64_t x, float& a, float& b) {
+  constexpr float kFloor = -127.0f + 0x1p-17f;
   float x0, x1;
   unpack2(x, x0, x1);
-  const std::uint64_t low = pack2(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
+  const std::uint64_t low = pack2(fmaxf(x0, kFloor), fmaxf(x1, kFloor));
   const std::uint64_t t = add2(low, pack2(12582912.0f, 12582912.0f)), n = add2(t, pack2(-12582912.0f, -12582912.0f));
   const std::uint64_t f = fma2(n, pack2(-1.0f, -1.0f), low);
   std::uint64_t p = fma2(f, pack2(0.009570102207362652f, 0.009570102207362652f), pack2(0.05591785907745361f, 0.05591785907745361f));

@@ -341,6 +341,21 @@ def check_decode(cache, q, window, sinks, scale, got, lse, dtype, weights=None, 
             assert torch.equal(weights_out[b, :, end:].double(), want[:, end:])
 
 
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (BF16, 64), (F16, 64)])
+@pytest.mark.parametrize("window", [0, 64])
+def test_prompt_keeps_the_largest_hidden_values_out(dtype, d, window):
+    """What is not seen has a weight of 0, not of the smallest number: times the type's largest value that would be a value like any other."""
+    cache = make_cache([300], 2, d, 32, dtype)
+    q = torch.randn((300, 8, d), generator=torch.Generator().manual_seed(5)).to(dtype).cuda()
+    place = (cache.block_table[0, 192 // 32].item(), slice(None), slice(0, 16))  # slots 192 to 207
+    outs = []
+    for value in (0.0, torch.finfo(dtype).max, torch.finfo(dtype).min):
+        cache.v[place] = value
+        got, _ = ops.attention_paged(q, cache, cu_of([300]), 300, d ** -0.5, window=window)
+        outs.append(torch.cat([got[:192], got[207 + window:] if window else got[:0]]))
+    assert torch.equal(outs[1], outs[0]) and torch.equal(outs[2], outs[0])
+
+
 @pytest.mark.parametrize("with_weights", [False, True])
 @pytest.mark.parametrize("lens,hq,hk,d,page,dtype,window,sinks,outside", DECODE)
 def test_decode(lens, hq, hk, d, page, dtype, window, sinks, outside, with_weights):
