@@ -74,9 +74,11 @@ __device__ __forceinline__ std::uint32_t seen_mask(int at, int hi, int lo, int f
   return below(hi + 1 - at) & (~below(lo + 1 - at) | below(first - at));
 }
 
-constexpr int kFmaPairs = 2;  // of every 8
-// 2^x for a pair of x on the FMA unit, which the softmax leaves half idle while the hardware's exponential, 16 results
-// a clock and SM, sets its pace: x = n + f with n whole and f in [-1/2, 1/2] (the sum with 1.5 * 2^23 rounds), 2^f by the polynomial
+// Pairs of exponentials, of every 8, that exp2_fma computes: 8192 tokens, 32 / 8 heads of 128, and 509 over 8192 slots, 14 / 2 of 64: none
+// 494 and 51.3 us, one 488 and 49.4, two 493 and 49.0, three 517 and 51.2.
+constexpr int kFmaPairs = 1;
+// 2^x for a pair of x on the FMA unit, which the softmax leaves half idle while the hardware's exponential has 16
+// results a clock and SM: x = n + f with n whole and f in [-1/2, 1/2] (the sum with 1.5 * 2^23 rounds), 2^f by the polynomial
 // of degree 4 with the least largest relative error on that interval (2.6e-6; Remez exchange), n added to its exponent. Below
 // -126.5 what is left is a subnormal number, and below -127 one that is 0 in 16 bits: kFloor is the float above -127, where the polynomial is
 // just above 1 and the exponent's field just empty. (2^-126 for what is not seen, times the largest bf16, would be 4.) What is past
@@ -242,14 +244,19 @@ __device__ __forceinline__ void add_nonfinite(const PromptArgs& a, const Work& w
 //   warp 1      of CTA 0: S(t + 2) = Q K^T once S(t) has been read, O += P(t) V(t) once P(t) is there
 //   warp 2      V's arrival, and in tiles that some row does not see whole what would make NaN of a 0 in P (see below)
 //   warp 3      the list of works; Q of the next one
-//   warps 4-7   softmax of the even tiles, one thread per row: S into registers, the tile's maximum, P = exp2(c S - m), 16 bits wide, into
+//   warps 4-7   softmax of the even tiles, one thread per row: S into registers, the row's maximum, P = exp2(c S - m), 16 bits wide, into
 //               tensor memory columns of its own, so that neither S nor P ever waits for an MMA that still reads the other
-//   warps 8-11  the same for the odd tiles
-// With two query tiles a CTA and a softmax warpgroup each (P over S's columns), a tile's scores waited for its own P.V: softmax 1900 of a period
-// of 3770 clocks, for MMAs of 2050. Both warpgroups refer a row's exponentials to one m, which they hand to each other tile by
-// tile: P, its sum and O are floating point, so m only has to keep P in range, and stays until a score is kRaise binades above
-// it; then O is scaled, once the P.V before have landed. Tiles are counted through all works (t), so that loads, scores and the first
+//   warps 8-11  the same for the odd tiles, at the same time
+// Both warpgroups refer a row's exponentials to one m: they swap the row's maximum of an even and the odd tile behind it. P, its sum
+// and O are floating point, so m only has to keep P in range, and stays until a score is kRaise binades above it; then the even tile's
+// warpgroup scales O, once the P.V before have landed. Tiles are counted through all works (t), so that loads, scores and the first
 // softmax of a work go on while the one before is stored; a CTA per work spent 22 of 80 thousand clocks on its start and its end.
+// Bound by the softmax: about 3750 clocks for two tiles, 2230 of them the exponentials with what goes with them (two warps of a scheduler; the
+// unit for exponentials alone 1800), the rest loads, maxima and barriers, under which that unit idles; the MMAs need 2050. 8192 tokens, 32 / 8
+// heads of 128: 488 us, 1.13 PFLOP/s (568 us under the power cap of a long run). Measured and slower: a warpgroup per 128 rows, P over
+// S's columns (657 us); the warpgroups by turns, m handed on tile by tile (613); the maximum checked after the exponentials, which are
+// repeated if it has grown too much, warpgroups not in step (593); two threads a row, 16 warps (529); S a quarter at a time
+// from tensor memory in a loop a fourth as long (608); 64-slot tiles.
 template <typename T, int D>
 __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
 prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -265,7 +272,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   extern __shared__ std::uint8_t smem_raw[];
   // Barriers of the leader (CTA 0 of the pair): Q, K, V, P, "S is read" and "O is read", by both CTAs; in each CTA: what the MMAs have done.
   __shared__ __align__(8) std::uint64_t s_q[2], s_k[S::kStages], s_v[S::kStages], s_read[2], s_p[2], s_o_free;
-  __shared__ __align__(8) std::uint64_t s_q_free[2], s_k_free[S::kStages], s_v_free[S::kStages], s_v_here[S::kStages], s_scores[2], s_pv[2], s_q_here, s_swap[4], s_done, s_left[kList];
+  __shared__ __align__(8) std::uint64_t s_q_free[2], s_k_free[S::kStages], s_v_free[S::kStages], s_v_here[S::kStages], s_scores[2], s_pv[2], s_q_here, s_left[kList];
   __shared__ List s_list;
   __shared__ float s_top[2][2][kTile], s_last[2][2][kTile][2];  // the largest scores of a pair of tiles; by work the warpgroups' sums and m
   __shared__ std::uint32_t s_tmem_base, s_nonfinite[kMarks];
@@ -293,8 +300,6 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     }
     mbar_init(smem_u32(&s_o_free), 16);
     mbar_init(smem_u32(&s_q_here), 1);
-    mbar_init(smem_u32(&s_done), 8);
-    for (int q = 0; q < 4; ++q) mbar_init(smem_u32(&s_swap[q]), 2);
     for (int i = 0; i < kList; ++i) {
       mbar_init(smem_u32(&s_list.here[i]), 1);
       mbar_init(smem_u32(&s_left[i]), 8);
@@ -552,6 +557,12 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     const std::uint32_t s_cols = tmem + lane_off + kColS + static_cast<std::uint32_t>(group) * kTile, p_cols = tmem + lane_off + kColP + static_cast<std::uint32_t>(group) * (kTile / 2);
     const float c = a.scale_log2;
     bool dead = false;
+    // The two warps that have the same rows meet at a barrier of their own (496 us where mbarriers took 510). One that gives up, having set the abort word, arrives there once
+    // more: the other leaves its meeting and sees the word.
+    const auto meet = [&] {
+      asm volatile("barrier.sync.aligned %0, 64;" ::"r"(1 + quarter) : "memory");
+      return *abort_word == 0;
+    };
     Reader reader{&s_list, abort_word};
     for (;;) {
       Work w;
@@ -609,9 +620,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         if (both) {  // of both tiles
           float(&tops)[2][kTile] = s_top[odd & 1];
           tops[group][r_local] = top;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&s_swap[quarter]));
-          if (!warp_wait(smem_u32(&s_swap[quarter]), static_cast<std::uint32_t>(odd) & 1u)) {
+          if (!meet()) {
             dead = true;
             break;
           }
@@ -682,10 +691,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       if (dead) break;
       float(&last)[2][kTile][2] = s_last[index & 1];
       last[group][r_local][0] = l, last[group][r_local][1] = m;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&s_done));
+      if (!meet()) break;
       const int last_group = (w.count - 1) & 1, last_nth = (last_group == 0 ? w.t0 : w.u0) + (w.count - 1) / 2;
-      if (!warp_wait(smem_u32(&s_done), static_cast<std::uint32_t>(index) & 1u) || !warp_wait(smem_u32(&s_pv[last_group]), static_cast<std::uint32_t>(last_nth) & 1u)) {
+      if (!warp_wait(smem_u32(&s_pv[last_group]), static_cast<std::uint32_t>(last_nth) & 1u)) {
         dead = true;
         break;
       }
@@ -753,6 +761,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&s_left[place]));
     }
+    if (__any_sync(0xffffffffu, *abort_word != 0)) asm volatile("barrier.arrive.aligned %0, 64;" ::"r"(1 + quarter) : "memory");
   }
 
   tc_fence_before();
