@@ -16,7 +16,7 @@ constexpr int kStages = 2;      // steps of a warp in shared memory: the one it 
 constexpr int kRows = 16;       // query heads of a CTA: the rows of an MMA
 constexpr int kMostCluster = 8, kClusterSteps = 16;  // CTAs that join their parts in shared memory; steps of each at most
 constexpr int kJoinThreads = 256;
-constexpr int kJoinSlots = 4;
+constexpr int kJoinSlots = 4, kJoinHeads = 4, kJoinPerSm = 8;
 constexpr int kMostGroup = 4096;  // (a float each in shared memory)
 
 struct DecodeArgs {
@@ -425,7 +425,7 @@ __device__ __forceinline__ float joined_lse(const float2* ml, int parts, int lan
 
 // The parts of a (sequence, key head) joined: the first CTAs have its query heads, the others ranges of its slots.
 template <typename T, int D, bool kScores>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a, int head_ctas) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a, int head_ctas, int slices) {
   extern __shared__ __align__(16) float s_lse[];  // [group]
   __shared__ __align__(16) float4 s_sum[kJoinThreads];
   __shared__ float2 s_ml[kJoinThreads];
@@ -436,11 +436,13 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a, 
   const std::int64_t head0 = static_cast<std::int64_t>(b) * a.q_heads + h * a.group;
 
   if (static_cast<int>(blockIdx.x) < head_ctas) {
-    // Four channels a thread, a slice of the parts each: one pass with a running maximum, so that no load waits for another.
-    constexpr int kQuads = D / 4, kSlices = kJoinThreads / kQuads;
-    const int quad = static_cast<int>(threadIdx.x) % kQuads, slice = static_cast<int>(threadIdx.x) / kQuads;
+    // Four channels a thread, a slice of a head's parts each: one pass with a running maximum, so that no load waits for another.
+    constexpr int kQuads = D / 4;
+    const int quad = static_cast<int>(threadIdx.x) % kQuads, unit = static_cast<int>(threadIdx.x) / kQuads, slice = unit % slices;
+    const int heads = kJoinThreads / kQuads / slices;  // of a CTA at a time
     wait_for_predecessors();
-    for (int g = blockIdx.x; g < a.group; g += head_ctas) {
+    for (int g0 = static_cast<int>(blockIdx.x) * heads; g0 < a.group; g0 += head_ctas * heads) {
+      const int g = min(g0 + unit / slices, a.group - 1);  // (behind the last: the last again, not stored)
       const float2* ml = a.part_ml + (head0 + g) * a.splits;
       const float* part = a.part_o + (head0 + g) * a.splits * D + quad * 4;
       float m = -INFINITY, l = 0.f;
@@ -452,23 +454,25 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a, 
         sum.x = fmaf(f, x.x, keep * sum.x), sum.y = fmaf(f, x.y, keep * sum.y);
         sum.z = fmaf(f, x.z, keep * sum.z), sum.w = fmaf(f, x.w, keep * sum.w);
       };
-      for (int i0 = slice; i0 < parts; i0 += 4 * kSlices) {
+      for (int i0 = slice; i0 < parts; i0 += 4 * slices) {
         float2 of[4];
         float4 x[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int at = i0 + i * kSlices;
+          const int at = i0 + i * slices;
           of[i] = at < parts ? ml[at] : make_float2(0.f, 0.f);
           if (at < parts) x[i] = *reinterpret_cast<const float4*>(part + static_cast<std::int64_t>(at) * D);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) add(of[i].x, of[i].y, x[i]);
       }
-      __syncthreads();  // (the slices of the head before are read)
-      s_sum[threadIdx.x] = sum, s_ml[threadIdx.x] = make_float2(m, l);
-      __syncthreads();
-      if (slice == 0) {
-        for (int i = 1; i < min(kSlices, parts); ++i) add(s_ml[i * kQuads + quad].x, s_ml[i * kQuads + quad].y, s_sum[i * kQuads + quad]);
+      if (slices > 1) {
+        __syncthreads();  // (the slices of the heads before are read)
+        s_sum[threadIdx.x] = sum, s_ml[threadIdx.x] = make_float2(m, l);
+        __syncthreads();
+      }
+      if (slice == 0 && g0 + unit / slices < a.group) {
+        for (int i = 1; i < min(slices, parts); ++i) add(s_ml[threadIdx.x + i * kQuads].x, s_ml[threadIdx.x + i * kQuads].y, s_sum[threadIdx.x + i * kQuads]);
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         T* out = static_cast<T*>(a.out) + b * a.o_row + (h * a.group + g) * a.o_head + quad * 4;
         *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(sum.x * inv, sum.y * inv), pack16<T>(sum.z * inv, sum.w * inv));
@@ -483,25 +487,41 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a, 
     constexpr int kRange = kJoinThreads * kJoinSlots;
     const int first = (static_cast<int>(blockIdx.x) - head_ctas) * kRange;
     if (first >= len) return;
-    wait_for_predecessors();
-    for (int g = warp; g < a.group; g += kJoinThreads / 32) {
-      const float lse2 = joined_lse(a.part_ml + (head0 + g) * a.splits, parts, lane);
-      if (lane == 0) s_lse[g] = lse2;
-    }
-    __syncthreads();
     const std::int64_t row = (static_cast<std::int64_t>(b) * a.c.kv_heads + h) * a.weights_ld;
-    for (int j0 = first + static_cast<int>(threadIdx.x); j0 < len; j0 += (static_cast<int>(gridDim.x) - head_ctas) * kRange) {
-      float sum[kJoinSlots], got[kJoinSlots] = {};
-      bool seen[kJoinSlots];
+    wait_for_predecessors();
+    // The scores of kJoinHeads heads and the sums so far are on their way while the heads' logarithms are made.
+    float sum[kJoinSlots], early[kJoinHeads][kJoinSlots];
+    bool seen[kJoinSlots];
+    const auto fetch = [&](int j0) {
 #pragma unroll
       for (int i = 0; i < kJoinSlots; ++i) {
         const int j = j0 + i * kJoinThreads;
         seen[i] = sees(a, len, j);
         sum[i] = j < len - 1 ? a.weights[row + j] : 0.f;
+#pragma unroll
+        for (int g = 0; g < kJoinHeads; ++g) early[g][i] = seen[i] && g < a.group ? a.scores[(head0 + g) * a.scores_ld + j] : 0.f;
+      }
+    };
+    fetch(first + static_cast<int>(threadIdx.x));
+    for (int g = warp; g < a.group; g += kJoinThreads / 32) {
+      const float lse2 = joined_lse(a.part_ml + (head0 + g) * a.splits, parts, lane);
+      if (lane == 0) s_lse[g] = lse2;
+    }
+    __syncthreads();
+    const int step = (static_cast<int>(gridDim.x) - head_ctas) * kRange;
+    for (int j0 = first + static_cast<int>(threadIdx.x); j0 < len; j0 += step) {
+      float got[kJoinSlots] = {};
+#pragma unroll
+      for (int g = 0; g < kJoinHeads; ++g) {
+        if (g >= a.group) break;
+#pragma unroll
+        for (int i = 0; i < kJoinSlots; ++i) {
+          if (seen[i]) got[i] += ex2(early[g][i] - s_lse[g]);
+        }
       }
       const float* s = a.scores + head0 * a.scores_ld + j0;
 #pragma unroll 4
-      for (int g = 0; g < a.group; ++g) {
+      for (int g = kJoinHeads; g < a.group; ++g) {
 #pragma unroll
         for (int i = 0; i < kJoinSlots; ++i) {
           if (seen[i]) got[i] += ex2(s[g * a.scores_ld + i * kJoinThreads] - s_lse[g]);
@@ -511,6 +531,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a, 
       for (int i = 0; i < kJoinSlots; ++i) {
         if (j0 + i * kJoinThreads < len) a.weights_out[row + j0 + i * kJoinThreads] = sum[i] + got[i];
       }
+      if (j0 + step < len) fetch(j0 + step);
     }
   }
 }
@@ -587,9 +608,15 @@ int launch(const char* op, const DecodeArgs& a, const Plan& p, const CUtensorMap
   if (const int rc = allow_shared(op, kernel, smem, allowed)) return rc;
   if (const int rc = enqueue(op, kernel, grid, kThreads, smem, st, 1, map_k, map_v, a)) return rc;
   if (!p.parts) return B2_OK;
-  const int head_ctas = std::min(a.group, 64), range = kJoinThreads * kJoinSlots, slot_ctas = kScores ? (a.c.most + range - 1) / range : 0;
+  // A slice has four parts in flight at once. Slot CTAs: eight per SM, so that the lengths of a batch even out.
+  constexpr int units = kJoinThreads / (D / 4), range = kJoinThreads * kJoinSlots;
+  int slices = 1;
+  while (slices < units && 4 * slices < p.splits) slices *= 2;
+  const int heads = units / slices, head_ctas = std::min((a.group + heads - 1) / heads, 64);
+  const std::int64_t most = (static_cast<std::int64_t>(a.c.most) + range - 1) / range, pairs = static_cast<std::int64_t>(a.c.kv_heads) * a.c.batch;
+  const int slot_ctas = kScores ? static_cast<int>(std::min(most, (static_cast<std::int64_t>(kJoinPerSm) * sm_count() + pairs - 1) / pairs)) : 0;
   return enqueue(op, join_kernel<T, D, kScores>, dim3(static_cast<unsigned>(head_ctas + slot_ctas), static_cast<unsigned>(a.c.kv_heads), batch), kJoinThreads,
-                 kScores ? static_cast<std::size_t>(a.group) * 4 : 0, st, 1, a, head_ctas);
+                 kScores ? static_cast<std::size_t>(a.group) * 4 : 0, st, 1, a, head_ctas, slices);
 }
 
 }  // namespace
