@@ -14,7 +14,7 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kKeys = 16;       // slots of a step of a warp: a page holds a multiple of it
 constexpr int kStages = 2;      // steps of a warp in shared memory: the one it works on and the one on its way
 constexpr int kRows = 16;       // query heads of a CTA: the rows of an MMA
-constexpr int kMostCluster = 8, kClusterSteps = 16;  // CTAs that join their parts in shared memory; steps of each at most
+constexpr int kMostCluster = 8, kClusterSteps = 24;  // CTAs that join their parts in shared memory; steps of each at most
 constexpr int kJoinThreads = 256;
 constexpr int kJoinSlots = 4, kJoinHeads = 4, kJoinPerSm = 8;
 constexpr int kMostGroup = 4096;  // (a float each in shared memory)
@@ -540,10 +540,14 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a, 
 // slots, 4 key heads: 53 us; three per SM 58, six 76). Several, whose lengths differ: eighteen, handed out as SMs come free (64 of up to 8101, 8
 // key heads: 196 us; three per SM 233), but of kLongEnough steps at least, since each has its start and its part to join
 // (4 of up to 30001: 76 us; as eighteen per SM 79).
-// Few short ones, whose clusters all run at once, are joined by the CTAs of a cluster in shared memory: one launch instead of
-// two and no workspace, some 2 us of the host's time. Six of up to 500 slots, 8 key heads: 10.4 us, with the second kernel
-// 16.5; of up to 2000, 16.5 and 19.3; of up to 4000, 24.0 and 22.6, so it ends at kClusterSteps. One sequence has too few CTAs
-// that way sooner (160 slots: 6.9 us and 8.3; 517: 8.3 and 8.3; 1000: 9.8 and 8.3; 2000: 12.4 and 10.3) and ends at half of it.
+// Short ones are joined by the CTAs of a cluster in shared memory (by one CTA, where there are enough of them): one launch instead of two and
+// no workspace, some 2 us of the host's time. Slots, and us with the second kernel and so: 6 sequences, 32 / 8 heads of 128: 500 15.8 and
+// 10.8, 2000 18.5 and 16.7, 2600 19.2 and 19.9; 16: 500 16.5 and 12.6; 30, 14 / 2 of 64: 1000 16.0 and 11.0, 2000 16.6 and 14.4; so up to
+// kClusterSteps a CTA. Five sixths of what fits on the SMs by shared memory, since a cluster wants its SMs side by side (60 clusters of
+// seven at 3 CTAs an SM: 21 us, of six 14.4; 55 of six where 2 fit on an SM: 30.5, with the second kernel 20.6). One sequence has too few
+// CTAs that way sooner (160 slots: 6.9 and 8.3; 517: 8.3 and 8.3; 1000: 9.8 and 8.3) and ends at a third of the steps.
+constexpr std::int64_t kSharedOfSm = 228 * 1024;
+constexpr int ring_bytes(int d) { return kWarps * kStages * 2 * kKeys * d * 2; }
 constexpr int kOneSequence = 2, kSeveral = 18, kLongEnough = 32, kShortest = kWarps;
 
 struct Plan {
@@ -562,8 +566,11 @@ Plan plan(const PagedArgs& c, int q_heads, int head_dim, int window, int sinks, 
   std::int64_t chunk = (steps * units + ctas - 1) / ctas;
   if (c.batch > 1) chunk = std::max<std::int64_t>(chunk, kLongEnough);
   chunk = std::max<std::int64_t>(chunk, kShortest);
-  p.cluster = group <= kRows && units * kMostCluster <= 3LL * sm_count() && steps <= kMostCluster * (c.batch <= 1 ? kClusterSteps / 2 : kClusterSteps);
-  if (p.cluster) chunk = std::max<std::int64_t>((steps + kMostCluster - 1) / kMostCluster, kShortest);
+  const std::int64_t at_once = 5LL * sm_count() / 6, each = std::max<std::int64_t>(1, std::min<std::int64_t>(kMostCluster, 3 * at_once / units));
+  const std::int64_t share = std::max<std::int64_t>((steps + each - 1) / each, kShortest);
+  const std::int64_t per_sm = kSharedOfSm / (ring_bytes(head_dim) + (weights ? group * share * kKeys * 4 : 0) + 4096);
+  p.cluster = group <= kRows && share <= (c.batch <= 1 ? kClusterSteps / 3 : kClusterSteps) && (per_sm >= 3 || units * each <= per_sm * at_once);
+  if (p.cluster) chunk = share;
   p.chunk = static_cast<int>(std::min<std::int64_t>(chunk, INT_MAX / 2));
   p.splits = static_cast<int>(std::max<std::int64_t>(1, (steps + p.chunk - 1) / p.chunk));
   p.parts = !p.cluster && (p.splits > 1 || weights);
@@ -590,7 +597,7 @@ int check(const char* op, const b2_paged_cache* cache, PagedArgs* c, int q_heads
 
 template <typename T, int D, bool kScores>
 int launch(const char* op, const DecodeArgs& a, const Plan& p, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t st) {
-  constexpr int ring = kWarps * kStages * 2 * kKeys * D * 2, meet = (kWarps * kRows * (D + 4 + 2) + 2 * kRows) * 4;
+  constexpr int ring = ring_bytes(D), meet = (kWarps * kRows * (D + 4 + 2) + 2 * kRows) * 4;
   static_assert(meet <= ring);
   const LaunchChain chain(st);
   const unsigned blocks = static_cast<unsigned>((a.group + kRows - 1) / kRows), batch = static_cast<unsigned>(a.c.batch);
