@@ -423,7 +423,9 @@ __device__ __forceinline__ float joined_lse(const float2* ml, int parts, int lan
   return ll == 0.f ? INFINITY : mm + log2f(ll);
 }
 
-// The parts of a (sequence, key head) joined: the first CTAs have its query heads, the others ranges of its slots.
+// The parts of a (sequence, key head) joined: the first CTAs have its query heads, the others ranges of its slots, which add up what those
+// got: ex2 of the scores that the first kernel left minus the row's logarithm. Bound by latency (lengths, parts, scores one after the
+// other): 64 sequences of up to 8101 slots, 32 / 8 heads, 20 us behind the first kernel for 50 MB; as a CTA per 1024 slots and head, 27.
 template <typename T, int D, bool kScores>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a, int head_ctas, int slices) {
   extern __shared__ __align__(16) float s_lse[];  // [group]
