@@ -256,7 +256,8 @@ __device__ __forceinline__ void add_nonfinite(const PromptArgs& a, const Work& w
 // heads of 128: 488 us, 1.13 PFLOP/s (568 us under the power cap of a long run). Measured and slower: a warpgroup per 128 rows, P over
 // S's columns (657 us); the warpgroups by turns, m handed on tile by tile (613); the maximum checked after the exponentials, which are
 // repeated if it has grown too much, warpgroups not in step (593); two threads a row, 16 warps (529); S a quarter at a time
-// from tensor memory in a loop a fourth as long (608); 64-slot tiles.
+// from tensor memory in a loop a fourth as long (608); two threads a row and the groups by turns (532: the warp that issues the MMAs is then
+// busy all the time, 2100 clocks a tile, half of them waits and instructions between the MMAs); P.V issued by a warp of its own (695).
 template <typename T, int D>
 __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
 prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -634,8 +635,14 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
           alpha = m == -INFINITY ? 0.f : ex2(m - (top - kShift));  // (nothing seen yet: O is 0)
           m = top - kShift, l *= alpha;
         }
+        if (!warp_wait(smem_u32(&s_pv[group]), phase ^ 1u)) {  // the P before this one has been read
+          dead = true;
+          break;
+        }
+        tc_fence_after();
         if (__builtin_expect(group == 0 && j > 1 && __any_sync(0xffffffffu, raise), 0)) {
-          // O times alpha, once the P.V of the tiles before have landed and ahead of this warpgroup's P, whose P.V comes first.
+          // O times alpha, once the P.V of the tiles before have landed and ahead of this warpgroup's P, whose P.V comes first. (The wait above
+          // has seen to it that the odd tile's barrier is at most one phase behind.)
           if (!warp_wait(smem_u32(&s_pv[1]), static_cast<std::uint32_t>(odd - 1) & 1u)) {
             dead = true;
             break;
@@ -652,11 +659,6 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             tmem_st_32x16(o_cols + cc, o);
           }
         }
-        if (!warp_wait(smem_u32(&s_pv[group]), phase ^ 1u)) {  // the P before this one has been read
-          dead = true;
-          break;
-        }
-        tc_fence_after();
         const float bias = m == -INFINITY ? 0.f : -m;  // (a row that has seen nothing: 2^-infinity)
         const std::uint64_t c2 = pack2(c, c), m2 = pack2(bias, bias);
         std::uint64_t sum_a = pack2(0.f, 0.f), sum_b = sum_a;
