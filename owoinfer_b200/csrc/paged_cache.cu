@@ -278,15 +278,12 @@ __device__ __forceinline__ unsigned sum_before(unsigned v, unsigned (&s_warp)[kS
 // which the running count from above reaches what may stay. (Bytes put the weights of a cache into a dozen bins of the first
 // histogram, where a warp's additions to one word wait for one another.) Then every CTA counts what stays of its share, and
 // writes it behind what the CTAs before it keep. Bound by the latency of its dozen steps between barriers, not by the weights' bytes.
-__global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs a) {
-  dependents_may_start();
+__device__ __forceinline__ void select(const EvictArgs& a, int h, int b, int len, int ctas, int rank) {
   __shared__ __align__(16) unsigned s_hist[2][kBins];
   __shared__ unsigned s_warp[kSelectWarps];
   __shared__ __align__(8) uint2 s_count;
   __shared__ unsigned s_pick[2];
-  const int ctas = gridDim.x, rank = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
-  const int len = paged_len(a.c, b);
   const std::int64_t row = static_cast<std::int64_t>(b) * a.c.kv_heads + h;
   const float* w = a.weights + row * a.weights_ld;
   float* w_out = a.weights_out == nullptr ? nullptr : a.weights_out + row * a.weights_out_ld;
@@ -430,27 +427,17 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs 
   }
 }
 
-constexpr int kMoveThreads = 256;
-constexpr int kMoveRows = 4;  // rows of K and of V that a group of lanes has in flight
-
-// kept -> the new pages: a group of D / 8 lanes moves kMoveRows rows of K and of V, 16 bytes a lane. 64 heads of 4096 kept slots of 128: 46 us,
-// 5.8 TB/s. (Within the select kernel, a CTA a head, it saved a launch and lost what the few CTAs cannot stream: 512 slots of 8 heads
-// 11.7 and 16.3 us.)
-template <int D>
-__global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictArgs a) {
-  constexpr int kLanes = D / 8, kGroups = kMoveThreads / kLanes;
-  const int h = blockIdx.y, b = blockIdx.z, lane = static_cast<int>(threadIdx.x) % kLanes, group = static_cast<int>(threadIdx.x) / kLanes;
-  wait_for_predecessors();
-  const int len = min(paged_len(a.c, b), a.budget);
-  const int row0 = static_cast<int>(blockIdx.x) * (kGroups * kMoveRows) + group;
-  if (row0 >= len) return;
+// Rows row0, row0 + step, … of the new pages from the slots in `kept`, kRows of K and of V in flight: a group of D / 8 lanes, 16 bytes each.
+template <int D, int kRows>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int b, int h, int row0, int step, int len) {
+  const int lane = static_cast<int>(threadIdx.x) % (D / 8);
   const std::int32_t* kept = a.kept + (static_cast<std::int64_t>(b) * a.c.kv_heads + h) * a.budget;
   const std::uint16_t *k = static_cast<const std::uint16_t*>(a.c.k), *v = static_cast<const std::uint16_t*>(a.c.v);
-  uint4 kr[kMoveRows], vr[kMoveRows];
-  std::int64_t to[kMoveRows];
+  uint4 kr[kRows], vr[kRows];
+  std::int64_t to[kRows];
 #pragma unroll
-  for (int i = 0; i < kMoveRows; ++i) {
-    const int r = row0 + i * kGroups;
+  for (int i = 0; i < kRows; ++i) {
+    const int r = row0 + i * step;
     to[i] = -1;
     if (r >= len) continue;
     const int slot = kept[r], page = paged_page(a.c, b, slot), page_to = a.table_out[b * a.table_out_ld + (r >> a.c.page_shift)];
@@ -462,11 +449,42 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictArgs a) {
     vr[i] = *reinterpret_cast<const uint4*>(v + from);
   }
 #pragma unroll
-  for (int i = 0; i < kMoveRows; ++i) {
+  for (int i = 0; i < kRows; ++i) {
     if (to[i] < 0) continue;
     *reinterpret_cast<uint4*>(static_cast<std::uint16_t*>(a.c.k) + to[i]) = kr[i];
     *reinterpret_cast<uint4*>(static_cast<std::uint16_t*>(a.c.v) + to[i]) = vr[i];
   }
+}
+
+__global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictArgs a) {
+  dependents_may_start();
+  select(a, blockIdx.y, blockIdx.z, paged_len(a.c, blockIdx.z), gridDim.x, blockIdx.x);
+}
+
+constexpr int kMoveThreads = 256;
+constexpr int kMoveRows = 4;  // rows of K and of V that a group of lanes has in flight
+
+// kept -> the new pages. 64 heads of 4096 kept slots of 128: 46 us, 5.8 TB/s.
+template <int D>
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictArgs a) {
+  constexpr int kGroups = kMoveThreads / (D / 8);
+  const int h = blockIdx.y, b = blockIdx.z;
+  wait_for_predecessors();
+  move_rows<D, kMoveRows>(a, b, h, static_cast<int>(blockIdx.x) * (kGroups * kMoveRows) + static_cast<int>(threadIdx.x) / (D / 8), kGroups,
+                          min(paged_len(a.c, b), a.budget));
+}
+
+// Both at once for a few heads: the first CTA of a cluster selects, all of them move. One launch less, 2 us of the host's time; on the device
+// 8 heads of 1100 slots to 512 10.3 us (two kernels 10.9), 2000 to 1024 12.4 (12.4). Past two rows a group of lanes the move wants more
+// SMs (4000 to 2048: 16.5 and 14.4), and 16 heads are more clusters than fit at a time (1000 to 512: 19.8 and 12.4).
+constexpr int kEvictCtas = 8, kEvictRows = 2;
+template <int D>
+__global__ void __launch_bounds__(kSelectThreads) evict_kernel(const EvictArgs a) {
+  const int h = blockIdx.y, b = blockIdx.z, len = paged_len(a.c, b);
+  if (blockIdx.x == 0) select(a, h, b, len, 1, 0);
+  cluster_sync_all();  // (releases and acquires what the first CTA wrote, too)
+  constexpr int kGroups = kSelectThreads / (D / 8);
+  move_rows<D, kEvictRows>(a, b, h, static_cast<int>(blockIdx.x) * kGroups + static_cast<int>(threadIdx.x) / (D / 8), kEvictCtas * kGroups, min(len, a.budget));
 }
 
 template <typename T, int D>
@@ -640,9 +658,15 @@ int b2_kv_evict(const b2_paged_cache* cache, const float* weights, int64_t weigh
   int ctas = 1;
   while (ctas < kMostSelectCtas && static_cast<std::int64_t>(ctas) * kSelectRound < slots) ctas *= 2;
   const unsigned heads = static_cast<unsigned>(cache->kv_heads), batch = static_cast<unsigned>(cache->batch);
+  const std::int64_t most = std::min<std::int64_t>(budget, slots);
+  if (ctas == 1 && most <= kEvictCtas * kEvictRows * (kSelectThreads / (cache->head_dim / 8)) &&
+      static_cast<std::int64_t>(heads) * batch * kEvictCtas <= sm_count() * 5 / 8) {
+    const dim3 grid(kEvictCtas, heads, batch);
+    return cache->head_dim == 128 ? enqueue(op, evict_kernel<128>, grid, kSelectThreads, 0, st, kEvictCtas, a)
+                                  : enqueue(op, evict_kernel<64>, grid, kSelectThreads, 0, st, kEvictCtas, a);
+  }
   if (const int rc = enqueue(op, select_kernel, dim3(static_cast<unsigned>(ctas), heads, batch), kSelectThreads, 0, st, ctas, a)) return rc;
   const int rows = kMoveThreads / (cache->head_dim / 8) * kMoveRows;
-  const std::int64_t most = std::min<std::int64_t>(budget, slots);
   if (most == 0) return B2_OK;
   const dim3 grid(static_cast<unsigned>((most + rows - 1) / rows), heads, batch);
   return cache->head_dim == 128 ? enqueue(op, move_kernel<128>, grid, kMoveThreads, 0, st, 1, a) : enqueue(op, move_kernel<64>, grid, kMoveThreads, 0, st, 1, a);

@@ -440,6 +440,8 @@ EVICT = [
     ([500, 301], 2, 128, 64, BF16, 4, 50, 300, "equal", False),
     ([500], 2, 128, 16, BF16, 0, 0, 77, "few", False),
     ([500], 1, 64, 16, BF16, 3, 0, 100, "odd", False),
+    ([700, 3, 0], 8, 128, 32, BF16, 4, 30, 200, "random", True),    # many heads, few slots
+    ([3000], 2, 128, 64, BF16, 4, 500, 2100, "few", False),        # few heads, many slots that stay
     ([9000, 8193], 2, 64, 128, F16, 4, 100, 4000, "few", False),   # two CTAs to a head
     ([70000], 1, 64, 256, BF16, 4, 1000, 20001, "random", False),  # the most CTAs, more than one round of each
     ([70000, 69999], 1, 64, 256, BF16, 0, 0, 65537, "few", False),
