@@ -92,8 +92,8 @@ constexpr float kRaise = 8.0f;
 // bring its own steps of 16 slots (whose 16 rows a page holds in one piece) and keeps its own maxima, sums and output rows in
 // registers; they meet at the end. Q·K^T and P·V are 16-row MMAs with the group's query heads as rows: the cache is read once
 // for all of them. At one byte of cache to every group / 2 multiply-adds the memory bounds it; 128-row tensor tiles would be
-// filled to group / 128. 64 sequences of up to 8101 slots, 32 / 8 heads of 128: 194 us, 6.5 TB/s with the join; one of 131001,
-// 16 / 4 heads: 53 us, 5.1 TB/s.
+// filled to group / 128. 64 sequences of up to 8101 slots, 32 / 8 heads of 128, with weights: 200 us, 6.3 TB/s (the
+// call 219); one of 131001, 32 / 4 heads in fp16: 50 us, 5.3 TB/s (59).
 template <typename T, int D, bool kScores, bool kCluster>
 __global__ void __launch_bounds__(kThreads, 3)
 decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const DecodeArgs a) {
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a, 
 }
 
 // How a call is cut into CTAs, by their number per SM, of which three fit at a time. One sequence: two equal CTAs per SM (131001
-// slots, 4 key heads: 53 us; three per SM 58, six 76). Several, whose lengths differ: eighteen, handed out as SMs come free (64 of up to 8101, 8
+// slots, 4 key heads, this kernel: 53 us; three per SM 58, six 76). Several, whose lengths differ: eighteen, handed out as SMs come free (64 of up to 8101, 8
 // key heads: 196 us; three per SM 233), but of kLongEnough steps at least, since each has its start and its part to join
 // (4 of up to 30001: 76 us; as eighteen per SM 79).
 // Short ones are joined by the CTAs of a cluster in shared memory (by one CTA, where there are enough of them): one launch instead of two and
