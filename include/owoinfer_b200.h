@@ -709,7 +709,8 @@ int b2_qk_norm_rope_append(const b2_paged_cache* cache, const void* qkv, int64_t
 /* Attention of a prompt's tokens over the cache that holds their keys and values already. Token i of the n a sequence has
  * in the call sits at slot p = seq_len - n + i and sees the slots j <= p with j < sinks or p - j < window (window 0: every
  * j <= p). out = softmax(scale * q k^T) v; lse (fp32 [tokens, q_heads], or NULL) = log sum exp(scale * q k^T). A token that
- * sees nothing (a cache shorter than the call's tokens) gets zeros and -infinity. q, out: views of one dtype [tokens,
+ * sees nothing (a cache shorter than the call's tokens, or scores that are all -infinity) gets zeros and -infinity; one that sees a score
+ * of NaN or +infinity gets NaN in out and lse. q, out: views of one dtype [tokens,
  * q_heads, head_dim]; max_q: no sequence has more tokens in the call. Keys and values of slots that a token does not see do
  * not reach its output, NaN and infinities included.
  * workspace: b2_attention_paged_workspace_bytes() of the same arguments, 256-byte aligned (few tokens over a long cache: parts of the

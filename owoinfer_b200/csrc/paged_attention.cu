@@ -701,10 +701,12 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       }
       tc_fence_after();
       m = fmaxf(last[0][r_local][1], last[1][r_local][1]);  // (a last even tile may have raised it alone)
-      l = 0.f;
+      // A row that has seen nothing still has m at minus infinity; so has one with a NaN or an infinity among the scores of every pair of tiles,
+      // whose sums say so. (What the polynomial leaves of an unseen score is in the sums too: they are no sign of the former.)
+      const bool undefined = isnan(last[0][r_local][0]) || isnan(last[1][r_local][0]), empty = m == -INFINITY && !undefined;
+      l = undefined ? __int_as_float(0x7FC00000) : 0.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i) l += last[i][r_local][0] == 0.f ? 0.f : last[i][r_local][0] * ex2(last[i][r_local][1] - m);
-      const bool empty = m == -INFINITY;
       const float inv = empty ? 0.f : 1.0f / l;
       const bool repair = *const_cast<volatile std::uint32_t*>(&s_nonfinite[index % kMarks]) == static_cast<std::uint32_t>(index) + 1u;
       // Half of the channels a warpgroup; O is free for the next work once they are in registers.

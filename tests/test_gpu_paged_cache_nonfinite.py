@@ -1,0 +1,99 @@
+"""Scores, keys, queries and values that are not finite, on paged key-value caches, against the definitions in 64 bits.
+
+A NaN or an infinity among the scores that a token sees makes its output and its lse NaN (the definition subtracts the largest score); a score
+of minus infinity is a weight of 0, and a token all of whose scores are that is one that sees nothing: zeros and minus infinity. The tolerances
+of finite values are those of test_gpu_paged_cache.py, where they are derived.
+"""
+import math
+
+import pytest
+import torch
+
+from owoinfer_b200 import ops
+from tests.test_gpu_paged_cache import BF16, F, F16, U, attention_64, cu_of, make_cache, near, rows_of, seen_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _clean_status():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    ops.paged_cache_status(clear=True)
+    yield
+    torch.cuda.synchronize()
+
+
+def put(cache, pool, b, slot, value, head=slice(None), channel=slice(None)):
+    pool[cache.block_table[b, slot // cache.page_size].item(), head, slot % cache.page_size, channel] = value
+
+
+def expect(cache, b, q, slots, window, sinks, scale):
+    """(out, lse, sum p |v|) of the tokens at `slots` of sequence b."""
+    end = int(cache.seq_lens[b])
+    want, lse, size, _ = attention_64(q, rows_of(cache, cache.k, b, end), rows_of(cache, cache.v, b, end), seen_of(slots, end, window, sinks), scale)
+    want[lse == -math.inf] = 0.0
+    size[lse == -math.inf] = 0.0
+    return want, torch.where(lse == math.inf, math.nan, lse), size
+
+
+def check(cache, q, new, scale, got, lse, dtype, window=0, sinks=0):
+    at = 0
+    for b, n in enumerate(new):
+        end = int(cache.seq_lens[b])
+        want, want_lse, size = expect(cache, b, q[at:at + n], torch.arange(end - n, end, device="cuda"), window, sinks, scale)
+        near(got[at:at + n], want, U[dtype] * want.abs() + (U[dtype] + F) * size + 1e-7, "out")
+        near(lse[at:at + n], want_lse, F * (1 + want_lse.abs()), "lse")
+        at += n
+
+
+def queries(tokens, heads, d, dtype):
+    return torch.randn((tokens, heads, d), generator=torch.Generator().manual_seed(9)).to(dtype).cuda()
+
+
+# ---------------------------------------------------------------------------------------------------- scores of a prompt
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 128), (BF16, 64), (F16, 64)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("n,slot", [(1, 0), (40, 0), (40, 1), (40, 5), (130, 129), (200, 16), (256, 128), (300, 0), (300, 260), (700, 300)])
+def test_prompt_with_a_key_that_is_not_finite(dtype, d, bad, n, slot):
+    """One channel of one key: every row that sees it, in the first pair of key tiles or behind it, and no others."""
+    cache = make_cache([n], 2, d, 16, dtype)
+    put(cache, cache.k, 0, slot, bad, channel=3)
+    q = queries(n, 4, d, dtype)
+    got, lse = ops.attention_paged(q, cache, cu_of([n]), n, d ** -0.5)
+    check(cache, q, [n], d ** -0.5, got, lse, dtype)
+    assert ops.paged_cache_status() == 0
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("n,window,sinks", [(1, 0, 0), (40, 0, 0), (300, 0, 0), (700, 64, 3)])
+def test_prompt_with_queries_that_are_not_finite(dtype, d, bad, n, window, sinks):
+    cache = make_cache([n], 2, d, 16, dtype)
+    q = queries(n, 4, d, dtype)
+    for token in {0, 1 % n, 7 % n, n // 2, n - 1}:
+        q[token, token % 4, 5] = bad
+    got, lse = ops.attention_paged(q, cache, cu_of([n]), n, d ** -0.5, window=window, sinks=sinks)
+    check(cache, q, [n], d ** -0.5, got, lse, dtype, window, sinks)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("slots", [[0], [1], [5], [3900], range(1300, 2600, 128), range(0, 5000, 128)])
+def test_prompt_in_parts_with_keys_that_are_not_finite(dtype, d, bad, slots):
+    """Few tokens over many slots: parts all of whose tiles have such a score, in a long sequence and in one of a single tile."""
+    lens, new = [5000, 100], [3, 2]
+    cache = make_cache(lens, 1, d, 32, dtype)
+    q = queries(sum(new), 4, d, dtype)
+    assert ops.attention_paged_workspace_bytes(cache, sum(new), 4, max(new)) > 256
+    for b in range(2):
+        for slot in slots:
+            if slot < lens[b]:
+                put(cache, cache.k, b, slot, bad, channel=slice(0, 2))
+    got, lse = ops.attention_paged(q, cache, cu_of(new), max(new), d ** -0.5)
+    check(cache, q, new, d ** -0.5, got, lse, dtype)
+    q[0, 0, 0] = q[4, 1, 0] = math.nan
+    clean = make_cache(lens, 1, d, 32, dtype)
+    got, lse = ops.attention_paged(q, clean, cu_of(new), max(new), d ** -0.5)
+    check(clean, q, new, d ** -0.5, got, lse, dtype)
