@@ -722,7 +722,8 @@ int b2_attention_paged(const b2_paged_cache* cache, const b2_view3* q, const b2_
 /* The same for one token per sequence (token b of q and out is sequence b's newest, at slot seq_len - 1), the cache's length
  * split over the GPU and joined. With weights_out != NULL the attention each slot got is added up besides:
  *   weights_out[b, h, j] = (j < seq_len - 1 ? weights[b, h, j] : 0) + sum of the softmax weight of slot j over h's query heads
- * for every slot j < seq_len; the others are left alone. weights, weights_out: device fp32, [batch, kv_heads, slots] with
+ * for every slot j < seq_len; the others are left alone. An infinity or NaN of V that the token sees is its channel's output, infinities of
+ * both signs are NaN. weights, weights_out: device fp32, [batch, kv_heads, slots] with
  * rows weights_ld apart (at least max_len, or the table's slots), the same buffer or two that do not overlap.
  * max_len: no sequence is longer (0: as long as the block table allows); the split goes by it.
  * workspace: b2_attention_paged_decode_workspace_bytes() of the same arguments (with_weights: whether weights_out is given), 256-byte aligned

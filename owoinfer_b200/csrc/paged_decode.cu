@@ -87,6 +87,32 @@ __device__ __forceinline__ void mma16<__half>(float (&d)[4], const std::uint32_t
 // keeps its relative precision however large it is (fp16: up to 2^8 of 2^16).
 constexpr float kRaise = 8.0f;
 
+// Four channels of an output in which something is not finite: where the token sees infinities or NaN of V in steps [begin, end), they are
+// the output, whatever their weights. P in two parts makes NaN of them, the second part being 0 or negative.
+template <typename T>
+__device__ __forceinline__ void take_nonfinite(const DecodeArgs& a, const Steps& steps, int begin, int end, int len, int b, int h, int d, float4& sum) {
+  float odd[4] = {};
+  unsigned found = 0;
+#pragma unroll 1
+  for (int i = begin * kKeys; i < end * kKeys; ++i) {
+    const int slot = steps.slot(i / kKeys) + i % kKeys;
+    const int page = sees(a, len, slot) ? paged_page(a.c, b, slot) : -1;
+    if (page < 0) continue;
+    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.c.v) + paged_row(a.c, page, h, slot) + d);
+    float x[4];
+    unpack16<T>(v.x, x[0], x[1]);
+    unpack16<T>(v.y, x[2], x[3]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (!isfinite(x[e])) odd[e] += x[e], found |= 1u << e;
+    }
+  }
+  if ((found & 1u) != 0u) sum.x = odd[0];
+  if ((found & 2u) != 0u) sum.y = odd[1];
+  if ((found & 4u) != 0u) sum.z = odd[2];
+  if ((found & 8u) != 0u) sum.w = odd[3];
+}
+
 // softmax(scale q·K^T)·V of one query row per head: o = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m), s in binades, m a running
 // reference. A CTA per (part of the cache, key head and block of 16 query heads, sequence). Its warps work apart: each has TMA
 // bring its own steps of 16 slots (whose 16 rows a page holds in one piece) and keeps its own maxima, sums and output rows in
@@ -329,6 +355,10 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       const float4 x = *reinterpret_cast<const float4*>(s_o + (w * kRows + row) * kLd + d);
       ll = fmaf(f, lw, ll);
       sum.x = fmaf(f, x.x, sum.x), sum.y = fmaf(f, x.y, sum.y), sum.z = fmaf(f, x.z, sum.z), sum.w = fmaf(f, x.w, sum.w);
+    }
+    if (__builtin_expect(!isfinite(sum.x + sum.y + sum.z + sum.w), 0)) {
+      if (ll == 0.f) sum = make_float4(0.f, 0.f, 0.f, 0.f);  // every score minus infinity
+      else take_nonfinite<T>(a, steps, begin, end, len, b, h, d, sum);
     }
     const std::int64_t head = static_cast<std::int64_t>(b) * a.q_heads + q_head0 + row;
     if constexpr (kCluster) {

@@ -97,3 +97,58 @@ def test_prompt_in_parts_with_keys_that_are_not_finite(dtype, d, bad, slots):
     clean = make_cache(lens, 1, d, 32, dtype)
     got, lse = ops.attention_paged(q, clean, cu_of(new), max(new), d ** -0.5)
     check(clean, q, new, d ** -0.5, got, lse, dtype)
+
+
+# ---------------------------------------------------------------------------------------------------- values that one token sees
+
+SEEN = [
+    # lens, q_heads, kv_heads, d, page, dtype, window, sinks, slots with a bad value
+    ([1], 4, 2, 128, 16, BF16, 0, 0, [0]),                          # its weight is 1: nothing is left for a second part
+    ([160], 4, 1, 64, 16, F16, 0, 0, [0, 77, 159]),                 # joined in a cluster
+    ([500, 33], 8, 2, 128, 32, BF16, 0, 0, [5, 32]),
+    ([300, 20], 80, 2, 64, 16, BF16, 0, 0, [19]),                   # one CTA to a sequence
+    ([5000], 8, 1, 128, 64, F16, 0, 0, [0, 4999]),                  # parts, joined by a second kernel
+    ([5000, 130], 6, 2, 64, 64, BF16, 64, 70, [3, 69, 129, 4990]),
+    ([9000, 8000, 7], 16, 2, 128, 128, BF16, 0, 0, [6, 8191]),
+]
+
+
+@pytest.mark.parametrize("with_weights", [False, True])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan, "both"])
+@pytest.mark.parametrize("lens,hq,hk,d,page,dtype,window,sinks,slots", SEEN)
+def test_decode_with_values_that_are_not_finite(lens, hq, hk, d, page, dtype, window, sinks, slots, bad, with_weights):
+    """An infinity that the token sees is its output's, infinities of both signs are NaN; the other channels and heads do not feel it."""
+    cache = make_cache(lens, hk, d, page, dtype, fill=math.nan)
+    for b, n in enumerate(lens):
+        for i, slot in enumerate(s for s in slots if s < n):
+            put(cache, cache.v, b, slot, math.inf if bad == "both" else bad, head=i % hk, channel=(7 * i) % d)
+            put(cache, cache.v, b, slot, -math.inf if bad == "both" else bad, head=hk - 1, channel=d - 1 - i)
+        if bad == "both" and slots[0] < n and n > 1:
+            put(cache, cache.v, b, n - 1, -math.inf, head=0, channel=0)
+    q = queries(len(lens), hq, d, dtype)
+    weights = torch.zeros((len(lens), hk, cache.slots), device="cuda") if with_weights else None
+    got, lse = ops.attention_paged_decode(q, cache, d ** -0.5, window=window, sinks=sinks, weights=weights)
+    for b, n in enumerate(lens):
+        want, want_lse, size = expect(cache, b, q[b:b + 1], torch.tensor([n - 1], device="cuda"), window, sinks, d ** -0.5)
+        near(got[b:b + 1], want, U[dtype] * want.abs() + (U[dtype] ** 2 + F) * size + 1e-7, "out")
+        near(lse[b:b + 1], want_lse, F * (1 + want_lse.abs()), "lse")
+    if with_weights:
+        assert bool(torch.isfinite(weights).all())
+    assert ops.paged_cache_status() == 0
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64)])
+def test_decode_with_an_infinite_value_of_no_weight(dtype, d):
+    """Where every score is minus infinity nothing is seen, infinities of V included; a small weight times infinity is infinity."""
+    cache = make_cache([40], 1, d, 16, dtype)
+    cache.k.zero_()
+    cache.k[..., 0] = -math.inf
+    put(cache, cache.v, 0, 9, math.inf, channel=2)
+    q = queries(1, 2, d, dtype)
+    q[..., 0] = 1.0
+    got, lse = ops.attention_paged_decode(q, cache, 0.5)
+    assert bool((got == 0).all()) and bool((lse == -math.inf).all())
+    cache.k[..., 0] = 0.0
+    put(cache, cache.k, 0, 20, 60.0, channel=0)  # a weight of e^-60 for the others
+    got, _ = ops.attention_paged_decode(q, cache, 1.0)
+    assert bool((got[..., 2] == math.inf).all()) and bool(torch.isfinite(got[..., 3:]).all())
