@@ -209,6 +209,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       qf[d][2] = at(r0, d * 16 + 8), qf[d][3] = at(r1, d * 16 + 8);
     }
   }
+  __syncthreads();  // s_abort is cleared before any wait looks at it (the copies and Q are on their way meanwhile)
   float o[D / 8][4] = {};
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
