@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "attention.cuh"
 #include "paged.cuh"
@@ -83,9 +84,15 @@ __device__ __forceinline__ void mma16<__half>(float (&d)[4], const std::uint32_t
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The reference of a row's exponentials is its first step's maximum, raised once a score is this many binades above it: P
-// keeps its relative precision however large it is (fp16: up to 2^8 of 2^16).
-constexpr float kRaise = 8.0f;
+// The reference of a row's exponentials is its first step's maximum less kShift binades, moved up once a score is kRaise binades above that
+// maximum. bf16 has fp32's range: P keeps its relative precision however large it is. fp16 ends at 2^16 and loses bits below 2^-14, P in two
+// parts below 2^-25 all of it: the largest of P is kept from 2^13 to 2^15, so that weights are held to 2^-38 of the largest. (From 1 to
+// 2^8, weights of 2^-18 lost a hundredth, and of 2^-25 everything.)
+template <typename T>
+struct Reference {
+  static constexpr bool kHalf = std::is_same<T, __half>::value;
+  static constexpr float kShift = kHalf ? 13.0f : 0.0f, kRaise = kHalf ? 2.0f : 8.0f;
+};
 
 // Four channels of an output in which something is not finite: where the token sees infinities or NaN of V in steps [begin, end), they are
 // the output, whatever their weights. P in two parts makes NaN of them, the second part being 0 or negative.
@@ -267,13 +274,13 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
     }
-    const auto above = [&](int i) { return m[i] == -INFINITY ? top[i] > -INFINITY : top[i] > m[i] + kRaise; };
+    const auto above = [&](int i) { return m[i] == -INFINITY ? top[i] > -INFINITY : top[i] > m[i] + (Reference<T>::kShift + Reference<T>::kRaise); };
     if (__any_sync(0xffffffffu, above(0) || above(1))) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (!above(i)) continue;
-        const float grow = ex2(m[i] - top[i]);  // 0 the first time
-        m[i] = top[i], l[i] *= grow;
+        const float to = top[i] - Reference<T>::kShift, grow = ex2(m[i] - to);  // 0 the first time
+        m[i] = to, l[i] *= grow;
 #pragma unroll
         for (int d = 0; d < D / 8; ++d) o[d][2 * i] *= grow, o[d][2 * i + 1] *= grow;
       }
