@@ -248,7 +248,7 @@ __device__ __forceinline__ void add_nonfinite(const PromptArgs& a, const Work& w
 //               tensor memory columns of its own, so that neither S nor P ever waits for an MMA that still reads the other
 //   warps 8-11  the same for the odd tiles, at the same time
 // Both warpgroups refer a row's exponentials to one m: they swap the row's maximum of an even and the odd tile behind it. P, its sum
-// and O are floating point, so m only has to keep P in range, and stays until a score is kRaise binades above it; then the even tile's
+// and O are floating point, so m only has to keep P in range, and stays until a score is kRaise binades above the one it was made from; then the even tile's
 // warpgroup scales O, once the P.V before have landed. Tiles are counted through all works (t), so that loads, scores and the first
 // softmax of a work go on while the one before is stored; a CTA per work spent 22 of 80 thousand clocks on its start and its end.
 // Bound by the softmax: about 3750 clocks for two tiles, 2230 of them the exponentials with what goes with them (two warps of a scheduler; the
@@ -264,8 +264,10 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
               const __grid_constant__ PromptArgs a) {
   using S = Shape<D>;
   constexpr bool kHalf = std::is_same<T, __half>::value;
-  // fp16 ends at 2^16 and loses bits below 2^-14: P starts at up to 2^6 and may grow to 2^14. bf16 has fp32's range.
-  constexpr float kShift = kHalf ? 6.0f : 0.0f, kRaise = kHalf ? 14.0f : 30.0f;
+  // m is the row's largest score so far less kShift, and moves once a score is kRaise above that. bf16 has fp32's range. fp16 ends at 2^16 and
+  // loses bits below 2^-14: the largest of P is kept from 2^13 to 2^15, so that weights are whole to 2^-27 of the largest and held to 2^-38 of it
+  // (from 2^6 to 2^8, weights of 2^-25 were off by a fiftieth).
+  constexpr float kShift = kHalf ? 13.0f : 0.0f, kRaise = kHalf ? 2.0f : 30.0f;
   constexpr int kMarks = 32;  // works that the V warp can be ahead of the stores, at most: a stage each and two
   const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
   const std::uint32_t rank = cluster_ctarank();
@@ -629,7 +631,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
           top = max3_nan(top, other, other);
         }
         if (__builtin_expect(!(top < INFINITY), 0)) l = __int_as_float(0x7FC00000), top = -INFINITY;  // NaN or infinity: so is the row, for good
-        const bool raise = m == -INFINITY ? top > -INFINITY : top > m + kRaise - kShift;
+        const bool raise = m == -INFINITY ? top > -INFINITY : top > m + (kShift + kRaise);
         float alpha = 1.0f;
         if (raise) {
           alpha = m == -INFINITY ? 0.f : ex2(m - (top - kShift));  // (nothing seen yet: O is 0)

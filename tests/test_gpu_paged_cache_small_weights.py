@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from owoinfer_b200 import ops
-from tests.test_gpu_paged_cache import BF16, F, F16, U, attention_64, make_cache, near, rows_of, seen_of
+from tests.test_gpu_paged_cache import BF16, F, F16, U, attention_64, cu_of, make_cache, near, rows_of, seen_of
 
 pytestmark = pytest.mark.gpu
 
@@ -55,4 +55,14 @@ def test_decode_keeps_small_weights(dtype, d, gap, n, top):
     for weights in (None, torch.zeros((1, 1, cache.slots), device="cuda")):
         got, lse = ops.attention_paged_decode(q, cache, 1.0, weights=weights)
         check(cache, q, n, got, lse, 2)
+    assert ops.paged_cache_status() == 0
+
+
+@pytest.mark.parametrize("dtype,d", [(F16, 64), (F16, 128), (BF16, 64)])
+@pytest.mark.parametrize("gap", [12.0, 18.5, 25.4])
+@pytest.mark.parametrize("n,top", CASES)
+def test_prompt_keeps_small_weights(dtype, d, gap, n, top):
+    cache, q = peaked(n, d, dtype, gap, top)
+    got, lse = ops.attention_paged(q, cache, cu_of([1]), 1, 1.0)
+    check(cache, q, n, got, lse, 1)
     assert ops.paged_cache_status() == 0
