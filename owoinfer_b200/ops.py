@@ -714,6 +714,8 @@ def _rows(t, name, dtype):
     stride, inner = t.stride()
     if inner != 1 and width > 1:
         raise ValueError(f"the rows of {name} must be contiguous")
+    if stride < width and rows > 1:
+        raise ValueError(f"the rows of {name} must not overlap")
     return rows, max(stride, width)
 
 
