@@ -675,7 +675,7 @@ void b2_dit_file_close(b2_dit_file* file);
  * p * page_stride + h * head_stride + r * row_stride), and for each sequence its pages in order and the number of slots
  * that are filled. Slot j of sequence b is row j % page_size of page block_table[b * table_ld + j / page_size]; entries
  * behind a sequence's last page are not read. Pools 16-byte aligned, strides multiples of 8 elements; page_size a power of
- * two from 16 to 1024; table_width * page_size < 2^31. What lies in slots behind seq_lens does not reach any output, NaN
+ * two from 16 to 1024; table_width * page_size at most 2^31 - 2^21. What lies in slots behind seq_lens does not reach any output, NaN
  * and infinities included. */
 typedef struct b2_paged_cache {
   size_t struct_size;
@@ -738,7 +738,7 @@ int b2_attention_paged_decode(const b2_paged_cache* cache, const b2_view3* q, co
  * keeps its first `sinks` slots, its last `recent` ones and, of those between, the ones of largest weight up to `budget` in all
  * (equal weights: the lower slot stays; NaN ranks below everything); a shorter one keeps all. What is kept moves, in
  * order, to the pages table_out[b, :] of the same pools (device int32, rows table_out_ld apart, table_out_width * page_size >=
- * budget): pages that none of the cache's sequences holds.
+ * budget, budget at most 2^31 - 2^21): pages that none of the cache's sequences holds.
  *   kept [batch, kv_heads, budget] int32: the slots that stayed, ascending, then -1;  lens_out [batch] int32: min(seq_len, budget);
  *   weights_out (or NULL) [batch, kv_heads, slots] fp32, rows weights_out_ld apart: the weights of the slots that stayed.
  * weights: fp32, rows weights_ld apart (at least table_width * page_size). weights_out must not overlap weights. */

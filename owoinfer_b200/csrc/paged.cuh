@@ -20,6 +20,10 @@ enum PagedFault : unsigned {
   kPagedWait = 16,        // a bounded wait expired
 };
 
+// Slots of a block table, at most: a slot is an int, and so is a loop's stride past the last one (the longest: 8 CTAs an SM of 1024 slots
+// each, in the join of single-token attention, 1.2 million).
+constexpr std::int64_t kMostSlots = (1LL << 31) - (1LL << 21);
+
 struct PagedArgs {
   void* k;
   void* v;

@@ -504,9 +504,9 @@ int check_paged_cache(const char* op, const b2_paged_cache* c, PagedArgs* a) {
     return fail_invalid(op, "page_size must be a power of two from 16 to 1024");
   }
   if (c->batch < 0 || c->batch > 65535 || c->kv_heads <= 0 || c->kv_heads > 65535) return fail_invalid(op, "batch and kv_heads must be at most 65535, kv_heads positive");
-  if (c->num_pages < 0 || c->num_pages > INT_MAX || c->table_width < 0 || static_cast<std::int64_t>(c->table_width) * c->page_size > INT_MAX ||
+  if (c->num_pages < 0 || c->num_pages > INT_MAX || c->table_width < 0 || static_cast<std::int64_t>(c->table_width) * c->page_size > kMostSlots ||
       c->table_ld < c->table_width) {
-    return fail_invalid(op, "num_pages and table_width * page_size must be below 2^31, table_ld at least table_width");
+    return fail_invalid(op, "num_pages must be below 2^31, table_width * page_size at most 2^31 - 2^21, table_ld at least table_width");
   }
   if (c->page_stride % 8 != 0 || c->head_stride % 8 != 0 || c->row_stride % 8 != 0 || c->row_stride < c->head_dim || c->page_stride < 0 || c->head_stride < 0) {
     return fail_invalid(op, "the pools' strides must be multiples of 8 elements, a row's at least head_dim");
@@ -639,6 +639,7 @@ int b2_kv_evict(const b2_paged_cache* cache, const float* weights, int64_t weigh
   if (sinks < 0 || recent < 0 || budget <= 0 || static_cast<std::int64_t>(sinks) + recent > budget) {
     return fail_invalid(op, "budget must be positive, sinks and recent not negative and together at most budget");
   }
+  if (budget > kMostSlots) return fail_invalid(op, "budget must be at most 2^31 - 2^21");
   if (table_out_width < 0 || table_out_ld < table_out_width || static_cast<std::int64_t>(table_out_width) * cache->page_size < budget) {
     return fail_invalid(op, "table_out must name pages for budget slots");
   }
