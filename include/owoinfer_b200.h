@@ -739,7 +739,7 @@ int b2_attention_paged_decode(const b2_paged_cache* cache, const b2_view3* q, co
  * (equal weights: the lower slot stays; NaN ranks below everything); a shorter one keeps all. What is kept moves, in
  * order, to the pages table_out[b, :] of the same pools (device int32, rows table_out_ld apart, table_out_width * page_size >=
  * budget, budget at most 2^31 - 2^21): pages that none of the cache's sequences holds.
- *   kept [batch, kv_heads, budget] int32: the slots that stayed, ascending, then -1;  lens_out [batch] int32: min(seq_len, budget);
+ *   kept [batch, kv_heads, budget] int32: the slots that stayed, ascending, then -1;  lens_out [batch] int32, not seq_lens itself: min(seq_len, budget);
  *   weights_out (or NULL) [batch, kv_heads, slots] fp32, rows weights_out_ld apart: the weights of the slots that stayed.
  * weights: fp32, rows weights_ld apart (at least table_width * page_size). weights_out must not overlap weights. */
 int b2_kv_evict(const b2_paged_cache* cache, const float* weights, int64_t weights_ld, int sinks, int recent, int budget,

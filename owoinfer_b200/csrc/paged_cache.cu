@@ -650,6 +650,8 @@ int b2_kv_evict(const b2_paged_cache* cache, const float* weights, int64_t weigh
   if (cache->batch == 0) return B2_OK;
   if (weights == nullptr || table_out == nullptr || kept == nullptr || lens_out == nullptr) return fail_invalid(op, "null weights, table_out, kept or lens_out");
   if (weights == weights_out) return fail_invalid(op, "weights_out must not be weights");
+  // (Every CTA reads the old lengths while the first ones write the new.)
+  if (lens_out < cache->seq_lens + cache->batch && cache->seq_lens < lens_out + cache->batch) return fail_invalid(op, "lens_out must not be the cache's seq_lens");
   a.weights = weights, a.weights_ld = weights_ld, a.table_out = table_out, a.table_out_ld = table_out_ld, a.kept = kept;
   a.lens_out = lens_out, a.weights_out = weights_out, a.weights_out_ld = weights_out_ld;
   a.sinks = sinks, a.recent = recent, a.budget = budget;

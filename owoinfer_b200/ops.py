@@ -857,7 +857,7 @@ def _slots_of(t, cache, name):
 def kv_evict(cache, weights, table_out, budget, sinks=0, recent=0, kept=None, lens_out=None, weights_out=None):
     """Sequences of more than `budget` slots keep their first `sinks`, their last `recent` and, of the rest, the slots of most weight
     (fp32 [batch, kv_heads, slots]), for each key head by itself; what is kept moves in order to the pages of table_out. Returns
-    (kept int32 [batch, kv_heads, budget], lens int32 [batch]); weights_out receives the weights of what is kept."""
+    (kept int32 [batch, kv_heads, budget], lens int32 [batch], not the cache's own); weights_out receives the weights of what is kept."""
     if budget <= 0:
         raise ValueError("budget must be positive")
     slots = _slots_of(weights, cache, "weights")
