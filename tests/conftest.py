@@ -20,3 +20,10 @@ def _built_library():
         from owoinfer_b200 import build
         build.build()
     yield
+
+
+def pytest_runtest_setup(item):
+    if item.get_closest_marker("gpu") is not None:
+        import torch
+        if not torch.cuda.is_available():
+            pytest.skip("needs a CUDA device")
