@@ -712,7 +712,8 @@ int b2_qk_norm_rope_append(const b2_paged_cache* cache, const void* qkv, int64_t
  * sees nothing (a cache shorter than the call's tokens, or scores that are all -infinity) gets zeros and -infinity; one that sees a score
  * of NaN or +infinity gets NaN in out and lse. q, out: views of one dtype [tokens,
  * q_heads, head_dim]; max_q: no sequence has more tokens in the call. Keys and values of slots that a token does not see do
- * not reach its output, NaN and infinities included.
+ * not reach its output, NaN and infinities included; an infinity or NaN of V that it sees is its channel's output, infinities of both signs
+ * are NaN. (Sums before the division are in fp32: finite |v| times the slots seen below 2^97.)
  * workspace: b2_attention_paged_workspace_bytes() of the same arguments, 256-byte aligned (few tokens over a long cache: parts of the
  * keys are worked on apart and joined; 256 where none is needed, and then NULL with 0 bytes will do). Nothing is kept in it. */
 size_t b2_attention_paged_workspace_bytes(const b2_paged_cache* cache, int64_t tokens, int q_heads, int max_q, int window, int sinks);

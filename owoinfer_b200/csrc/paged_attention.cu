@@ -235,6 +235,40 @@ __device__ __forceinline__ void add_nonfinite(const PromptArgs& a, const Work& w
   }
 }
 
+// The same for tiles that all rows of the pair see, where an infinity of V has met every weight, those among them that are 0 in 16 bits: it is the output.
+// 32 * kEach channels from `from` on, of the rows of a whole warp, kEach channels to a lane on the way; `sums`: shared memory for as many.
+template <typename T, int kEach, typename Out>
+__device__ __forceinline__ void take_nonfinite(const PromptArgs& a, const Work& w, int from, int lane, float* sums, Out* out, bool live, bool empty) {
+  float odd[kEach] = {};
+#pragma unroll 1
+  for (int j = 0; j < w.count; ++j) {
+    const int slot0 = w.slot(j);
+    if (!w.seen_by_all(a, slot0)) continue;
+#pragma unroll 1
+    for (int i0 = 0; i0 < kTile; i0 += 16) {  // (a page holds 16 slots at least)
+      const int page = paged_page(a.c, w.b, slot0 + i0);
+      if (page < 0) continue;
+      const T* v = static_cast<const T*>(a.c.v) + paged_row(a.c, page, w.h, slot0 + i0) + from + lane * kEach;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          const float x = to_float(v[i * a.c.row_stride + e]);
+          if (!isfinite(x)) odd[e] += x;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) sums[lane * kEach + e] = odd[e];
+  __syncwarp();
+#pragma unroll 1
+  for (int d = 0; d < 32 * kEach; ++d) {
+    if (live && (empty || !isfinite(sums[d]))) out[from + d] = static_cast<Out>(empty ? 0.f : sums[d]);
+  }
+  __syncwarp();
+}
+
 // Persistent CTA pairs; a work is 256 rows of a (sequence, key head). A row is a (token, query head of the group) pair, the group's heads of a
 // token side by side: they share their keys, and 256 rows have few tokens, so little of the causal edge is computed for nothing. Each
 // CTA has 128 rows; tcgen05.mma.cta_group::2 multiplies both CTAs' rows with one K or V tile of 128 slots, of which each CTA holds half (64
@@ -719,6 +753,11 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_tensor(at_leader(s_o_free));
+      // A weight that is 0 in 16 bits makes NaN of an infinity in V, and so does a row whose scores are all minus infinity.
+      float most[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < D / 2; i += 2) most[i / 2 % 4] = max3_nan(most[i / 2 % 4], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+      const bool spoilt = __any_sync(0xffffffffu, isnan(max3_nan(max3_nan(most[0], most[1], most[2]), most[3], most[3])) && !undefined);
       // The warp's rows, 64 bytes of each at a time, through shared memory, so that four lanes store them: a lane storing its own row touches 32
       // lines an instruction, and the eight warps kept each other waiting for 4500 clocks a work.
       const std::uint32_t at = smem_u32(&s_out[warp - 4][0]);
@@ -743,8 +782,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
           for (int e = 0; e < 4; ++e) put(e, make_uint4(x[i * 16 + e * 4], x[i * 16 + e * 4 + 1], x[i * 16 + e * 4 + 2], x[i * 16 + e * 4 + 3]));
           store(part_o, (group * (D / 2) + i * 16) * 4);
         }
+        if (__builtin_expect(spoilt, 0)) take_nonfinite<T, D / 64>(a, w, group * (D / 2), lane, reinterpret_cast<float*>(s_out[warp - 4]), part_o, live, empty);
         if (live) {
-          if (repair) add_nonfinite<T>(a, w, p, part_o, group * (D / 2), (group + 1) * (D / 2));
+          if (repair && !empty) add_nonfinite<T>(a, w, p, part_o, group * (D / 2), (group + 1) * (D / 2));
           if (group == 0) a.part_ml[part_at] = make_float2(m, empty ? 0.f : l);
         }
       } else {
@@ -759,8 +799,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
           }
           store(out, (group * (D / 2) + i * 32) * 2);
         }
+        if (__builtin_expect(spoilt, 0)) take_nonfinite<T, D / 64>(a, w, group * (D / 2), lane, reinterpret_cast<float*>(s_out[warp - 4]), out, live, empty);
         if (live) {
-          if (repair) add_nonfinite<T>(a, w, p, out, group * (D / 2), (group + 1) * (D / 2));
+          if (repair && !empty) add_nonfinite<T>(a, w, p, out, group * (D / 2), (group + 1) * (D / 2));
           if (group == 0 && a.lse != nullptr) a.lse[lse_at] = empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         }
       }

@@ -152,3 +152,42 @@ def test_decode_with_an_infinite_value_of_no_weight(dtype, d):
     put(cache, cache.k, 0, 20, 60.0, channel=0)  # a weight of e^-60 for the others
     got, _ = ops.attention_paged_decode(q, cache, 1.0)
     assert bool((got[..., 2] == math.inf).all()) and bool(torch.isfinite(got[..., 3:]).all())
+
+
+# ---------------------------------------------------------------------------------------------------- values of next to no weight
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 128), (BF16, 64), (F16, 64)])
+@pytest.mark.parametrize("gap", [20.0, 60.0, 110.0])
+@pytest.mark.parametrize("n,past,window,sinks", [(400, 0, 0, 0), (700, 0, 300, 5), (3, 5000, 0, 0), (300, 900, 0, 0)])
+def test_prompt_with_infinite_values_of_little_weight(dtype, d, gap, n, past, window, sinks):
+    """A weight of e^-gap is above 0, however 16 bits hold it: times infinity it is infinity."""
+    end = n + past
+    cache = make_cache([end], 2, d, 64, dtype)
+    cache.k.zero_()
+    for b_slot, channel, value in ((2, 3, math.inf), (133, d - 1, -math.inf), (140, 7, math.nan), (end - 140, 0, math.inf), (end - 2, 5, math.inf)):
+        if 0 <= b_slot < end:
+            put(cache, cache.k, 0, b_slot, -gap, channel=0)
+            put(cache, cache.v, 0, b_slot, value, head=b_slot % 2, channel=channel)
+    put(cache, cache.v, 0, 30, -math.inf, head=0, channel=3)  # meets the infinity of slot 2
+    put(cache, cache.k, 0, 30, -gap, channel=0)
+    q = torch.zeros((n, 6, d), dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    got, lse = ops.attention_paged(q, cache, cu_of([n]), n, 1.0, window=window, sinks=sinks)
+    check(cache, q, [n], 1.0, got, lse, dtype, window, sinks)
+    again, _ = ops.attention_paged(q, cache, cu_of([n]), n, 1.0, window=window, sinks=sinks)
+    assert torch.equal(again.view(torch.int16), got.view(torch.int16)) and ops.paged_cache_status() == 0
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64)])
+def test_prompt_that_sees_nothing_of_infinite_values(dtype, d):
+    """Every score minus infinity: zeros, infinities of V included."""
+    cache = make_cache([300], 1, d, 16, dtype)
+    cache.k.zero_()
+    cache.k[..., 0] = -math.inf
+    put(cache, cache.v, 0, 9, math.inf, channel=2)
+    put(cache, cache.v, 0, 290, math.nan, channel=3)
+    q = torch.zeros((300, 2, d), dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    got, lse = ops.attention_paged(q, cache, cu_of([300]), 300, 0.5)
+    assert bool((lse == -math.inf).all())
+    assert bool((got == 0).all())
