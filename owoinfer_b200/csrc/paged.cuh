@@ -96,6 +96,13 @@ __device__ __forceinline__ void paged_tokens(const PagedArgs& a, const std::int3
   first = 0, n = 0;
 }
 
+// f x + keep sum, the join of a part of an output: an infinity is one however small the part's factor, 0 included.
+__device__ __forceinline__ float joined(float f, float x, float keep, float sum) {
+  const float y = fmaf(f, x, keep * sum);
+  if (__builtin_expect(!isnan(y), 1)) return y;
+  return (isinf(x) ? x : f * x) + (isinf(sum) ? sum : keep * sum);
+}
+
 template <typename T>
 __device__ __forceinline__ float to_float(T v) { return static_cast<float>(v); }
 template <typename T>

@@ -850,7 +850,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) prompt_join_kernel(const Prom
     const float top = fmaxf(m, ml.x), f = ex2(ml.x - top), keep = l == 0.f ? 0.f : ex2(m - top);
     m = top, l = fmaf(f, ml.y, keep * l);
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) o[e] = fmaf(f, part[e], keep * o[e]);
+    for (int e = 0; e < kEach; ++e) o[e] = joined(f, part[e], keep, o[e]);
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   std::uint32_t packed[kEach / 2];

@@ -413,7 +413,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       for (int i = 0; i < kMostCluster; ++i) {
         if (ml[i].y == 0.f) continue;
         const float f = ex2(ml[i].x - mm);
-        sum.x = fmaf(f, x[i].x, sum.x), sum.y = fmaf(f, x[i].y, sum.y), sum.z = fmaf(f, x[i].z, sum.z), sum.w = fmaf(f, x[i].w, sum.w);
+        sum.x = joined(f, x[i].x, 1.f, sum.x), sum.y = joined(f, x[i].y, 1.f, sum.y), sum.z = joined(f, x[i].z, 1.f, sum.z), sum.w = joined(f, x[i].w, 1.f, sum.w);
       }
       const float inv = ll == 0.f ? 0.f : 1.0f / ll;
       T* out = static_cast<T*>(a.out) + b * a.o_row + (q_head0 + row) * a.o_head + d;
@@ -491,8 +491,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a, 
         if (li == 0.f) return;  // nothing seen
         const float top = fmaxf(m, mi), f = ex2(mi - top), keep = l == 0.f ? 0.f : ex2(m - top);
         m = top, l = fmaf(f, li, keep * l);
-        sum.x = fmaf(f, x.x, keep * sum.x), sum.y = fmaf(f, x.y, keep * sum.y);
-        sum.z = fmaf(f, x.z, keep * sum.z), sum.w = fmaf(f, x.w, keep * sum.w);
+        sum.x = joined(f, x.x, keep, sum.x), sum.y = joined(f, x.y, keep, sum.y);
+        sum.z = joined(f, x.z, keep, sum.z), sum.w = joined(f, x.w, keep, sum.w);
       };
       for (int i0 = slice; i0 < parts; i0 += 4 * slices) {
         float2 of[4];

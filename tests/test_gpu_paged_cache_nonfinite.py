@@ -191,3 +191,23 @@ def test_prompt_that_sees_nothing_of_infinite_values(dtype, d):
     got, lse = ops.attention_paged(q, cache, cu_of([300]), 300, 0.5)
     assert bool((lse == -math.inf).all())
     assert bool((got == 0).all())
+
+
+@pytest.mark.parametrize("form", ["prompt", "decode"])
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("n,low", [(500, 300), (20000, 12000)])
+@pytest.mark.parametrize("gap", [80.0, 100.0])
+def test_infinite_values_in_parts_of_little_weight(form, dtype, d, n, low, gap):
+    """The slots [0, low), whole parts of the keys, have e^-gap of the others' weight: less than fp32 keeps of 1."""
+    cache = make_cache([n], 1, d, 64, dtype)
+    cache.k.zero_()
+    for slot in range(0, low, 64):
+        cache.k[cache.block_table[0, slot // 64].item(), :, :min(64, low - slot), 0] = -gap
+    put(cache, cache.v, 0, 5, math.inf, channel=1)
+    put(cache, cache.v, 0, low // 2, -math.inf, channel=2)
+    put(cache, cache.v, 0, 8, math.inf, channel=3)
+    put(cache, cache.v, 0, low // 2 + 1, -math.inf, channel=3)
+    q = torch.zeros((1, 4, d), dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    got, lse = ops.attention_paged(q, cache, cu_of([1]), 1, 1.0) if form == "prompt" else ops.attention_paged_decode(q, cache, 1.0)
+    check(cache, q, [1], 1.0, got, lse, dtype)
