@@ -674,7 +674,7 @@ void b2_dit_file_close(b2_dit_file* file);
 /* A pool of pages for keys and one for values (of the same strides, in elements: row r of page p of head h starts at
  * p * page_stride + h * head_stride + r * row_stride), and for each sequence its pages in order and the number of slots
  * that are filled. Slot j of sequence b is row j % page_size of page block_table[b * table_ld + j / page_size]; entries
- * behind a sequence's last page are not read. Pools 16-byte aligned, strides multiples of 8 elements; page_size a power of
+ * behind a sequence's last page do not matter. Pools 16-byte aligned, strides multiples of 8 elements; page_size a power of
  * two from 16 to 1024; table_width * page_size at most 2^31 - 2^21. What lies in slots behind seq_lens does not reach any output, NaN
  * and infinities included. */
 typedef struct b2_paged_cache {

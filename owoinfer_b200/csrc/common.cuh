@@ -43,7 +43,9 @@ int gemm_debug_set(unsigned long long wait_limit_ns, int skip_stage);
 // it first thing, the tensor-core ones when their last load is issued and up to kHandOverRows rows only. Every kernel calls
 // wait_for_predecessors() before it touches memory that anything on the stream may still be writing or reading. The
 // chain's first launch is an ordinary one, so whatever a caller enqueued before a call of this library is finished before
-// the call's first kernel starts: data that no kernel of the call writes may be read ahead of the wait.
+// the call's first kernel starts: data that no kernel of the call writes may be read ahead of the wait. (The first kernels of
+// the calls on paged caches, append, prompt, decode, select and evict, do without the wait: they are the first of their
+// chains, and none of these calls may be made inside another's.)
 // At 2 x 320 tokens a launch takes the GPU about 2 us from the end of one kernel to the first instructions of the next
 // and another 1 to 2 us of set-up, thirteen times per block.
 // ---------------------------------------------------------------------------------------------------------------

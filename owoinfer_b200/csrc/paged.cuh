@@ -15,7 +15,7 @@ namespace b2 {
 enum PagedFault : unsigned {
   kPagedBadPage = 1,      // a page of the block table outside the pool
   kPagedBadLength = 2,    // seq_lens below 0 or past the block table or max_len
-  kPagedBadTokens = 4,    // cu_seqlens that do not rise from 0 to the call's tokens, or tokens without a slot
+  kPagedBadTokens = 4,    // cu_seqlens that fall or leave [0, the call's tokens]; in the append also tokens without a sequence or a slot
   kPagedBadPosition = 8,  // a position outside the rotation table
   kPagedWait = 16,        // a bounded wait expired
 };

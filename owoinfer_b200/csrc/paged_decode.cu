@@ -126,7 +126,7 @@ __device__ __forceinline__ void take_nonfinite(const DecodeArgs& a, const Steps&
 // registers; they meet at the end. Q·K^T and P·V are 16-row MMAs with the group's query heads as rows: the cache is read once
 // for all of them. At one byte of cache to every group / 2 multiply-adds the memory bounds it; 128-row tensor tiles would be
 // filled to group / 128. 64 sequences of up to 8101 slots, 32 / 8 heads of 128, with weights: 200 us, 6.3 TB/s (the
-// call 219); one of 131001, 32 / 4 heads in fp16: 50 us, 5.3 TB/s (59).
+// call 222); one of 131001, 32 / 4 heads in fp16: 50 us, 5.3 TB/s (59).
 template <typename T, int D, bool kScores, bool kCluster>
 __global__ void __launch_bounds__(kThreads, 3)
 decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const DecodeArgs a) {
@@ -579,7 +579,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs a, 
 // How a call is cut into CTAs, by their number per SM, of which three fit at a time. One sequence: two equal CTAs per SM (131001
 // slots, 4 key heads, this kernel: 53 us; three per SM 58, six 76). Several, whose lengths differ: eighteen, handed out as SMs come free (64 of up to 8101, 8
 // key heads: 196 us; three per SM 233), but of kLongEnough steps at least, since each has its start and its part to join
-// (4 of up to 30001: 76 us; as eighteen per SM 79).
+// (4 of up to 30001: 76 us; as eighteen per SM 79). The lengths are on the device, so the rule goes by the number of sequences: equal ones do
+// better as two per SM (the whole call behind a flushed L2, 32 / 4 heads of 128 in fp16: two of 65000 70.7 us, as eighteen 78.8; three of 43000
+// 70.7 and 76.8; two of 130000 130 both ways), uneven ones worse by more (65000, 20000 and 5000: 69.6, as eighteen 60.4).
 // Short ones are joined by the CTAs of a cluster in shared memory (by one CTA, where there are enough of them): one launch instead of two and
 // no workspace, some 2 us of the host's time. Slots, and us with the second kernel and so: 6 sequences, 32 / 8 heads of 128: 500 15.8 and
 // 10.8, 2000 18.5 and 16.7, 2600 19.2 and 19.9; 16: 500 16.5 and 12.6; 30, 14 / 2 of 64: 1000 16.0 and 11.0, 2000 16.6 and 14.4; so up to

@@ -21,7 +21,8 @@ def rope_table(positions, dim, base=1e6, device="cuda"):
 class TextCache:
     """Pages of `layers` caches for `batch` sequences of up to `slots` slots. With a budget a cache that is full shrinks to it: the first
     `sinks` slots, the last `recent` and of the rest those of most weight stay, for each layer and key head by itself; the
-    sequences keep counting positions. What stays moves to a second set of pages, which takes turns with the first."""
+    sequences keep counting positions. What stays moves to a second set of pages, which takes turns with the first. Weights are those that the
+    tokens written one by one gave; a prompt's own attention is not counted, so that of slots without any weight yet the lowest stay."""
 
     def __init__(self, layers, batch, kv_heads, head_dim, slots, page_size=64, budget=0, sinks=4, recent=0, dtype=torch.bfloat16, device="cuda"):
         width = -(-slots // page_size)
