@@ -211,3 +211,20 @@ def test_infinite_values_in_parts_of_little_weight(form, dtype, d, n, low, gap):
     q[..., 0] = 1.0
     got, lse = ops.attention_paged(q, cache, cu_of([1]), 1, 1.0) if form == "prompt" else ops.attention_paged_decode(q, cache, 1.0)
     check(cache, q, [1], 1.0, got, lse, dtype)
+
+
+# ---------------------------------------------------------------------------------------------------- eviction
+
+@pytest.mark.parametrize("n,heads", [(60, 1), (3000, 3), (20000, 1)])
+def test_evict_ranks_nan_below_minus_infinity(n, heads):
+    """Of weights that are NaN in every other slot and minus infinity in the others, the latter stay; then the lowest of the NaN."""
+    cache = make_cache([n], heads, 64, 16, BF16, spare=-(-(n // 2 + 7) // 16))
+    weights = torch.full((1, heads, cache.slots), math.nan, device="cuda")
+    weights[..., 1:n:2] = -math.inf
+    used = set(cache.block_table[cache.block_table >= 0].tolist())
+    table_out = torch.tensor([[p for p in range(cache.k.shape[0]) if p not in used]], dtype=torch.int32).cuda()
+    for budget in (n // 2 - 5, n // 2, n // 2 + 7):
+        kept, _ = ops.kv_evict(cache, weights, table_out, budget)
+        want = sorted(list(range(1, n, 2))[:budget] + list(range(0, n, 2))[:max(0, budget - n // 2)])
+        assert kept.tolist() == [[want] * heads]
+    assert ops.paged_cache_status() == 0
