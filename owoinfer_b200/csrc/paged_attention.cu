@@ -238,31 +238,46 @@ __device__ __forceinline__ void add_nonfinite(const PromptArgs& a, const Work& w
 }
 
 // The same for tiles that all rows of the pair see, where an infinity of V has met every weight, those among them that are 0 in 16 bits: it is the output.
-// 32 * kEach channels from `from` on, of the rows of a whole warp, kEach channels to a lane on the way; `sums`: shared memory for as many.
+// 32 * kEach channels from `from` on, of the rows of a whole warp; `sums`: shared memory for as many. 16 bytes a lane, eight in flight (131072 slots
+// take 2.4 ms; 2 bytes a lane 5.5): the other warps wait for this one, 200 ms at most.
 template <typename T, int kEach, typename Out>
 __device__ __forceinline__ void take_nonfinite(const PromptArgs& a, const Work& w, int from, int lane, float* sums, Out* out, bool live, bool empty) {
-  float odd[kEach] = {};
+  constexpr int kChunks = 4 * kEach, kSlots = 32 / kChunks, kBatch = 8;  // lanes to a row; rows to a load
+  const T* const v = static_cast<const T*>(a.c.v) + from + lane % kChunks * 8;
+  float odd[8] = {};
 #pragma unroll 1
   for (int j = 0; j < w.count; ++j) {
     const int slot0 = w.slot(j);
     if (!w.seen_by_all(a, slot0)) continue;
 #pragma unroll 1
-    for (int i0 = 0; i0 < kTile; i0 += 16) {  // (a page holds 16 slots at least)
-      const int page = paged_page(a.c, w.b, slot0 + i0);
-      if (page < 0) continue;
-      const T* v = static_cast<const T*>(a.c.v) + paged_row(a.c, page, w.h, slot0 + i0) + from + lane * kEach;
+    for (int i0 = lane / kChunks; i0 < kTile; i0 += kBatch * kSlots) {
+      uint4 x[kBatch];
+      std::uint32_t any = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < kBatch; ++i) {
+        const int slot = slot0 + i0 + i * kSlots, page = paged_page(a.c, w.b, slot);
+        x[i] = page < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(v + paged_row(a.c, page, w.h, slot));
+      }
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          const float x = to_float(v[i * a.c.row_stride + e]);
-          if (!isfinite(x)) odd[e] += x;
+      for (int i = 0; i < kBatch; ++i) any |= full_exponent<T>(x[i].x) | full_exponent<T>(x[i].y) | full_exponent<T>(x[i].z) | full_exponent<T>(x[i].w);
+      if (__builtin_expect((any & 0x80008000u) == 0u, 1)) continue;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        float y[8];
+        load8<T>(x[i], y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (!isfinite(y[e])) odd[e] += y[e];
         }
       }
     }
   }
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) sums[lane * kEach + e] = odd[e];
+  for (int e = 0; e < 8; ++e) {
+#pragma unroll
+    for (int m = kChunks; m < 32; m *= 2) odd[e] += __shfl_xor_sync(0xffffffffu, odd[e], m);
+    if (lane < kChunks) sums[lane * 8 + e] = odd[e];
+  }
   __syncwarp();
 #pragma unroll 1
   for (int d = 0; d < 32 * kEach; ++d) {
