@@ -752,6 +752,105 @@ int b2_kv_evict(const b2_paged_cache* cache, const float* weights, int64_t weigh
  * table, 16 a bounded wait that expired. Synchronises the device: for tests and post-mortems. */
 int b2_paged_cache_status(unsigned* host_value, int clear);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * What a text decoder's step runs around its attention: the norm ahead of an 8-bit projection, adapters beside one, log
+ * probabilities of what is written. No counterpart in the reference's DiT path.
+ *
+ * The calls follow the conventions above: they allocate nothing, do not synchronise and can be captured; sums and softmax statistics
+ * are in fp32, each output is rounded once. All tensors of a call lie on the current device.
+ * ------------------------------------------------------------------------------------------------------------- */
+
+#define B2_DTYPE_F32 2
+#define B2_CODES_INT8 0
+#define B2_CODES_E4M3 1
+
+/* s = x + residual (residual NULL: s = x), residual_out = s; y = s * rsqrt(mean(s^2) + eps) * weight (NULL: 1), of s before it is
+ * rounded; for every token, or every `group` channels of it, scale = max(max|y| / Q, 1e-30) with Q = 127 (int8) or 448 (e4m3), and
+ * q = round(y / scale), ties to even. norm_out, where given, is y in 16 bits besides.
+ * x bf16, fp16 or fp32; residual and residual_out of x's type or fp32; weight any of them. Rows 16-byte aligned, their strides (in elements)
+ * multiples of 16 bytes; q 8-byte aligned, ldq % 8 == 0; dim % 8 == 0, dim <= 32768. residual_out may be residual, or x where
+ * they have one type, and norm_out may be x; otherwise nothing that is written may overlap anything else (residual_out NULL: not written).
+ * scale: fp32 [tokens], or [tokens, dim / group] with group 32, 64, 128 or 256 (dim % group == 0; 0: none).
+ * A token with a NaN or an infinity in s, or whose squares add up past fp32 (|s| of 2^63 and more), has NaN for all of its scales and its
+ * norm_out; its int8 codes are 0, its e4m3 codes NaN. */
+typedef struct b2_norm_quantize {
+  size_t struct_size;
+  int64_t tokens;
+  int dim, group;
+  float eps;
+  int codes;                    /* B2_CODES_* */
+  const void* x;
+  int64_t ldx;
+  const void* residual;
+  int64_t ld_residual;
+  void* residual_out;
+  int64_t ld_residual_out;
+  const void* weight;
+  void* norm_out;
+  int64_t ld_norm;
+  void* q;
+  int64_t ldq;
+  float* scale;
+  int x_dtype, residual_dtype, weight_dtype, norm_dtype; /* B2_DTYPE_*; read where the tensor is given */
+} b2_norm_quantize;
+int b2_add_rms_norm_quantize(const b2_norm_quantize* args, void* stream);
+
+/* Of each row z = scale * logits[row, 0 .. vocab): lse = log sum exp z, entropy = -sum p log p with p = exp(z - lse) (0 log 0 = 0); of the
+ * token targets[row] its logprob = z[target] - lse and its rank, 1 for the first in the order of falling logits (equal logits: the
+ * lower token first); the first `top` tokens of that order and their log probabilities.
+ * logits bf16, fp16 or fp32, rows ld elements apart (any alignment of the type's own); vocab from 1 to 2^30, top from 0 to 32 and at most
+ * vocab. targets: device int64 [rows] or NULL; a negative target is none: logprob 0, rank 0; one past the vocabulary has NaN and rank 0.
+ * Any output may be NULL but for top_logprobs and top_tokens with top > 0, which come together: logprobs, entropy, lse fp32 [rows], ranks int32
+ * [rows], top_logprobs fp32 and top_tokens int32 [rows, top].
+ * Logits of -infinity have log probability -infinity and no part in the entropy. A row of nothing else has lse and all log probabilities -infinity
+ * and entropy 0. A row with a NaN or +infinity has NaN for lse, entropy and all log probabilities; NaN ranks below everything. */
+typedef struct b2_logprobs {
+  size_t struct_size;
+  const void* logits;
+  int64_t ld, rows;
+  int dtype, vocab, top;
+  float scale;                  /* above 0, at most 1e30 */
+  const int64_t* targets;
+  float* logprobs;
+  int32_t* ranks;
+  float* entropy;
+  float* lse;
+  float* top_logprobs;
+  int32_t* top_tokens;
+} b2_logprobs;
+int b2_token_logprobs(const b2_logprobs* args, void* stream);
+
+/* Low-rank adapters of many requests at once, beside a projection that they share:
+ *   out[t] = y[t] + scales[a] * (x[t] A[a]^T) B[a]^T,  a = the adapter of token t (negative: none, out[t] = y[t])
+ * x [tokens, dim], y and out [tokens, width], A [adapters, rank, dim], B [adapters, width, rank], all of one type, bf16 or fp16; scales fp32
+ * [adapters] or NULL (1); ranks int32 [adapters] or NULL: adapter a has ranks[a] <= rank rows of A and columns of B, what lies behind them is not
+ * used, NaN and infinities included (ranks outside 0 .. rank raise a bit of b2_lora_status and are cut). x A^T is held to 16 bits and more; an
+ * infinity in what is used of B may make NaN where it would make an infinity.
+ * Rows and matrices 16-byte aligned, strides in elements, multiples of 8; dim, width and rank multiples of 8, rank <= 128; adapters <= 4096.
+ * out may be y itself (rows without an adapter are then left alone); x may be either.
+ *
+ * b2_lora_plan sorts the tokens by their adapter (token_adapters, device int32 [tokens]; an adapter past the last raises a bit of
+ * b2_lora_status and counts as none) into `plan`, which b2_lora_add of any layer and projection then reads: once for a step.
+ * plan and workspace are 256-byte aligned, of the sizes that the _bytes calls give (0: invalid arguments). Nothing is kept in the workspace. */
+typedef struct b2_lora {
+  size_t struct_size;
+  const void* a;
+  const void* b;
+  int64_t a_adapter_stride, a_row_stride, b_adapter_stride, b_row_stride;
+  const float* scales;
+  const int32_t* ranks;
+  int64_t dim, width;
+  int adapters, rank, dtype;
+} b2_lora;
+size_t b2_lora_plan_bytes(int64_t tokens, int adapters);
+int b2_lora_plan(const int32_t* token_adapters, int64_t tokens, int adapters, void* plan, size_t plan_bytes, void* stream);
+size_t b2_lora_workspace_bytes(int64_t tokens, int adapters, int64_t dim, int rank);
+int b2_lora_add(const b2_lora* lora, const void* plan, size_t plan_bytes, int64_t tokens, const void* x, int64_t ldx, const void* y, int64_t ldy,
+                void* out, int64_t ldo, void* workspace, size_t workspace_bytes, void* stream);
+/* Bits raised on the current device since the last clear: 1 an adapter past the last one, 2 a rank outside 0 .. rank. Synchronises the
+ * device: for tests and post-mortems. */
+int b2_lora_status(unsigned* host_value, int clear);
+
 /* Every mbarrier wait inside the tensor-core kernels is bounded (200 ms); a CTA whose wait expired raises a device word,
  * drains and returns instead of hanging. This reads the two words (GEMM, attention): 0 = no wait ever expired on this device.
  * Synchronises the device; for tests and post-mortems, not for the hot path. No counterpart in the reference (its

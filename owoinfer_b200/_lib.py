@@ -25,7 +25,8 @@ EXPORTS = [
     "b2_dit_graphs_create", "b2_dit_graphs_clear", "b2_dit_graphs_destroy", "b2_dit_graphs_stats", "b2_dit_forward_graphed",
     "b2_dit_file_open", "b2_dit_file_get_info", "b2_dit_file_model", "b2_dit_file_time_embedding", "b2_dit_file_time_mlp_bf16", "b2_dit_file_close",
     "b2_qk_norm_rope_append", "b2_attention_paged", "b2_attention_paged_workspace_bytes", "b2_attention_paged_decode_workspace_bytes", "b2_attention_paged_decode",
-    "b2_kv_evict", "b2_paged_cache_status",
+    "b2_kv_evict", "b2_paged_cache_status", "b2_add_rms_norm_quantize", "b2_token_logprobs", "b2_lora_plan_bytes", "b2_lora_plan", "b2_lora_workspace_bytes",
+    "b2_lora_add", "b2_lora_status",
 ]
 
 
@@ -143,6 +144,26 @@ class SpRun(C.Structure):
     _fields_ = [("struct_size", C.c_size_t), ("local", BlockRun), ("seq_lens_host", C.c_void_p)]
 
 
+class NormQuantize(C.Structure):
+    _fields_ = [("struct_size", C.c_size_t), ("tokens", C.c_int64), ("dim", C.c_int), ("group", C.c_int), ("eps", C.c_float), ("codes", C.c_int),
+                ("x", C.c_void_p), ("ldx", C.c_int64), ("residual", C.c_void_p), ("ld_residual", C.c_int64), ("residual_out", C.c_void_p),
+                ("ld_residual_out", C.c_int64), ("weight", C.c_void_p), ("norm_out", C.c_void_p), ("ld_norm", C.c_int64), ("q", C.c_void_p),
+                ("ldq", C.c_int64), ("scale", C.c_void_p), ("x_dtype", C.c_int), ("residual_dtype", C.c_int), ("weight_dtype", C.c_int),
+                ("norm_dtype", C.c_int)]
+
+
+class Logprobs(C.Structure):
+    _fields_ = [("struct_size", C.c_size_t), ("logits", C.c_void_p), ("ld", C.c_int64), ("rows", C.c_int64), ("dtype", C.c_int), ("vocab", C.c_int),
+                ("top", C.c_int), ("scale", C.c_float), ("targets", C.c_void_p), ("logprobs", C.c_void_p), ("ranks", C.c_void_p),
+                ("entropy", C.c_void_p), ("lse", C.c_void_p), ("top_logprobs", C.c_void_p), ("top_tokens", C.c_void_p)]
+
+
+class Lora(C.Structure):
+    _fields_ = [("struct_size", C.c_size_t), ("a", C.c_void_p), ("b", C.c_void_p), ("a_adapter_stride", C.c_int64), ("a_row_stride", C.c_int64),
+                ("b_adapter_stride", C.c_int64), ("b_row_stride", C.c_int64), ("scales", C.c_void_p), ("ranks", C.c_void_p), ("dim", C.c_int64),
+                ("width", C.c_int64), ("adapters", C.c_int), ("rank", C.c_int), ("dtype", C.c_int)]
+
+
 _lib = None
 
 
@@ -194,6 +215,15 @@ def lib() -> C.CDLL:
         l.b2_attention_paged_decode.argtypes = [cache, view, view, p, i, C.c_float, i, i, p, p, n, p, C.c_size_t, p]
         l.b2_kv_evict.argtypes = [cache, p, n, i, i, i, p, n, i, p, p, p, n, p]
         l.b2_paged_cache_status.argtypes = [C.POINTER(C.c_uint), i]
+        l.b2_add_rms_norm_quantize.argtypes = [C.POINTER(NormQuantize), p]
+        l.b2_token_logprobs.argtypes = [C.POINTER(Logprobs), p]
+        l.b2_lora_plan_bytes.restype = C.c_size_t
+        l.b2_lora_plan_bytes.argtypes = [n, i]
+        l.b2_lora_plan.argtypes = [p, n, i, p, C.c_size_t, p]
+        l.b2_lora_workspace_bytes.restype = C.c_size_t
+        l.b2_lora_workspace_bytes.argtypes = [n, i, n, i]
+        l.b2_lora_add.argtypes = [C.POINTER(Lora), p, C.c_size_t, n, p, n, p, n, p, n, p, C.c_size_t, p]
+        l.b2_lora_status.argtypes = [C.POINTER(C.c_uint), i]
         _lib = l
     return _lib
 

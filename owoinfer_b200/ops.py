@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import typing
 
 import torch
 
@@ -879,6 +880,191 @@ def paged_cache_status(clear=False) -> int:
     """Bits that the kernels on paged caches raised (b2_paged_cache_status): 0 when every length, page and position was in bounds."""
     v = C.c_uint(0)
     check(_lib.lib().b2_paged_cache_status(C.byref(v), int(clear)))
+    return int(v.value)
+
+
+# ------------------------------------------------------------------------------------------------ around a text decoder's attention
+
+_DTYPES_ALL = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+_NORM_BYTES, _LOGPROBS_BYTES, _LORA_BYTES = C.sizeof(_lib.NormQuantize), C.sizeof(_lib.Logprobs), C.sizeof(_lib.Lora)
+
+
+def _here(device, **tensors):
+    """All tensors lie on the current CUDA device (`device`: that of the call's first one)."""
+    if device.type != "cuda" or device.index != (torch.cuda.current_device() if _get_device is None else _get_device()):
+        raise ValueError("the tensors must be on the current CUDA device")
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} must be on the device of the other tensors")
+
+
+def _like(t, name, shape, dtypes):
+    """Row stride of a matrix of this shape, of one of `dtypes`, whose rows are contiguous."""
+    if t.dtype not in dtypes or t.shape != shape:
+        raise ValueError(f"{name} must be a {list(shape)} matrix of {' or '.join(map(str, dtypes))}")
+    return _rows(t, name, t.dtype)[1]
+
+
+def add_rms_norm_quantize(x, weight=None, residual=None, eps=1e-6, dtype=torch.int8, group=0, residual_out=None, norm_out=None, q=None, scale=None):
+    """The sum s = x + residual ([tokens, dim]; into residual_out, or the residual itself) and its root-mean-square norm times weight [dim] in 8 bits
+    for the projection that follows: codes of `dtype` (int8 or float8_e4m3fn) with an fp32 scale per token, or per `group` channels
+    (32, 64, 128 or 256). x bf16, fp16 or fp32, the residual of x's type or fp32. norm_out (bf16 or fp16 [tokens, dim]) receives the norm
+    unquantised besides, for adapters. Returns (q, scale): scale [tokens], or [tokens, dim / group]."""
+    code, types = _DTYPES_ALL.get(x.dtype), _DTYPES_ALL
+    if code is None or dtype not in _CODES:
+        raise ValueError("x must be bf16, fp16 or fp32, the codes int8 or float8_e4m3fn")
+    tokens, ldx = _rows(x, "x", x.dtype)
+    shape, device = x.shape, x.device
+    dim = shape[1]
+    if group < 0 or (group and dim % group):
+        raise ValueError("group must be 0, 32, 64, 128 or 256 and divide dim")
+    ld_res = ld_res_out = ld_norm = 0
+    if residual is not None:
+        ld_res = ld_res_out = _like(residual, "residual", shape, (x.dtype, torch.float32))
+        if residual_out is None:
+            residual_out = residual
+        elif residual_out is not residual:
+            ld_res_out = _like(residual_out, "residual_out", shape, (residual.dtype,))
+    elif residual_out is not None:
+        raise ValueError("residual_out needs a residual")
+    if norm_out is not None:
+        ld_norm = _like(norm_out, "norm_out", shape, (torch.bfloat16, torch.float16))
+    if weight is not None and (weight.dtype not in types or weight.dim() != 1 or weight.numel() != dim or not weight.is_contiguous()):
+        raise ValueError("weight must be a contiguous [dim] tensor of bf16, fp16 or fp32")
+    scales = (tokens, dim // group) if group else (tokens,)
+    if q is None:
+        q = torch.empty(shape, dtype=dtype, device=device)
+        ldq = dim
+    else:
+        ldq = _like(q, "q", shape, (dtype,))
+    if scale is None:
+        scale = torch.empty(scales, dtype=torch.float32, device=device)
+    elif scale.dtype != torch.float32 or scale.shape != scales or not scale.is_contiguous():
+        raise ValueError(f"scale must be a contiguous fp32 {list(scales)} tensor")
+    _here(device, residual=residual, residual_out=residual_out, norm_out=norm_out, weight=weight, q=q, scale=scale)
+    check(_lib.lib().b2_add_rms_norm_quantize(
+        _lib.NormQuantize(_NORM_BYTES, tokens, dim, group, eps, _CODES[dtype], x.data_ptr(), ldx, _at(residual), ld_res, _at(residual_out), ld_res_out,
+                          _at(weight), _at(norm_out), ld_norm, q.data_ptr(), ldq, scale.data_ptr(), code, 0 if residual is None else types[residual.dtype],
+                          0 if weight is None else types[weight.dtype], 0 if norm_out is None else types[norm_out.dtype]), _raw_stream()))
+    return q, scale
+
+
+class TokenLogprobs(typing.NamedTuple):
+    """What token_logprobs returns; logprobs and ranks are None without targets, the last two without alternatives."""
+    logprobs: typing.Optional[torch.Tensor]      # fp32 [rows]
+    ranks: typing.Optional[torch.Tensor]         # int32 [rows], from 1
+    entropy: torch.Tensor                        # fp32 [rows]
+    lse: torch.Tensor                            # fp32 [rows]
+    top_logprobs: typing.Optional[torch.Tensor]  # fp32 [rows, top]
+    top_tokens: typing.Optional[torch.Tensor]    # int32 [rows, top]
+
+
+def token_logprobs(logits, targets=None, top=0, scale=1.0):
+    """Of logits [rows, vocab] (bf16, fp16 or fp32 rows of any stride) times scale (one over the temperature): the log probability and the rank
+    of targets (int64 [rows]; a negative one is none and has 0 for both), the entropy, the log of the sum of exponentials, and the `top` (up to 32)
+    most probable tokens with their log probabilities, equal ones by number. Returns TokenLogprobs."""
+    code = _DTYPES_ALL.get(logits.dtype)
+    if code is None:
+        raise ValueError("logits must be bf16, fp16 or fp32")
+    rows, ld = _rows(logits, "logits", logits.dtype)
+    if targets is not None and (targets.dtype != torch.int64 or targets.dim() != 1 or targets.numel() != rows or not targets.is_contiguous()):
+        raise ValueError("targets must be a contiguous int64 [rows] tensor")
+    device = logits.device
+    if top < 0 or top > 32:
+        raise ValueError("top must be from 0 to 32 and at most vocab")
+    _here(device, targets=targets)
+    # (One allocation for all outputs: each costs a microsecond.)
+    out = torch.empty((4 + 2 * top) * rows, dtype=torch.float32, device=device)
+    logprobs, entropy, lse, ranks, top_logprobs, top_tokens = out.split([rows, rows, rows, rows, rows * top, rows * top])
+    at = out.data_ptr()
+    check(_lib.lib().b2_token_logprobs(
+        _lib.Logprobs(_LOGPROBS_BYTES, logits.data_ptr(), ld, rows, code, logits.shape[1], top, scale, _at(targets), at, at + 12 * rows, at + 4 * rows,
+                      at + 8 * rows, at + 16 * rows if top else 0, at + (16 + 4 * top) * rows if top else 0), _raw_stream()))
+    return TokenLogprobs(None if targets is None else logprobs, None if targets is None else ranks.view(torch.int32), entropy, lse,
+                         top_logprobs.view(rows, top) if top else None, top_tokens.view(torch.int32).view(rows, top) if top else None)
+
+
+class LoraAdapters:
+    """b2_lora: the low-rank adapters of one projection, a [adapters, rank, dim] and b [adapters, width, rank] (bf16 or fp16, rows contiguous), scales
+    fp32 [adapters] (None: 1) and, where some have a lower rank than the tensors, ranks int32 [adapters]. The struct holds addresses, so the
+    contents may change between calls."""
+
+    def __init__(self, a, b, scales=None, ranks=None):
+        code = _DTYPES.get(a.dtype)
+        if code is None or a.dtype != b.dtype or a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise ValueError("a and b must be bf16 or fp16 tensors [adapters, rank, dim] and [adapters, width, rank]")
+        n, rank, dim = a.shape
+        for name, t in (("a", a), ("b", b)):
+            if (t.stride(2) != 1 and t.shape[2] > 1) or (t.stride(1) < t.shape[2] and t.shape[1] > 1):
+                raise ValueError(f"the rows of {name} must be contiguous and not overlap")
+        if scales is not None and (scales.dtype != torch.float32 or scales.dim() != 1 or scales.numel() != n or not scales.is_contiguous()):
+            raise ValueError("scales must be a contiguous fp32 [adapters] tensor")
+        if ranks is not None:
+            _vector(ranks, "ranks", n)
+        for name, t in (("b", b), ("scales", scales), ("ranks", ranks)):
+            if t is not None and t.device != a.device:
+                raise ValueError(f"{name} must be on a's device")
+        self.a, self.b, self.scales, self.ranks, self.dtype, self.device = a, b, scales, ranks, a.dtype, a.device
+        self.adapters, self.rank, self.dim, self.width = n, rank, dim, b.shape[1]
+        self.struct = _lib.Lora(_LORA_BYTES, a.data_ptr(), b.data_ptr(), a.stride(0), max(a.stride(1), dim), b.stride(0), max(b.stride(1), rank), _at(scales),
+                                _at(ranks), dim, self.width, n, rank, code)
+
+
+class LoraPlan:
+    """b2_lora_plan: a step's tokens sorted by their adapter, token_adapters int32 [tokens] (negative: none), for every lora_add of the step. Where
+    the tensor's contents change, fill() sorts them anew (on the current stream; it can be captured along with the calls that use it)."""
+
+    def __init__(self, token_adapters, adapters):
+        self.tokens, self.adapters, self.token_adapters = token_adapters.numel(), adapters, token_adapters
+        _vector(token_adapters, "token_adapters", self.tokens)
+        self._sizes = {}
+        need = _lib.lib().b2_lora_plan_bytes(self.tokens, adapters)
+        if need == 0:
+            check(-1)
+        _here(token_adapters.device)
+        self.buffer = torch.empty(need, dtype=torch.uint8, device=token_adapters.device)
+        self.fill()
+
+    def fill(self):
+        _here(self.buffer.device)
+        check(_lib.lib().b2_lora_plan(self.token_adapters.data_ptr(), self.tokens, self.adapters, self.buffer.data_ptr(), self.buffer.numel(), _raw_stream()))
+
+    def workspace_bytes(self, dim, rank) -> int:
+        need = self._sizes.get((dim, rank))
+        if need is None:
+            need = _lib.lib().b2_lora_workspace_bytes(self.tokens, self.adapters, dim, rank)
+            if need == 0:
+                check(-1)
+            self._sizes[(dim, rank)] = need
+        return need
+
+
+def lora_add(y, x, adapters, plan, out=None, workspace=None):
+    """y [tokens, width] plus, for each token with an adapter, scale (x A^T) B^T of its row of x [tokens, dim]: in y's place, or into `out`. y and x
+    are views with contiguous rows (a slice of a fused projection's columns, say). Returns out."""
+    if plan.adapters != adapters.adapters:
+        raise ValueError("the plan is of another number of adapters")
+    ldx = _like(x, "x", (plan.tokens, adapters.dim), (adapters.dtype,))
+    ldy = ldo = _like(y, "y", (plan.tokens, adapters.width), (adapters.dtype,))
+    if out is None:
+        out = y
+    else:
+        ldo = _like(out, "out", (plan.tokens, adapters.width), (adapters.dtype,))
+    need = plan.workspace_bytes(adapters.dim, adapters.rank)
+    device = y.device
+    _here(device, x=x, out=out, a=adapters.a, plan=plan.buffer, workspace=workspace)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    check(_lib.lib().b2_lora_add(adapters.struct, plan.buffer.data_ptr(), plan.buffer.numel(), plan.tokens, x.data_ptr(), ldx, y.data_ptr(), ldy,
+                                 out.data_ptr(), ldo, workspace.data_ptr(), workspace.numel(), _raw_stream()))
+    return out
+
+
+def lora_status(clear=False) -> int:
+    """Bits that the kernels on adapters raised (b2_lora_status): 0 when every adapter and rank was in bounds."""
+    v = C.c_uint(0)
+    check(_lib.lib().b2_lora_status(C.byref(v), int(clear)))
     return int(v.value)
 
 
