@@ -365,6 +365,12 @@ __device__ __forceinline__ void st_cluster_v4(std::uint32_t cluster_addr, std::u
 __device__ __forceinline__ void st_cluster_u32(std::uint32_t cluster_addr, std::uint32_t x) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(x) : "memory");
 }
+// 16 bytes from the shared memory of a CTA of the cluster.
+__device__ __forceinline__ float4 ld_cluster_f32x4(std::uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 // Arrive on an mbarrier given by its shared::cluster address (own or peer CTA).
 __device__ __forceinline__ void mbar_arrive_cluster(std::uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");

@@ -66,11 +66,6 @@ __device__ __forceinline__ float2 ld_cluster_f32x2(std::uint32_t addr) {
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ float4 ld_cluster_f32x4(std::uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
 template <typename T>
 __device__ __forceinline__ void mma16(float (&d)[4], const std::uint32_t (&a)[4], std::uint32_t b0, std::uint32_t b1);
 template <>
