@@ -802,6 +802,7 @@ int b2_add_rms_norm_quantize(const b2_norm_quantize* args, void* stream);
  * vocab. targets: device int64 [rows] or NULL; a negative target is none: logprob 0, rank 0; one past the vocabulary has NaN and rank 0.
  * Any output may be NULL but for top_logprobs and top_tokens with top > 0, which come together: logprobs, entropy, lse fp32 [rows], ranks int32
  * [rows], top_logprobs fp32 and top_tokens int32 [rows, top].
+ * (An expired bounded wait, bit 16 of b2_paged_cache_status, makes NaN of a row's numbers.)
  * Logits of -infinity have log probability -infinity and no part in the entropy. A row of nothing else has lse and all log probabilities -infinity
  * and entropy 0. A row with a NaN or +infinity has NaN for lse, entropy and all log probabilities; NaN ranks below everything. */
 typedef struct b2_logprobs {
@@ -831,7 +832,8 @@ int b2_token_logprobs(const b2_logprobs* args, void* stream);
  *
  * b2_lora_plan sorts the tokens by their adapter (token_adapters, device int32 [tokens]; an adapter past the last raises a bit of
  * b2_lora_status and counts as none) into `plan`, which b2_lora_add of any layer and projection then reads: once for a step.
- * plan and workspace are 256-byte aligned, of the sizes that the _bytes calls give (0: invalid arguments). Nothing is kept in the workspace. */
+ * plan and workspace are 256-byte aligned, of the sizes that the _bytes calls give (0: invalid arguments; 256: none is used, and then a workspace of
+ * NULL with 0 bytes will do). Nothing is kept in the workspace. */
 typedef struct b2_lora {
   size_t struct_size;
   const void* a;
@@ -847,8 +849,8 @@ int b2_lora_plan(const int32_t* token_adapters, int64_t tokens, int adapters, vo
 size_t b2_lora_workspace_bytes(int64_t tokens, int adapters, int64_t dim, int rank);
 int b2_lora_add(const b2_lora* lora, const void* plan, size_t plan_bytes, int64_t tokens, const void* x, int64_t ldx, const void* y, int64_t ldy,
                 void* out, int64_t ldo, void* workspace, size_t workspace_bytes, void* stream);
-/* Bits raised on the current device since the last clear: 1 an adapter past the last one, 2 a rank outside 0 .. rank. Synchronises the
- * device: for tests and post-mortems. */
+/* Bits raised on the current device since the last clear: 1 an adapter past the last one, 2 a rank outside 0 .. rank, 4 a bounded wait that
+ * expired. Synchronises the device: for tests and post-mortems. */
 int b2_lora_status(unsigned* host_value, int clear);
 
 /* Every mbarrier wait inside the tensor-core kernels is bounded (200 ms); a CTA whose wait expired raises a device word,

@@ -3,58 +3,62 @@
 #include <algorithm>
 #include <cmath>
 
+#include "attention.cuh"
 #include "text.cuh"
 
 namespace b2 {
 namespace {
 
 __device__ unsigned g_lora_status = 0;
-enum LoraFault : unsigned { kLoraBadAdapter = 1, kLoraBadRank = 2 };
+enum LoraFault : unsigned { kLoraBadAdapter = 1, kLoraBadRank = 2, kLoraWait = 4 };  // (a bounded wait expired)
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kPlanThreads = 1024;
 constexpr int kMostAdapters = 4096, kMostRank = 128;
-constexpr int kMostParts = 8;  // CTAs of a cluster that divide the channels
+constexpr int kMostParts = 8, kMostManyParts = 4;  // CTAs of a cluster that divide the channels, of few and of many tokens
 
-// Tokens of a tile: one warp's rows of few tokens, eight warps' of many, for A and B to be read once for more of them.
-constexpr int kFewTokens = 256, kFewRows = 16, kManyRows = 128;
-inline int tile_rows(std::int64_t tokens) { return tokens <= kFewTokens ? kFewRows : kManyRows; }
-inline std::int64_t most_tiles(std::int64_t tokens, int adapters) {
-  const int rows = tile_rows(tokens);
-  return std::min(tokens, tokens / rows + adapters + 1);
+// A plan sorts the tokens by adapter and cuts them into tiles, of one warp's rows, where there are few tokens, and of eight warps', for A and B to be
+// read once for more of them: [0] and [1] below.
+constexpr int kFewRows = 16, kManyRows = 128, kFewTokens = 1024;
+inline std::int64_t most_tiles(std::int64_t tokens, int adapters, int rows) {
+  return rows == kFewRows && tokens > kFewTokens ? 0 : std::min(tokens, tokens / rows + adapters + 1);
 }
-
-// A plan: how many tiles there are, the tiles, the tokens in the order of their adapters.
 struct PlanHead {
-  int tiles, pad[3];
+  int tiles[2], pad[2];
 };
 struct Tile {
   int adapter, first, count, pad;  // -1: tokens without an adapter
 };
 struct Plan {
-  const PlanHead* head;
+  PlanHead* head;
+  Tile* tiles[2];
+  std::int32_t* order;
+};
+inline std::size_t plan_bytes(std::int64_t tokens, int adapters) {
+  const std::size_t tiles = static_cast<std::size_t>(most_tiles(tokens, adapters, kFewRows) + most_tiles(tokens, adapters, kManyRows));
+  return (sizeof(PlanHead) + tiles * sizeof(Tile) + static_cast<std::size_t>(tokens) * 4 + 255) / 256 * 256;
+}
+inline Plan plan_at(void* p, std::int64_t tokens, int adapters) {
+  char* at = static_cast<char*>(p);
+  Tile* tiles = reinterpret_cast<Tile*>(at + sizeof(PlanHead));
+  Tile* large = tiles + most_tiles(tokens, adapters, kFewRows);
+  return {reinterpret_cast<PlanHead*>(at), {tiles, large}, reinterpret_cast<std::int32_t*>(large + most_tiles(tokens, adapters, kManyRows))};
+}
+// What a kernel reads of it: one kind of tiles.
+struct Tiles {
+  const int* count;
   const Tile* tiles;
   const std::int32_t* order;
 };
-inline std::size_t plan_bytes(std::int64_t tokens, int adapters) {
-  const std::size_t bytes = sizeof(PlanHead) + static_cast<std::size_t>(most_tiles(tokens, adapters)) * sizeof(Tile) + static_cast<std::size_t>(tokens) * 4;
-  return (bytes + 255) / 256 * 256;
-}
-inline Plan plan_at(const void* p, std::int64_t tokens, int adapters) {
-  const char* at = static_cast<const char*>(p);
-  const Tile* tiles = reinterpret_cast<const Tile*>(at + sizeof(PlanHead));
-  return {reinterpret_cast<const PlanHead*>(at), tiles, reinterpret_cast<const std::int32_t*>(tiles + most_tiles(tokens, adapters))};
-}
 
 // A CTA per adapter, and one for the tokens without: each counts all tokens by adapter (a thread a run of neighbouring tokens, which mostly have
 // the same one), and puts its own in their places, in their order.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const std::int32_t* ids, int tokens, int adapters, int rows, PlanHead* head, Tile* tiles,
-                                                            std::int32_t* order) {
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const std::int32_t* ids, int tokens, int adapters, const Plan plan) {
   extern __shared__ int s_count[];  // [adapters + 1]
-  __shared__ int s_warp[kPlanThreads / 32], s_before[2];
+  __shared__ int s_warp[kPlanThreads / 32], s_before[3];
   const int tid = static_cast<int>(threadIdx.x), own = static_cast<int>(blockIdx.x);
   for (int i = tid; i <= adapters; i += kPlanThreads) s_count[i] = 0;
-  if (tid < 2) s_before[tid] = 0;
+  if (tid < 3) s_before[tid] = 0;
   __syncthreads();
   const int per = (tokens + kPlanThreads - 1) / kPlanThreads, begin = static_cast<int>(min(static_cast<long long>(tid) * per, static_cast<long long>(tokens)));
   const int end = min(tokens, begin + per);
@@ -76,9 +80,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const std::int32_t* 
   if (length > 0) atomicAdd(&s_count[run], length);
   __syncthreads();
   // Tokens and tiles of the adapters before this one.
-  int tokens_before = 0, tiles_before = 0;
-  for (int i = tid; i < own; i += kPlanThreads) tokens_before += s_count[i], tiles_before += (s_count[i] + rows - 1) / rows;
-  if (tokens_before > 0) atomicAdd(&s_before[0], tokens_before), atomicAdd(&s_before[1], tiles_before);
+  int tokens_before = 0, tiles_before[2] = {};
+  for (int i = tid; i < own; i += kPlanThreads) {
+    tokens_before += s_count[i], tiles_before[0] += (s_count[i] + kFewRows - 1) / kFewRows, tiles_before[1] += (s_count[i] + kManyRows - 1) / kManyRows;
+  }
+  if (tokens_before > 0) atomicAdd(&s_before[0], tokens_before), atomicAdd(&s_before[1], tiles_before[0]), atomicAdd(&s_before[2], tiles_before[1]);
   // This thread's place among the CTA's tokens.
   const int lane = tid % 32;
   int sum = mine;
@@ -93,16 +99,23 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const std::int32_t* 
   for (int i = 0; i < tid / 32; ++i) place += s_warp[i];
   if (mine > 0) {
     for (int i = begin; i < end; ++i) {
-      if (id_of(i) == own) order[place++] = i;
+      if (id_of(i) == own) plan.order[place++] = i;
     }
   }
-  const int count = s_count[own], num = (count + rows - 1) / rows;
-  for (int i = tid; i < num; i += kPlanThreads) tiles[s_before[1] + i] = Tile{own < adapters ? own : -1, s_before[0] + i * rows, min(rows, count - i * rows), 0};
-  if (own == adapters && tid == 0) head->tiles = s_before[1] + num;
+  const int count = s_count[own];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int rows = k == 0 ? kFewRows : kManyRows, num = (count + rows - 1) / rows;
+    if (k == 0 && tokens > kFewTokens) continue;
+    for (int i = tid; i < num; i += kPlanThreads) {
+      plan.tiles[k][s_before[1 + k] + i] = Tile{own < adapters ? own : -1, s_before[0] + i * rows, min(rows, count - i * rows), 0};
+    }
+    if (own == adapters && tid == 0) plan.head->tiles[k] = s_before[1 + k] + num;
+  }
 }
 
 struct LoraArgs {
-  Plan plan;
+  Tiles plan;
   const void* a;
   const void* b;
   std::int64_t a_adapter, a_row, b_adapter, b_row;
@@ -112,13 +125,14 @@ struct LoraArgs {
   const void* y;
   void* out;
   std::int64_t ldx, ldy, ldo;
-  // t = scale x A^T by [tile, row of the tile]: in two 16-bit parts [ranks, padded] each, and what a row was divided by.
-  void* t_hi;
-  void* t_lo;
+  // Of few and several tokens: t = scale x A^T, by [tile, row of the tile], in two 16-bit parts in operand order, and what a row was divided by.
+  std::uint32_t* t_hi;
+  std::uint32_t* t_lo;
   float* t_back;
   int adapters, rank, dim, width;
   int parts, slice;  // parts of the channels, channels of each (a multiple of 64)
   int columns;        // columns of an output CTA
+  int groups;         // clusters to a tile
 };
 
 template <typename T>
@@ -146,6 +160,26 @@ __device__ __forceinline__ int rank_of(const LoraArgs& a, int adapter) {
   atomicOr(&g_lora_status, kLoraBadRank);
   return r < 0 ? 0 : a.rank;
 }
+
+// fp32 values of a row, the largest of them `top`, as two 16-bit parts. fp16 ends at 2^16 and loses bits below 2^-14: there the largest is brought between
+// 2^14 and 2^15 by a power of two, which `back` undoes.
+template <typename T>
+struct Halves {
+  float by = 1.f, back = 1.f;
+  __device__ __forceinline__ explicit Halves(float top) {
+    if constexpr (std::is_same<T, __half>::value) {
+      const int e = top < INFINITY ? max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14, -100) : 0;
+      by = __uint_as_float(static_cast<unsigned>(127 - e) << 23), back = __uint_as_float(static_cast<unsigned>(127 + e) << 23);
+    }
+  }
+  __device__ __forceinline__ void split(float x, float y, std::uint32_t& hi, std::uint32_t& lo) const {
+    if constexpr (std::is_same<T, __half>::value) x *= by, y *= by;
+    hi = pack16<T>(x, y);
+    float xh, yh;
+    unpack16<T>(hi, xh, yh);
+    lo = pack16<T>(isfinite(xh) ? x - xh : 0.f, isfinite(yh) ? y - yh : 0.f);
+  }
+};
 
 // Where t's ranks r and r + 1 of a row lie, r + 2 and r + 3 two words on (r a multiple of 4): in the order of an MMA's A operands, four words of a lane
 // for each 16 rows and K of 16. Ranks of a K go to lanes as they come from B in one load: 8 neighbouring ones of 32 for two MMAs, or (16 ranks and fewer)
@@ -183,28 +217,18 @@ __device__ __forceinline__ void leave_sums(const LoraArgs& a, const Tile& tile, 
       v[e] = lane * 4 + e < rank ? v[e] * scale : 0.f;  // (infinities of x have made NaN of what lies behind the rank)
       top = fmaxf(top, fabsf(v[e]));
     }
-    float by = 1.f, back = 1.f;
     if constexpr (std::is_same<T, __half>::value) {
-      // fp16 ends at 2^16 and loses bits below 2^-14: a row's largest value is brought between 2^14 and 2^15 by a power of two.
 #pragma unroll
       for (int m = kLanes / 2; m > 0; m /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-      const int e = top < INFINITY ? max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14, -100) : 0;
-      by = __uint_as_float(static_cast<unsigned>(127 - e) << 23), back = __uint_as_float(static_cast<unsigned>(127 + e) << 23);
     }
     if (row >= kRows) continue;
+    const Halves<T> by(top);
     std::uint32_t hi[2], lo[2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float x = v[2 * e] * by, y = v[2 * e + 1] * by;
-      hi[e] = pack16<T>(x, y);
-      float xh, yh;
-      unpack16<T>(hi[e], xh, yh);
-      lo[e] = pack16<T>(isfinite(xh) ? x - xh : 0.f, isfinite(yh) ? y - yh : 0.f);
-    }
+    for (int e = 0; e < 2; ++e) by.split(v[2 * e], v[2 * e + 1], hi[e], lo[e]);
     const std::int64_t to = low_word<kRanks>(tile_number * kRows + row, lane * 4);
-    static_cast<std::uint32_t*>(a.t_hi)[to] = hi[0], static_cast<std::uint32_t*>(a.t_hi)[to + 2] = hi[1];
-    static_cast<std::uint32_t*>(a.t_lo)[to] = lo[0], static_cast<std::uint32_t*>(a.t_lo)[to + 2] = lo[1];
-    if (lane == 0) a.t_back[tile_number * kRows + row] = back;
+    a.t_hi[to] = hi[0], a.t_hi[to + 2] = hi[1], a.t_lo[to] = lo[0], a.t_lo[to + 2] = lo[1];
+    if (lane == 0) a.t_back[tile_number * kRows + row] = by.back;
   }
   if (a.parts > 1) cluster_sync_all();  // (nobody leaves while others read its sums)
 }
@@ -218,7 +242,7 @@ __global__ void __launch_bounds__(kThreads) shrink_few_kernel(const LoraArgs a) 
   constexpr int kRanks = kNT * 8;
   __shared__ __align__(16) float s_sum[kWarps][kFewRows * kRanks];
   const int tile_number = static_cast<int>(blockIdx.x) / a.parts, part = static_cast<int>(blockIdx.x) % a.parts;
-  if (tile_number >= a.plan.head->tiles) return;
+  if (tile_number >= *a.plan.count) return;
   const Tile tile = a.plan.tiles[tile_number];
   if (tile.adapter < 0) return;
   const int rank = rank_of(a, tile.adapter);
@@ -282,19 +306,19 @@ __device__ __forceinline__ uint4 matrices(std::uint32_t addr) {
   return r;
 }
 
-// The same for many tokens: four warps of 32 rows each with all ranks, 64 channels at a time through three stages of shared memory, rows of 128 bytes whose
+// The same for several tokens: four warps of 32 rows each with all ranks, 64 channels at a time through three stages of shared memory, rows of 128 bytes whose
 // 16-byte pieces are permuted by the row. (With the lanes' own pieces as operands, as above, each MMA had four moves beside it to bring its
 // registers together: 8191 tokens, 4096 channels, rank 64: 30 us.)
 template <int kNT>
 constexpr int kShrinkStage = kManyRows * 128 + kNT * 8 * 128;
 constexpr int kShrinkStages = 3;
 template <typename T, int kNT>
-__global__ void __launch_bounds__(kThreads) shrink_many_kernel(const LoraArgs a) {
+__global__ void __launch_bounds__(kThreads) shrink_several_kernel(const LoraArgs a) {
   dependents_may_start();
   constexpr int kRanks = kNT * 8;
   extern __shared__ __align__(128) std::uint8_t smem[];
   const int tile_number = static_cast<int>(blockIdx.x) / a.parts, part = static_cast<int>(blockIdx.x) % a.parts;
-  if (tile_number >= a.plan.head->tiles) return;
+  if (tile_number >= *a.plan.count) return;
   const Tile tile = a.plan.tiles[tile_number];
   if (tile.adapter < 0) return;
   const int rank = rank_of(a, tile.adapter);
@@ -382,7 +406,7 @@ struct Low {
     for (int s = 0; s < kSteps; ++s) {
       const std::int64_t at = (row0 / 16 * kSteps + s) * 32 + g * 4 + c;
       hi[s] = lo[s] = make_uint4(0, 0, 0, 0);
-      if (c * kPer < kNT * 8) hi[s] = static_cast<const uint4*>(a.t_hi)[at], lo[s] = static_cast<const uint4*>(a.t_lo)[at];  // (8 ranks: the upper lanes have none)
+      if (c * kPer < kNT * 8) hi[s] = reinterpret_cast<const uint4*>(a.t_hi)[at], lo[s] = reinterpret_cast<const uint4*>(a.t_lo)[at];  // (8 ranks: the upper lanes have none)
     }
   }
 };
@@ -455,7 +479,7 @@ struct OutRows {
 };
 // The tile of a CTA; one that has nothing to do says so.
 __device__ __forceinline__ bool tile_to_add(const LoraArgs& a, Tile& tile) {
-  const bool exists = static_cast<int>(blockIdx.x) < a.plan.head->tiles;
+  const bool exists = static_cast<int>(blockIdx.x) < *a.plan.count;
   if (exists) tile = a.plan.tiles[blockIdx.x];
   return exists && (tile.adapter >= 0 || a.y != a.out);
 }
@@ -514,13 +538,13 @@ __global__ void __launch_bounds__(kThreads) expand_few_kernel(const LoraArgs a) 
 // bits that `fold` takes.
 __device__ __forceinline__ int folded(int piece, int fold) { return (piece & ~7) | ((piece & 7) ^ fold); }
 
-// Many: eight warps of 16 rows each, 32 columns at a time through four stages of shared memory: a lane copies the pieces of y that it adds to, B is
+// Several: eight warps of 16 rows each, 32 columns at a time through four stages of shared memory: a lane copies the pieces of y that it adds to, B is
 // everybody's. What bounds it is memory: y is read and out written once.
 constexpr int kManyThreads = 256, kExpandStages = 4;
 template <int kNT>
 constexpr int kExpandStage = 32 * kNT * 16 + kManyRows * 64;
 template <typename T, int kNT>
-__global__ void __launch_bounds__(kManyThreads, kNT <= 8 ? 3 : 2) expand_many_kernel(const LoraArgs a) {
+__global__ void __launch_bounds__(kManyThreads, kNT <= 8 ? 3 : 2) expand_several_kernel(const LoraArgs a) {
   using L = Low<T, kNT>;
   constexpr int kRanks = kNT * 8, kBBytes = 32 * kNT * 16;
   extern __shared__ __align__(128) std::uint8_t smem[];
@@ -618,54 +642,384 @@ __global__ void __launch_bounds__(kManyThreads, kNT <= 8 ? 3 : 2) expand_many_ke
   else add_all(std::false_type{});
 }
 
+// What the kernels of many tokens share: a bounded wait that gave up, barriers of MMAs, where the accumulators are.
+struct Tensor {
+  std::uint64_t done[4];
+  std::uint32_t memory;
+  int abort;
+};
+template <int kColumns>
+__device__ __forceinline__ void begin_tensor(Tensor& s) {
+  if (threadIdx.x / 32 == 0) {
+    tmem_alloc(smem_u32(&s.memory), kColumns);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0) {
+    s.abort = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&s.done[i]), 1);
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+}
+// Frees the tensor memory once everybody is done with it. A wait that expired is reported; what was issued has had time to end by then.
+template <int kColumns>
+__device__ __forceinline__ void end_tensor(Tensor& s) {
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (s.abort != 0) {
+    if (threadIdx.x == 0) atomicOr(&g_lora_status, kLoraWait);
+    const std::uint64_t t0 = global_ns();
+    while (global_ns() - t0 < 2000000ull) {
+    }
+  }
+  if (threadIdx.x / 32 == 0) tmem_dealloc(s.memory, kColumns);
+}
+
+// Many tokens: 128 of a tile in one kernel, both products by tcgen05. A cluster of CTAs divides the channels, then the columns: each adds up x A^T over its
+// own channels (64 at a time), they exchange the sums through distributed shared memory, and each adds t B^T to its own columns of y (64 at a time), t in
+// tensor memory in its two 16-bit parts. Both kinds of steps run through the same stages of shared memory, rows of 128 bytes with the 128-byte swizzle,
+// so that y and B are on their way while the sums are exchanged. A tile's tokens need not be neighbours, so that the threads copy the rows, piece by
+// piece. Where tiles are few several clusters share one: each makes the tile's sums and has some of the columns. Memory bounds it: x and y are read, out written.
+// (As two kernels, x A^T left in global memory: 8191 tokens, 4096 to 4096, rank 64: 71 us, on mma.sync, whose rate is a quarter, 69.)
+template <int kNT>
+struct ManyShape {
+  static constexpr int kN = kNT < 2 ? 16 : kNT * 8;                               // ranks of an MMA
+  static constexpr int kOperand = kN > 64 ? 128 * 128 : 64 * 128;                 // of a step: A's ranks by 64 channels, or B's 64 columns by its ranks
+  static constexpr int kStage = kOperand + kManyRows * 128, kStages = kN > 64 ? 3 : 4;
+  static constexpr int kLow = 128, kColumns = 256;                                // accumulators (of x A^T, then of two steps' t B^T); from kLow on t
+  static constexpr int kBytes = kStages * kStage + 1024;                          // and what aligns it
+  // The sums that are exchanged: blocks of ranks, 16 KB at most each, as many to a stage as two stages take them all.
+  static constexpr int kBlock = kN < 32 ? 16 : 32, kBlocks = kN / kBlock, kPerStage = (kBlocks + 1) / 2;
+  static_assert(kManyRows * kBlock * 4 * kPerStage <= kStage && kManyRows * kN * 2 <= kStage, "the sums, then t's parts, lie in two stages' places");
+};
+template <typename T, int kNT>
+__global__ void __launch_bounds__(kManyThreads, 2) many_kernel(const LoraArgs a) {
+  using S = ManyShape<kNT>;
+  extern __shared__ std::uint8_t smem_raw[];
+  __shared__ Tensor sh;
+  __shared__ float s_back[kManyRows];
+  const int part = static_cast<int>(blockIdx.x) % a.parts, group = static_cast<int>(blockIdx.x) / a.parts % a.groups;
+  const int tile_number = static_cast<int>(blockIdx.x) / a.parts / a.groups;
+  if (tile_number >= *a.plan.count) return;
+  const Tile tile = a.plan.tiles[tile_number];
+  if (tile.adapter < 0 && a.y == a.out) return;
+  const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
+  const int from_k = part * a.slice, to_k = min(a.dim, from_k + a.slice), k_steps = a.slice / 64;  // (as many for every part)
+  const int from = min(a.width, (group * a.parts + part) * a.columns), to = min(a.width, from + a.columns), steps = k_steps + (to - from + 63) / 64;
+  // A warp has 32 rows of the tile and one half of a step's 128 bytes of each. Lane l moves piece l % 4 of rows l / 4, l / 4 + 8, l / 4 + 16, l / 4 + 24.
+  const int row0 = warp % 4 * 32, half = warp / 4, column = half * 32 + lane % 4 * 8;
+  const T* x_from[4];
+  const T* y_from[4];
+  T* out_to[4];
+  bool there[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = row0 + lane / 4 + i * 8;
+    there[i] = r < tile.count;
+    const std::int64_t token = there[i] ? a.plan.order[tile.first + r] : 0;
+    x_from[i] = static_cast<const T*>(a.x) + token * a.ldx + from_k + column;
+    y_from[i] = static_cast<const T*>(a.y) + token * a.ldy + from + column, out_to[i] = static_cast<T*>(a.out) + token * a.ldo + from + column;
+  }
+  if (tile.adapter < 0) {  // (they only move)
+    for (int n = 0; n < to - from; n += 64) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (there[i] && n + column < to - from) *reinterpret_cast<uint4*>(out_to[i] + n) = load16(y_from[i] + n);
+      }
+    }
+    return;
+  }
+  const int rank = rank_of(a, tile.adapter);
+  std::uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const std::uint32_t ring = smem_u32(smem);
+  const T* const wa = static_cast<const T*>(a.a) + tile.adapter * a.a_adapter + from_k;
+  const T* const wb = static_cast<const T*>(a.b) + tile.adapter * a.b_adapter + from * a.b_row;
+  const auto at_piece = [](int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); };
+  constexpr int kPieces = S::kN / 8;
+  const auto copy_step = [&](int s) {
+    if (s < steps) {
+      const std::uint32_t at = ring + s % S::kStages * S::kStage;
+      const bool first = s < k_steps;
+      const int n = (first ? s : s - k_steps) * 64, left = (first ? to_k - from_k : to - from) - n;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool in = there[i] && column < left;
+        copy16(at + S::kOperand + at_piece(row0 + lane / 4 + i * 8, half * 4 + lane % 4), in ? (first ? x_from[i] : y_from[i]) + n : a.x, in);
+      }
+      if (first) {
+#pragma unroll
+        for (int i = 0; i < (S::kN * 8 + kManyThreads - 1) / kManyThreads; ++i) {
+          const int row = tid / 8 + i * (kManyThreads / 8), piece = tid % 8;
+          if (S::kN < kManyThreads / 8 && row >= S::kN) continue;
+          const bool in = row < rank && piece * 8 < left;
+          copy16(at + at_piece(row, piece), in ? wa + row * a.a_row + n + piece * 8 : wa, in);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < (64 * kPieces + kManyThreads - 1) / kManyThreads; ++i) {
+          const int j = tid + i * kManyThreads, row = j / kPieces, piece = j % kPieces;
+          if (64 * kPieces < kManyThreads && row >= 64) continue;
+          const bool in = row < left && piece * 8 < rank;
+          copy16(at + piece / 8 * (64 * 128) + at_piece(row, piece & 7), in ? wb + (n + row) * a.b_row + piece * 8 : wb, in);
+        }
+      }
+    }
+    copies_are_one_group();
+  };
+  // The two stages that are free last ahead of the exchange stay free until it is over.
+  const int held = k_steps + S::kStages - 2;
+#pragma unroll
+  for (int i = 0; i < S::kStages; ++i) {
+    if (i < held) copy_step(i);
+  }
+  begin_tensor<S::kColumns>(sh);
+  const std::uint32_t lanes = static_cast<std::uint32_t>(row0) << 16, accumulators = sh.memory, low = sh.memory + S::kLow;
+  constexpr int kFormat = std::is_same<T, __half>::value ? 0 : 1;
+  constexpr std::uint32_t idesc_a = umma_idesc(/*f32*/ 1, kFormat, kFormat, 0, 0, kManyRows, S::kN), idesc_b = umma_idesc(1, kFormat, kFormat, 0, 0, kManyRows, 64);
+  bool lost = false;
+  const auto wait_done = [&](int s) {  // the MMAs of step s
+    if (!lost) lost = !warp_wait_bar(smem_u32(&sh.done[s % S::kStages]), static_cast<std::uint32_t>(s / S::kStages) & 1u, &sh.abort);
+    tc_fence_after();
+  };
+  const auto copies_are_there = [&] {  // of the step that is next; everybody's
+    wait_for_copies<S::kStages - 2>();
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  };
+  for (int s = 0; s < k_steps; ++s) {
+    copies_are_there();
+    if (warp == 0 && elect_one()) {
+      const std::uint32_t at = ring + s % S::kStages * S::kStage;
+      const std::uint64_t dx = umma_desc_sw128(at + S::kOperand), dw = umma_desc_sw128(at);
+#pragma unroll
+      for (std::uint32_t i = 0; i < 4; ++i) umma_f16(accumulators, dx + 2 * i, dw + 2 * i, idesc_a, static_cast<std::uint32_t>(s) + i);
+      tc_commit(smem_u32(&sh.done[s % S::kStages]));
+    }
+    if (s > 0) {
+      wait_done(s - 1);
+      if (s - 1 + S::kStages < held) copy_step(s - 1 + S::kStages);
+    }
+  }
+  wait_done(k_steps - 1);
+
+  // The sums of all parts, joined by every CTA for itself: lanes side by side read a row's neighbouring ranks. (A thread a row, 144 bytes from the next
+  // thread's, took 25 us of reads from the other CTAs' shared memory.)
+  float back;
+  {
+    constexpr int kRowBytes = S::kBlock * 4, kLanes = S::kBlock / 4, kRows = kManyThreads / kLanes, kRounds = kManyRows / kRows;
+    const auto stage_of = [&](int i) { return smem + (k_steps + S::kStages - 1 - i) % S::kStages * S::kStage; };
+    const auto swizzled = [](int row, int piece) { return S::kBlock == 32 ? piece ^ (row & 7) : piece ^ (row >> 1 & 3); };
+    const auto sum_at = [&](int b, int row, int piece) { return stage_of(b / S::kPerStage) + b % S::kPerStage * (kManyRows * kRowBytes) + row * kRowBytes + swizzled(row, piece) * 16; };
+#pragma unroll
+    for (int b = half; b < S::kBlocks; b += 2) {
+      std::uint32_t r[S::kBlock];
+      if constexpr (S::kBlock == 16) tmem_ld_32x16(accumulators + lanes + b * S::kBlock, r);
+      else tmem_ld_32x32(accumulators + lanes + b * S::kBlock, r);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < kLanes; ++i) *reinterpret_cast<uint4*>(sum_at(b, row0 + lane, i)) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+    }
+    if (a.parts > 1) cluster_sync_all();
+    else __syncthreads();
+    const float scale = a.scales != nullptr ? a.scales[tile.adapter] : 1.f;
+    const int piece = tid % kLanes;
+    float v[kRounds][S::kBlocks][4];
+    const auto gather = [&](auto parts) {  // (the parts' number at compile time: all of a block's loads are on their way together)
+      constexpr int kParts = decltype(parts)::value;
+#pragma unroll
+      for (int i = 0; i < kRounds; ++i) {
+        const int row = tid / kLanes + i * kRows;
+#pragma unroll
+        for (int b = 0; b < S::kBlocks; ++b) {
+          const std::uint32_t at = smem_u32(sum_at(b, row, piece));
+          float4 o[kParts];
+#pragma unroll
+          for (int q = 0; q < kParts; ++q) o[q] = ld_cluster_f32x4(map_to_cta(at, static_cast<std::uint32_t>(q)));
+#pragma unroll
+          for (int q = 1; q < kParts; ++q) o[0].x += o[q].x, o[0].y += o[q].y, o[0].z += o[q].z, o[0].w += o[q].w;
+          v[i][b][0] = o[0].x, v[i][b][1] = o[0].y, v[i][b][2] = o[0].z, v[i][b][3] = o[0].w;
+        }
+      }
+    };
+    if (a.parts == 1) gather(std::integral_constant<int, 1>{});
+    else if (a.parts == 2) gather(std::integral_constant<int, 2>{});
+    else gather(std::integral_constant<int, kMostManyParts>{});
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+#pragma unroll
+      for (int b = 0; b < S::kBlocks; ++b) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][b][e] = b * S::kBlock + piece * 4 + e < rank ? v[i][b][e] * scale : 0.f;  // (infinities of x have made NaN of the others)
+      }
+    }
+    if (a.parts > 1) cluster_sync_all();  // (read by all)
+    else __syncthreads();
+    // Its two parts as rows, in the same place, then a row to a thread and into tensor memory.
+    constexpr int kTRow = S::kN * 2;
+    const auto t_at = [&](int which, int row, int at) { return stage_of(which) + row * kTRow + (S::kN >= 64 ? (at & ~7) | ((at & 7) ^ (row & 7)) : at) * 16; };
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int row = tid / kLanes + i * kRows;
+      float top = 0.f;
+      if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+        for (int b = 0; b < S::kBlocks; ++b) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[i][b][e]));
+        }
+#pragma unroll
+        for (int m = kLanes / 2; m > 0; m /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+      }
+      const Halves<T> by(top);
+#pragma unroll
+      for (int b = 0; b < S::kBlocks; ++b) {
+        uint2 hi, lo;
+        by.split(v[i][b][0], v[i][b][1], hi.x, lo.x), by.split(v[i][b][2], v[i][b][3], hi.y, lo.y);
+        const int at = b * S::kBlock + piece * 4;  // (the rank)
+        *reinterpret_cast<uint2*>(t_at(0, row, at / 8) + at % 8 * 2) = hi, *reinterpret_cast<uint2*>(t_at(1, row, at / 8) + at % 8 * 2) = lo;
+      }
+      if (std::is_same<T, __half>::value && piece == 0) s_back[row] = by.back;
+    }
+    __syncthreads();
+    back = std::is_same<T, __half>::value ? s_back[row0 + lane] : 1.f;
+#pragma unroll
+    for (int i = 0; i < S::kN / 8; ++i) {
+      const uint4 p = load16(t_at(half, row0 + lane, i));
+      const std::uint32_t r[4] = {p.x, p.y, p.z, p.w};
+      tmem_st_32x4(low + lanes + half * (S::kN / 2) + i * 4, r);
+    }
+    tmem_st_wait();
+    __syncthreads();  // (read by all)
+  }
+  copy_step(held);
+
+  for (int s = k_steps; s <= steps; ++s) {
+    if (s < steps) {
+      if (rank % 8 != 0) {  // the last piece that is used has ranks behind the last one: whatever they hold, they are zeros
+        wait_for_copies<S::kStages - 2>();
+        __syncthreads();
+        const int piece = rank / 8;
+        for (int r = tid; r < 64; r += kManyThreads) {
+          std::uint16_t* const p = reinterpret_cast<std::uint16_t*>(smem + s % S::kStages * S::kStage + piece / 8 * (64 * 128) + at_piece(r, piece & 7));
+          for (int e = rank % 8; e < 8; ++e) p[e] = 0;
+        }
+      }
+      copies_are_there();  // (and the accumulator of the step before the last has been read)
+      if (warp == 0 && elect_one()) {
+        const std::uint32_t at = ring + s % S::kStages * S::kStage, d = accumulators + (s & 1) * 64;
+#pragma unroll
+        for (int i = 0; i < S::kN / 16; ++i) {
+          const std::uint64_t db = umma_desc_sw128(at + i / 4 * (64 * 128)) + 2 * (i % 4);
+          umma_f16_ts(d, low + i * 8, db, idesc_b, static_cast<std::uint32_t>(i));
+          umma_f16_ts(d, low + S::kN / 2 + i * 8, db, idesc_b, 1u);
+        }
+        tc_commit(smem_u32(&sh.done[s % S::kStages]));
+      }
+    }
+    const int e = s - 1;  // the step that is added
+    if (e >= k_steps) {
+      wait_done(e);
+      std::uint32_t v[32];
+      tmem_ld_32x32(accumulators + (e & 1) * 64 + lanes + half * 32, v);
+      tmem_ld_wait();
+      std::uint8_t* const at = smem + e % S::kStages * S::kStage + S::kOperand;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint4* const p = reinterpret_cast<uint4*>(at + at_piece(row0 + lane, half * 4 + i));
+        float f[8];
+        load8<T>(*p, f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = fmaf(__uint_as_float(v[8 * i + j]), back, f[j]);
+        *p = store8<T>(f);
+      }
+      __syncwarp();
+      const int n = (e - k_steps) * 64;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 p = load16(at + at_piece(row0 + lane / 4 + i * 8, half * 4 + lane % 4));
+        if (there[i] && n + column < to - from) *reinterpret_cast<uint4*>(out_to[i] + n) = p;
+      }
+      __syncwarp();  // (this warp's pieces of the stage are read: it is the next to be copied into)
+    }
+    copy_step(e + S::kStages);
+  }
+  wait_for_copies<0>();
+  end_tensor<S::kColumns>(sh);
+}
+
 inline int padded_tiles(int rank) {  // ranks / 8, up to a power of two
   int n = 1;
   while (n * 8 < rank) n *= 2;
   return n;
 }
-// Parts of the channels (a power of two): CTAs for the whole GPU twice (of few tokens) or three times over, of 256 channels at least.
-inline int parts_of(std::int64_t tokens, int adapters, std::int64_t dim) {
-  const std::int64_t tiles = most_tiles(tokens, adapters), room = (tokens <= kFewTokens ? 2 : 3) * 148;
+// Which kernels a call runs, by the rows of its tiles times the ranks: what they do with tiles that are not full, and what mma.sync's rate costs. Measured with
+// 4096 channels and columns, few / several / many tokens' kernels, us: 300 tokens of 3 adapters, rank 128 (2688 by small tiles) 20 / 23 / 24, 700 of
+// 4, rank 64 (3072) 22 / 17 / 27; 3000 of 4, rank 128 (3584 by large ones) several 50, many 48, 5000 of 6, rank 64 (2944) 45 / 50, 8191 of 6, rank 64 (4544)
+// 65 / 57, rank 128 99 / 70.
+enum class Way { kFew, kSeveral, kMany };
+inline Way way_of(std::int64_t tokens, int adapters, int rank) {
+  if (tokens <= kFewTokens && most_tiles(tokens, adapters, kFewRows) * rank <= 2800) return Way::kFew;
+  return most_tiles(tokens, adapters, kManyRows) * rank >= 3500 ? Way::kMany : Way::kSeveral;
+}
+inline int rows_of(Way way) { return way == Way::kFew ? kFewRows : kManyRows; }
+// Parts of the channels (a power of two): CTAs for the whole GPU twice over (thrice of several tokens), of 256 channels at least.
+inline int parts_of(Way way, std::int64_t tiles, std::int64_t dim) {
+  const std::int64_t room = (way == Way::kSeveral ? 3 : 2) * 148, most = way == Way::kMany ? kMostManyParts : kMostParts;
   int parts = 1;
-  while (parts < kMostParts && tiles * parts * 2 <= room && dim >= parts * 2 * 256) parts *= 2;
+  while (parts < most && tiles * parts * 2 <= room && dim >= parts * 2 * 256) parts *= 2;
   return parts;
 }
-inline std::size_t rows_of(std::int64_t tokens, int adapters) { return static_cast<std::size_t>(most_tiles(tokens, adapters)) * tile_rows(tokens); }
-inline std::size_t part_bytes(std::int64_t tokens, int adapters, int rank) {  // (an operand has 16 ranks at least)
-  return (rows_of(tokens, adapters) * std::max(2, padded_tiles(rank)) * 16 + 255) / 256 * 256;
-}
+// Of few and several tokens: one of t's two parts (an operand has 16 ranks at least).
+inline std::size_t part_bytes(std::int64_t rows, int rank) { return (static_cast<std::size_t>(rows) * std::max(2, padded_tiles(rank)) * 16 + 255) / 256 * 256; }
 inline std::size_t workspace_bytes(std::int64_t tokens, int adapters, int rank) {
-  return std::max<std::size_t>(256, 2 * part_bytes(tokens, adapters, rank) + rows_of(tokens, adapters) * 4);
+  const Way way = way_of(tokens, adapters, rank);
+  if (way == Way::kMany) return 0;
+  const std::int64_t rows = most_tiles(tokens, adapters, rows_of(way)) * rows_of(way);
+  return 2 * part_bytes(rows, rank) + static_cast<std::size_t>(rows) * 4;
 }
 
 template <typename T, int kNT>
-int launch(const char* op, LoraArgs a, std::int64_t tokens, cudaStream_t stream) {
-  const unsigned tiles = static_cast<unsigned>(most_tiles(tokens, a.adapters));
+int launch(const char* op, LoraArgs a, Way way, unsigned tiles, cudaStream_t stream) {
   const LaunchChain chain(stream);
-  // Columns of a CTA: as many as leave 8 small or 4 large CTAs to an SM, 128 at least.
-  const bool few = tokens <= kFewTokens;
-  const std::int64_t most = std::max<std::int64_t>(1, (few ? 8LL : 4LL) * sm_count() / tiles);
-  a.columns = static_cast<int>(std::max<std::int64_t>(128, ((a.width + most - 1) / most + 127) / 128 * 128));
-  const dim3 grid(tiles, static_cast<unsigned>((a.width + a.columns - 1) / a.columns));
-  if (few) {
-    if (const int s = enqueue(op, shrink_few_kernel<T, kNT>, dim3(tiles * a.parts), dim3(kThreads), 0, stream, a.parts, a); s != B2_OK) return s;
-    return enqueue(op, expand_few_kernel<T, kNT>, grid, dim3(kThreads), 0, stream, 1, a);
+  if (way != Way::kMany) {
+    // Columns of a CTA: as many as leave 8 small or 4 large CTAs to an SM, 128 at least.
+    const std::int64_t most = std::max<std::int64_t>(1, (way == Way::kFew ? 8LL : 4LL) * sm_count() / tiles);
+    a.columns = static_cast<int>(std::max<std::int64_t>(128, ((a.width + most - 1) / most + 127) / 128 * 128));
+    const dim3 grid(tiles, static_cast<unsigned>((a.width + a.columns - 1) / a.columns));
+    if (way == Way::kFew) {
+      if (const int s = enqueue(op, shrink_few_kernel<T, kNT>, dim3(tiles * a.parts), dim3(kThreads), 0, stream, a.parts, a); s != B2_OK) return s;
+      return enqueue(op, expand_few_kernel<T, kNT>, grid, dim3(kThreads), 0, stream, 1, a);
+    }
+    static std::atomic<std::uint64_t> shrink_done{0}, expand_done{0};
+    constexpr int kShrinkBytes = kShrinkStages * kShrinkStage<kNT>, kExpandBytes = kExpandStages * kExpandStage<kNT>;
+    if (const int s = allow_shared(op, shrink_several_kernel<T, kNT>, kShrinkBytes, shrink_done); s != B2_OK) return s;
+    if (const int s = allow_shared(op, expand_several_kernel<T, kNT>, kExpandBytes, expand_done); s != B2_OK) return s;
+    if (const int s = enqueue(op, shrink_several_kernel<T, kNT>, dim3(tiles * a.parts), dim3(kThreads), kShrinkBytes, stream, a.parts, a); s != B2_OK) return s;
+    return enqueue(op, expand_several_kernel<T, kNT>, grid, dim3(kManyThreads), kExpandBytes, stream, 1, a);
   }
-  static std::atomic<std::uint64_t> shrink_done{0}, expand_done{0};
-  constexpr int kShrinkBytes = kShrinkStages * kShrinkStage<kNT>, kExpandBytes = kExpandStages * kExpandStage<kNT>;
-  if (const int s = allow_shared(op, shrink_many_kernel<T, kNT>, kShrinkBytes, shrink_done); s != B2_OK) return s;
-  if (const int s = allow_shared(op, expand_many_kernel<T, kNT>, kExpandBytes, expand_done); s != B2_OK) return s;
-  if (const int s = enqueue(op, shrink_many_kernel<T, kNT>, dim3(tiles * a.parts), dim3(kThreads), kShrinkBytes, stream, a.parts, a); s != B2_OK) return s;
-  return enqueue(op, expand_many_kernel<T, kNT>, grid, dim3(kManyThreads), kExpandBytes, stream, 1, a);
+  static std::atomic<std::uint64_t> done{0};
+  if (const int s = allow_shared(op, many_kernel<T, kNT>, ManyShape<kNT>::kBytes, done); s != B2_OK) return s;
+  // Clusters to a tile: as many as the GPU has room for (2 CTAs to an SM), of 128 columns a CTA at least.
+  const std::int64_t room = std::max<std::int64_t>(1, 2LL * sm_count() / (static_cast<std::int64_t>(tiles) * a.parts));
+  a.groups = static_cast<int>(std::max<std::int64_t>(1, std::min<std::int64_t>(room, a.width / (128 * a.parts))));
+  a.columns = (a.width + a.parts * a.groups - 1) / (a.parts * a.groups);
+  a.columns = (a.columns + 63) / 64 * 64;
+  return enqueue(op, many_kernel<T, kNT>, dim3(tiles * a.parts * a.groups), dim3(kManyThreads), ManyShape<kNT>::kBytes, stream, a.parts, a);
 }
 template <typename T>
-int launch(const char* op, const LoraArgs& a, std::int64_t tokens, cudaStream_t stream) {
+int launch(const char* op, const LoraArgs& a, Way way, unsigned tiles, cudaStream_t stream) {
   switch (padded_tiles(a.rank)) {
-    case 1: return launch<T, 1>(op, a, tokens, stream);
-    case 2: return launch<T, 2>(op, a, tokens, stream);
-    case 4: return launch<T, 4>(op, a, tokens, stream);
-    case 8: return launch<T, 8>(op, a, tokens, stream);
-    default: return launch<T, 16>(op, a, tokens, stream);
+    case 1: return launch<T, 1>(op, a, way, tiles, stream);
+    case 2: return launch<T, 2>(op, a, way, tiles, stream);
+    case 4: return launch<T, 4>(op, a, way, tiles, stream);
+    case 8: return launch<T, 8>(op, a, way, tiles, stream);
+    default: return launch<T, 16>(op, a, way, tiles, stream);
   }
 }
 
@@ -697,17 +1051,15 @@ int b2_lora_plan(const int32_t* token_adapters, int64_t tokens, int adapters, vo
   if (plan == nullptr || !aligned_to(plan, 256) || bytes < plan_bytes(tokens, adapters)) return fail_invalid(op, "plan is missing, too small or not 256-byte aligned");
   if (tokens == 0) return B2_OK;
   if (token_adapters == nullptr || !aligned_to(token_adapters, 4)) return fail_invalid(op, "token_adapters is missing or not aligned");
-  const Plan p = plan_at(plan, tokens, adapters);
   return enqueue(op, plan_kernel, dim3(static_cast<unsigned>(adapters + 1)), dim3(kPlanThreads), static_cast<std::size_t>(adapters + 1) * 4, as_stream(stream), 1,
-                 token_adapters, static_cast<int>(tokens), adapters, tile_rows(tokens), const_cast<PlanHead*>(p.head), const_cast<Tile*>(p.tiles),
-                 const_cast<std::int32_t*>(p.order));
+                 token_adapters, static_cast<int>(tokens), adapters, plan_at(plan, tokens, adapters));
 }
 
 size_t b2_lora_workspace_bytes(int64_t tokens, int adapters, int64_t dim, int rank) {
   using namespace b2;
   const char* const op = "lora_add";
   if (check_sizes(op, tokens, adapters) != B2_OK || check_shape(op, dim, rank) != B2_OK) return 0;
-  return workspace_bytes(tokens, adapters, rank);
+  return std::max<std::size_t>(256, workspace_bytes(tokens, adapters, rank));
 }
 
 int b2_lora_add(const b2_lora* l, const void* plan, size_t bytes, int64_t tokens, const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, int64_t ldo,
@@ -731,16 +1083,19 @@ int b2_lora_add(const b2_lora* l, const void* plan, size_t bytes, int64_t tokens
   if (out == y && ldo != ldy) return fail_invalid(op, "out in y's place must have y's rows");
   if (const int s = check_workspace(op, workspace, ws_bytes, workspace_bytes(tokens, l->adapters, l->rank)); s != B2_OK) return s;
   LoraArgs a{};
-  a.plan = plan_at(plan, tokens, l->adapters);
+  const Way way = way_of(tokens, l->adapters, l->rank);
+  const std::int64_t tiles = most_tiles(tokens, l->adapters, rows_of(way));
+  const Plan p = plan_at(const_cast<void*>(plan), tokens, l->adapters);
+  a.plan = Tiles{&p.head->tiles[way != Way::kFew], p.tiles[way != Way::kFew], p.order};
   a.a = l->a, a.b = l->b, a.a_adapter = l->a_adapter_stride, a.a_row = l->a_row_stride, a.b_adapter = l->b_adapter_stride, a.b_row = l->b_row_stride;
   a.scales = l->scales, a.ranks = l->ranks, a.x = x, a.y = y, a.out = out, a.ldx = ldx, a.ldy = ldy, a.ldo = ldo;
   a.adapters = l->adapters, a.rank = l->rank, a.dim = static_cast<int>(l->dim), a.width = static_cast<int>(l->width);
   char* const at = static_cast<char*>(workspace);
-  const std::size_t part = part_bytes(tokens, l->adapters, l->rank);
-  a.t_hi = at, a.t_lo = at + part, a.t_back = reinterpret_cast<float*>(at + 2 * part);
-  a.parts = parts_of(tokens, l->adapters, l->dim);
+  const std::size_t part = part_bytes(tiles * rows_of(way), l->rank);
+  a.t_hi = reinterpret_cast<std::uint32_t*>(at), a.t_lo = reinterpret_cast<std::uint32_t*>(at + part), a.t_back = reinterpret_cast<float*>(at + 2 * part);
+  a.parts = parts_of(way, tiles, l->dim);
   a.slice = static_cast<int>(((l->dim + a.parts - 1) / a.parts + 63) / 64 * 64);
-  return l->dtype == B2_DTYPE_F16 ? launch<__half>(op, a, tokens, as_stream(stream)) : launch<__nv_bfloat16>(op, a, tokens, as_stream(stream));
+  return l->dtype == B2_DTYPE_F16 ? launch<__half>(op, a, way, static_cast<unsigned>(tiles), as_stream(stream)) : launch<__nv_bfloat16>(op, a, way, static_cast<unsigned>(tiles), as_stream(stream));
 }
 
 int b2_lora_status(unsigned* host_value, int clear) {

@@ -890,20 +890,21 @@ _CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _NORM_BYTES, _LOGPROBS_BYTES, _LORA_BYTES = C.sizeof(_lib.NormQuantize), C.sizeof(_lib.Logprobs), C.sizeof(_lib.Lora)
 
 
-def _here(device, **tensors):
-    """All tensors lie on the current CUDA device (`device`: that of the call's first one)."""
-    if device.type != "cuda" or device.index != (torch.cuda.current_device() if _get_device is None else _get_device()):
+def _here(first, *others):
+    """All tensors that are given lie on the current CUDA device."""
+    at = first.get_device()
+    if at < 0 or at != (torch.cuda.current_device() if _get_device is None else _get_device()):
         raise ValueError("the tensors must be on the current CUDA device")
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} must be on the device of the other tensors")
+    for t in others:
+        if t is not None and t.get_device() != at:
+            raise ValueError("the tensors must be on the current CUDA device")
 
 
 def _like(t, name, shape, dtypes):
     """Row stride of a matrix of this shape, of one of `dtypes`, whose rows are contiguous."""
     if t.dtype not in dtypes or t.shape != shape:
         raise ValueError(f"{name} must be a {list(shape)} matrix of {' or '.join(map(str, dtypes))}")
-    return _rows(t, name, t.dtype)[1]
+    return shape[1] if t.is_contiguous() else _rows(t, name, t.dtype)[1]
 
 
 def add_rms_norm_quantize(x, weight=None, residual=None, eps=1e-6, dtype=torch.int8, group=0, residual_out=None, norm_out=None, q=None, scale=None):
@@ -911,42 +912,44 @@ def add_rms_norm_quantize(x, weight=None, residual=None, eps=1e-6, dtype=torch.i
     for the projection that follows: codes of `dtype` (int8 or float8_e4m3fn) with an fp32 scale per token, or per `group` channels
     (32, 64, 128 or 256). x bf16, fp16 or fp32, the residual of x's type or fp32. norm_out (bf16 or fp16 [tokens, dim]) receives the norm
     unquantised besides, for adapters. Returns (q, scale): scale [tokens], or [tokens, dim / group]."""
-    code, types = _DTYPES_ALL.get(x.dtype), _DTYPES_ALL
-    if code is None or dtype not in _CODES:
+    types = _DTYPES_ALL
+    x_dtype = x.dtype
+    code, codes = types.get(x_dtype), _CODES.get(dtype)
+    if code is None or codes is None:
         raise ValueError("x must be bf16, fp16 or fp32, the codes int8 or float8_e4m3fn")
-    tokens, ldx = _rows(x, "x", x.dtype)
+    tokens, ldx = _rows(x, "x", x_dtype)
     shape, device = x.shape, x.device
     dim = shape[1]
     if group < 0 or (group and dim % group):
         raise ValueError("group must be 0, 32, 64, 128 or 256 and divide dim")
-    ld_res = ld_res_out = ld_norm = 0
+    ld_res = ld_res_out = ld_norm = at_res = at_res_out = r_code = 0
     if residual is not None:
-        ld_res = ld_res_out = _like(residual, "residual", shape, (x.dtype, torch.float32))
+        ld_res = ld_res_out = _like(residual, "residual", shape, (x_dtype, torch.float32))
+        r_code, at_res = types[residual.dtype], residual.data_ptr()
         if residual_out is None:
-            residual_out = residual
-        elif residual_out is not residual:
-            ld_res_out = _like(residual_out, "residual_out", shape, (residual.dtype,))
+            at_res_out = at_res
+        else:
+            ld_res_out, at_res_out = _like(residual_out, "residual_out", shape, (residual.dtype,)), residual_out.data_ptr()
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
     if norm_out is not None:
         ld_norm = _like(norm_out, "norm_out", shape, (torch.bfloat16, torch.float16))
     if weight is not None and (weight.dtype not in types or weight.dim() != 1 or weight.numel() != dim or not weight.is_contiguous()):
         raise ValueError("weight must be a contiguous [dim] tensor of bf16, fp16 or fp32")
-    scales = (tokens, dim // group) if group else (tokens,)
+    ldq = dim if q is None else _like(q, "q", shape, (dtype,))
+    if scale is not None and (scale.dtype != torch.float32 or scale.shape != ((tokens, dim // group) if group else (tokens,)) or not scale.is_contiguous()):
+        raise ValueError("scale must be a contiguous fp32 tensor [tokens], or [tokens, dim / group]")
+    _here(x, residual, residual_out, norm_out, weight, q, scale)
+    # (empty_strided takes half of empty's time, a microsecond.)
     if q is None:
-        q = torch.empty(shape, dtype=dtype, device=device)
-        ldq = dim
-    else:
-        ldq = _like(q, "q", shape, (dtype,))
+        q = torch.empty_strided(shape, (dim, 1), dtype=dtype, device=device)
     if scale is None:
-        scale = torch.empty(scales, dtype=torch.float32, device=device)
-    elif scale.dtype != torch.float32 or scale.shape != scales or not scale.is_contiguous():
-        raise ValueError(f"scale must be a contiguous fp32 {list(scales)} tensor")
-    _here(device, residual=residual, residual_out=residual_out, norm_out=norm_out, weight=weight, q=q, scale=scale)
+        groups = dim // group if group else 1
+        scale = torch.empty_strided((tokens, groups) if group else (tokens,), (groups, 1) if group else (1,), dtype=torch.float32, device=device)
     check(_lib.lib().b2_add_rms_norm_quantize(
-        _lib.NormQuantize(_NORM_BYTES, tokens, dim, group, eps, _CODES[dtype], x.data_ptr(), ldx, _at(residual), ld_res, _at(residual_out), ld_res_out,
-                          _at(weight), _at(norm_out), ld_norm, q.data_ptr(), ldq, scale.data_ptr(), code, 0 if residual is None else types[residual.dtype],
-                          0 if weight is None else types[weight.dtype], 0 if norm_out is None else types[norm_out.dtype]), _raw_stream()))
+        _lib.NormQuantize(_NORM_BYTES, tokens, dim, group, eps, codes, x.data_ptr(), ldx, at_res, ld_res, at_res_out, ld_res_out,
+                          0 if weight is None else weight.data_ptr(), 0 if norm_out is None else norm_out.data_ptr(), ld_norm, q.data_ptr(), ldq, scale.data_ptr(),
+                          code, r_code, 0 if weight is None else types[weight.dtype], 0 if norm_out is None else types[norm_out.dtype]), _raw_stream()))
     return q, scale
 
 
@@ -970,19 +973,25 @@ def token_logprobs(logits, targets=None, top=0, scale=1.0):
     rows, ld = _rows(logits, "logits", logits.dtype)
     if targets is not None and (targets.dtype != torch.int64 or targets.dim() != 1 or targets.numel() != rows or not targets.is_contiguous()):
         raise ValueError("targets must be a contiguous int64 [rows] tensor")
-    device = logits.device
     if top < 0 or top > 32:
         raise ValueError("top must be from 0 to 32 and at most vocab")
-    _here(device, targets=targets)
-    # (One allocation for all outputs: each costs a microsecond.)
-    out = torch.empty((4 + 2 * top) * rows, dtype=torch.float32, device=device)
-    logprobs, entropy, lse, ranks, top_logprobs, top_tokens = out.split([rows, rows, rows, rows, rows * top, rows * top])
-    at = out.data_ptr()
+    _here(logits, targets)
+    device, new, one = logits.device, torch.empty_strided, (1,)
+    entropy = new((rows,), one, dtype=torch.float32, device=device)
+    lse = torch.empty_like(entropy)
+    logprobs = ranks = top_logprobs = top_tokens = None
+    at = [0, 0, 0, 0]
+    if targets is not None:
+        logprobs, ranks = torch.empty_like(entropy), new((rows,), one, dtype=torch.int32, device=device)
+        at[0], at[1] = logprobs.data_ptr(), ranks.data_ptr()
+    if top:
+        top_logprobs = new((rows, top), (top, 1), dtype=torch.float32, device=device)
+        top_tokens = new((rows, top), (top, 1), dtype=torch.int32, device=device)
+        at[2], at[3] = top_logprobs.data_ptr(), top_tokens.data_ptr()
     check(_lib.lib().b2_token_logprobs(
-        _lib.Logprobs(_LOGPROBS_BYTES, logits.data_ptr(), ld, rows, code, logits.shape[1], top, scale, _at(targets), at, at + 12 * rows, at + 4 * rows,
-                      at + 8 * rows, at + 16 * rows if top else 0, at + (16 + 4 * top) * rows if top else 0), _raw_stream()))
-    return TokenLogprobs(None if targets is None else logprobs, None if targets is None else ranks.view(torch.int32), entropy, lse,
-                         top_logprobs.view(rows, top) if top else None, top_tokens.view(torch.int32).view(rows, top) if top else None)
+        _lib.Logprobs(_LOGPROBS_BYTES, logits.data_ptr(), ld, rows, code, logits.shape[1], top, scale, 0 if targets is None else targets.data_ptr(), at[0], at[1],
+                      entropy.data_ptr(), lse.data_ptr(), at[2], at[3]), _raw_stream()))
+    return TokenLogprobs(logprobs, ranks, entropy, lse, top_logprobs, top_tokens)
 
 
 class LoraAdapters:
@@ -1005,7 +1014,7 @@ class LoraAdapters:
         for name, t in (("b", b), ("scales", scales), ("ranks", ranks)):
             if t is not None and t.device != a.device:
                 raise ValueError(f"{name} must be on a's device")
-        self.a, self.b, self.scales, self.ranks, self.dtype, self.device = a, b, scales, ranks, a.dtype, a.device
+        self.a, self.b, self.scales, self.ranks, self.dtype, self.dtypes, self.device = a, b, scales, ranks, a.dtype, (a.dtype,), a.device
         self.adapters, self.rank, self.dim, self.width = n, rank, dim, b.shape[1]
         self.struct = _lib.Lora(_LORA_BYTES, a.data_ptr(), b.data_ptr(), a.stride(0), max(a.stride(1), dim), b.stride(0), max(b.stride(1), rank), _at(scales),
                                 _at(ranks), dim, self.width, n, rank, code)
@@ -1022,13 +1031,15 @@ class LoraPlan:
         need = _lib.lib().b2_lora_plan_bytes(self.tokens, adapters)
         if need == 0:
             check(-1)
-        _here(token_adapters.device)
-        self.buffer = torch.empty(need, dtype=torch.uint8, device=token_adapters.device)
+        _here(token_adapters)
+        self.device, self.bytes = token_adapters.device, need
+        self.buffer = torch.empty(need, dtype=torch.uint8, device=self.device)
+        self.at = self.buffer.data_ptr()
         self.fill()
 
     def fill(self):
-        _here(self.buffer.device)
-        check(_lib.lib().b2_lora_plan(self.token_adapters.data_ptr(), self.tokens, self.adapters, self.buffer.data_ptr(), self.buffer.numel(), _raw_stream()))
+        _here(self.buffer, self.token_adapters)
+        check(_lib.lib().b2_lora_plan(self.token_adapters.data_ptr(), self.tokens, self.adapters, self.at, self.bytes, _raw_stream()))
 
     def workspace_bytes(self, dim, rank) -> int:
         need = self._sizes.get((dim, rank))
@@ -1043,21 +1054,25 @@ class LoraPlan:
 def lora_add(y, x, adapters, plan, out=None, workspace=None):
     """y [tokens, width] plus, for each token with an adapter, scale (x A^T) B^T of its row of x [tokens, dim]: in y's place, or into `out`. y and x
     are views with contiguous rows (a slice of a fused projection's columns, say). Returns out."""
+    tokens, dtypes = plan.tokens, adapters.dtypes
     if plan.adapters != adapters.adapters:
         raise ValueError("the plan is of another number of adapters")
-    ldx = _like(x, "x", (plan.tokens, adapters.dim), (adapters.dtype,))
-    ldy = ldo = _like(y, "y", (plan.tokens, adapters.width), (adapters.dtype,))
+    ldx = _like(x, "x", (tokens, adapters.dim), dtypes)
+    ldy = ldo = _like(y, "y", (tokens, adapters.width), dtypes)
     if out is None:
         out = y
     else:
-        ldo = _like(out, "out", (plan.tokens, adapters.width), (adapters.dtype,))
+        ldo = _like(out, "out", (tokens, adapters.width), dtypes)
+    _here(y, x, out, adapters.a, plan.buffer, workspace)
     need = plan.workspace_bytes(adapters.dim, adapters.rank)
-    device = y.device
-    _here(device, x=x, out=out, a=adapters.a, plan=plan.buffer, workspace=workspace)
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    check(_lib.lib().b2_lora_add(adapters.struct, plan.buffer.data_ptr(), plan.buffer.numel(), plan.tokens, x.data_ptr(), ldx, y.data_ptr(), ldy,
-                                 out.data_ptr(), ldo, workspace.data_ptr(), workspace.numel(), _raw_stream()))
+    if workspace is not None:
+        given = workspace.numel() * workspace.element_size()
+    elif need > 256:
+        workspace, given = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=plan.device), need
+    else:
+        given = 0  # (256: none is used)
+    check(_lib.lib().b2_lora_add(adapters.struct, plan.at, plan.bytes, tokens, x.data_ptr(), ldx, y.data_ptr(), ldy, out.data_ptr(), ldo, _at(workspace), given,
+                                 _raw_stream()))
     return out
 
 

@@ -50,7 +50,8 @@ def check(got, want, off, dtype):
 @pytest.mark.parametrize("dtype", [bf16, f16], ids=["bf16", "f16"])
 @pytest.mark.parametrize("tokens,dim,width,rank,adapters", [
     (1, 8, 8, 8, 1), (1, 2048, 2048, 16, 4), (15, 64, 24, 16, 3), (16, 40, 136, 24, 1), (17, 520, 1000, 40, 5), (100, 256, 512, 128, 60), (64, 4096, 640, 16, 48),
-    (1024, 72, 264, 8, 3), (1025, 136, 200, 64, 7), (3000, 512, 384, 32, 2), (1100, 2056, 72, 128, 2), (2000, 64, 128, 16, 700), (40, 104, 8, 56, 4096),
+    (4000, 1032, 200, 128, 6), (2500, 264, 72, 64, 50), (3000, 520, 1000, 24, 200), (500, 520, 264, 8, 450), (6000, 512, 72, 32, 90), (900, 1544, 520, 128, 30),
+    (64, 136, 264, 128, 40), (1024, 72, 264, 8, 3), (1025, 136, 200, 64, 7), (3000, 512, 384, 32, 2), (1100, 2056, 72, 128, 2), (2000, 64, 128, 16, 700), (40, 104, 8, 56, 4096),
 ])
 def test_against_the_formula(tokens, dim, width, rank, adapters, dtype):
     x, y, a, b, scales, ids = make(tokens, dim, width, rank, adapters, dtype, seed=tokens + dim)
@@ -65,27 +66,28 @@ def test_against_the_formula(tokens, dim, width, rank, adapters, dtype):
     assert torch.equal(y, out)
 
 
-@pytest.mark.parametrize("tokens", [50, 1500])
-def test_ranks_and_what_lies_behind_them(tokens):
-    x, y, a, b, scales, ids = make(tokens, 264, 72, 32, 6, bf16, seed=3)
-    ranks = torch.tensor([32, 0, 1, 7, 16, 30], dtype=torch.int32)
+# (each of the ways that a call can go: few tokens, several, and many by tiles times ranks)
+@pytest.mark.parametrize("tokens,rank,adapters", [(50, 32, 6), (1500, 32, 6), (1500, 32, 120), (300, 128, 30)])
+def test_ranks_and_what_lies_behind_them(tokens, rank, adapters):
+    x, y, a, b, scales, ids = make(tokens, 264, 72, rank, adapters, bf16, seed=3)
+    ranks = torch.tensor(([rank, 0, 1, 7, 16, rank - 2] * adapters)[:adapters], dtype=torch.int32)
     for n, r in enumerate(ranks.tolist()):
         a[n, r:] = float("nan")
         b[n, :, r:] = float("inf")
     want, off = exact(x, y, a, b, None, ids, ranks)
-    got = ops.lora_add(y, x, ops.LoraAdapters(a, b, None, ranks.cuda()), ops.LoraPlan(ids, 6), out=torch.empty_like(y))
+    got = ops.lora_add(y, x, ops.LoraAdapters(a, b, None, ranks.cuda()), ops.LoraPlan(ids, adapters), out=torch.empty_like(y))
     check(got, want, off, bf16)
 
 
-@pytest.mark.parametrize("tokens", [40, 1300])
-def test_views_leave_the_rest_alone(tokens):
-    x, y, a, b, scales, ids = make(tokens, 128, 256, 16, 4, bf16, seed=4)
+@pytest.mark.parametrize("tokens,adapters", [(40, 4), (1300, 4), (1300, 250)])
+def test_views_leave_the_rest_alone(tokens, adapters):
+    x, y, a, b, scales, ids = make(tokens, 128, 256, 16, adapters, bf16, seed=4)
     wide_x, wide_y = torch.full((tokens, 400), 3.0, dtype=bf16, device="cuda"), torch.full((tokens, 1000), 5.0, dtype=bf16, device="cuda")
     wide_x[:, 8:136], wide_y[:, 504:760] = x, y
-    wide_a, wide_b = torch.full((4, 48, 136), float("nan"), dtype=bf16, device="cuda"), torch.full((4, 260, 48), float("nan"), dtype=bf16, device="cuda")
+    wide_a, wide_b = torch.full((adapters, 48, 136), float("nan"), dtype=bf16, device="cuda"), torch.full((adapters, 260, 48), float("nan"), dtype=bf16, device="cuda")
     wide_a[:, 16:32, :128], wide_b[:, 2:258, 8:24] = a, b
-    want = ops.lora_add(y, x, ops.LoraAdapters(a, b, scales), ops.LoraPlan(ids, 4), out=torch.empty_like(y))
-    ops.lora_add(wide_y[:, 504:760], wide_x[:, 8:136], ops.LoraAdapters(wide_a[:, 16:32, :128], wide_b[:, 2:258, 8:24], scales), ops.LoraPlan(ids, 4))
+    want = ops.lora_add(y, x, ops.LoraAdapters(a, b, scales), ops.LoraPlan(ids, adapters), out=torch.empty_like(y))
+    ops.lora_add(wide_y[:, 504:760], wide_x[:, 8:136], ops.LoraAdapters(wide_a[:, 16:32, :128], wide_b[:, 2:258, 8:24], scales), ops.LoraPlan(ids, adapters))
     assert torch.equal(wide_y[:, 504:760], want)
     assert (wide_y[:, :504] == 5.0).all() and (wide_y[:, 760:] == 5.0).all()
 
@@ -98,28 +100,49 @@ def test_one_tensor_read_and_written():
     assert torch.equal(x, want)
 
 
+@pytest.mark.parametrize("tokens,rank,adapters", [(70, 16, 2), (1100, 16, 2), (1100, 64, 50)])
 @pytest.mark.parametrize("std", [2.0 ** -20, 1.0, 3000.0])
-def test_half_precision_products_far_from_one(std):
-    x, y, a, b, scales, ids = make(70, 64, 64, 16, 2, f16, seed=7, std=std)
+def test_half_precision_products_far_from_one(std, tokens, rank, adapters):
+    x, y, a, b, scales, ids = make(tokens, 64, 64, rank, adapters, f16, seed=7, std=std)
     y, a = y * 0, a * 40  # (x A^T past fp16's largest number, or below its smallest)
     b = (b.float() * min(1.0, 1.0 / (std * 40))).to(f16)
     want, off = exact(x, y, a, b, scales, ids)
-    check(ops.lora_add(y, x, ops.LoraAdapters(a, b, scales), ops.LoraPlan(ids, 2)), want, off, f16)
+    check(ops.lora_add(y, x, ops.LoraAdapters(a, b, scales), ops.LoraPlan(ids, adapters)), want, off, f16)
 
 
-def test_infinities_of_one_token_stay_its_own():
-    x, y, a, b, scales, ids = make(40, 64, 64, 16, 2, bf16, seed=8)
+@pytest.mark.parametrize("tokens,adapters", [(40, 2), (1200, 2), (1200, 230)])
+def test_infinities_of_one_token_stay_its_own(tokens, adapters):
+    x, y, a, b, scales, ids = make(tokens, 64, 64, 16, adapters, bf16, seed=8)
     ids[:] = 1
     want, off = exact(x, y, a, b, scales, ids)
     x[3, 5], x[4, 6] = float("inf"), float("nan")
-    got = ops.lora_add(y, x, ops.LoraAdapters(a, b, scales), ops.LoraPlan(ids, 2), out=torch.empty_like(y))
+    got = ops.lora_add(y, x, ops.LoraAdapters(a, b, scales), ops.LoraPlan(ids, adapters), out=torch.empty_like(y))
     assert not got[3].isfinite().any() and got[4].isnan().all()
-    rest = torch.tensor([i for i in range(40) if i not in (3, 4)], device="cuda")
+    rest = torch.tensor([i for i in range(tokens) if i not in (3, 4)], device="cuda")
     check(got[rest], want[rest], off[rest], bf16)
     # one rank: an infinity stays an infinity
     a1, b1 = a[:, :8].clone(), b[:, :, :8].clone()
-    got = ops.lora_add(y, x, ops.LoraAdapters(a1, b1, scales, torch.tensor([1, 1], dtype=torch.int32, device="cuda")), ops.LoraPlan(ids, 2), out=torch.empty_like(y))
+    got = ops.lora_add(y, x, ops.LoraAdapters(a1, b1, scales, torch.ones(adapters, dtype=torch.int32, device="cuda")), ops.LoraPlan(ids, adapters), out=torch.empty_like(y))
     assert torch.equal(got[3].float(), float("inf") * (torch.sign(a1[1, 0, 5]) * torch.sign(b1[1, :, 0])).float())
+
+
+def test_rows_behind_the_last_and_two_streams_at_once():
+    # Calls of every way on two streams; each has its own workspace, and what lies behind the tokens stays as it was.
+    made = []
+    for seed, (tokens, rank, adapters) in enumerate([(60, 16, 3), (1300, 32, 3), (1300, 64, 60)] * 2):
+        x, y, a, b, scales, ids = make(tokens, 256, 320, rank, adapters, bf16, seed=20 + seed)
+        out = torch.full((tokens + 40, 320), 7.0, dtype=bf16, device="cuda")
+        made.append((x, y, ops.LoraAdapters(a, b, scales), ops.LoraPlan(ids, adapters), out, exact(x, y, a, b, scales, ids), tokens))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, (x, y, adapters, plan, out, _, tokens) in enumerate(made):
+            with torch.cuda.stream(streams[i % 2]):
+                ops.lora_add(y, x, adapters, plan, out=out[:tokens])
+    torch.cuda.synchronize()
+    for _, _, _, _, out, (want, off), tokens in made:
+        check(out[:tokens], want, off, bf16)
+        assert (out[tokens:] == 7.0).all()
 
 
 @pytest.mark.parametrize("tokens", [30, 1200])

@@ -93,7 +93,7 @@ def adapters(n=3, rank=16, dim=64, width=128, dtype=torch.bfloat16, **how):
 
 
 class Plan:
-    tokens, adapters, buffer = 4, 3, torch.zeros(512, dtype=torch.uint8)
+    tokens, adapters, buffer, device, at, bytes = 4, 3, torch.zeros(512, dtype=torch.uint8), torch.device("cpu"), 0, 512
 
     def workspace_bytes(self, dim, rank):
         return 256
