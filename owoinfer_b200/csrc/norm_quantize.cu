@@ -65,7 +65,8 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], float by) {
 
 // s = x + residual; y = s rsqrt(mean s^2 + eps) w; codes round(y / scale). A row's threads hold 8 neighbouring channels each, kPer times over, from
 // the load to the codes: one pass over memory, and one block barrier, for the sum of squares and the largest |s w| (the scale of a
-// whole row does not need the norm's factor first) are reduced together. What bounds it is memory.
+// whole row does not need the norm's factor first) are reduced together. What bounds it is memory: 16384 x 8192, bf16 with its residual to
+// e4m3, takes 141 us, as long as a copy of as many bytes; a row alone takes the 2.4 us of a launch, a load and a store.
 template <typename X, typename R, bool kE4m3, int kPer, int kThreads>
 __global__ void __launch_bounds__(kThreads) norm_kernel(const NormArgs a) {
   __shared__ float2 s_part[32];
@@ -128,8 +129,10 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const NormArgs a) {
       sum += p.x, top = fmaxf(top, p.y);
     }
   }
-  // A row with a NaN or an infinity, or whose squares pass fp32, has NaN for its scales: rsqrt of infinity would make zeros of the rest.
-  const float r = sum < INFINITY ? rsqrtf(sum / static_cast<float>(a.dim) + a.eps) : __int_as_float(0x7fc00000);
+  // A row with a NaN or an infinity, or whose squares pass fp32, has NaN for its scales (rsqrt of infinity would make zeros of the rest), and so
+  // has one of zeros without an eps.
+  const float square = sum / static_cast<float>(a.dim) + a.eps;
+  const float r = square > 0.f && square < INFINITY ? rsqrtf(square) : __int_as_float(0x7fc00000);
   constexpr float kLargest = kE4m3 ? 448.f : 127.f;
   const auto scale_of = [&](float most) { return isnan(r) ? r : fmaxf(most * r / kLargest, kSmallestScale); };
   float scale = 0.f, by = 0.f;
@@ -162,9 +165,12 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const NormArgs a) {
 
 template <typename X, typename R, bool kE4m3>
 int launch(const char* op, NormArgs a, cudaStream_t stream) {
-  // Few rows: a thread per 8 channels, for the latency. Many: up to four times as much a thread, whose loads are on their way together.
+  // Few rows: a thread per 8 channels, for the latency. Many: up to four times as much a thread, whose loads are on their way together, and
+  // as few threads behind a row's barrier. Once, twice, four times, us on B200 (bf16, INT8): 200 x 4096: 3.7, 3.6, 4.5;
+  // 400 x 4096: 5.0, 4.6, 5.4; 1500 x 4096: 13.8, 11.4, 12.4; 2011 x 4096 (fp32 residual): 19.2, 17.7, 19.6; 2011 x 8192: 36.9, 29.9, 24.8;
+  // 8000 x 8192: 132, 100, 74.
   const int chunks = a.dim / 8;
-  int per = a.tokens <= 2 * sm_count() ? 1 : 4;
+  int per = a.tokens <= sm_count() ? 1 : a.tokens * chunks <= 1 << 20 ? 2 : 4;
   while (per < 4 && (chunks + per - 1) / per > 1024) per *= 2;
   while (per > 1 && chunks <= 32 * (per / 2)) per /= 2;
   a.row_threads = ((chunks + per - 1) / per + 31) / 32 * 32;
@@ -173,7 +179,7 @@ int launch(const char* op, NormArgs a, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>(blocks)), block(static_cast<unsigned>(rows * a.row_threads));
   if (per == 1) return enqueue(op, norm_kernel<X, R, kE4m3, 1, 1024>, grid, block, 0, stream, 1, a);
   if (per == 2) return enqueue(op, norm_kernel<X, R, kE4m3, 2, 1024>, grid, block, 0, stream, 1, a);
-  // (Four times 8 channels of fp32 twice do not fit the registers that 1024 threads leave a thread.)
+  // (Four times 8 channels of x and an fp32 residual do not quite fit the registers that 1024 threads leave a thread.)
   if (block.x <= 256) return enqueue(op, norm_kernel<X, R, kE4m3, 4, 256>, grid, block, 0, stream, 1, a);
   return enqueue(op, norm_kernel<X, R, kE4m3, 4, 1024>, grid, block, 0, stream, 1, a);
 }

@@ -116,6 +116,14 @@ def test_rows_that_are_not_finite_zero_or_extreme(dim, codes, group):
     check(x[fine], None, None, codes, group, 1e-6, q[fine], scale[fine].view(-1) if not group else scale[fine], None, y[fine], None)
 
 
+@pytest.mark.parametrize("group", [0, 32])
+def test_zeros_without_an_eps(group):
+    x = torch.ones(3, 64, device="cuda", dtype=bf16)
+    x[1] = 0
+    q, scale = ops.add_rms_norm_quantize(x, eps=0.0, group=group)
+    assert scale[1].isnan().all() and (q[1] == 0).all() and (q[::2] == 127).all() and ((scale[::2] * 127 - 1).abs() < 1e-6).all()
+
+
 def test_no_tokens_and_a_captured_call_on_another_stream():
     q, scale = ops.add_rms_norm_quantize(torch.empty(0, 64, dtype=bf16, device="cuda"), group=32)
     assert q.shape == (0, 64) and scale.shape == (0, 2)
