@@ -769,7 +769,7 @@ int b2_paged_cache_status(unsigned* host_value, int clear);
  * q = round(y / scale), ties to even. norm_out, where given, is y in 16 bits besides.
  * x bf16, fp16 or fp32; residual and residual_out of x's type or fp32; weight any of them. Rows 16-byte aligned, their strides (in elements)
  * multiples of 16 bytes; q 8-byte aligned, ldq % 8 == 0; dim % 8 == 0, dim <= 32768. residual_out may be residual, or x where
- * they have one type, and norm_out may be x; otherwise nothing that is written may overlap anything else (residual_out NULL: not written).
+ * they have one type, and norm_out may be a 16-bit x; otherwise nothing that is written may overlap anything else (residual_out NULL: not written).
  * scale: fp32 [tokens], or [tokens, dim / group] with group 32, 64, 128 or 256 (dim % group == 0; 0: none).
  * A token with a NaN or an infinity in s, whose squares add up past fp32 (|s| of 2^63 and more), or with neither squares nor eps, has NaN
  * for all of its scales and its norm_out; its int8 codes are 0, its e4m3 codes NaN. */
@@ -828,7 +828,8 @@ int b2_token_logprobs(const b2_logprobs* args, void* stream);
  * used, NaN and infinities included (ranks outside 0 .. rank raise a bit of b2_lora_status and are cut). x A^T is held to 16 bits and more; an
  * infinity in what is used of B may make NaN where it would make an infinity.
  * Rows and matrices 16-byte aligned, strides in elements, multiples of 8; dim, width and rank multiples of 8, rank <= 128; adapters <= 4096.
- * out may be y itself (rows without an adapter are then left alone); x may be either.
+ * out may be y itself (rows without an adapter are then left alone), and x may be either, with the same row stride; otherwise nothing that is
+ * written may overlap what is read.
  *
  * b2_lora_plan sorts the tokens by their adapter (token_adapters, device int32 [tokens]; an adapter past the last raises a bit of
  * b2_lora_status and counts as none) into `plan`, which b2_lora_add of any layer and projection then reads: once for a step.

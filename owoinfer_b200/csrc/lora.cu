@@ -690,7 +690,9 @@ struct ManyShape {
   static constexpr int kN = kNT < 2 ? 16 : kNT * 8;                               // ranks of an MMA
   static constexpr int kOperand = kN > 64 ? 128 * 128 : 64 * 128;                 // of a step: A's ranks by 64 channels, or B's 64 columns by its ranks
   static constexpr int kStage = kOperand + kManyRows * 128, kStages = kN > 64 ? 3 : 4;
-  static constexpr int kLow = 128, kColumns = 256;                                // accumulators (of x A^T, then of two steps' t B^T); from kLow on t
+  // Tensor memory: accumulators (of x A^T, then of two steps' t B^T), from kLow on t. Two CTAs of an SM have all of it; a kernel of the framework that
+  // allocates some and waits for its neighbours has more than half of the shared memory, and does not fit beside one: no two wait for one another.
+  static constexpr int kLow = 128, kColumns = 256;
   static constexpr int kBytes = kStages * kStage + 1024;                          // and what aligns it
   // The sums that are exchanged: blocks of ranks, 16 KB at most each, as many to a stage as two stages take them all.
   static constexpr int kBlock = kN < 32 ? 16 : 32, kBlocks = kN / kBlock, kPerStage = (kBlocks + 1) / 2;
@@ -1005,8 +1007,9 @@ int launch(const char* op, LoraArgs a, Way way, unsigned tiles, cudaStream_t str
   }
   static std::atomic<std::uint64_t> done{0};
   if (const int s = allow_shared(op, many_kernel<T, kNT>, ManyShape<kNT>::kBytes, done); s != B2_OK) return s;
-  // Clusters to a tile: as many as the GPU has room for (2 CTAs to an SM), of 128 columns a CTA at least.
-  const std::int64_t room = std::max<std::int64_t>(1, 2LL * sm_count() / (static_cast<std::int64_t>(tiles) * a.parts));
+  // Clusters to a tile: as many as the GPU has room for (2 CTAs to an SM), of 128 columns a CTA at least. One where x is out: all of a cluster's channels are
+  // read before one of its columns is written, those of another cluster may not be.
+  const std::int64_t room = a.x == a.out ? 1 : std::max<std::int64_t>(1, 2LL * sm_count() / (static_cast<std::int64_t>(tiles) * a.parts));
   a.groups = static_cast<int>(std::max<std::int64_t>(1, std::min<std::int64_t>(room, a.width / (128 * a.parts))));
   a.columns = (a.width + a.parts * a.groups - 1) / (a.parts * a.groups);
   a.columns = (a.columns + 63) / 64 * 64;
@@ -1081,6 +1084,7 @@ int b2_lora_add(const b2_lora* l, const void* plan, size_t bytes, int64_t tokens
   if (!matrix_ok(y, ldy, l->width, 2)) return fail_invalid(op, "y must be 16-byte aligned rows of at least width elements");
   if (!matrix_ok(out, ldo, l->width, 2)) return fail_invalid(op, "out must be 16-byte aligned rows of at least width elements");
   if (out == y && ldo != ldy) return fail_invalid(op, "out in y's place must have y's rows");
+  if (out == x && ldo != ldx && tokens > 1) return fail_invalid(op, "out in x's place must have x's rows");
   if (const int s = check_workspace(op, workspace, ws_bytes, workspace_bytes(tokens, l->adapters, l->rank)); s != B2_OK) return s;
   LoraArgs a{};
   const Way way = way_of(tokens, l->adapters, l->rank);

@@ -100,6 +100,20 @@ def test_one_tensor_read_and_written():
     assert torch.equal(x, want)
 
 
+# (each way that a call can go, the last two in the kernel of many tokens, which otherwise has several clusters to a tile)
+@pytest.mark.parametrize("y_too", [True, False])
+@pytest.mark.parametrize("tokens,dim,width,rank,adapters", [(50, 512, 512, 32, 6), (1500, 512, 512, 32, 6), (3000, 1024, 1024, 128, 4), (3500, 1024, 2048, 128, 1)])
+def test_x_in_the_place_of_out(tokens, dim, width, rank, adapters, y_too):
+    x, y, a, b, scales, ids = make(tokens, dim, width, rank, adapters, bf16, seed=tokens)
+    if y_too:
+        y[:, :dim] = x
+    want, off = exact(x, y, a, b, scales, ids)
+    out = y if y_too else torch.zeros_like(y)
+    out[:, :dim] = x
+    ops.lora_add(y, out[:, :dim], ops.LoraAdapters(a, b, scales), ops.LoraPlan(ids, adapters), out=out)
+    check(out, want, off, bf16)
+
+
 @pytest.mark.parametrize("tokens,rank,adapters", [(70, 16, 2), (1100, 16, 2), (1100, 64, 50)])
 @pytest.mark.parametrize("std", [2.0 ** -20, 1.0, 3000.0])
 def test_half_precision_products_far_from_one(std, tokens, rank, adapters):
