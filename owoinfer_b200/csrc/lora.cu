@@ -193,6 +193,7 @@ __device__ __forceinline__ std::int64_t low_word(std::int64_t row, int r) {
 
 // Sums of x A^T over the channels' parts, [rows][ranks] in the shared memory of each CTA of a cluster at `sums`, joined, scaled and left for the product with
 // B: a row by ranks / 4 neighbouring lanes, every CTA some of the rows. In two 16-bit parts t keeps 16 (bf16) or 22 (fp16) of its bits.
+// (Rows behind the tile's tokens are left out: what t has there ends up in rows that nobody stores.)
 template <typename T, int kRanks, int kRows>
 __device__ __forceinline__ void leave_sums(const LoraArgs& a, const Tile& tile, std::int64_t tile_number, int rank, const float* sums) {
   constexpr int kLanes = kRanks / 4;
@@ -201,10 +202,10 @@ __device__ __forceinline__ void leave_sums(const LoraArgs& a, const Tile& tile, 
   const int part = static_cast<int>(blockIdx.x) % a.parts, lane = static_cast<int>(threadIdx.x) % kLanes;
   const float scale = a.scales != nullptr ? a.scales[tile.adapter] : 1.f;
   const std::uint32_t own = smem_u32(sums);
-  for (int first = part * (kThreads / kLanes); first < kRows; first += a.parts * (kThreads / kLanes)) {  // (the same number of rounds for a warp's lanes)
+  for (int first = part * (kThreads / kLanes); first < tile.count; first += a.parts * (kThreads / kLanes)) {  // (the same number of rounds for a warp's lanes)
     const int row = first + static_cast<int>(threadIdx.x) / kLanes;
     float v[4] = {};
-    if (row < kRows) {
+    if (row < tile.count) {
       const std::uint32_t at = own + (row * kRanks + lane * 4) * 4;
       for (int p = 0; p < a.parts; ++p) {
         const float4 s = a.parts > 1 ? ld_cluster_f32x4(map_to_cta(at, static_cast<std::uint32_t>(p))) : *reinterpret_cast<const float4*>(sums + row * kRanks + lane * 4);
@@ -221,7 +222,7 @@ __device__ __forceinline__ void leave_sums(const LoraArgs& a, const Tile& tile, 
 #pragma unroll
       for (int m = kLanes / 2; m > 0; m /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
     }
-    if (row >= kRows) continue;
+    if (row >= tile.count) continue;
     const Halves<T> by(top);
     std::uint32_t hi[2], lo[2];
 #pragma unroll
@@ -231,64 +232,6 @@ __device__ __forceinline__ void leave_sums(const LoraArgs& a, const Tile& tile, 
     if (lane == 0) a.t_back[tile_number * kRows + row] = by.back;
   }
   if (a.parts > 1) cluster_sync_all();  // (nobody leaves while others read its sums)
-}
-
-// x A^T of a tile's tokens over a part of the channels, in 16-row MMAs with the ranks as columns. Which channels a place of an MMA's K stands for does
-// not matter as long as x and A agree: a lane takes 8 neighbouring ones of each, in one load, as the K of two MMAs. kNT: ranks / 8, up to a
-// power of two. Few tokens: a tile's warps divide the part's channels and are added up in shared memory.
-template <typename T, int kNT>
-__global__ void __launch_bounds__(kThreads) shrink_few_kernel(const LoraArgs a) {
-  dependents_may_start();
-  constexpr int kRanks = kNT * 8;
-  __shared__ __align__(16) float s_sum[kWarps][kFewRows * kRanks];
-  const int tile_number = static_cast<int>(blockIdx.x) / a.parts, part = static_cast<int>(blockIdx.x) % a.parts;
-  if (tile_number >= *a.plan.count) return;
-  const Tile tile = a.plan.tiles[tile_number];
-  if (tile.adapter < 0) return;
-  const int rank = rank_of(a, tile.adapter);
-  const int warp = static_cast<int>(threadIdx.x) / 32, lane = static_cast<int>(threadIdx.x) % 32, g = lane / 4, c = lane % 4;
-  const T* x[2];
-  bool there[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = g + 8 * i;
-    there[i] = r < tile.count;
-    x[i] = static_cast<const T*>(a.x) + (there[i] ? a.plan.order[tile.first + r] : 0) * a.ldx + c * 8;
-  }
-  const T* const w = static_cast<const T*>(a.a) + tile.adapter * a.a_adapter + g * a.a_row + c * 8;
-  const int from = part * a.slice, to = min(a.dim, from + a.slice);
-  float acc[kNT][4] = {};
-  constexpr int kStep = 32 * kWarps, kUnroll = kNT <= 2 ? 4 : kNT <= 4 ? 2 : 1;
-  const auto block = [&](int k, bool in, uint4 (&xv)[2], uint4 (&wv)[kNT]) {
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int j = 0; j < kNT; ++j) wv[j] = in && j * 8 + g < rank ? load16(w + j * 8 * a.a_row + k) : zero;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) xv[i] = in && there[i] ? load16(x[i] + k) : zero;
-  };
-  for (int k = from + warp * 32; k < to; k += kStep * kUnroll) {
-    uint4 xv[kUnroll][2], wv[kUnroll][kNT];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) block(k + u * kStep, k + u * kStep + c * 8 < to, xv[u], wv[u]);
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-#pragma unroll
-      for (int j = 0; j < kNT; ++j) mma_twice<T>(acc[j], xv[u][0], xv[u][1], wv[u][j]);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < kNT; ++j) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) *reinterpret_cast<float2*>(&s_sum[warp][(g + 8 * i) * kRanks + j * 8 + c * 2]) = make_float2(acc[j][2 * i], acc[j][2 * i + 1]);
-  }
-  __syncthreads();
-  for (int i = static_cast<int>(threadIdx.x); i < kFewRows * kRanks; i += kThreads) {
-    float sum = s_sum[0][i];
-#pragma unroll
-    for (int v = 1; v < kWarps; ++v) sum += s_sum[v][i];
-    s_sum[0][i] = sum;
-  }
-  leave_sums<T, kRanks, kFewRows>(a, tile, tile_number, rank, s_sum[0]);
 }
 
 __device__ __forceinline__ void copy16(std::uint32_t to, const void* from, bool there) {  // (zeros where there is nothing)
@@ -304,6 +247,97 @@ __device__ __forceinline__ uint4 matrices(std::uint32_t addr) {
   uint4 r;
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr) : "memory");
   return r;
+}
+
+// x A^T of a tile's tokens over a part of the channels, in 16-row MMAs with the ranks as columns, kNT: ranks / 8, up to a power of two. Few tokens: a tile's warps
+// take 64 of the part's channels each in turn, through stages of shared memory of their own, rows of 128 bytes whose 16-byte pieces are permuted by the
+// row, and are added up in shared memory. What bounds it is how much of A is on its way: a warp has all that two stages hold in flight at once.
+template <int kNT>
+constexpr int kFewStage = (kFewRows + kNT * 8) * 128;
+template <int kNT>
+constexpr int kFewStages = kNT <= 4 ? 3 : 2;
+template <typename T, int kNT>
+__global__ void __launch_bounds__(kThreads) shrink_few_kernel(const LoraArgs a) {
+  dependents_may_start();
+  constexpr int kRanks = kNT * 8, kStages = kFewStages<kNT>, kRing = kStages * kFewStage<kNT>;
+  extern __shared__ __align__(128) std::uint8_t smem[];
+  const int tile_number = static_cast<int>(blockIdx.x) / a.parts, part = static_cast<int>(blockIdx.x) % a.parts;
+  if (tile_number >= *a.plan.count) return;
+  const Tile tile = a.plan.tiles[tile_number];
+  if (tile.adapter < 0) return;
+  const int rank = rank_of(a, tile.adapter);
+  const int warp = static_cast<int>(threadIdx.x) / 32, lane = static_cast<int>(threadIdx.x) % 32, g = lane / 4, c = lane % 4;
+  // A lane copies piece lane % 8 of rows lane / 8, lane / 8 + 4, ...
+  const int piece = lane % 8;
+  const T* x[kFewRows / 4];
+#pragma unroll
+  for (int i = 0; i < kFewRows / 4; ++i) {
+    const int r = lane / 8 + i * 4;
+    x[i] = r < tile.count ? static_cast<const T*>(a.x) + a.plan.order[tile.first + r] * a.ldx + piece * 8 : nullptr;
+  }
+  const T* const w = static_cast<const T*>(a.a) + tile.adapter * a.a_adapter + lane / 8 * a.a_row + piece * 8;
+  const int from = part * a.slice, to = min(a.dim, from + a.slice);
+  const std::uint32_t ring = smem_u32(smem) + warp * kRing;
+  int to_copy = from + warp * 64, copied = 0;
+  const auto copy_stage = [&] {
+    if (to_copy < to) {
+      const std::uint32_t at = ring + copied * kFewStage<kNT> + lane / 8 * 128;
+      const bool in = to_copy + piece * 8 < to;
+      const auto piece_at = [&](int i) { return at + i * 512 + ((piece ^ (lane / 8 + i * 4 & 7)) << 4); };
+#pragma unroll
+      for (int i = 0; i < kRanks / 4; ++i) {
+        const bool there = in && lane / 8 + i * 4 < rank;
+        copy16(piece_at(i), there ? w + i * 4 * a.a_row + to_copy : w, there);
+      }
+#pragma unroll
+      for (int i = 0; i < kFewRows / 4; ++i) copy16(piece_at(kRanks / 4 + i), x[i] != nullptr && in ? x[i] + to_copy : a.x, x[i] != nullptr && in);
+      to_copy += 64 * kWarps;
+      copied = copied == kStages - 1 ? 0 : copied + 1;
+    }
+    copies_are_one_group();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) copy_stage();
+  float acc[kNT][4] = {};
+  // Lane addresses within a stage: A as B operands of two MMAs (8 channels, the next 8, then the next 8 ranks), x as A operands (rows 0..7, 8..15, then
+  // the next 8 channels).
+  const int wr = (lane >> 4) * 8 + (lane & 7), wp = lane >> 3 & 1, xr = lane & 15, xp = lane >> 4;
+  int stage = 0;
+  for (int k = from + warp * 64; k < to; k += 64 * kWarps) {
+    wait_for_copies<kStages - 1>();
+    __syncwarp();  // (the warp's pieces of this stage are there)
+    const std::uint32_t at = ring + stage * kFewStage<kNT>;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const uint4 xv = matrices(at + kRanks * 128 + xr * 128 + (((2 * s + xp) ^ (xr & 7)) << 4));
+#pragma unroll
+      for (int j = 0; j < (kNT + 1) / 2; ++j) {
+        const uint4 wv = matrices(at + ((kNT == 1 ? wr & 7 : wr) + j * 16) * 128 + (((2 * s + wp) ^ (wr & 7)) << 4));
+        mma<T>(acc[2 * j], xv, wv.x, wv.y);
+        if constexpr (kNT > 1) mma<T>(acc[2 * j + 1], xv, wv.z, wv.w);
+      }
+    }
+    __syncwarp();  // (the stage is read)
+    copy_stage();
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+  }
+  wait_for_copies<0>();
+  __syncwarp();
+  constexpr int kNext = kRing / 4;  // floats from a warp's sums to the next one's
+  float* const sums = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int j = 0; j < kNT; ++j) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) *reinterpret_cast<float2*>(sums + warp * kNext + (g + 8 * i) * kRanks + j * 8 + c * 2) = make_float2(acc[j][2 * i], acc[j][2 * i + 1]);
+  }
+  __syncthreads();
+  for (int i = static_cast<int>(threadIdx.x); i < tile.count * kRanks; i += kThreads) {
+    float sum = sums[i];
+#pragma unroll
+    for (int v = 1; v < kWarps; ++v) sum += sums[v * kNext + i];
+    sums[i] = sum;
+  }
+  leave_sums<T, kRanks, kFewRows>(a, tile, tile_number, rank, sums);
 }
 
 // The same for several tokens: four warps of 32 rows each with all ranks, 64 channels at a time through three stages of shared memory, rows of 128 bytes whose
@@ -995,7 +1029,10 @@ int launch(const char* op, LoraArgs a, Way way, unsigned tiles, cudaStream_t str
     a.columns = static_cast<int>(std::max<std::int64_t>(128, ((a.width + most - 1) / most + 127) / 128 * 128));
     const dim3 grid(tiles, static_cast<unsigned>((a.width + a.columns - 1) / a.columns));
     if (way == Way::kFew) {
-      if (const int s = enqueue(op, shrink_few_kernel<T, kNT>, dim3(tiles * a.parts), dim3(kThreads), 0, stream, a.parts, a); s != B2_OK) return s;
+      static std::atomic<std::uint64_t> few_done{0};
+      constexpr int kBytes = kWarps * kFewStages<kNT> * kFewStage<kNT>;
+      if (const int s = allow_shared(op, shrink_few_kernel<T, kNT>, kBytes, few_done); s != B2_OK) return s;
+      if (const int s = enqueue(op, shrink_few_kernel<T, kNT>, dim3(tiles * a.parts), dim3(kThreads), kBytes, stream, a.parts, a); s != B2_OK) return s;
       return enqueue(op, expand_few_kernel<T, kNT>, grid, dim3(kThreads), 0, stream, 1, a);
     }
     static std::atomic<std::uint64_t> shrink_done{0}, expand_done{0};
