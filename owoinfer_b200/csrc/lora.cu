@@ -518,11 +518,47 @@ __device__ __forceinline__ bool tile_to_add(const LoraArgs& a, Tile& tile) {
   return exists && (tile.adapter >= 0 || a.y != a.out);
 }
 
-// Few tokens: a tile's warps take columns in turn, B comes straight from memory.
+// Where a 16-byte piece of a row of 128 bytes lies so that eight lanes, four pieces of two rows, meet no bank twice: rows alike but for the
+// bits that `fold` takes.
+__device__ __forceinline__ int folded(int piece, int fold) { return (piece & ~7) | ((piece & 7) ^ fold); }
+
+// Of 16 bytes of 8 ranks of a column, of 32 columns.
+template <int kNT>
+__device__ __forceinline__ int fold_of(int column) { return kNT >= 8 ? (column & 1) << 2 | (column >> 3 & 3) : 0; }
+// Where a lane's operands of a step lie among its B.
+template <typename T, int kNT>
+__device__ __forceinline__ void place_operands(int g, int c, std::uint32_t (&at)[4][Low<T, kNT>::kBlocks]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int q = 0; q < Low<T, kNT>::kBlocks; ++q) {
+      const int n = column_of(j, g);
+      at[j][q] = n * (kNT * 16) + (Low<T, kNT>::kPer == 8 ? folded(q * 4 + c, fold_of<kNT>(n)) * 16 : c * 8);
+    }
+  }
+}
+template <typename T, int kNT>
+__device__ __forceinline__ uint4 operand(const std::uint8_t* p, int c) {
+  if constexpr (Low<T, kNT>::kPer == 8) {
+    return load16(p);
+  } else {
+    if (c * 4 >= kNT * 8) return make_uint4(0, 0, 0, 0);
+    const uint2 r = *reinterpret_cast<const uint2*>(p);
+    return make_uint4(r.x, r.y, 0, 0);
+  }
+}
+
+// Few tokens: a tile's warps take 32 columns in turn, y and B through stages of shared memory of their own: the first ones come while the kernel before still
+// makes t.
+template <int kNT>
+constexpr int kFewAddStage = 32 * kNT * 16 + 1024;
+template <int kNT>
+constexpr int kFewAddStages = kNT <= 4 ? 4 : kNT <= 8 ? 3 : 2;
 template <typename T, int kNT>
 __global__ void __launch_bounds__(kThreads) expand_few_kernel(const LoraArgs a) {
   using L = Low<T, kNT>;
-  constexpr int kStep = 32 * kWarps;
+  constexpr int kStep = 32 * kWarps, kStages = kFewAddStages<kNT>, kStage = kFewAddStage<kNT>, kBBytes = 32 * kNT * 16;
+  extern __shared__ __align__(128) std::uint8_t smem[];
   Tile tile;
   if (!tile_to_add(a, tile)) {
     wait_for_predecessors();  // (this kernel is not done before the one that it follows)
@@ -537,27 +573,51 @@ __global__ void __launch_bounds__(kThreads) expand_few_kernel(const LoraArgs a) 
     return;
   }
   const int rank = rank_of(a, tile.adapter);
-  const T* const w = static_cast<const T*>(a.b) + tile.adapter * a.b_adapter + c * L::kPer;
+  // A lane copies piece lane % kNT of column lane / kNT and of those kColumns on.
+  constexpr int kColumns = 32 / kNT;
+  const int column = lane / kNT, piece = lane % kNT;
+  const T* const w = static_cast<const T*>(a.b) + tile.adapter * a.b_adapter + column * a.b_row + piece * 8;
+  std::uint8_t* const ring = smem + warp * (kStages * kStage);
+  const std::uint32_t ring_at = smem_u32(ring);
+  int to_copy = from, copied = 0;
+  const auto copy_stage = [&] {
+    if (to_copy < to) {
+      const std::uint32_t at = ring_at + copied * kStage;
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) {
+        const int n = column + i * kColumns;
+        const bool in = piece * 8 < rank && to_copy + n < to;
+        copy16(at + n * (kNT * 16) + folded(piece, fold_of<kNT>(n)) * 16, in ? w + (to_copy + i * kColumns) * a.b_row : a.b, in);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool in = rows.there[i] && to_copy + c * 8 < to;
+        copy16(at + kBBytes + (i * 32 + lane) * 16, in ? rows.y[i] + to_copy : a.y, in);
+      }
+      to_copy += kStep;
+      copied = copied == kStages - 1 ? 0 : copied + 1;
+    }
+    copies_are_one_group();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) copy_stage();
+  std::uint32_t b_from[4][L::kBlocks];
+  place_operands<T, kNT>(g, c, b_from);
   wait_for_predecessors();
   const L low(a, static_cast<std::int64_t>(blockIdx.x) * kFewRows, g, c);
   const auto add_all = [&](auto ragged) {
+    int stage = 0;
     for (int n = from; n < to; n += kStep) {
+      wait_for_copies<kStages - 1>();
+      __syncwarp();  // (the warp's pieces of this step are there)
+      const std::uint8_t* const at = ring + stage * kStage;
       uint4 y[2], out[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) y[i] = rows.there[i] && n + c * 8 < to ? load16(rows.y[i] + n) : make_uint4(0, 0, 0, 0);
-      add_block<T, kNT, decltype(ragged)::value>(low, c, rank, y, [&](int j, int q) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        const int column = n + column_of(j, g);
-        if (column >= to || q * 32 + c * L::kPer >= rank) return v;
-        const T* const p = w + column * a.b_row + q * 32;
-        if constexpr (L::kPer == 8) {
-          v = load16(p);
-        } else {
-          const uint2 r = *reinterpret_cast<const uint2*>(p);
-          v.x = r.x, v.y = r.y;
-        }
-        return v;
-      }, out);
+      for (int i = 0; i < 2; ++i) y[i] = load16(at + kBBytes + (i * 32 + lane) * 16);
+      add_block<T, kNT, decltype(ragged)::value>(low, c, rank, y, [&](int j, int q) { return operand<T, kNT>(at + b_from[j][q], c); }, out);
+      __syncwarp();  // (the stage is read)
+      copy_stage();
+      stage = stage == kStages - 1 ? 0 : stage + 1;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (rows.there[i] && n + c * 8 < to) *reinterpret_cast<uint4*>(rows.out[i] + n) = out[i];
@@ -566,11 +626,8 @@ __global__ void __launch_bounds__(kThreads) expand_few_kernel(const LoraArgs a) 
   };
   if (rank % 8 != 0) add_all(std::true_type{});
   else add_all(std::false_type{});
+  wait_for_copies<0>();
 }
-
-// Where a 16-byte piece of a row of 128 bytes lies so that eight lanes, four pieces of two rows, meet no bank twice: rows alike but for the
-// bits that `fold` takes.
-__device__ __forceinline__ int folded(int piece, int fold) { return (piece & ~7) | ((piece & 7) ^ fold); }
 
 // Several: eight warps of 16 rows each, 32 columns at a time through four stages of shared memory: a lane copies the pieces of y that it adds to, B is
 // everybody's. What bounds it is memory: y is read and out written once.
@@ -580,7 +637,7 @@ constexpr int kExpandStage = 32 * kNT * 16 + kManyRows * 64;
 template <typename T, int kNT>
 __global__ void __launch_bounds__(kManyThreads, kNT <= 8 ? 3 : 2) expand_several_kernel(const LoraArgs a) {
   using L = Low<T, kNT>;
-  constexpr int kRanks = kNT * 8, kBBytes = 32 * kNT * 16;
+  constexpr int kBBytes = 32 * kNT * 16;
   extern __shared__ __align__(128) std::uint8_t smem[];
   Tile tile;
   if (!tile_to_add(a, tile)) {
@@ -596,7 +653,6 @@ __global__ void __launch_bounds__(kManyThreads, kNT <= 8 ? 3 : 2) expand_several
     return;
   }
   const int rank = rank_of(a, tile.adapter);
-  const auto fold_of = [](int column) { return kNT >= 8 ? (column & 1) << 2 | (column >> 3 & 3) : 0; };
   // What this thread copies of B at each step: piece tid % kNT of column tid / kNT and of those kColumns on; where its own operands lie.
   constexpr int kColumns = kManyThreads / kNT < 32 ? kManyThreads / kNT : 32, kCopies = 32 / kColumns;
   const int column = tid / kNT, piece = tid % kNT;
@@ -606,7 +662,7 @@ __global__ void __launch_bounds__(kManyThreads, kNT <= 8 ? 3 : 2) expand_several
 #pragma unroll
   for (int i = 0; i < kCopies; ++i) {
     w[i] = static_cast<const T*>(a.b) + tile.adapter * a.b_adapter + (from + column + i * kColumns) * a.b_row + piece * 8;
-    w_to[i] = (column + i * kColumns) * (kNT * 16) + folded(piece, fold_of(column + i * kColumns)) * 16;
+    w_to[i] = (column + i * kColumns) * (kNT * 16) + folded(piece, fold_of<kNT>(column + i * kColumns)) * 16;
   }
   const std::int64_t w_step = 32 * a.b_row;
   const std::uint32_t ring = smem_u32(smem);
@@ -637,14 +693,7 @@ __global__ void __launch_bounds__(kManyThreads, kNT <= 8 ? 3 : 2) expand_several
   wait_for_predecessors();
   const L low(a, static_cast<std::int64_t>(blockIdx.x) * kManyRows + warp * 16, g, c);
   std::uint32_t b_from[4][L::kBlocks];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-#pragma unroll
-    for (int q = 0; q < L::kBlocks; ++q) {
-      const int n = column_of(j, g);
-      b_from[j][q] = n * (kNT * 16) + (L::kPer == 8 ? folded(q * 4 + c, fold_of(n)) * 16 : c * 8);
-    }
-  }
+  place_operands<T, kNT>(g, c, b_from);
   T* out_to[2] = {rows.out[0] + from, rows.out[1] + from};
   const auto add_all = [&](auto ragged) {
     for (int s = 0; s < steps; ++s) {
@@ -655,15 +704,7 @@ __global__ void __launch_bounds__(kManyThreads, kNT <= 8 ? 3 : 2) expand_several
       uint4 y[2], out[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) y[i] = load16(at + kBBytes + ((warp * 2 + i) * 32 + lane) * 16);
-      add_block<T, kNT, decltype(ragged)::value>(low, c, rank, y, [&](int j, int q) {
-        if constexpr (L::kPer == 8) {
-          return load16(at + b_from[j][q]);
-        } else {
-          if (c * 4 >= kRanks) return make_uint4(0, 0, 0, 0);
-          const uint2 r = *reinterpret_cast<const uint2*>(at + b_from[j][q]);
-          return make_uint4(r.x, r.y, 0, 0);
-        }
-      }, out);
+      add_block<T, kNT, decltype(ragged)::value>(low, c, rank, y, [&](int j, int q) { return operand<T, kNT>(at + b_from[j][q], c); }, out);
       const bool in = c * 8 < to - from - s * 32;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -1024,8 +1065,8 @@ template <typename T, int kNT>
 int launch(const char* op, LoraArgs a, Way way, unsigned tiles, cudaStream_t stream) {
   const LaunchChain chain(stream);
   if (way != Way::kMany) {
-    // Columns of a CTA: as many as leave 8 small or 4 large CTAs to an SM, 128 at least.
-    const std::int64_t most = std::max<std::int64_t>(1, (way == Way::kFew ? 8LL : 4LL) * sm_count() / tiles);
+    // Columns of a CTA: as many as leave 6 small or 4 large CTAs to an SM, 128 at least.
+    const std::int64_t most = std::max<std::int64_t>(1, (way == Way::kFew ? 6LL : 4LL) * sm_count() / tiles);
     a.columns = static_cast<int>(std::max<std::int64_t>(128, ((a.width + most - 1) / most + 127) / 128 * 128));
     const dim3 grid(tiles, static_cast<unsigned>((a.width + a.columns - 1) / a.columns));
     if (way == Way::kFew) {
@@ -1033,7 +1074,10 @@ int launch(const char* op, LoraArgs a, Way way, unsigned tiles, cudaStream_t str
       constexpr int kBytes = kWarps * kFewStages<kNT> * kFewStage<kNT>;
       if (const int s = allow_shared(op, shrink_few_kernel<T, kNT>, kBytes, few_done); s != B2_OK) return s;
       if (const int s = enqueue(op, shrink_few_kernel<T, kNT>, dim3(tiles * a.parts), dim3(kThreads), kBytes, stream, a.parts, a); s != B2_OK) return s;
-      return enqueue(op, expand_few_kernel<T, kNT>, grid, dim3(kThreads), 0, stream, 1, a);
+      static std::atomic<std::uint64_t> few_add_done{0};
+      constexpr int kAddBytes = kWarps * kFewAddStages<kNT> * kFewAddStage<kNT>;
+      if (const int s = allow_shared(op, expand_few_kernel<T, kNT>, kAddBytes, few_add_done); s != B2_OK) return s;
+      return enqueue(op, expand_few_kernel<T, kNT>, grid, dim3(kThreads), kAddBytes, stream, 1, a);
     }
     static std::atomic<std::uint64_t> shrink_done{0}, expand_done{0};
     constexpr int kShrinkBytes = kShrinkStages * kShrinkStage<kNT>, kExpandBytes = kExpandStages * kExpandStage<kNT>;
