@@ -19,7 +19,7 @@ constexpr int kMostParts = 8, kMostManyParts = 4;  // CTAs of a cluster that div
 
 // A plan sorts the tokens by adapter and cuts them into tiles, of one warp's rows, where there are few tokens, and of eight warps', for A and B to be
 // read once for more of them: [0] and [1] below.
-constexpr int kFewRows = 16, kManyRows = 128, kFewTokens = 1024;
+constexpr int kFewRows = 16, kManyRows = 128, kFewTokens = 16384;
 inline std::int64_t most_tiles(std::int64_t tokens, int adapters, int rows) {
   return rows == kFewRows && tokens > kFewTokens ? 0 : std::min(tokens, tokens / rows + adapters + 1);
 }
@@ -915,9 +915,11 @@ __global__ void __launch_bounds__(kManyThreads, 2) many_kernel(const LoraArgs a)
 #pragma unroll
         for (int b = 0; b < S::kBlocks; ++b) {
           const std::uint32_t at = smem_u32(sum_at(b, row, piece));
-          float4 o[kParts];
+          float4 o[kParts] = {};
+          if (row < tile.count) {
 #pragma unroll
-          for (int q = 0; q < kParts; ++q) o[q] = ld_cluster_f32x4(map_to_cta(at, static_cast<std::uint32_t>(q)));
+            for (int q = 0; q < kParts; ++q) o[q] = ld_cluster_f32x4(map_to_cta(at, static_cast<std::uint32_t>(q)));
+          }
 #pragma unroll
           for (int q = 1; q < kParts; ++q) o[0].x += o[q].x, o[0].y += o[q].y, o[0].z += o[q].z, o[0].w += o[q].w;
           v[i][b][0] = o[0].x, v[i][b][1] = o[0].y, v[i][b][2] = o[0].z, v[i][b][3] = o[0].w;
@@ -1002,27 +1004,29 @@ __global__ void __launch_bounds__(kManyThreads, 2) many_kernel(const LoraArgs a)
     const int e = s - 1;  // the step that is added
     if (e >= k_steps) {
       wait_done(e);
-      std::uint32_t v[32];
-      tmem_ld_32x32(accumulators + (e & 1) * 64 + lanes + half * 32, v);
-      tmem_ld_wait();
-      std::uint8_t* const at = smem + e % S::kStages * S::kStage + S::kOperand;
+      if (row0 < tile.count) {
+        std::uint32_t v[32];
+        tmem_ld_32x32(accumulators + (e & 1) * 64 + lanes + half * 32, v);
+        tmem_ld_wait();
+        std::uint8_t* const at = smem + e % S::kStages * S::kStage + S::kOperand;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint4* const p = reinterpret_cast<uint4*>(at + at_piece(row0 + lane, half * 4 + i));
-        float f[8];
-        load8<T>(*p, f);
+        for (int i = 0; i < 4; ++i) {
+          uint4* const p = reinterpret_cast<uint4*>(at + at_piece(row0 + lane, half * 4 + i));
+          float f[8];
+          load8<T>(*p, f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = fmaf(__uint_as_float(v[8 * i + j]), back, f[j]);
-        *p = store8<T>(f);
+          for (int j = 0; j < 8; ++j) f[j] = fmaf(__uint_as_float(v[8 * i + j]), back, f[j]);
+          *p = store8<T>(f);
+        }
+        __syncwarp();
+        const int n = (e - k_steps) * 64;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 p = load16(at + at_piece(row0 + lane / 4 + i * 8, half * 4 + lane % 4));
+          if (there[i] && n + column < to - from) *reinterpret_cast<uint4*>(out_to[i] + n) = p;
+        }
+        __syncwarp();  // (this warp's pieces of the stage are read: it is the next to be copied into)
       }
-      __syncwarp();
-      const int n = (e - k_steps) * 64;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 p = load16(at + at_piece(row0 + lane / 4 + i * 8, half * 4 + lane % 4));
-        if (there[i] && n + column < to - from) *reinterpret_cast<uint4*>(out_to[i] + n) = p;
-      }
-      __syncwarp();  // (this warp's pieces of the stage are read: it is the next to be copied into)
     }
     copy_step(e + S::kStages);
   }
@@ -1035,14 +1039,17 @@ inline int padded_tiles(int rank) {  // ranks / 8, up to a power of two
   while (n * 8 < rank) n *= 2;
   return n;
 }
-// Which kernels a call runs, by the rows of its tiles times the ranks: what they do with tiles that are not full, and what mma.sync's rate costs. Measured with
-// 4096 channels and columns, few / several / many tokens' kernels, us: 300 tokens of 3 adapters, rank 128 (2688 by small tiles) 20 / 23 / 24, 700 of
-// 4, rank 64 (3072) 22 / 17 / 27; 3000 of 4, rank 128 (3584 by large ones) several 50, many 48, 5000 of 6, rank 64 (2944) 45 / 50, 8191 of 6, rank 64 (4544)
-// 65 / 57, rank 128 99 / 70.
+// Which kernels a call runs. Small tiles read A and B again every 16 tokens, large ones are mostly empty where adapters are many: small ones go by their number
+// times the ranks for each large tile. Of large tiles, the kernel of many tokens wins by its products (mma.sync's rate is a quarter) and has more to set up. With
+// 4096 channels and columns from memory, few / several / many tokens' kernels, us: 64 tokens of as many adapters, rank 64 (a small tile for each large one)
+// 15 / 44 / 42; 300 of 3, rank 128 (470) 22 / 25 / 26; 1000 of 6, rank 128 (630) 36 / 28 / 40; 3000 of 4, rank 16 (110) 22 / 23 / 32, rank 32 (220)
+// 27 / 25 / 33, rank 128 85 / 53 / 50; 3000 of 60, rank 64 (189) 39 / 58 / 59, rank 128 (380) 90 / 93 / 73; 8191 of 6, rank 64 85 / 69 / 59; 16000 of 60, 2048
+// channels and columns, rank 32 55 / 53 / 71.
 enum class Way { kFew, kSeveral, kMany };
 inline Way way_of(std::int64_t tokens, int adapters, int rank) {
-  if (tokens <= kFewTokens && most_tiles(tokens, adapters, kFewRows) * rank <= 2800) return Way::kFew;
-  return most_tiles(tokens, adapters, kManyRows) * rank >= 3500 ? Way::kMany : Way::kSeveral;
+  const std::int64_t large = most_tiles(tokens, adapters, kManyRows);
+  if (tokens <= kFewTokens && most_tiles(tokens, adapters, kFewRows) * rank <= large * (tokens <= 1024 ? 500 : 200)) return Way::kFew;
+  return rank > 32 && large * rank >= 3500 ? Way::kMany : Way::kSeveral;
 }
 inline int rows_of(Way way) { return way == Way::kFew ? kFewRows : kManyRows; }
 // Parts of the channels (a power of two): CTAs for the whole GPU twice over (thrice of several tokens), of 256 channels at least.

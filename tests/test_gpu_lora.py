@@ -52,6 +52,7 @@ def check(got, want, off, dtype):
     (1, 8, 8, 8, 1), (1, 2048, 2048, 16, 4), (15, 64, 24, 16, 3), (16, 40, 136, 24, 1), (17, 520, 1000, 40, 5), (100, 256, 512, 128, 60), (64, 4096, 640, 16, 48),
     (4000, 1032, 200, 128, 6), (2500, 264, 72, 64, 50), (3000, 520, 1000, 24, 200), (500, 520, 264, 8, 450), (6000, 512, 72, 32, 90), (900, 1544, 520, 128, 30),
     (64, 136, 264, 128, 40), (1024, 72, 264, 8, 3), (1025, 136, 200, 64, 7), (3000, 512, 384, 32, 2), (1100, 2056, 72, 128, 2), (2000, 64, 128, 16, 700), (40, 104, 8, 56, 4096),
+    (17000, 72, 136, 8, 3), (16500, 264, 72, 24, 5), (1600, 520, 1000, 56, 2), (1100, 136, 520, 120, 40), (12000, 328, 200, 48, 9),
 ])
 def test_against_the_formula(tokens, dim, width, rank, adapters, dtype):
     x, y, a, b, scales, ids = make(tokens, dim, width, rank, adapters, dtype, seed=tokens + dim)
@@ -67,7 +68,7 @@ def test_against_the_formula(tokens, dim, width, rank, adapters, dtype):
 
 
 # (each of the ways that a call can go: few tokens, several, and many by tiles times ranks)
-@pytest.mark.parametrize("tokens,rank,adapters", [(50, 32, 6), (1500, 32, 6), (1500, 32, 120), (300, 128, 30)])
+@pytest.mark.parametrize("tokens,rank,adapters", [(50, 32, 6), (1500, 32, 6), (1500, 32, 120), (300, 128, 30), (1600, 64, 2), (1200, 24, 1), (20000, 16, 3), (1100, 128, 40)])
 def test_ranks_and_what_lies_behind_them(tokens, rank, adapters):
     x, y, a, b, scales, ids = make(tokens, 264, 72, rank, adapters, bf16, seed=3)
     ranks = torch.tensor(([rank, 0, 1, 7, 16, rank - 2] * adapters)[:adapters], dtype=torch.int32)
@@ -79,7 +80,7 @@ def test_ranks_and_what_lies_behind_them(tokens, rank, adapters):
     check(got, want, off, bf16)
 
 
-@pytest.mark.parametrize("tokens,adapters", [(40, 4), (1300, 4), (1300, 250)])
+@pytest.mark.parametrize("tokens,adapters", [(40, 4), (1300, 4), (1300, 250), (17000, 4)])
 def test_views_leave_the_rest_alone(tokens, adapters):
     x, y, a, b, scales, ids = make(tokens, 128, 256, 16, adapters, bf16, seed=4)
     wide_x, wide_y = torch.full((tokens, 400), 3.0, dtype=bf16, device="cuda"), torch.full((tokens, 1000), 5.0, dtype=bf16, device="cuda")
@@ -102,7 +103,7 @@ def test_one_tensor_read_and_written():
 
 # (each way that a call can go, the last two in the kernel of many tokens, which otherwise has several clusters to a tile)
 @pytest.mark.parametrize("y_too", [True, False])
-@pytest.mark.parametrize("tokens,dim,width,rank,adapters", [(50, 512, 512, 32, 6), (1500, 512, 512, 32, 6), (3000, 1024, 1024, 128, 4), (3500, 1024, 2048, 128, 1)])
+@pytest.mark.parametrize("tokens,dim,width,rank,adapters", [(50, 512, 512, 32, 6), (1500, 512, 512, 32, 6), (3000, 1024, 1024, 128, 4), (3500, 1024, 2048, 128, 1), (1600, 512, 512, 64, 2)])
 def test_x_in_the_place_of_out(tokens, dim, width, rank, adapters, y_too):
     x, y, a, b, scales, ids = make(tokens, dim, width, rank, adapters, bf16, seed=tokens)
     if y_too:
@@ -114,7 +115,7 @@ def test_x_in_the_place_of_out(tokens, dim, width, rank, adapters, y_too):
     check(out, want, off, bf16)
 
 
-@pytest.mark.parametrize("tokens,rank,adapters", [(70, 16, 2), (1100, 16, 2), (1100, 64, 50)])
+@pytest.mark.parametrize("tokens,rank,adapters", [(70, 16, 2), (1100, 16, 2), (1100, 64, 50), (1500, 64, 2), (17000, 16, 2), (1100, 128, 40)])
 @pytest.mark.parametrize("std", [2.0 ** -20, 1.0, 3000.0])
 def test_half_precision_products_far_from_one(std, tokens, rank, adapters):
     x, y, a, b, scales, ids = make(tokens, 64, 64, rank, adapters, f16, seed=7, std=std)
@@ -124,7 +125,7 @@ def test_half_precision_products_far_from_one(std, tokens, rank, adapters):
     check(ops.lora_add(y, x, ops.LoraAdapters(a, b, scales), ops.LoraPlan(ids, adapters)), want, off, f16)
 
 
-@pytest.mark.parametrize("tokens,adapters", [(40, 2), (1200, 2), (1200, 230)])
+@pytest.mark.parametrize("tokens,adapters", [(40, 2), (1200, 2), (1200, 230), (17000, 3)])
 def test_infinities_of_one_token_stay_its_own(tokens, adapters):
     x, y, a, b, scales, ids = make(tokens, 64, 64, 16, adapters, bf16, seed=8)
     ids[:] = 1
