@@ -114,6 +114,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const std::int32_t* 
   }
 }
 
+struct LowWords {
+  std::uint32_t* hi;
+  std::uint32_t* lo;
+  float* back;
+};
 struct LoraArgs {
   Tiles plan;
   const void* a;
@@ -125,10 +130,8 @@ struct LoraArgs {
   const void* y;
   void* out;
   std::int64_t ldx, ldy, ldo;
-  // Of few and several tokens: t = scale x A^T, by [tile, row of the tile], in two 16-bit parts in operand order, and what a row was divided by.
-  std::uint32_t* t_hi;
-  std::uint32_t* t_lo;
-  float* t_back;
+  // Of several tokens: t = scale x A^T, by [tile, row of the tile], in two 16-bit parts in operand order, and what a row was divided by.
+  LowWords low;
   int adapters, rank, dim, width;
   int parts, slice;  // parts of the channels, channels of each (a multiple of 64)
   int columns;        // columns of an output CTA
@@ -192,17 +195,15 @@ __device__ __forceinline__ std::int64_t low_word(std::int64_t row, int r) {
 }
 
 // Sums of x A^T over the channels' parts, [rows][ranks] in the shared memory of each CTA of a cluster at `sums`, joined, scaled and left for the product with
-// B: a row by ranks / 4 neighbouring lanes, every CTA some of the rows. In two 16-bit parts t keeps 16 (bf16) or 22 (fp16) of its bits.
-// (Rows behind the tile's tokens are left out: what t has there ends up in rows that nobody stores.)
-template <typename T, int kRanks, int kRows>
-__device__ __forceinline__ void leave_sums(const LoraArgs& a, const Tile& tile, std::int64_t tile_number, int rank, const float* sums) {
+// B, as rows from `to_row` of an operand: a row by ranks / 4 neighbouring lanes, rows first, first + step, ... (Rows behind the tile's tokens are left out: what
+// t has there ends up in rows that nobody stores.) In two 16-bit parts t keeps 16 (bf16) or 22 (fp16) of its bits.
+template <typename T, int kRanks>
+__device__ __forceinline__ void leave_sums(const LoraArgs& a, const Tile& tile, int rank, const float* sums, int first, int step, const LowWords& to, std::int64_t to_row) {
   constexpr int kLanes = kRanks / 4;
-  if (a.parts > 1) cluster_sync_all();
-  else __syncthreads();
-  const int part = static_cast<int>(blockIdx.x) % a.parts, lane = static_cast<int>(threadIdx.x) % kLanes;
+  const int lane = static_cast<int>(threadIdx.x) % kLanes;
   const float scale = a.scales != nullptr ? a.scales[tile.adapter] : 1.f;
   const std::uint32_t own = smem_u32(sums);
-  for (int first = part * (kThreads / kLanes); first < tile.count; first += a.parts * (kThreads / kLanes)) {  // (the same number of rounds for a warp's lanes)
+  for (; first < tile.count; first += step) {  // (the same number of rounds for a warp's lanes)
     const int row = first + static_cast<int>(threadIdx.x) / kLanes;
     float v[4] = {};
     if (row < tile.count) {
@@ -227,11 +228,10 @@ __device__ __forceinline__ void leave_sums(const LoraArgs& a, const Tile& tile, 
     std::uint32_t hi[2], lo[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) by.split(v[2 * e], v[2 * e + 1], hi[e], lo[e]);
-    const std::int64_t to = low_word<kRanks>(tile_number * kRows + row, lane * 4);
-    a.t_hi[to] = hi[0], a.t_hi[to + 2] = hi[1], a.t_lo[to] = lo[0], a.t_lo[to + 2] = lo[1];
-    if (lane == 0) a.t_back[tile_number * kRows + row] = by.back;
+    const std::int64_t word = low_word<kRanks>(to_row + row, lane * 4);
+    to.hi[word] = hi[0], to.hi[word + 2] = hi[1], to.lo[word] = lo[0], to.lo[word + 2] = lo[1];
+    if (lane == 0) to.back[to_row + row] = by.back;
   }
-  if (a.parts > 1) cluster_sync_all();  // (nobody leaves while others read its sums)
 }
 
 __device__ __forceinline__ void copy16(std::uint32_t to, const void* from, bool there) {  // (zeros where there is nothing)
@@ -247,97 +247,6 @@ __device__ __forceinline__ uint4 matrices(std::uint32_t addr) {
   uint4 r;
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr) : "memory");
   return r;
-}
-
-// x A^T of a tile's tokens over a part of the channels, in 16-row MMAs with the ranks as columns, kNT: ranks / 8, up to a power of two. Few tokens: a tile's warps
-// take 64 of the part's channels each in turn, through stages of shared memory of their own, rows of 128 bytes whose 16-byte pieces are permuted by the
-// row, and are added up in shared memory. What bounds it is how much of A is on its way: a warp has all that two stages hold in flight at once.
-template <int kNT>
-constexpr int kFewStage = (kFewRows + kNT * 8) * 128;
-template <int kNT>
-constexpr int kFewStages = kNT <= 4 ? 3 : 2;
-template <typename T, int kNT>
-__global__ void __launch_bounds__(kThreads) shrink_few_kernel(const LoraArgs a) {
-  dependents_may_start();
-  constexpr int kRanks = kNT * 8, kStages = kFewStages<kNT>, kRing = kStages * kFewStage<kNT>;
-  extern __shared__ __align__(128) std::uint8_t smem[];
-  const int tile_number = static_cast<int>(blockIdx.x) / a.parts, part = static_cast<int>(blockIdx.x) % a.parts;
-  if (tile_number >= *a.plan.count) return;
-  const Tile tile = a.plan.tiles[tile_number];
-  if (tile.adapter < 0) return;
-  const int rank = rank_of(a, tile.adapter);
-  const int warp = static_cast<int>(threadIdx.x) / 32, lane = static_cast<int>(threadIdx.x) % 32, g = lane / 4, c = lane % 4;
-  // A lane copies piece lane % 8 of rows lane / 8, lane / 8 + 4, ...
-  const int piece = lane % 8;
-  const T* x[kFewRows / 4];
-#pragma unroll
-  for (int i = 0; i < kFewRows / 4; ++i) {
-    const int r = lane / 8 + i * 4;
-    x[i] = r < tile.count ? static_cast<const T*>(a.x) + a.plan.order[tile.first + r] * a.ldx + piece * 8 : nullptr;
-  }
-  const T* const w = static_cast<const T*>(a.a) + tile.adapter * a.a_adapter + lane / 8 * a.a_row + piece * 8;
-  const int from = part * a.slice, to = min(a.dim, from + a.slice);
-  const std::uint32_t ring = smem_u32(smem) + warp * kRing;
-  int to_copy = from + warp * 64, copied = 0;
-  const auto copy_stage = [&] {
-    if (to_copy < to) {
-      const std::uint32_t at = ring + copied * kFewStage<kNT> + lane / 8 * 128;
-      const bool in = to_copy + piece * 8 < to;
-      const auto piece_at = [&](int i) { return at + i * 512 + ((piece ^ (lane / 8 + i * 4 & 7)) << 4); };
-#pragma unroll
-      for (int i = 0; i < kRanks / 4; ++i) {
-        const bool there = in && lane / 8 + i * 4 < rank;
-        copy16(piece_at(i), there ? w + i * 4 * a.a_row + to_copy : w, there);
-      }
-#pragma unroll
-      for (int i = 0; i < kFewRows / 4; ++i) copy16(piece_at(kRanks / 4 + i), x[i] != nullptr && in ? x[i] + to_copy : a.x, x[i] != nullptr && in);
-      to_copy += 64 * kWarps;
-      copied = copied == kStages - 1 ? 0 : copied + 1;
-    }
-    copies_are_one_group();
-  };
-#pragma unroll
-  for (int i = 0; i < kStages; ++i) copy_stage();
-  float acc[kNT][4] = {};
-  // Lane addresses within a stage: A as B operands of two MMAs (8 channels, the next 8, then the next 8 ranks), x as A operands (rows 0..7, 8..15, then
-  // the next 8 channels).
-  const int wr = (lane >> 4) * 8 + (lane & 7), wp = lane >> 3 & 1, xr = lane & 15, xp = lane >> 4;
-  int stage = 0;
-  for (int k = from + warp * 64; k < to; k += 64 * kWarps) {
-    wait_for_copies<kStages - 1>();
-    __syncwarp();  // (the warp's pieces of this stage are there)
-    const std::uint32_t at = ring + stage * kFewStage<kNT>;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const uint4 xv = matrices(at + kRanks * 128 + xr * 128 + (((2 * s + xp) ^ (xr & 7)) << 4));
-#pragma unroll
-      for (int j = 0; j < (kNT + 1) / 2; ++j) {
-        const uint4 wv = matrices(at + ((kNT == 1 ? wr & 7 : wr) + j * 16) * 128 + (((2 * s + wp) ^ (wr & 7)) << 4));
-        mma<T>(acc[2 * j], xv, wv.x, wv.y);
-        if constexpr (kNT > 1) mma<T>(acc[2 * j + 1], xv, wv.z, wv.w);
-      }
-    }
-    __syncwarp();  // (the stage is read)
-    copy_stage();
-    stage = stage == kStages - 1 ? 0 : stage + 1;
-  }
-  wait_for_copies<0>();
-  __syncwarp();
-  constexpr int kNext = kRing / 4;  // floats from a warp's sums to the next one's
-  float* const sums = reinterpret_cast<float*>(smem);
-#pragma unroll
-  for (int j = 0; j < kNT; ++j) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) *reinterpret_cast<float2*>(sums + warp * kNext + (g + 8 * i) * kRanks + j * 8 + c * 2) = make_float2(acc[j][2 * i], acc[j][2 * i + 1]);
-  }
-  __syncthreads();
-  for (int i = static_cast<int>(threadIdx.x); i < tile.count * kRanks; i += kThreads) {
-    float sum = sums[i];
-#pragma unroll
-    for (int v = 1; v < kWarps; ++v) sum += sums[v * kNext + i];
-    sums[i] = sum;
-  }
-  leave_sums<T, kRanks, kFewRows>(a, tile, tile_number, rank, sums);
 }
 
 // The same for several tokens: four warps of 32 rows each with all ranks, 64 channels at a time through three stages of shared memory, rows of 128 bytes whose
@@ -424,7 +333,11 @@ __global__ void __launch_bounds__(kThreads) shrink_several_kernel(const LoraArgs
       }
     }
   }
-  leave_sums<T, kRanks, kManyRows>(a, tile, tile_number, rank, sums);
+  if (a.parts > 1) cluster_sync_all();
+  else __syncthreads();
+  constexpr int kRound = kThreads / (kRanks / 4);
+  leave_sums<T, kRanks>(a, tile, rank, sums, part * kRound, a.parts * kRound, a.low, static_cast<std::int64_t>(tile_number) * kManyRows);
+  if (a.parts > 1) cluster_sync_all();  // (nobody leaves while others read its sums)
 }
 
 // t of a warp's 16 rows as A operands.
@@ -433,14 +346,14 @@ struct Low {
   static constexpr int kPer = kNT <= 2 ? 4 : 8, kBlocks = kNT <= 2 ? 1 : kNT / 4, kSteps = kNT <= 2 ? 1 : kNT / 2;
   uint4 hi[kSteps], lo[kSteps];
   float back[2];
-  __device__ __forceinline__ Low(const LoraArgs& a, std::int64_t row0, int g, int c) {
+  __device__ __forceinline__ Low(const LowWords& from, std::int64_t row0, int g, int c) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) back[i] = a.t_back[row0 + g + 8 * i];
+    for (int i = 0; i < 2; ++i) back[i] = from.back[row0 + g + 8 * i];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const std::int64_t at = (row0 / 16 * kSteps + s) * 32 + g * 4 + c;
       hi[s] = lo[s] = make_uint4(0, 0, 0, 0);
-      if (c * kPer < kNT * 8) hi[s] = reinterpret_cast<const uint4*>(a.t_hi)[at], lo[s] = reinterpret_cast<const uint4*>(a.t_lo)[at];  // (8 ranks: the upper lanes have none)
+      if (c * kPer < kNT * 8) hi[s] = reinterpret_cast<const uint4*>(from.hi)[at], lo[s] = reinterpret_cast<const uint4*>(from.lo)[at];  // (8 ranks: the upper lanes have none)
     }
   }
 };
@@ -548,76 +461,170 @@ __device__ __forceinline__ uint4 operand(const std::uint8_t* p, int c) {
   }
 }
 
-// Few tokens: a tile's warps take 32 columns in turn, y and B through stages of shared memory of their own: the first ones come while the kernel before still
-// makes t.
+// Few tokens: 16 of a tile in one kernel. A cluster of CTAs divides the channels, then the columns; a CTA's warps take 64 of its channels each in turn, are
+// added up with each other and with the other CTAs' through distributed shared memory, and take 32 of its columns each in turn. A, x, B and y come through
+// stages of shared memory of each warp, the first of B and y ahead of A's last. What bounds it is latency, and how much of A and B is on its way.
+// Where tiles are few several clusters share one: each makes the tile's sums and has some of the columns.
 template <int kNT>
-constexpr int kFewAddStage = 32 * kNT * 16 + 1024;
-template <int kNT>
-constexpr int kFewAddStages = kNT <= 4 ? 4 : kNT <= 8 ? 3 : 2;
+struct FewShape {
+  static constexpr int kRanks = kNT * 8;
+  static constexpr int kStageA = (kFewRows + kRanks) * 128, kStagesA = kNT <= 4 ? 3 : kNT <= 8 ? 2 : 1, kRingA = kStagesA * kStageA;
+  // Of B's stages so many are its own, the others lie where A's were: two CTAs fit an SM. (With more on its way but one CTA to an SM, us: 64 users of 32 ranks
+  // 17 for 11, 300 tokens of 3 adapters of 128 ranks 31 for 21.)
+  static constexpr int kBBytes = 32 * kNT * 16, kStageB = kBBytes + 1024, kStagesB = kNT <= 8 ? 4 : 2, kOwnB = kNT <= 2 ? 4 : kNT <= 4 ? 2 : kNT <= 8 ? 1 : 0, kRingB = kOwnB * kStageB;
+  static constexpr int kSumBytes = kFewRows * kRanks * 4, kLowBytes = kFewRows * (kRanks < 16 ? 16 : kRanks) * 2;  // of the sums, of one of t's parts
+  static constexpr int kSums = kWarps * (kRingA + kRingB), kLow = kSums + kSumBytes, kBytes = kLow + 2 * kLowBytes + kFewRows * 4;
+  static_assert((kStagesB - kOwnB) * kStageB <= kRingA && kSumBytes <= kRingA, "some of B's stages, and a warp's sums, lie in its stages of A");
+};
 template <typename T, int kNT>
-__global__ void __launch_bounds__(kThreads) expand_few_kernel(const LoraArgs a) {
-  using L = Low<T, kNT>;
-  constexpr int kStep = 32 * kWarps, kStages = kFewAddStages<kNT>, kStage = kFewAddStage<kNT>, kBBytes = 32 * kNT * 16;
+__global__ void __launch_bounds__(kThreads) few_kernel(const LoraArgs a) {
+  using S = FewShape<kNT>;
+  constexpr int kRanks = S::kRanks;
   extern __shared__ __align__(128) std::uint8_t smem[];
-  Tile tile;
-  if (!tile_to_add(a, tile)) {
-    wait_for_predecessors();  // (this kernel is not done before the one that it follows)
-    return;
-  }
+  const int part = static_cast<int>(blockIdx.x) % a.parts, group = static_cast<int>(blockIdx.x) / a.parts % a.groups;
+  const int tile_number = static_cast<int>(blockIdx.x) / a.parts / a.groups;
+  if (tile_number >= *a.plan.count) return;
+  const Tile tile = a.plan.tiles[tile_number];
+  if (tile.adapter < 0 && a.y == a.out) return;
   const int warp = static_cast<int>(threadIdx.x) / 32, lane = static_cast<int>(threadIdx.x) % 32, g = lane / 4, c = lane % 4;
+  constexpr int kStep = 32 * kWarps;
   const OutRows<T> rows(a, tile, 0, g, c);
-  const int from = static_cast<int>(blockIdx.y) * a.columns + warp * 32, to = min(a.width, (static_cast<int>(blockIdx.y) + 1) * a.columns);
+  const int first = min(a.width, (group * a.parts + part) * a.columns), from = first + warp * 32, to = min(a.width, first + a.columns);
   if (tile.adapter < 0) {
     rows.move(from, to, kStep, c);
-    wait_for_predecessors();
     return;
   }
   const int rank = rank_of(a, tile.adapter);
-  // A lane copies piece lane % kNT of column lane / kNT and of those kColumns on.
+
+  // Of A and x a lane copies piece lane % 8 of rows lane / 8, lane / 8 + 4, ...: 64 channels, rows of 128 bytes whose pieces are permuted by the row.
+  const int piece = lane % 8;
+  const T* x[kFewRows / 4];
+#pragma unroll
+  for (int i = 0; i < kFewRows / 4; ++i) {
+    const int r = lane / 8 + i * 4;
+    x[i] = r < tile.count ? static_cast<const T*>(a.x) + a.plan.order[tile.first + r] * a.ldx + piece * 8 : nullptr;
+  }
+  const T* const wa = static_cast<const T*>(a.a) + tile.adapter * a.a_adapter + lane / 8 * a.a_row + piece * 8;
+  const int from_k = part * a.slice, to_k = min(a.dim, from_k + a.slice);
+  const std::uint32_t ring_a = smem_u32(smem) + warp * S::kRingA;
+  int next_k = from_k + warp * 64, copied_a = 0;
+  const auto copy_a = [&] {
+    if (next_k < to_k) {
+      const std::uint32_t at = ring_a + copied_a * S::kStageA + lane / 8 * 128;
+      const bool in = next_k + piece * 8 < to_k;
+      const auto piece_at = [&](int i) { return at + i * 512 + ((piece ^ (lane / 8 + i * 4 & 7)) << 4); };
+#pragma unroll
+      for (int i = 0; i < kRanks / 4; ++i) {
+        const bool there = in && lane / 8 + i * 4 < rank;
+        copy16(piece_at(i), there ? wa + i * 4 * a.a_row + next_k : wa, there);
+      }
+#pragma unroll
+      for (int i = 0; i < kFewRows / 4; ++i) copy16(piece_at(kRanks / 4 + i), x[i] != nullptr && in ? x[i] + next_k : a.x, x[i] != nullptr && in);
+      next_k += 64 * kWarps;
+      copied_a = copied_a == S::kStagesA - 1 ? 0 : copied_a + 1;
+    }
+    copies_are_one_group();
+  };
+  // Of B piece lane % kNT of column lane / kNT and of those kColumns on, of y the pieces that it adds to.
   constexpr int kColumns = 32 / kNT;
-  const int column = lane / kNT, piece = lane % kNT;
-  const T* const w = static_cast<const T*>(a.b) + tile.adapter * a.b_adapter + column * a.b_row + piece * 8;
-  std::uint8_t* const ring = smem + warp * (kStages * kStage);
-  const std::uint32_t ring_at = smem_u32(ring);
-  int to_copy = from, copied = 0;
-  const auto copy_stage = [&] {
-    if (to_copy < to) {
-      const std::uint32_t at = ring_at + copied * kStage;
+  const int b_column = lane / kNT, b_piece = lane % kNT;
+  const T* const wb = static_cast<const T*>(a.b) + tile.adapter * a.b_adapter + b_column * a.b_row + b_piece * 8;
+  std::uint8_t* const rings[2] = {smem + kWarps * S::kRingA + warp * S::kRingB, smem + warp * S::kRingA};
+  const auto stage_b = [&](int i) { return i < S::kOwnB ? rings[0] + i * S::kStageB : rings[1] + (i - S::kOwnB) * S::kStageB; };
+  int next_n = from, copied_b = 0;
+  const auto copy_b = [&] {
+    if (next_n < to) {
+      const std::uint32_t at = smem_u32(stage_b(copied_b));
 #pragma unroll
       for (int i = 0; i < kNT; ++i) {
-        const int n = column + i * kColumns;
-        const bool in = piece * 8 < rank && to_copy + n < to;
-        copy16(at + n * (kNT * 16) + folded(piece, fold_of<kNT>(n)) * 16, in ? w + (to_copy + i * kColumns) * a.b_row : a.b, in);
+        const int n = b_column + i * kColumns;
+        const bool in = b_piece * 8 < rank && next_n + n < to;
+        copy16(at + n * (kNT * 16) + folded(b_piece, fold_of<kNT>(n)) * 16, in ? wb + (next_n + i * kColumns) * a.b_row : a.b, in);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const bool in = rows.there[i] && to_copy + c * 8 < to;
-        copy16(at + kBBytes + (i * 32 + lane) * 16, in ? rows.y[i] + to_copy : a.y, in);
+        const bool in = rows.there[i] && next_n + c * 8 < to;
+        copy16(at + S::kBBytes + (i * 32 + lane) * 16, in ? rows.y[i] + next_n : a.y, in);
       }
-      to_copy += kStep;
-      copied = copied == kStages - 1 ? 0 : copied + 1;
+      next_n += kStep;
+      copied_b = copied_b == S::kStagesB - 1 ? 0 : copied_b + 1;
     }
     copies_are_one_group();
   };
 #pragma unroll
-  for (int i = 0; i < kStages; ++i) copy_stage();
-  std::uint32_t b_from[4][L::kBlocks];
+  for (int i = 0; i < S::kStagesA; ++i) copy_a();
+#pragma unroll
+  for (int i = 0; i < S::kOwnB; ++i) copy_b();
+
+  float acc[kNT][4] = {};
+  {
+    // Lane addresses within a stage: A as B operands of two MMAs (8 channels, the next 8, then the next 8 ranks), x as A operands (rows 0..7, 8..15, then
+    // the next 8 channels).
+    const int wr = (lane >> 4) * 8 + (lane & 7), wp = lane >> 3 & 1, xr = lane & 15, xp = lane >> 4;
+    int stage = 0, number = 0;
+    for (int k = from_k + warp * 64; k < to_k; k += 64 * kWarps, ++number) {
+      if (number < S::kStagesA) wait_for_copies<S::kStagesA + S::kOwnB - 1>();  // (B's first stages are behind these)
+      else wait_for_copies<S::kStagesA - 1>();
+      __syncwarp();  // (the warp's pieces of this stage are there)
+      const std::uint32_t at = ring_a + stage * S::kStageA;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const uint4 xv = matrices(at + kRanks * 128 + xr * 128 + (((2 * s + xp) ^ (xr & 7)) << 4));
+#pragma unroll
+        for (int j = 0; j < (kNT + 1) / 2; ++j) {
+          const uint4 wv = matrices(at + ((kNT == 1 ? wr & 7 : wr) + j * 16) * 128 + (((2 * s + wp) ^ (wr & 7)) << 4));
+          mma<T>(acc[2 * j], xv, wv.x, wv.y);
+          if constexpr (kNT > 1) mma<T>(acc[2 * j + 1], xv, wv.z, wv.w);
+        }
+      }
+      __syncwarp();  // (the stage is read)
+      copy_a();
+      stage = stage == S::kStagesA - 1 ? 0 : stage + 1;
+    }
+  }
+  wait_for_copies<0>();
+  __syncwarp();
+  constexpr int kNext = S::kRingA / 4;  // floats from a warp's sums to the next one's
+  float* const own = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int j = 0; j < kNT; ++j) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) *reinterpret_cast<float2*>(own + warp * kNext + (g + 8 * i) * kRanks + j * 8 + c * 2) = make_float2(acc[j][2 * i], acc[j][2 * i + 1]);
+  }
+  __syncthreads();
+  float* const sums = reinterpret_cast<float*>(smem + S::kSums);
+  for (int i = static_cast<int>(threadIdx.x); i < tile.count * kRanks; i += kThreads) {
+    float sum = own[i];
+#pragma unroll
+    for (int v = 1; v < kWarps; ++v) sum += own[v * kNext + i];
+    sums[i] = sum;
+  }
+  if (a.parts > 1) cluster_sync_all();
+  else __syncthreads();
+#pragma unroll
+  for (int i = S::kOwnB; i < S::kStagesB; ++i) copy_b();
+  std::uint8_t* const t = smem + S::kLow;
+  const LowWords words{reinterpret_cast<std::uint32_t*>(t), reinterpret_cast<std::uint32_t*>(t + S::kLowBytes), reinterpret_cast<float*>(t + 2 * S::kLowBytes)};
+  leave_sums<T, kRanks>(a, tile, rank, sums, 0, kThreads / (kRanks / 4), words, 0);
+  __syncthreads();
+  if (a.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (it has read the others' sums)
+
+  const Low<T, kNT> low(words, 0, g, c);
+  std::uint32_t b_from[4][Low<T, kNT>::kBlocks];
   place_operands<T, kNT>(g, c, b_from);
-  wait_for_predecessors();
-  const L low(a, static_cast<std::int64_t>(blockIdx.x) * kFewRows, g, c);
   const auto add_all = [&](auto ragged) {
     int stage = 0;
     for (int n = from; n < to; n += kStep) {
-      wait_for_copies<kStages - 1>();
+      wait_for_copies<S::kStagesB - 1>();
       __syncwarp();  // (the warp's pieces of this step are there)
-      const std::uint8_t* const at = ring + stage * kStage;
+      const std::uint8_t* const at = stage_b(stage);
       uint4 y[2], out[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) y[i] = load16(at + kBBytes + (i * 32 + lane) * 16);
+      for (int i = 0; i < 2; ++i) y[i] = load16(at + S::kBBytes + (i * 32 + lane) * 16);
       add_block<T, kNT, decltype(ragged)::value>(low, c, rank, y, [&](int j, int q) { return operand<T, kNT>(at + b_from[j][q], c); }, out);
       __syncwarp();  // (the stage is read)
-      copy_stage();
-      stage = stage == kStages - 1 ? 0 : stage + 1;
+      copy_b();
+      stage = stage == S::kStagesB - 1 ? 0 : stage + 1;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (rows.there[i] && n + c * 8 < to) *reinterpret_cast<uint4*>(rows.out[i] + n) = out[i];
@@ -627,6 +634,7 @@ __global__ void __launch_bounds__(kThreads) expand_few_kernel(const LoraArgs a) 
   if (rank % 8 != 0) add_all(std::true_type{});
   else add_all(std::false_type{});
   wait_for_copies<0>();
+  if (a.parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // (nobody leaves while others read its sums)
 }
 
 // Several: eight warps of 16 rows each, 32 columns at a time through four stages of shared memory: a lane copies the pieces of y that it adds to, B is
@@ -691,7 +699,7 @@ __global__ void __launch_bounds__(kManyThreads, kNT <= 8 ? 3 : 2) expand_several
 #pragma unroll
   for (int i = 0; i < kExpandStages - 1; ++i) copy_step();
   wait_for_predecessors();
-  const L low(a, static_cast<std::int64_t>(blockIdx.x) * kManyRows + warp * 16, g, c);
+  const L low(a.low, static_cast<std::int64_t>(blockIdx.x) * kManyRows + warp * 16, g, c);
   std::uint32_t b_from[4][L::kBlocks];
   place_operands<T, kNT>(g, c, b_from);
   T* out_to[2] = {rows.out[0] + from, rows.out[1] + from};
@@ -1052,40 +1060,31 @@ inline Way way_of(std::int64_t tokens, int adapters, int rank) {
   return rank > 32 && large * rank >= 3500 ? Way::kMany : Way::kSeveral;
 }
 inline int rows_of(Way way) { return way == Way::kFew ? kFewRows : kManyRows; }
-// Parts of the channels (a power of two): CTAs for the whole GPU twice over (thrice of several tokens), of 256 channels at least.
+// Parts of the channels (a power of two): CTAs for the whole GPU twice over (of few tokens some more, as not all tiles that there may be are there; thrice of several),
+// of 256 channels at least.
 inline int parts_of(Way way, std::int64_t tiles, std::int64_t dim) {
-  const std::int64_t room = (way == Way::kSeveral ? 3 : 2) * 148, most = way == Way::kMany ? kMostManyParts : kMostParts;
+  const std::int64_t room = way == Way::kFew ? 370 : (way == Way::kSeveral ? 3 : 2) * 148, most = way == Way::kMany ? kMostManyParts : kMostParts;
   int parts = 1;
   while (parts < most && tiles * parts * 2 <= room && dim >= parts * 2 * 256) parts *= 2;
   return parts;
 }
-// Of few and several tokens: one of t's two parts (an operand has 16 ranks at least).
+// Of several tokens: one of t's two parts (an operand has 16 ranks at least).
 inline std::size_t part_bytes(std::int64_t rows, int rank) { return (static_cast<std::size_t>(rows) * std::max(2, padded_tiles(rank)) * 16 + 255) / 256 * 256; }
 inline std::size_t workspace_bytes(std::int64_t tokens, int adapters, int rank) {
   const Way way = way_of(tokens, adapters, rank);
-  if (way == Way::kMany) return 0;
-  const std::int64_t rows = most_tiles(tokens, adapters, rows_of(way)) * rows_of(way);
+  if (way != Way::kSeveral) return 0;
+  const std::int64_t rows = most_tiles(tokens, adapters, kManyRows) * kManyRows;
   return 2 * part_bytes(rows, rank) + static_cast<std::size_t>(rows) * 4;
 }
 
 template <typename T, int kNT>
 int launch(const char* op, LoraArgs a, Way way, unsigned tiles, cudaStream_t stream) {
-  const LaunchChain chain(stream);
-  if (way != Way::kMany) {
-    // Columns of a CTA: as many as leave 6 small or 4 large CTAs to an SM, 128 at least.
-    const std::int64_t most = std::max<std::int64_t>(1, (way == Way::kFew ? 6LL : 4LL) * sm_count() / tiles);
+  if (way == Way::kSeveral) {
+    const LaunchChain chain(stream);
+    // Columns of a CTA: as many as leave 4 CTAs to an SM, 128 at least.
+    const std::int64_t most = std::max<std::int64_t>(1, 4LL * sm_count() / tiles);
     a.columns = static_cast<int>(std::max<std::int64_t>(128, ((a.width + most - 1) / most + 127) / 128 * 128));
     const dim3 grid(tiles, static_cast<unsigned>((a.width + a.columns - 1) / a.columns));
-    if (way == Way::kFew) {
-      static std::atomic<std::uint64_t> few_done{0};
-      constexpr int kBytes = kWarps * kFewStages<kNT> * kFewStage<kNT>;
-      if (const int s = allow_shared(op, shrink_few_kernel<T, kNT>, kBytes, few_done); s != B2_OK) return s;
-      if (const int s = enqueue(op, shrink_few_kernel<T, kNT>, dim3(tiles * a.parts), dim3(kThreads), kBytes, stream, a.parts, a); s != B2_OK) return s;
-      static std::atomic<std::uint64_t> few_add_done{0};
-      constexpr int kAddBytes = kWarps * kFewAddStages<kNT> * kFewAddStage<kNT>;
-      if (const int s = allow_shared(op, expand_few_kernel<T, kNT>, kAddBytes, few_add_done); s != B2_OK) return s;
-      return enqueue(op, expand_few_kernel<T, kNT>, grid, dim3(kThreads), kAddBytes, stream, 1, a);
-    }
     static std::atomic<std::uint64_t> shrink_done{0}, expand_done{0};
     constexpr int kShrinkBytes = kShrinkStages * kShrinkStage<kNT>, kExpandBytes = kExpandStages * kExpandStage<kNT>;
     if (const int s = allow_shared(op, shrink_several_kernel<T, kNT>, kShrinkBytes, shrink_done); s != B2_OK) return s;
@@ -1093,15 +1092,20 @@ int launch(const char* op, LoraArgs a, Way way, unsigned tiles, cudaStream_t str
     if (const int s = enqueue(op, shrink_several_kernel<T, kNT>, dim3(tiles * a.parts), dim3(kThreads), kShrinkBytes, stream, a.parts, a); s != B2_OK) return s;
     return enqueue(op, expand_several_kernel<T, kNT>, grid, dim3(kManyThreads), kExpandBytes, stream, 1, a);
   }
-  static std::atomic<std::uint64_t> done{0};
-  if (const int s = allow_shared(op, many_kernel<T, kNT>, ManyShape<kNT>::kBytes, done); s != B2_OK) return s;
   // Clusters to a tile: as many as the GPU has room for (2 CTAs to an SM), of 128 columns a CTA at least. One where x is out: all of a cluster's channels are
   // read before one of its columns is written, those of another cluster may not be.
   const std::int64_t room = a.x == a.out ? 1 : std::max<std::int64_t>(1, 2LL * sm_count() / (static_cast<std::int64_t>(tiles) * a.parts));
   a.groups = static_cast<int>(std::max<std::int64_t>(1, std::min<std::int64_t>(room, a.width / (128 * a.parts))));
   a.columns = (a.width + a.parts * a.groups - 1) / (a.parts * a.groups);
-  a.columns = (a.columns + 63) / 64 * 64;
-  return enqueue(op, many_kernel<T, kNT>, dim3(tiles * a.parts * a.groups), dim3(kManyThreads), ManyShape<kNT>::kBytes, stream, a.parts, a);
+  a.columns = way == Way::kFew ? (a.columns + 31) / 32 * 32 : (a.columns + 63) / 64 * 64;
+  const dim3 grid(tiles * a.parts * a.groups);
+  static std::atomic<std::uint64_t> few_done{0}, many_done{0};
+  if (way == Way::kFew) {
+    if (const int s = allow_shared(op, few_kernel<T, kNT>, FewShape<kNT>::kBytes, few_done); s != B2_OK) return s;
+    return enqueue(op, few_kernel<T, kNT>, grid, dim3(kThreads), FewShape<kNT>::kBytes, stream, a.parts, a);
+  }
+  if (const int s = allow_shared(op, many_kernel<T, kNT>, ManyShape<kNT>::kBytes, many_done); s != B2_OK) return s;
+  return enqueue(op, many_kernel<T, kNT>, grid, dim3(kManyThreads), ManyShape<kNT>::kBytes, stream, a.parts, a);
 }
 template <typename T>
 int launch(const char* op, const LoraArgs& a, Way way, unsigned tiles, cudaStream_t stream) {
@@ -1184,7 +1188,7 @@ int b2_lora_add(const b2_lora* l, const void* plan, size_t bytes, int64_t tokens
   a.adapters = l->adapters, a.rank = l->rank, a.dim = static_cast<int>(l->dim), a.width = static_cast<int>(l->width);
   char* const at = static_cast<char*>(workspace);
   const std::size_t part = part_bytes(tiles * rows_of(way), l->rank);
-  a.t_hi = reinterpret_cast<std::uint32_t*>(at), a.t_lo = reinterpret_cast<std::uint32_t*>(at + part), a.t_back = reinterpret_cast<float*>(at + 2 * part);
+  a.low = LowWords{reinterpret_cast<std::uint32_t*>(at), reinterpret_cast<std::uint32_t*>(at + part), reinterpret_cast<float*>(at + 2 * part)};
   a.parts = parts_of(way, tiles, l->dim);
   a.slice = static_cast<int>(((l->dim + a.parts - 1) / a.parts + 63) / 64 * 64);
   return l->dtype == B2_DTYPE_F16 ? launch<__half>(op, a, way, static_cast<unsigned>(tiles), as_stream(stream)) : launch<__nv_bfloat16>(op, a, way, static_cast<unsigned>(tiles), as_stream(stream));
