@@ -398,7 +398,7 @@ struct RowOutputs {
 // largest of their largest elements is a bound that `top` elements reach, so that only the threads whose largest one reaches it can hold one of the first
 // `top`: their elements are read once more (the batches of loads that have those, from L2), and those at or above the bound sorted by counting.
 // A warp's loads are bulk copies into shared memory, units ahead of the one that it works on.
-// Exponentials bound it after memory: 4096 rows of 160000 in bf16 with one alternative take 256 us, 78 % of a copy's rate, the exponentials' unit 67 % busy. Few rows take
+// Exponentials bound it after memory: 4096 rows of 160000 in bf16 with one alternative take 240 to 253 us, 80 % of a copy's rate, the exponentials' unit 64 % busy. Few rows take
 // a chain of latencies: one row of 150001 with 5 alternatives 12 us, 6 of them for its sums, 2 for the target, 4 for the alternatives.
 template <typename T, bool kLong>
 __global__ void __launch_bounds__(kThreads, Shape<kLong>::kPerSm) logprobs_kernel(const LogprobArgs a) {
@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kLong>::kPerSm) logprobs_kerne
         if (u >= valid) v[u].raw = make_uint4(least, least, least, least);
       }
     }
-    if (!(sums.cuts && top == -INFINITY && blank(v))) sums.add(v, from, valid, top, c);
+    if (kLong || !(sums.cuts && top == -INFINITY && blank(v))) sums.add(v, from, valid, top, c);
     if (counts && (top >= mine || mine_nan)) {
       const int token = first_token + first * n;
       const bool ahead = token + ((kBatch - 1) * 32 + 1) * n <= target;
@@ -510,9 +510,10 @@ __global__ void __launch_bounds__(kThreads, Shape<kLong>::kPerSm) logprobs_kerne
       see(v, from, first, valid);
     }
     lost = __any_sync(kAll, lost);  // (the unit is read)
-    // What a lane has to cut is a mask's, mostly, and then all cut: lanes that go on differently would take turns. (2000 rows of 150000 in bf16 of which one in 500
-    // is allowed: 181 us without this and the look at whole loads, 141 with; without a mask 114 and 117.)
-    sums.cuts = __any_sync(kAll, sums.cuts);
+    // What a lane has to cut is a mask's, mostly, and then all cut: lanes that go on differently would take turns. (509 rows of 32003 in fp16 of which one in 500
+    // is allowed: 24.5 us without this and the look at whole loads, 21.2 with. Long rows without a mask would take 5 % more: 4096 of 160000 238 and 250;
+    // with one 2000 of 150000 181 and 139.)
+    if constexpr (!kLong) sums.cuts = __any_sync(kAll, sums.cuts);
     if (!lost && lane == 0) copy_unit(unit + kStages * kWarps, stage);
     stage = stage == kStages - 1 ? 0 : stage + 1;
     parity ^= stage == 0 ? 1u : 0u;
