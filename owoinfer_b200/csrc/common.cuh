@@ -465,14 +465,9 @@ __device__ __forceinline__ void tmem_st_32x16(std::uint32_t taddr, const std::ui
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
 }
-// The same for 4 and 8 consecutive columns.
+// The same for 4 consecutive columns.
 __device__ __forceinline__ void tmem_st_32x4(std::uint32_t taddr, const std::uint32_t (&r)[4]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%4], {%0, %1, %2, %3};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(taddr) : "memory");
-}
-__device__ __forceinline__ void tmem_st_32x8(std::uint32_t taddr, const std::uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
-               ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
-               : "memory");
 }
 // The same 32-bit value into this warp's 32 lanes x 32 consecutive columns.
 __device__ __forceinline__ void tmem_fill_32x32(std::uint32_t taddr, std::uint32_t v) {

@@ -19,7 +19,7 @@ constexpr int kMostParts = 8, kMostManyParts = 4;  // CTAs of a cluster that div
 
 // A plan sorts the tokens by adapter and cuts them into tiles, of one warp's rows, where there are few tokens, and of eight warps', for A and B to be
 // read once for more of them: [0] and [1] below.
-constexpr int kFewRows = 16, kManyRows = 128, kFewTokens = 16384;
+constexpr int kFewRows = 16, kManyRows = 128, kFewTokens = 4096;
 inline std::int64_t most_tiles(std::int64_t tokens, int adapters, int rows) {
   return rows == kFewRows && tokens > kFewTokens ? 0 : std::min(tokens, tokens / rows + adapters + 1);
 }
@@ -148,12 +148,6 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint4& a, std::uint32_t
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
   }
 }
-// K of 32: 8 neighbouring elements of a lane in each operand.
-template <typename T>
-__device__ __forceinline__ void mma_twice(float (&d)[4], const uint4& a0, const uint4& a1, const uint4& b) {
-  mma<T>(d, make_uint4(a0.x, a1.x, a0.y, a1.y), b.x, b.y);
-  mma<T>(d, make_uint4(a0.z, a1.z, a0.w, a1.w), b.z, b.w);
-}
 __device__ __forceinline__ uint4 load16(const void* p) { return *reinterpret_cast<const uint4*>(p); }
 
 __device__ __forceinline__ int rank_of(const LoraArgs& a, int adapter) {
@@ -249,9 +243,10 @@ __device__ __forceinline__ uint4 matrices(std::uint32_t addr) {
   return r;
 }
 
-// The same for several tokens: four warps of 32 rows each with all ranks, 64 channels at a time through three stages of shared memory, rows of 128 bytes whose
-// 16-byte pieces are permuted by the row. (With the lanes' own pieces as operands, as above, each MMA had four moves beside it to bring its
-// registers together: 8191 tokens, 4096 channels, rank 64: 30 us.)
+// Several tokens: x A^T of a tile over a part of the channels, the ranks as columns, kNT: ranks / 8, up to a power of two. Four warps of 32 rows each with all ranks, 64
+// channels at a time through three stages of shared memory, rows of 128 bytes whose 16-byte pieces are permuted by the row. (With operands straight
+// from memory each MMA had four moves beside it to bring its registers together: 8191 tokens, 4096 channels, rank 64: 30 us.) What bounds it is memory and, between
+// its copies and its last MMA, latency: 3000 tokens of 4 adapters, 4096 to 4096, rank 32 take 24 us with the kernel behind it, twice what their bytes take.
 template <int kNT>
 constexpr int kShrinkStage = kManyRows * 128 + kNT * 8 * 128;
 constexpr int kShrinkStages = 3;
@@ -464,7 +459,8 @@ __device__ __forceinline__ uint4 operand(const std::uint8_t* p, int c) {
 // Few tokens: 16 of a tile in one kernel. A cluster of CTAs divides the channels, then the columns; a CTA's warps take 64 of its channels each in turn, are
 // added up with each other and with the other CTAs' through distributed shared memory, and take 32 of its columns each in turn. A, x, B and y come through
 // stages of shared memory of each warp, the first of B and y ahead of A's last. What bounds it is latency, and how much of A and B is on its way.
-// Where tiles are few several clusters share one: each makes the tile's sums and has some of the columns.
+// Where tiles are few several clusters share one: each makes the tile's sums and has some of the columns. One token of rank 16 over 2048 channels takes 4.5 us, 64 of as many
+// users, 48 adapters, 4096 to 6144, from memory 8.5 (their bytes: 2.0). (As two kernels 4.4 and 10.2, and another launch of 2.5 us for the host.)
 template <int kNT>
 struct FewShape {
   static constexpr int kRanks = kNT * 8;
@@ -766,7 +762,8 @@ __device__ __forceinline__ void end_tensor(Tensor& s) {
 // own channels (64 at a time), they exchange the sums through distributed shared memory, and each adds t B^T to its own columns of y (64 at a time), t in
 // tensor memory in its two 16-bit parts. Both kinds of steps run through the same stages of shared memory, rows of 128 bytes with the 128-byte swizzle,
 // so that y and B are on their way while the sums are exchanged. A tile's tokens need not be neighbours, so that the threads copy the rows, piece by
-// piece. Where tiles are few several clusters share one: each makes the tile's sums and has some of the columns. Memory bounds it: x and y are read, out written.
+// piece. Where tiles are few several clusters share one: each makes the tile's sums and has some of the columns. Memory should bound it (x and y are read, out written):
+// 8191 tokens of 6 adapters, 4096 to 4096, rank 64 take 59 to 64 us, half of a copy's rate; a CTA's parts, the exchange among them, do not overlap each other.
 // (As two kernels, x A^T left in global memory: 8191 tokens, 4096 to 4096, rank 64: 71 us, on mma.sync, whose rate is a quarter, 69.)
 template <int kNT>
 struct ManyShape {
@@ -1049,10 +1046,10 @@ inline int padded_tiles(int rank) {  // ranks / 8, up to a power of two
 }
 // Which kernels a call runs. Small tiles read A and B again every 16 tokens, large ones are mostly empty where adapters are many: small ones go by their number
 // times the ranks for each large tile. Of large tiles, the kernel of many tokens wins by its products (mma.sync's rate is a quarter) and has more to set up. With
-// 4096 channels and columns from memory, few / several / many tokens' kernels, us: 64 tokens of as many adapters, rank 64 (a small tile for each large one)
-// 15 / 44 / 42; 300 of 3, rank 128 (470) 22 / 25 / 26; 1000 of 6, rank 128 (630) 36 / 28 / 40; 3000 of 4, rank 16 (110) 22 / 23 / 32, rank 32 (220)
-// 27 / 25 / 33, rank 128 85 / 53 / 50; 3000 of 60, rank 64 (189) 39 / 58 / 59, rank 128 (380) 90 / 93 / 73; 8191 of 6, rank 64 85 / 69 / 59; 16000 of 60, 2048
-// channels and columns, rank 32 55 / 53 / 71.
+// 4096 channels and columns from memory, few / several / many tokens' kernels, us (in brackets small tiles times ranks for each large tile): 64 tokens of as many
+// adapters, rank 64 (64) 16 / 44 / 37; 300 of 3, rank 128 (470) 21 / 24 / 25; 1000 of 6, rank 64 (320) 17 / 21 / 29, rank 128 (630) 31 / 28 / 39; 1500 of 4, rank 64
+// (390) 26 / 23 / 30; 3000 of 4, rank 16 (110) 25 / 23 / 31, rank 128 88 / 52 / 49; 3000 of 60, rank 64 (190) 46 / 58 / 59, rank 128 (380) 91 / 94 / 73; 5000 of 6, rank
+// 16 (110; a wave and a bit of CTAs, each a tile's whole work) 45 / 32 / 44; 8191 of 6, rank 64 85 / 68 / 59; 16000 of 60, 2048 channels and columns, rank 32 63 / 51 / 69.
 enum class Way { kFew, kSeveral, kMany };
 inline Way way_of(std::int64_t tokens, int adapters, int rank) {
   const std::int64_t large = most_tiles(tokens, adapters, kManyRows);
