@@ -144,7 +144,7 @@ def test_infinities_of_one_token_stay_its_own(tokens, adapters):
 def test_rows_behind_the_last_and_two_streams_at_once():
     # Calls of every way on two streams; each has its own workspace, and what lies behind the tokens stays as it was.
     made = []
-    for seed, (tokens, rank, adapters) in enumerate([(60, 16, 3), (1300, 32, 3), (1300, 64, 60)] * 2):
+    for seed, (tokens, rank, adapters) in enumerate([(60, 16, 3), (1300, 32, 3), (1300, 64, 60), (1300, 128, 3), (1100, 128, 40)] * 2):
         x, y, a, b, scales, ids = make(tokens, 256, 320, rank, adapters, bf16, seed=20 + seed)
         out = torch.full((tokens + 40, 320), 7.0, dtype=bf16, device="cuda")
         made.append((x, y, ops.LoraAdapters(a, b, scales), ops.LoraPlan(ids, adapters), out, exact(x, y, a, b, scales, ids), tokens))
@@ -160,7 +160,7 @@ def test_rows_behind_the_last_and_two_streams_at_once():
         assert (out[tokens:] == 7.0).all()
 
 
-@pytest.mark.parametrize("tokens", [30, 1200])
+@pytest.mark.parametrize("tokens", [30, 1200, 17000])
 def test_adapters_and_ranks_outside_raise_a_bit(tokens):
     x, y, a, b, scales, ids = make(tokens, 64, 64, 16, 3, bf16, seed=9)
     plan = ops.LoraPlan(ids, 3)
@@ -175,20 +175,22 @@ def test_adapters_and_ranks_outside_raise_a_bit(tokens):
     assert ops.lora_status(clear=True) == 2
 
 
-def test_nobody_has_an_adapter_and_no_tokens():
-    x, y, a, b, scales, ids = make(33, 64, 64, 16, 3, bf16, seed=10)
+@pytest.mark.parametrize("tokens,rank,adapters", [(33, 16, 3), (1600, 64, 3), (1100, 128, 40)])
+def test_nobody_has_an_adapter_and_no_tokens(tokens, rank, adapters):
+    x, y, a, b, scales, ids = make(tokens, 64, 64, rank, adapters, bf16, seed=10)
     ids[:] = -1
-    out = ops.lora_add(y, x, ops.LoraAdapters(a, b, scales), ops.LoraPlan(ids, 3), out=torch.empty_like(y))
+    out = ops.lora_add(y, x, ops.LoraAdapters(a, b, scales), ops.LoraPlan(ids, adapters), out=torch.empty_like(y))
     assert torch.equal(out, y)
-    none = ops.LoraPlan(ids[:0], 3)
+    none = ops.LoraPlan(ids[:0], adapters)
     assert ops.lora_add(y[:0], x[:0], ops.LoraAdapters(a, b, scales), none).shape == (0, 64)
 
 
-def test_a_captured_step_with_its_plan():
-    x, y, a, b, scales, ids = make(48, 512, 512, 16, 5, bf16, seed=11)
+@pytest.mark.parametrize("tokens,rank,n", [(48, 16, 5), (1600, 64, 2), (1100, 128, 40)])
+def test_a_captured_step_with_its_plan(tokens, rank, n):
+    x, y, a, b, scales, ids = make(tokens, 512, 512, rank, n, bf16, seed=11)
     adapters, out = ops.LoraAdapters(a, b, scales), torch.empty_like(y)
     changing = ids.clone()
-    plan = ops.LoraPlan(changing, 5)
+    plan = ops.LoraPlan(changing, n)
     ops.lora_add(y, x, adapters, plan, out=out)
     graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
@@ -197,10 +199,19 @@ def test_a_captured_step_with_its_plan():
         ops.lora_add(y, x, adapters, plan, out=out)
         second = ops.lora_add(out, x, adapters, plan, out=torch.empty_like(y))
     for shift in range(3):
-        changing.copy_((ids + shift) % 5 - (ids + shift) % 2)
+        changing.copy_((ids + shift) % n - (ids + shift) % 2)
         graph.replay()
         torch.cuda.synchronize()
         want, off = exact(x, y, a, b, scales, changing)
         check(out, want, off, bf16)
         want, off = exact(x, out, a, b, scales, changing)
         check(second, want, off, bf16)
+
+
+@pytest.mark.parametrize("tokens,rank,adapters", [(300, 32, 20), (1600, 64, 2), (1100, 128, 40)])
+def test_the_same_call_gives_the_same_bits(tokens, rank, adapters):
+    x, y, a, b, scales, ids = make(tokens, 1032, 520, rank, adapters, bf16, seed=12)
+    plan, adapters = ops.LoraPlan(ids, adapters), ops.LoraAdapters(a, b, scales)
+    first = ops.lora_add(y, x, adapters, plan, out=torch.empty_like(y))
+    for _ in range(20):
+        assert torch.equal(ops.lora_add(y, x, adapters, plan, out=torch.empty_like(y)), first)

@@ -58,6 +58,7 @@ def plan(ids=A, tokens=4, adapters=3, at=A, size=1 << 20):
     (lora, dict(ranks=A + 2), "ranks"), (lora, dict(plan=None), "plan"), (lora, dict(plan=A + 64), "plan"), (lora, dict(plan_bytes=16), "plan"), (lora, dict(x=A + 2), "x must"),
     (lora, dict(ldx=60), "x must"), (lora, dict(y=None), "y must"), (lora, dict(ldy=120), "y must"), (lora, dict(out=A + 8), "out must"), (lora, dict(ldo=132), "out must"),
     (lora, dict(out=A, ldo=136), "y's"), (lora, dict(out=A, y=A + 4096), "x's"), (lora, dict(ws=None), "workspace"), (lora, dict(ws_bytes=64), "workspace"), (lora, dict(ws=A + 128), "workspace"),
+    (lora, dict(tokens=20000, plan_bytes=1 << 22, ws_bytes=4096), "workspace"), (lora, dict(tokens=20000, plan_bytes=1 << 22, ws=None, ws_bytes=0), "workspace"),
     (plan, dict(tokens=-1), "tokens"), (plan, dict(adapters=0), "adapters"), (plan, dict(at=None), "plan"), (plan, dict(size=0), "plan"), (plan, dict(at=A + 16), "plan"),
     (plan, dict(ids=None), "token_adapters"), (plan, dict(ids=A + 2), "token_adapters"),
 ], ids=lambda v: v.__name__ if callable(v) else "-".join(f"{k}={x}" for k, x in v.items()) if isinstance(v, dict) else "")
