@@ -398,7 +398,7 @@ struct RowOutputs {
 // largest of their largest elements is a bound that `top` elements reach, so that only the threads whose largest one reaches it can hold one of the first
 // `top`: their elements are read once more (the batches of loads that have those, from L2), and those at or above the bound sorted by counting.
 // A warp's loads are bulk copies into shared memory, units ahead of the one that it works on.
-// Exponentials bound it after memory: 4096 rows of 160000 in bf16 with one alternative take 240 to 253 us, 80 % of a copy's rate, the exponentials' unit 64 % busy. Few rows take
+// Exponentials bound it after memory: 4096 rows of 160000 in bf16 with one alternative take 240 to 253 us, 80 % of a copy's rate, the exponentials' unit 67 % busy. Few rows take
 // a chain of latencies: one row of 150001 with 5 alternatives 12 us, 6 of them for its sums, 2 for the target, 4 for the alternatives.
 template <typename T, bool kLong>
 __global__ void __launch_bounds__(kThreads, Shape<kLong>::kPerSm) logprobs_kernel(const LogprobArgs a) {

@@ -459,8 +459,8 @@ __device__ __forceinline__ uint4 operand(const std::uint8_t* p, int c) {
 // Few tokens: 16 of a tile in one kernel. A cluster of CTAs divides the channels, then the columns; a CTA's warps take 64 of its channels each in turn, are
 // added up with each other and with the other CTAs' through distributed shared memory, and take 32 of its columns each in turn. A, x, B and y come through
 // stages of shared memory of each warp, the first of B and y ahead of A's last. What bounds it is latency, and how much of A and B is on its way.
-// Where tiles are few several clusters share one: each makes the tile's sums and has some of the columns. One token of rank 16 over 2048 channels takes 4.5 us, 64 of as many
-// users, 48 adapters, 4096 to 6144, from memory 8.5 (their bytes: 2.0). (As two kernels 4.4 and 10.2, and another launch of 2.5 us for the host.)
+// Where tiles are few several clusters share one: each makes the tile's sums and has some of the columns. One token of rank 16, 2048 to 2048, takes 4.9 us, 64 of as many
+// users, 48 adapters, 4096 to 6144, from memory 8.5 (their bytes: 2.0). (As two kernels 4.4 to 5.0 and 10.2, and another launch of 2.5 us for the host.)
 template <int kNT>
 struct FewShape {
   static constexpr int kRanks = kNT * 8;
