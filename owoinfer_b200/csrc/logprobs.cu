@@ -393,7 +393,7 @@ struct RowOutputs {
   }
 };
 
-// A cluster of CTAs per row, each with a run of it, or CTAs that take row after row; one pass over the logits. Every thread keeps its sums against its own
+// A CTA per row, or where rows are few a cluster, each CTA with a run of it; one pass over the logits. Every thread keeps its sums against its own
 // reference, how many of its elements come before the target, and its largest element. The alternatives come from what the threads saw: the `top`-th
 // largest of their largest elements is a bound that `top` elements reach, so that only the threads whose largest one reaches it can hold one of the first
 // `top`: their elements are read once more (the batches of loads that have those, from L2), and those at or above the bound sorted by counting.
