@@ -605,7 +605,9 @@ __global__ void __launch_bounds__(kThreads, Shape<kLong>::kPerSm) logprobs_kerne
     };
     find_bound();
     if (sh.bound == 0u) {
-      // Fewer than `top` threads have seen anything above -infinity: for the others their first -infinity, or NaN.
+      // Fewer than `top` threads have seen anything above -infinity: for the others their first -infinity, or NaN. (The bound may be one of these
+      // then. Of a thread with a number it is not known whether another of its batches reaches that: it is looked through.)
+      if (sh.second[tid] == 0u) sh.second[tid] = order_of<T>(-INFINITY);
       if (best == 0u) {
         int where = -1;
         for (int j = 0; j < units_each * kBatch && best <= 1u; ++j) {
