@@ -157,7 +157,7 @@ __device__ __forceinline__ int count_from(const Chunk<T>& c, float least) {
     return __popc((t & 0x00ff00ffu) | (s & 0xff00ff00u));
   }
 }
-// The value of T above x, a number that is not the last.
+// The value of T above x: a number, or NaN of infinity.
 template <typename T>
 __device__ __forceinline__ float next_of(float x) {
   return value_of<T>(order_of<T>(x) + 1u);
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kLong>::kPerSm) logprobs_kerne
   const bool mine_nan = isnan(mine);
   const auto is_before = [&](float l, int token) { return l > mine || (l == mine && token < target) || (mine_nan && (!isnan(l) || token < target)); };
   const bool counts = has_target && a.ranks != nullptr;
-  const float next = counts && mine < INFINITY ? next_of<T>(mine) : INFINITY;  // what is behind the target comes before it from here on
+  const float next = counts && !mine_nan ? next_of<T>(mine) : nan;  // what is behind the target comes before it from here on (of infinity NaN: nothing does)
   // The loads v, which lie at `from` too: first, first + 32, ...; behind `valid` of them the first again.
   const auto see = [&](Chunk<T>(&v)[kBatch], const uint4* from, int first, int valid) {
     const float top = top_of(v);
