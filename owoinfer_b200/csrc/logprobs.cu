@@ -207,8 +207,12 @@ struct Running {
   template <typename T>
   __device__ __forceinline__ void rise(float top, float c) {
     if (!(top > ref) || (ref > -INFINITY && (top - ref) * c <= kAhead)) return;
-    const Sums m = finished(c).moved(top, c);
+    Sums m = finished(c).moved(top, c);
     ref = top, base = top * c;
+    if (!wide() && m.s != 0.f) {  // (what finished() will undo)
+      const float d = fmaf(ref, c, -base), f = ex2(d);
+      m.w = f * fmaf(d, m.s, m.w), m.s *= f;
+    }
     s[0] = pack2(m.s, 0.f), w[0] = pack2(m.w, 0.f), s[1] = w[1] = pack2(0.f, 0.f);
     limit = wide() ? -INFINITY : top + kAhead / c;
     least = fmaxf(kLowest<T>, -2.9e38f / c);
