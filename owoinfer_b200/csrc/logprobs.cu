@@ -163,6 +163,9 @@ __device__ __forceinline__ float next_of(float x) {
   return value_of<T>(order_of<T>(x) + 1u);
 }
 
+// (a - b) c, which may be a number where a - b is none.
+__device__ __forceinline__ float apart(float a, float b, float c) { return fmaf(a, 0.5f, -0.5f * b) * (2.f * c); }
+
 // Sums over part of a row against a reference `ref` near its largest logit: s = sum 2^x, w = sum x 2^x with x = (l - ref) c, c = scale log2(e).
 // The reference is the largest of what came first and follows once something is kAhead binades above it.
 struct Sums {
@@ -170,7 +173,7 @@ struct Sums {
   __device__ __forceinline__ Sums moved(float to, float c) const {
     Sums r{to, 0.f, 0.f};
     if (s != 0.f) {  // (nothing, or only what weighs nothing, so far: nothing to scale, and -infinity times 0 to avoid)
-      const float d = (ref - to) * c, f = ex2(d);
+      const float d = apart(ref, to, c), f = ex2(d);
       r.s = s * f;
       r.w = f == 0.f ? 0.f : f * fmaf(d, s, w);
     }
@@ -208,7 +211,7 @@ struct Running {
   // Ahead of elements of which `top` is the largest (NaN: no number among them).
   template <typename T>
   __device__ __forceinline__ void rise(float top, float c) {
-    if (!(top > ref) || (ref > -INFINITY && (top - ref) * c <= kAhead)) return;
+    if (!(top > ref) || (ref > -INFINITY && apart(top, ref, c) <= kAhead)) return;
     Sums m = finished(c).moved(top, c);
     const bool was_wide = wide();
     ref = top, base = top * c;
@@ -220,7 +223,7 @@ struct Running {
     s[0] = pack2(m.s, 0.f), w[0] = pack2(m.w, 0.f), s[1] = w[1] = pack2(0.f, 0.f);
     limit = wide() ? -INFINITY : top + kAhead / c;
     least = fmaxf(kLowest<T>, -2.9e38f / c);
-    if (wide() || !((least - top) * c < -200.f)) least = -INFINITY;
+    if (wide() || !(apart(least, top, c) < -200.f)) least = -INFINITY;
   }
   // The sums of 2^x and x 2^x go on over loads, the elements cut to `least` where that is asked for.
   template <typename T, int count, bool kCut>
@@ -287,7 +290,7 @@ struct Running {
   }
   // Any elements: what is 2^-200 and less of the reference is 2^-200, 0 in fp32 and times x no NaN.
   __device__ __forceinline__ void add_two(float l, float m, float c) {
-    const float by = wide() ? 1.f : c, less = wide() ? ref : base, times = wide() ? c : 1.f;
+    const float by = wide() ? 0.5f : c, less = wide() ? 0.5f * ref : base, times = wide() ? 2.f * c : 1.f;  // (as apart() does)
     float x, y;
     unpack2(mul2(fma2(pack2(l, m), pack2(by, by), pack2(-less, -less)), pack2(times, times)), x, y);
     x = max_nan(x, -200.f), y = max_nan(y, -200.f);
@@ -386,7 +389,7 @@ struct RowOutputs {
     nothing = s.ref == -INFINITY && !isnan(s.s);
   }
   __device__ __forceinline__ float logprob(float l) const {
-    return nothing ? -INFINITY : isnan(sums.s) ? __int_as_float(0x7fc00000) : (l - sums.ref) * a.scale - log_s;
+    return nothing ? -INFINITY : isnan(sums.s) ? __int_as_float(0x7fc00000) : apart(l, sums.ref, a.scale) - log_s;
   }
   __device__ __forceinline__ void row(std::int64_t target, float logit, unsigned before) const {  // (before: four times)
     const bool has_target = target >= 0 && target < a.vocab;
