@@ -152,11 +152,17 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const NormArgs a) {
       if (mine && c * 8 % a.group == 0) a.scale[row * (a.dim / a.group) + c * 8 / a.group] = scale;
     }
     if (!mine) continue;
-    *reinterpret_cast<uint2*>(static_cast<std::uint8_t*>(a.q) + row * a.ldq + c * 8) = codes8<kE4m3>(v[i], by);
+    // r / scale may pass fp32 where the row and what its scale is of are tiny (neither factor does): then one after the other.
+    const bool tiny = isinf(by);
+    if (tiny) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] *= r;
+    }
+    *reinterpret_cast<uint2*>(static_cast<std::uint8_t*>(a.q) + row * a.ldq + c * 8) = codes8<kE4m3>(v[i], tiny ? 1.f / scale : by);
     if (a.norm_out != nullptr) {
       float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = v[i][e] * r;
+      for (int e = 0; e < 8; ++e) y[e] = tiny ? v[i][e] : v[i][e] * r;
       std::uint16_t* const p = static_cast<std::uint16_t*>(a.norm_out) + row * a.ld_norm + c * 8;
       *reinterpret_cast<uint4*>(p) = a.norm_f16 != 0 ? store8<__half>(y) : store8<__nv_bfloat16>(y);
     }
