@@ -766,7 +766,8 @@ int b2_paged_cache_status(unsigned* host_value, int clear);
 
 /* s = x + residual (residual NULL: s = x), residual_out = s; y = s * rsqrt(mean(s^2) + eps) * weight (NULL: 1), of s before it is
  * rounded; for every token, or every `group` channels of it, scale = max(max|y| / Q, 1e-30) with Q = 127 (int8) or 448 (e4m3), and
- * q = round(y / scale), ties to even. norm_out, where given, is y in 16 bits besides.
+ * q = round(y / scale), ties to even (y / scale as s * weight * (Q / max|s * weight|), two roundings ahead of this one: what lies
+ * closer than those to the middle of two codes may go either way). norm_out, where given, is y in 16 bits besides. s * weight is formed in fp32.
  * x bf16, fp16 or fp32; residual and residual_out of x's type or fp32; weight any of them. Rows 16-byte aligned, their strides (in elements)
  * multiples of 16 bytes; q 8-byte aligned, ldq % 8 == 0; dim % 8 == 0, dim <= 32768. residual_out may be residual, or x where
  * they have one type, and norm_out may be a 16-bit x; otherwise nothing that is written may overlap anything else (residual_out NULL: not written).

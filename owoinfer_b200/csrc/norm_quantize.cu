@@ -135,9 +135,12 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const NormArgs a) {
   const float r = square > 0.f && square < INFINITY ? rsqrtf(square) : __int_as_float(0x7fc00000);
   constexpr float kLargest = kE4m3 ? 448.f : 127.f;
   const auto scale_of = [&](float most) { return isnan(r) ? r : fmaxf(most * r / kLargest, kSmallestScale); };
+  // y / scale is s w times this: the norm's factor is in both, and its roundings would move what lies between two codes. (Of NaN NaN; infinity where the
+  // scale is the smallest one.)
+  const auto factor_of = [&](float most, float scale) { return scale > kSmallestScale ? kLargest / most : isnan(r) ? r : INFINITY; };
   float scale = 0.f, by = 0.f;
   if (a.group == 0) {
-    scale = scale_of(top), by = r / scale;
+    scale = scale_of(top), by = factor_of(top, scale);
     if (there && lane == 0) a.scale[row] = scale;
   }
 #pragma unroll
@@ -148,11 +151,11 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const NormArgs a) {
       float most = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[i][e]));
-      scale = scale_of(warp_max(most, a.group / 8)), by = r / scale;
+      most = warp_max(most, a.group / 8), scale = scale_of(most), by = factor_of(most, scale);
       if (mine && c * 8 % a.group == 0) a.scale[row * (a.dim / a.group) + c * 8 / a.group] = scale;
     }
     if (!mine) continue;
-    // r / scale may pass fp32 where the row and what its scale is of are tiny (neither factor does): then one after the other.
+    // Where that passes fp32, or the scale is the smallest one: y, then times 1 / scale, which do not.
     const bool tiny = isinf(by);
     if (tiny) {
 #pragma unroll
