@@ -159,13 +159,13 @@ __device__ __forceinline__ int rank_of(const LoraArgs& a, int adapter) {
 }
 
 // fp32 values of a row, the largest of them `top`, as two 16-bit parts. fp16 ends at 2^16 and loses bits below 2^-14: there the largest is brought between
-// 2^14 and 2^15 by a power of two, which `back` undoes.
+// 2^14 and 2^15 by a power of two, which `back` undoes. (Where it is an infinity the others may be any number: 2^-114 keeps them below one.)
 template <typename T>
 struct Halves {
   float by = 1.f, back = 1.f;
   __device__ __forceinline__ explicit Halves(float top) {
     if constexpr (std::is_same<T, __half>::value) {
-      const int e = top < INFINITY ? max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14, -100) : 0;
+      const int e = max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14, -100);
       by = __uint_as_float(static_cast<unsigned>(127 - e) << 23), back = __uint_as_float(static_cast<unsigned>(127 + e) << 23);
     }
   }
