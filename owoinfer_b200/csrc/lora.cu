@@ -767,15 +767,16 @@ __device__ __forceinline__ void end_tensor(Tensor& s) {
 // (As two kernels, x A^T left in global memory: 8191 tokens, 4096 to 4096, rank 64: 71 us, on mma.sync, whose rate is a quarter, 69.)
 template <int kNT>
 struct ManyShape {
-  static constexpr int kN = kNT < 2 ? 16 : kNT * 8;                               // ranks of an MMA
+  static_assert(kNT >= 8, "ranks above 32 only: way_of()");
+  static constexpr int kN = kNT * 8;                                              // ranks of an MMA
   static constexpr int kOperand = kN > 64 ? 128 * 128 : 64 * 128;                 // of a step: A's ranks by 64 channels, or B's 64 columns by its ranks
   static constexpr int kStage = kOperand + kManyRows * 128, kStages = kN > 64 ? 3 : 4;
   // Tensor memory: accumulators (of x A^T, then of two steps' t B^T), from kLow on t. Two CTAs of an SM have all of it; a kernel of the framework that
   // allocates some and waits for its neighbours has more than half of the shared memory, and does not fit beside one: no two wait for one another.
   static constexpr int kLow = 128, kColumns = 256;
   static constexpr int kBytes = kStages * kStage + 1024;                          // and what aligns it
-  // The sums that are exchanged: blocks of ranks, 16 KB at most each, as many to a stage as two stages take them all.
-  static constexpr int kBlock = kN < 32 ? 16 : 32, kBlocks = kN / kBlock, kPerStage = (kBlocks + 1) / 2;
+  // The sums that are exchanged: blocks of ranks, 16 KB each, as many to a stage as two stages take them all.
+  static constexpr int kBlock = 32, kBlocks = kN / kBlock, kPerStage = kBlocks / 2;
   static_assert(kManyRows * kBlock * 4 * kPerStage <= kStage && kManyRows * kN * 2 <= kStage, "the sums, then t's parts, lie in two stages' places");
 };
 template <typename T, int kNT>
@@ -834,17 +835,15 @@ __global__ void __launch_bounds__(kManyThreads, 2) many_kernel(const LoraArgs a)
       }
       if (first) {
 #pragma unroll
-        for (int i = 0; i < (S::kN * 8 + kManyThreads - 1) / kManyThreads; ++i) {
+        for (int i = 0; i < S::kN * 8 / kManyThreads; ++i) {
           const int row = tid / 8 + i * (kManyThreads / 8), piece = tid % 8;
-          if (S::kN < kManyThreads / 8 && row >= S::kN) continue;
           const bool in = row < rank && piece * 8 < left;
           copy16(at + at_piece(row, piece), in ? wa + row * a.a_row + n + piece * 8 : wa, in);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < (64 * kPieces + kManyThreads - 1) / kManyThreads; ++i) {
+        for (int i = 0; i < 64 * kPieces / kManyThreads; ++i) {
           const int j = tid + i * kManyThreads, row = j / kPieces, piece = j % kPieces;
-          if (64 * kPieces < kManyThreads && row >= 64) continue;
           const bool in = row < left && piece * 8 < rank;
           copy16(at + piece / 8 * (64 * 128) + at_piece(row, piece & 7), in ? wb + (n + row) * a.b_row + piece * 8 : wb, in);
         }
@@ -896,13 +895,11 @@ __global__ void __launch_bounds__(kManyThreads, 2) many_kernel(const LoraArgs a)
   {
     constexpr int kRowBytes = S::kBlock * 4, kLanes = S::kBlock / 4, kRows = kManyThreads / kLanes, kRounds = kManyRows / kRows;
     const auto stage_of = [&](int i) { return smem + (k_steps + S::kStages - 1 - i) % S::kStages * S::kStage; };
-    const auto swizzled = [](int row, int piece) { return S::kBlock == 32 ? piece ^ (row & 7) : piece ^ (row >> 1 & 3); };
-    const auto sum_at = [&](int b, int row, int piece) { return stage_of(b / S::kPerStage) + b % S::kPerStage * (kManyRows * kRowBytes) + row * kRowBytes + swizzled(row, piece) * 16; };
+    const auto sum_at = [&](int b, int row, int piece) { return stage_of(b / S::kPerStage) + b % S::kPerStage * (kManyRows * kRowBytes) + row * kRowBytes + (piece ^ (row & 7)) * 16; };
 #pragma unroll
     for (int b = half; b < S::kBlocks; b += 2) {
       std::uint32_t r[S::kBlock];
-      if constexpr (S::kBlock == 16) tmem_ld_32x16(accumulators + lanes + b * S::kBlock, r);
-      else tmem_ld_32x32(accumulators + lanes + b * S::kBlock, r);
+      tmem_ld_32x32(accumulators + lanes + b * S::kBlock, r);
       tmem_ld_wait();
 #pragma unroll
       for (int i = 0; i < kLanes; ++i) *reinterpret_cast<uint4*>(sum_at(b, row0 + lane, i)) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
@@ -946,7 +943,7 @@ __global__ void __launch_bounds__(kManyThreads, 2) many_kernel(const LoraArgs a)
     else __syncthreads();
     // Its two parts as rows, in the same place, then a row to a thread and into tensor memory.
     constexpr int kTRow = S::kN * 2;
-    const auto t_at = [&](int which, int row, int at) { return stage_of(which) + row * kTRow + (S::kN >= 64 ? (at & ~7) | ((at & 7) ^ (row & 7)) : at) * 16; };
+    const auto t_at = [&](int which, int row, int at) { return stage_of(which) + row * kTRow + folded(at, row & 7) * 16; };
 #pragma unroll
     for (int i = 0; i < kRounds; ++i) {
       const int row = tid / kLanes + i * kRows;
@@ -1103,13 +1100,16 @@ int launch(const char* op, LoraArgs a, Way way, unsigned tiles, cudaStream_t str
   a.columns = (a.width + a.parts * a.groups - 1) / (a.parts * a.groups);
   a.columns = way == Way::kFew ? (a.columns + 31) / 32 * 32 : (a.columns + 63) / 64 * 64;
   const dim3 grid(tiles * a.parts * a.groups);
-  static std::atomic<std::uint64_t> few_done{0}, many_done{0};
-  if (way == Way::kFew) {
-    if (const int s = allow_shared(op, few_kernel<T, kNT>, FewShape<kNT>::kBytes, few_done); s != B2_OK) return s;
-    return enqueue(op, few_kernel<T, kNT>, grid, dim3(kThreads), FewShape<kNT>::kBytes, stream, a.parts, a);
+  if constexpr (kNT >= 8) {
+    if (way == Way::kMany) {
+      static std::atomic<std::uint64_t> many_done{0};
+      if (const int s = allow_shared(op, many_kernel<T, kNT>, ManyShape<kNT>::kBytes, many_done); s != B2_OK) return s;
+      return enqueue(op, many_kernel<T, kNT>, grid, dim3(kManyThreads), ManyShape<kNT>::kBytes, stream, a.parts, a);
+    }
   }
-  if (const int s = allow_shared(op, many_kernel<T, kNT>, ManyShape<kNT>::kBytes, many_done); s != B2_OK) return s;
-  return enqueue(op, many_kernel<T, kNT>, grid, dim3(kManyThreads), ManyShape<kNT>::kBytes, stream, a.parts, a);
+  static std::atomic<std::uint64_t> few_done{0};
+  if (const int s = allow_shared(op, few_kernel<T, kNT>, FewShape<kNT>::kBytes, few_done); s != B2_OK) return s;
+  return enqueue(op, few_kernel<T, kNT>, grid, dim3(kThreads), FewShape<kNT>::kBytes, stream, a.parts, a);
 }
 template <typename T>
 int launch(const char* op, const LoraArgs& a, Way way, unsigned tiles, cudaStream_t stream) {
