@@ -1063,7 +1063,7 @@ inline std::int64_t likely_tiles(std::int64_t tokens, int adapters) {
 // Parts of the channels (a power of two): CTAs for the whole GPU twice over (thrice of several tokens), of 256 channels at least. (Of few tokens by the tiles
 // that are likely; by those that there may be, 300 tokens of 60 adapters of 128 ranks took 42 us for 31.)
 inline int parts_of(Way way, std::int64_t tokens, int adapters, std::int64_t dim) {
-  const std::int64_t room = (way == Way::kSeveral ? 3 : 2) * 148, most = way == Way::kMany ? kMostManyParts : kMostParts;
+  const std::int64_t room = (way == Way::kSeveral ? 3LL : 2LL) * sm_count(), most = way == Way::kMany ? kMostManyParts : kMostParts;
   const std::int64_t tiles = way == Way::kFew ? likely_tiles(tokens, adapters) : most_tiles(tokens, adapters, kManyRows);
   int parts = 1;
   while (parts < most && tiles * parts * 2 <= room && dim >= parts * 2 * 256) parts *= 2;
