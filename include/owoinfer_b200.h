@@ -770,7 +770,7 @@ int b2_paged_cache_status(unsigned* host_value, int clear);
  * closer than those to the middle of two codes may go either way). norm_out, where given, is y in 16 bits besides. s * weight is formed in fp32.
  * x bf16, fp16 or fp32; residual and residual_out of x's type or fp32; weight any of them. Rows 16-byte aligned, their strides (in elements)
  * multiples of 16 bytes; q 8-byte aligned, ldq % 8 == 0; dim % 8 == 0, dim <= 32768. residual_out may be residual, or x where
- * they have one type, and norm_out may be a 16-bit x; otherwise nothing that is written may overlap anything else (residual_out NULL: not written).
+ * they have one type, and norm_out may be a 16-bit x, with the same row stride; otherwise nothing that is written may overlap anything else (residual_out NULL: not written).
  * scale: fp32 [tokens], or [tokens, dim / group] with group 32, 64, 128 or 256 (dim % group == 0; 0: none).
  * A token with a NaN or an infinity in s, whose squares add up past fp32 (|s| of 2^63 and more), or with neither squares nor eps, has NaN
  * for all of its scales and its norm_out; its int8 codes are 0, its e4m3 codes NaN. */

@@ -223,6 +223,16 @@ extern "C" int b2_add_rms_norm_quantize(const b2_norm_quantize* p, void* stream)
   if (p->weight != nullptr && !aligned_to(p->weight, 16)) return fail_invalid(op, "weight must be 16-byte aligned");
   if (p->q == nullptr || !aligned_to(p->q, 8) || p->ldq < p->dim || p->ldq % 8 != 0) return fail_invalid(op, "q must be 8-byte aligned rows of at least dim codes");
   if (p->scale == nullptr || !aligned_to(p->scale, 4)) return fail_invalid(op, "scale is missing or not aligned");
+  // A row is read by its own threads alone: what is written in a tensor's place has its rows where that has them.
+  const auto in_place = [&](const void* out, std::int64_t ld_out, int out_dtype, const void* in, std::int64_t ld, int dtype) {
+    return out != in || (dtype_bytes(out_dtype) == dtype_bytes(dtype) && (ld_out == ld || p->tokens == 1));
+  };
+  if (p->residual_out != nullptr && (!in_place(p->residual_out, p->ld_residual_out, r_dtype, p->x, p->ldx, p->x_dtype) ||
+                                     !in_place(p->residual_out, p->ld_residual_out, r_dtype, p->residual, p->ld_residual, r_dtype)))
+    return fail_invalid(op, "residual_out in the place of x or of the residual must have its rows and its type");
+  if (p->norm_out != nullptr && !in_place(p->norm_out, p->ld_norm, p->norm_dtype, p->x, p->ldx, p->x_dtype))
+    return fail_invalid(op, "norm_out in x's place must have x's rows, of 16 bits");
+  if (p->norm_out != nullptr && p->norm_out == p->residual_out) return fail_invalid(op, "norm_out and residual_out must be two matrices");
   NormArgs a{p->x, p->ldx, p->residual, p->ld_residual, p->residual_out, p->ld_residual_out, p->weight, p->weight_dtype, p->norm_out, p->ld_norm,
              p->norm_dtype == B2_DTYPE_F16, p->q, p->ldq, p->scale, p->tokens, p->dim, p->group, 0, p->eps};
   const cudaStream_t s = as_stream(stream);
