@@ -135,12 +135,20 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const NormArgs a) {
   const float r = square > 0.f && square < INFINITY ? rsqrtf(square) : __int_as_float(0x7fc00000);
   constexpr float kLargest = kE4m3 ? 448.f : 127.f;
   const auto scale_of = [&](float most) { return isnan(r) ? r : fmaxf(most * r / kLargest, kSmallestScale); };
-  // y / scale is s w times this: the norm's factor is in both, and its roundings would move what lies between two codes. (Of NaN NaN; infinity where the
-  // scale is the smallest one.)
-  const auto factor_of = [&](float most, float scale) { return scale > kSmallestScale ? kLargest / most : isnan(r) ? r : INFINITY; };
-  float scale = 0.f, by = 0.f;
+  // y / scale is s w times Q / max|s w|: the norm's factor is in both, and its roundings would move what lies between two codes. Where that passes fp32, or
+  // the scale is the smallest one (or NaN): y itself, then times 1 / scale.
+  const auto by_largest = [](float most, float scale) { return scale > kSmallestScale && most > kLargest / 3e38f; };
+  float scale = 0.f, by = 0.f, rest = r;  // (rest: of y = v rest)
   if (a.group == 0) {
-    scale = scale_of(top), by = factor_of(top, scale);
+    scale = scale_of(top), by = kLargest / top;
+    if (!by_largest(top, scale)) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] *= r;
+      }
+      by = 1.f / scale, rest = 1.f;
+    }
     if (there && lane == 0) a.scale[row] = scale;
   }
 #pragma unroll
@@ -151,21 +159,20 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const NormArgs a) {
       float most = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[i][e]));
-      most = warp_max(most, a.group / 8), scale = scale_of(most), by = factor_of(most, scale);
+      most = warp_max(most, a.group / 8), scale = scale_of(most), by = kLargest / most, rest = r;
+      if (!by_largest(most, scale)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] *= r;
+        by = 1.f / scale, rest = 1.f;
+      }
       if (mine && c * 8 % a.group == 0) a.scale[row * (a.dim / a.group) + c * 8 / a.group] = scale;
     }
     if (!mine) continue;
-    // Where that passes fp32, or the scale is the smallest one: y, then times 1 / scale, which do not.
-    const bool tiny = isinf(by);
-    if (tiny) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] *= r;
-    }
-    *reinterpret_cast<uint2*>(static_cast<std::uint8_t*>(a.q) + row * a.ldq + c * 8) = codes8<kE4m3>(v[i], tiny ? 1.f / scale : by);
+    *reinterpret_cast<uint2*>(static_cast<std::uint8_t*>(a.q) + row * a.ldq + c * 8) = codes8<kE4m3>(v[i], by);
     if (a.norm_out != nullptr) {
       float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = tiny ? v[i][e] : v[i][e] * r;
+      for (int e = 0; e < 8; ++e) y[e] = v[i][e] * rest;
       std::uint16_t* const p = static_cast<std::uint16_t*>(a.norm_out) + row * a.ld_norm + c * 8;
       *reinterpret_cast<uint4*>(p) = a.norm_f16 != 0 ? store8<__half>(y) : store8<__nv_bfloat16>(y);
     }
