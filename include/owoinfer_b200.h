@@ -833,7 +833,8 @@ int b2_token_logprobs(const b2_logprobs* args, void* stream);
  * written may overlap what is read.
  *
  * b2_lora_plan sorts the tokens by their adapter (token_adapters, device int32 [tokens]; an adapter past the last raises a bit of
- * b2_lora_status and counts as none) into `plan`, which b2_lora_add of any layer and projection then reads: once for a step.
+ * b2_lora_status and counts as none) into `plan`, which b2_lora_add of any layer and projection then reads: once for a step. A plan of another number of
+ * tokens or adapters raises a bit and leaves out as it was.
  * plan and workspace are 256-byte aligned, of the sizes that the _bytes calls give (0: invalid arguments; 256: none is used, and then a workspace of
  * NULL with 0 bytes will do). Nothing is kept in the workspace. */
 typedef struct b2_lora {
@@ -852,7 +853,7 @@ size_t b2_lora_workspace_bytes(int64_t tokens, int adapters, int64_t dim, int ra
 int b2_lora_add(const b2_lora* lora, const void* plan, size_t plan_bytes, int64_t tokens, const void* x, int64_t ldx, const void* y, int64_t ldy,
                 void* out, int64_t ldo, void* workspace, size_t workspace_bytes, void* stream);
 /* Bits raised on the current device since the last clear: 1 an adapter past the last one, 2 a rank outside 0 .. rank, 4 a bounded wait that
- * expired. Synchronises the device: for tests and post-mortems. */
+ * expired, 8 a plan of another number of tokens or adapters. Synchronises the device: for tests and post-mortems. */
 int b2_lora_status(unsigned* host_value, int clear);
 
 /* Every mbarrier wait inside the tensor-core kernels is bounded (200 ms); a CTA whose wait expired raises a device word,

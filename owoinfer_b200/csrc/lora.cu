@@ -10,7 +10,7 @@ namespace b2 {
 namespace {
 
 __device__ unsigned g_lora_status = 0;
-enum LoraFault : unsigned { kLoraBadAdapter = 1, kLoraBadRank = 2, kLoraWait = 4 };  // (a bounded wait expired)
+enum LoraFault : unsigned { kLoraBadAdapter = 1, kLoraBadRank = 2, kLoraWait = 4, kLoraOtherPlan = 8 };  // (4: a bounded wait expired)
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kPlanThreads = 1024;
@@ -23,8 +23,8 @@ constexpr int kFewRows = 16, kManyRows = 128, kFewTokens = 4096;
 inline std::int64_t most_tiles(std::int64_t tokens, int adapters, int rows) {
   return rows == kFewRows && tokens > kFewTokens ? 0 : std::min(tokens, tokens / rows + adapters + 1);
 }
-struct PlanHead {
-  int tiles[2], pad[2];
+struct alignas(16) PlanHead {
+  int tiles[2], tokens, adapters;
 };
 struct Tile {
   int adapter, first, count, pad;  // -1: tokens without an adapter
@@ -46,9 +46,17 @@ inline Plan plan_at(void* p, std::int64_t tokens, int adapters) {
 }
 // What a kernel reads of it: one kind of tiles.
 struct Tiles {
-  const int* count;
+  const PlanHead* head;
   const Tile* tiles;
   const std::int32_t* order;
+  int tokens, adapters, kind;  // kind: which tiles
+  // How many; none of a plan of other tokens or adapters, whose tiles lie elsewhere.
+  __device__ __forceinline__ int count() const {
+    const int4 h = *reinterpret_cast<const int4*>(head);
+    if (h.z == tokens && h.w == adapters) return kind == 0 ? h.x : h.y;
+    atomicOr(&g_lora_status, kLoraOtherPlan);
+    return 0;
+  }
 };
 
 // A CTA per adapter, and one for the tokens without: each counts all tokens by adapter (a thread a run of neighbouring tokens, which mostly have
@@ -110,7 +118,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const std::int32_t* 
     for (int i = tid; i < num; i += kPlanThreads) {
       plan.tiles[k][s_before[1 + k] + i] = Tile{own < adapters ? own : -1, s_before[0] + i * rows, min(rows, count - i * rows), 0};
     }
-    if (own == adapters && tid == 0) plan.head->tiles[k] = s_before[1 + k] + num;
+    if (own == adapters && tid == 0) plan.head->tiles[k] = s_before[1 + k] + num, plan.head->tokens = tokens, plan.head->adapters = adapters;
   }
 }
 
@@ -132,7 +140,7 @@ struct LoraArgs {
   std::int64_t ldx, ldy, ldo;
   // Of several tokens: t = scale x A^T, by [tile, row of the tile], in two 16-bit parts in operand order, and what a row was divided by.
   LowWords low;
-  int adapters, rank, dim, width;
+  int rank, dim, width;
   int parts, slice;  // parts of the channels, channels of each (a multiple of 64)
   int columns;        // columns of an output CTA
   int groups;         // clusters to a tile
@@ -256,7 +264,7 @@ __global__ void __launch_bounds__(kThreads) shrink_several_kernel(const LoraArgs
   constexpr int kRanks = kNT * 8;
   extern __shared__ __align__(128) std::uint8_t smem[];
   const int tile_number = static_cast<int>(blockIdx.x) / a.parts, part = static_cast<int>(blockIdx.x) % a.parts;
-  if (tile_number >= *a.plan.count) return;
+  if (tile_number >= a.plan.count()) return;
   const Tile tile = a.plan.tiles[tile_number];
   if (tile.adapter < 0) return;
   const int rank = rank_of(a, tile.adapter);
@@ -421,7 +429,7 @@ struct OutRows {
 };
 // The tile of a CTA; one that has nothing to do says so.
 __device__ __forceinline__ bool tile_to_add(const LoraArgs& a, Tile& tile) {
-  const bool exists = static_cast<int>(blockIdx.x) < *a.plan.count;
+  const bool exists = static_cast<int>(blockIdx.x) < a.plan.count();
   if (exists) tile = a.plan.tiles[blockIdx.x];
   return exists && (tile.adapter >= 0 || a.y != a.out);
 }
@@ -479,7 +487,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const LoraArgs a) {
   extern __shared__ __align__(128) std::uint8_t smem[];
   const int part = static_cast<int>(blockIdx.x) % a.parts, group = static_cast<int>(blockIdx.x) / a.parts % a.groups;
   const int tile_number = static_cast<int>(blockIdx.x) / a.parts / a.groups;
-  if (tile_number >= *a.plan.count) return;
+  if (tile_number >= a.plan.count()) return;
   const Tile tile = a.plan.tiles[tile_number];
   if (tile.adapter < 0 && a.y == a.out) return;
   const int warp = static_cast<int>(threadIdx.x) / 32, lane = static_cast<int>(threadIdx.x) % 32, g = lane / 4, c = lane % 4;
@@ -787,7 +795,7 @@ __global__ void __launch_bounds__(kManyThreads, 2) many_kernel(const LoraArgs a)
   __shared__ float s_back[kManyRows];
   const int part = static_cast<int>(blockIdx.x) % a.parts, group = static_cast<int>(blockIdx.x) / a.parts % a.groups;
   const int tile_number = static_cast<int>(blockIdx.x) / a.parts / a.groups;
-  if (tile_number >= *a.plan.count) return;
+  if (tile_number >= a.plan.count()) return;
   const Tile tile = a.plan.tiles[tile_number];
   if (tile.adapter < 0 && a.y == a.out) return;
   const int tid = static_cast<int>(threadIdx.x), warp = tid / 32, lane = tid % 32;
@@ -1186,10 +1194,10 @@ int b2_lora_add(const b2_lora* l, const void* plan, size_t bytes, int64_t tokens
   const Way way = way_of(tokens, l->adapters, l->rank);
   const std::int64_t tiles = most_tiles(tokens, l->adapters, rows_of(way));
   const Plan p = plan_at(const_cast<void*>(plan), tokens, l->adapters);
-  a.plan = Tiles{&p.head->tiles[way != Way::kFew], p.tiles[way != Way::kFew], p.order};
+  a.plan = Tiles{p.head, p.tiles[way != Way::kFew], p.order, static_cast<int>(tokens), l->adapters, way != Way::kFew};
   a.a = l->a, a.b = l->b, a.a_adapter = l->a_adapter_stride, a.a_row = l->a_row_stride, a.b_adapter = l->b_adapter_stride, a.b_row = l->b_row_stride;
   a.scales = l->scales, a.ranks = l->ranks, a.x = x, a.y = y, a.out = out, a.ldx = ldx, a.ldy = ldy, a.ldo = ldo;
-  a.adapters = l->adapters, a.rank = l->rank, a.dim = static_cast<int>(l->dim), a.width = static_cast<int>(l->width);
+  a.rank = l->rank, a.dim = static_cast<int>(l->dim), a.width = static_cast<int>(l->width);
   char* const at = static_cast<char*>(workspace);
   const std::size_t part = part_bytes(tiles * rows_of(way), l->rank);
   a.low = LowWords{reinterpret_cast<std::uint32_t*>(at), reinterpret_cast<std::uint32_t*>(at + part), reinterpret_cast<float*>(at + 2 * part)};

@@ -1077,7 +1077,7 @@ def lora_add(y, x, adapters, plan, out=None, workspace=None):
 
 
 def lora_status(clear=False) -> int:
-    """Bits that the kernels on adapters raised (b2_lora_status): 0 when every adapter and rank was in bounds."""
+    """Bits that the kernels on adapters raised (b2_lora_status): 0 when every adapter, rank and plan was as it should be."""
     v = C.c_uint(0)
     check(_lib.lib().b2_lora_status(C.byref(v), int(clear)))
     return int(v.value)
