@@ -1063,6 +1063,8 @@ def lora_add(y, x, adapters, plan, out=None, workspace=None):
         out = y
     else:
         ldo = _like(out, "out", (tokens, adapters.width), dtypes)
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
     _here(y, x, out, adapters.a, plan.buffer, workspace)
     need = plan.workspace_bytes(adapters.dim, adapters.rank)
     if workspace is not None:
