@@ -826,8 +826,8 @@ int b2_token_logprobs(const b2_logprobs* args, void* stream);
  *   out[t] = y[t] + scales[a] * (x[t] A[a]^T) B[a]^T,  a = the adapter of token t (negative: none, out[t] = y[t])
  * x [tokens, dim], y and out [tokens, width], A [adapters, rank, dim], B [adapters, width, rank], all of one type, bf16 or fp16; scales fp32
  * [adapters] or NULL (1); ranks int32 [adapters] or NULL: adapter a has ranks[a] <= rank rows of A and columns of B, what lies behind them is not
- * used, NaN and infinities included (ranks outside 0 .. rank raise a bit of b2_lora_status and are cut). x A^T is held to 16 bits and more; an
- * infinity in what is used of B may make NaN where it would make an infinity.
+ * used, NaN and infinities included (ranks outside 0 .. rank raise a bit of b2_lora_status and are cut). x A^T is held to 16 bits and more (in fp16
+ * a token's numbers below 2^-22 of its largest to 2^-39 of that); an infinity in what is used of B may make NaN where it would make an infinity.
  * Rows and matrices 16-byte aligned, strides in elements, multiples of 8; dim, width and rank multiples of 8, rank <= 128; adapters <= 4096.
  * out may be y itself (rows without an adapter are then left alone), and x may be either, with the same row stride; otherwise nothing that is
  * written may overlap what is read.

@@ -189,7 +189,7 @@ struct Sums {
 };
 // A thread's sums while it reads. x = l c - base is one fma of a pair, base = ref c as it is rounded: what that is off is put right at the end. That is 64
 // binades at most below kWide, where different logits are as far apart; a reference beyond is subtracted first. (2000 rows of 150000 in bf16, one in 500 allowed,
-// the others at -1e9: 182 us; at -1e10, beyond: 262.)
+// the others at -1e9: 165 us; at -1e10, beyond: 244.)
 struct Running {
   static constexpr float kAhead = 8.f, kWide = 2147483648.f;
   float ref = -INFINITY, base = 0.f;
@@ -412,7 +412,7 @@ struct RowOutputs {
 // largest of their largest elements is a bound that `top` elements reach, so that only the threads whose largest one reaches it can hold one of the first
 // `top`: their elements are read once more (the batches of loads that have those, from L2), and those at or above the bound sorted by counting.
 // A warp's loads are bulk copies into shared memory, units ahead of the one that it works on.
-// Exponentials bound it after memory: 4096 rows of 160000 in bf16 with one alternative take 240 to 253 us, 80 % of a copy's rate, the exponentials' unit 67 % busy. Few rows take
+// Exponentials bound it after memory: 4096 rows of 160000 in bf16 with one alternative take 242 us, 83 % of a copy's rate, the exponentials' unit 67 % busy. Few rows take
 // a chain of latencies: one row of 150001 with 5 alternatives 12 us, 6 of them for its sums, 2 for the target, 4 for the alternatives.
 template <typename T, bool kLong>
 __global__ void __launch_bounds__(kThreads, Shape<kLong>::kPerSm) logprobs_kernel(const LogprobArgs a) {

@@ -467,8 +467,8 @@ __device__ __forceinline__ uint4 operand(const std::uint8_t* p, int c) {
 // Few tokens: 16 of a tile in one kernel. A cluster of CTAs divides the channels, then the columns; a CTA's warps take 64 of its channels each in turn, are
 // added up with each other and with the other CTAs' through distributed shared memory, and take 32 of its columns each in turn. A, x, B and y come through
 // stages of shared memory of each warp, the first of B and y ahead of A's last. What bounds it is latency, and how much of A and B is on its way.
-// Where tiles are few several clusters share one: each makes the tile's sums and has some of the columns. One token of rank 16, 2048 to 2048, takes 4.9 us, 64 of as many
-// users, 48 adapters, 4096 to 6144, from memory 8.5 (their bytes: 2.0). (As two kernels 4.4 to 5.0 and 10.2, and another launch of 2.5 us for the host.)
+// Where tiles are few several clusters share one: each makes the tile's sums and has some of the columns. One token of rank 16, 2048 to 2048, takes 4.1 us, 64 of as many
+// users, 48 adapters, 4096 to 6144, 7.3, from memory 11 (their bytes: 1.2). (As two kernels 1.7 from memory more, and another launch of 2.5 us for the host.)
 template <int kNT>
 struct FewShape {
   static constexpr int kRanks = kNT * 8;
@@ -771,7 +771,7 @@ __device__ __forceinline__ void end_tensor(Tensor& s) {
 // tensor memory in its two 16-bit parts. Both kinds of steps run through the same stages of shared memory, rows of 128 bytes with the 128-byte swizzle,
 // so that y and B are on their way while the sums are exchanged. A tile's tokens need not be neighbours, so that the threads copy the rows, piece by
 // piece. Where tiles are few several clusters share one: each makes the tile's sums and has some of the columns. Memory should bound it (x and y are read, out written):
-// 8191 tokens of 6 adapters, 4096 to 4096, rank 64 take 59 to 64 us, half of a copy's rate; a CTA's parts, the exchange among them, do not overlap each other.
+// 8191 tokens of 6 adapters, 4096 to 4096, rank 64 take 64 us, half of a copy's rate; a CTA's parts, the exchange among them, do not overlap each other.
 // (As two kernels, x A^T left in global memory: 8191 tokens, 4096 to 4096, rank 64: 71 us, on mma.sync, whose rate is a quarter, 69.)
 template <int kNT>
 struct ManyShape {

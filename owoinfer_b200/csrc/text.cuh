@@ -1,5 +1,5 @@
 // What the operators around a text decoder's attention share (norm_quantize.cu, lora.cu, logprobs.cu): element types, eight neighbouring elements as
-// fp32 and back, warp sums. No counterpart in the reference.
+// fp32 and back. No counterpart in the reference.
 #pragma once
 
 #include <type_traits>
